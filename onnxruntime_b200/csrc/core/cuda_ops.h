@@ -40,5 +40,6 @@ at::Tensor GemmAllReduce(OpKernelContext& ctx, const at::Tensor& partial, const 
 void RegisterMoreCudaKernels(KernelRegistry& r);
 void RegisterCudaKernels3(KernelRegistry& r);
 void RegisterCudaKernels4(KernelRegistry& r);
+void RegisterCudaKernels5(KernelRegistry& r);
 
 }  // namespace ortb

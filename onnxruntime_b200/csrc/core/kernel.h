@@ -201,6 +201,7 @@ at::Tensor ToFloat8(const at::Tensor& x, at::ScalarType type, bool saturate);
 void RegisterControlFlowKernels(KernelRegistry& r);
 void RegisterCollectiveKernels(KernelRegistry& r);
 void RegisterHybridKernels(KernelRegistry& r);
+void RegisterServingKernels(KernelRegistry& r);
 void RegisterCudaKernels(KernelRegistry& r);
 void EnsureKernelsRegistered();
 

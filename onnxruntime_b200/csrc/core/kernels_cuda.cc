@@ -532,6 +532,7 @@ void RegisterCudaKernels(KernelRegistry& r) {
   RegisterMoreCudaKernels(r);
   RegisterCudaKernels3(r);
   RegisterCudaKernels4(r);
+  RegisterCudaKernels5(r);
 }
 
 }  // namespace ortb

@@ -682,6 +682,33 @@ void RegisterBuiltinSchemas(std::map<std::string, OpSchema>& t) {
   Reg(t, FUSED, "LatentPagedAttention", 9, 12);
   Reg(t, FUSED, "ClampedSwiGLU", 2, 2);
   Reg(t, FUSED, "SoftCap", 1, 1);
+  Reg(t, FUSED, "PagedBatchLayout", 5, 5, [](Ctx& c) {
+    if (c.HasShape(2)) c.SetOutput(0, pb::INT32, c.Dims(2));
+    if (c.Rank(0) == 1) c.SetOutput(1, pb::INT32, {c.Dims(0)[0].has_value ? Known(c.Dims(0)[0].value + 1) : c.FreshDim()});
+    for (size_t i : {2, 3})
+      if (c.Rank(4) >= 1) c.SetOutput(i, pb::INT64, {c.Dims(4)[0]});
+    c.SetOutput(4, pb::INT32, {Known(1)});
+  });
+  Reg(t, FUSED, "SharedPrefixPagedAttention", 9, 13, [](Ctx& c) {
+    if (!c.HasShape(0) || c.Rank(0) != 2) return;
+    Dims out = c.Dims(0);
+    const int64_t N = c.node.attr_i("num_heads", 0), Nk = c.node.attr_i("kv_num_heads", 0);
+    if (!c.node.has_input(1) && out[1].has_value && N > 0) out[1] = Known(out[1].value / (N + 2 * Nk) * N);
+    c.SetOutput(0, c.ElemType(0), out);
+    c.PassThrough(3, 1);
+    c.PassThrough(4, 2);
+  });
+  Reg(t, FUSED, "TokenLogProbs", 2, 2, [](Ctx& c) {
+    if (c.Rank(0) < 1) return;
+    Dims lead = c.Dims(0);
+    lead.pop_back();
+    Dims top = lead;
+    top.push_back(Known(c.node.attr_i("top_k", 0)));
+    for (size_t i : {0, 1, 4}) c.SetOutput(i, pb::FLOAT, lead);
+    c.SetOutput(2, pb::FLOAT, top);
+    c.SetOutput(3, pb::INT64, top);
+  });
+  Reg(t, FUSED, "TokenLogProbsGrad", 3, 9, Same);
   Reg(t, FUSED, "SwiGLU", 1, 1, [](Ctx& c) {
     if (!c.HasShape(0) || c.Rank(0) < 1) return;
     Dims out = c.Dims(0);
