@@ -148,6 +148,10 @@ class SharedPrefixPagedAttentionKernel final : public WithGeneric {
       a.scale = z.scale;
       a.softcap = z.softcap;
       a.dtype = dt;
+      // 16-bit heads of 64 or 128 over blocks that a tile of 64 keys divides, or that divide it
+      const bool blocks = z.block_size % 64 == 0 || z.block_size == 8 || z.block_size == 16 || z.block_size == 32;
+      const bool aligned = ((reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache)) & 15) == 0;
+      a.tensor_cores = dt != ORTB200_F32 && (z.H == 64 || z.H == 128) && blocks && aligned && z.N / z.Nk <= 128 ? 1 : 0;
       a.use_pdl = Pdl(ctx);
       a.status = ctx.session()->StatusWord().data_ptr<int>();
       const int64_t bytes = ortb200_prefix_attn_workspace_bytes(a.T, a.B, a.N, a.Nk, a.H, a.tensor_cores);
@@ -155,7 +159,7 @@ class SharedPrefixPagedAttentionKernel final : public WithGeneric {
       a.workspace = ws.data_ptr();
       a.workspace_bytes = bytes;
       CheckLaunch(ortb200_prefix_attn(&a, ctx.cuda_stream()), "ortb200_prefix_attn");
-      ctx.session()->AddLaunches(2);
+      ctx.session()->AddLaunches(a.tensor_cores ? 3 : 2);
     }
     ctx.SetOutput(0, out);
     if (ctx.OutputCount() > 1) ctx.SetOutput(1, kc);

@@ -3,11 +3,24 @@
 // softmax(q K^T) V splits over any partition of the keys: with m the largest score of a part, l = sum exp(s - m) and
 // o = sum exp(s - m) v, two parts join as m = max(m1, m2), l = l1 e^(m1 - m) + l2 e^(m2 - m), o likewise; the result is o / l.
 //
-// Step 1 rotates the queries and the new keys and appends keys and values to the cache; step 2 attends.
+// Step 1 rotates the queries and the new keys and appends keys and values to the cache; step 2 attends; step 3 joins the parts.
+//
+// Tensor-core form.  A unit of work is a tile of up to 128 query rows (a row is one token and one of the G query heads that
+// share a key head) against the keys of one key head: rows of all sequences against the prefix, or rows of one sequence
+// against its own keys.  The units' 64-key tiles are numbered consecutively and every CTA takes an equal share of the numbers,
+// so that one long prefix and many short tails fill the machine alike, without a word about it from the host, which does not
+// know the lengths.  A CTA's share of a unit is a segment; it leaves (m, l, o) of its rows in 32 bits, and step 3 joins the
+// segments of a row.  Which CTA wrote what follows from the same arithmetic: nothing is counted, nothing waited for.
+//
+// Within a CTA (192 threads, two per SM): warp 0 loads tiles by TMA through the block table, warp 1 issues the products
+// (S = Q K^T into tensor memory, O += P V with P in tensor memory over the scores), warps 2 to 5 hold one row per thread.
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <math.h>
+#include "attn_internal.h"
 #include "launch_util.cuh"
 #include "serving_ops.h"
+#include "tensor_map.h"
 
 namespace ortb200 {
 namespace {
@@ -85,7 +98,7 @@ __global__ void __launch_bounds__(128) prefix_rows_kernel(const ortb200_prefix_a
   for (int r = 0; r < R; ++r) o[r] = 0.f;
   if (t < last_row(a)) {
     const int b = sequence_of(a.cu_seqlens, a.B, t);
-    const Span s = span_of(a, b);
+    const Span s = span_of(a, b);   // (cumulative lengths that start behind 0 leave rows to nobody: no keys)
     const long long cap = static_cast<long long>(a.max_blocks) * a.block_size;
     const int keys = static_cast<int>(min(static_cast<long long>(s.past) + (t - s.row0) + 1, cap));
     const float scale = a.scale != 0.f ? a.scale : 1.f / sqrtf(static_cast<float>(H));
@@ -116,6 +129,658 @@ __global__ void __launch_bounds__(128) prefix_rows_kernel(const ortb200_prefix_a
     if (r * 32 + lane < H) out[r * 32 + lane] = from_float<T>(o[r] * inv);
 }
 
+// ------------------------------------------------------------------------------------------------------- tensor-core form
+constexpr int kQT = 128;          // query rows of a unit
+constexpr int kKT = 64;           // keys of a tile
+constexpr int kThreads = 192;
+constexpr int kGrid = 296;        // two CTAs on each of 148 SMs
+constexpr int kTmemCols = 256;    // two score buffers of 64 columns, O in up to 128
+constexpr int kPlanInSmem = 1024; // sequences whose running sums a CTA keeps in shared memory
+
+// What step 1 finds out about the lengths.
+struct Plan {
+  long long total;       // tiles of all units
+  int prefix_tiles;      // tiles of the prefix
+  int prefix_row;        // row of the block table that the prefix is read from
+  // then: long long first[B + 1], the tiles of the own units in front of each sequence's
+};
+
+struct Work {            // the workspace's parts
+  Plan* plan;
+  long long* first;
+  uint16_t* q;           // [Nk, T G, H]
+  float2* ml;            // per row of a segment: m (in units of log 2) and l
+  float* o;              // per row of a segment: H values
+};
+__host__ __device__ inline long long up256(long long n) { return (n + 255) / 256 * 256; }
+__host__ __device__ inline long long segment_rows(long long T, int N) { return 2 * T * N + static_cast<long long>(kGrid) * kQT; }
+__host__ __device__ inline Work work_of(const ortb200_prefix_attn_args& a) {
+  char* p = static_cast<char*>(a.workspace);
+  Work w;
+  w.plan = reinterpret_cast<Plan*>(p);
+  w.first = reinterpret_cast<long long*>(p + sizeof(Plan));
+  p += up256(sizeof(Plan) + 8ll * (a.B + 1));
+  w.q = reinterpret_cast<uint16_t*>(p);
+  p += up256(a.T * a.N * a.H * 2);
+  w.ml = reinterpret_cast<float2*>(p);
+  p += up256(segment_rows(a.T, a.N) * 8);
+  w.o = reinterpret_cast<float*>(p);
+  return w;
+}
+
+// The share of CTA i of `total` tiles starts at share(i); tile x belongs to CTA owner(x).
+__device__ __forceinline__ long long share(long long total, int i) { return total * i / kGrid; }
+__device__ __forceinline__ int owner(long long total, long long x) { return static_cast<int>(((x + 1) * kGrid - 1) / total); }
+
+// Unit `rt` (rows [128 rt, 128 rt + 128) of the sequence's rows x G) of a sequence: its keys [prefix keys, end) in tiles of 64.
+__device__ __forceinline__ int own_end(const ortb200_prefix_attn_args& a, const Span& s, int rt) {
+  const int G = a.N / a.Nk, last = min(rt * kQT + kQT, s.rows * G) - 1;
+  return static_cast<int>(min(static_cast<long long>(s.past) + last / G + 1, static_cast<long long>(a.max_blocks) * a.block_size));
+}
+__device__ __forceinline__ int own_tiles(const ortb200_prefix_attn_args& a, const Span& s, int rt, int prefix_tiles) {
+  return max((own_end(a, s, rt) + kKT - 1) / kKT - prefix_tiles, 0);
+}
+__device__ __forceinline__ int row_tiles(const ortb200_prefix_attn_args& a, int rows) { return (rows * (a.N / a.Nk) + kQT - 1) / kQT; }
+// first row that the segments of a unit may use, before 128 rows per CTA number: units follow one another without a gap
+__device__ __forceinline__ long long prefix_slot(const ortb200_prefix_attn_args& a, int rt, int kvh, int rows) {
+  return static_cast<long long>(rt) * kQT * a.Nk + static_cast<long long>(kvh) * rows;
+}
+__device__ __forceinline__ long long own_slot(const ortb200_prefix_attn_args& a, int row0, int rt, int kvh, int rows) {
+  return a.T * a.N + static_cast<long long>(a.Nk) * (static_cast<long long>(row0) * (a.N / a.Nk) + static_cast<long long>(rt) * kQT) + static_cast<long long>(kvh) * rows;
+}
+
+// One CTA: how many tokens all sequences share, and the running sums of their own tiles.
+__device__ void make_plan(const ortb200_prefix_attn_args& a, const Work& w) {
+  __shared__ int shortest, first_row;
+  __shared__ long long warp_sum64[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    shortest = 0x7fffffff;
+    first_row = 0x7fffffff;
+  }
+  __syncthreads();
+  int least = 0x7fffffff, row = 0x7fffffff;
+  for (int b = threadIdx.x; b < a.B; b += 128) {
+    const Span s = span_of(a, b);
+    if (s.rows == 0) continue;
+    least = min(least, s.past);
+    row = min(row, b);
+    if (a.past_seqlens[b] != s.past || s.past + static_cast<long long>(s.rows) > static_cast<long long>(a.max_blocks) * a.block_size)
+      if (a.status) atomicExch(a.status, kStatusBadLength);
+  }
+  atomicMin(&shortest, least);
+  atomicMin(&first_row, row);
+  __syncthreads();
+  const int prefix_tiles = shortest == 0x7fffffff ? 0 : max(min(*a.shared_prefix, shortest), 0) / kKT;
+  long long base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 128) {
+    const int b = b0 + threadIdx.x;
+    long long n = 0;
+    if (b < a.B) {
+      const Span s = span_of(a, b);
+      for (int rt = 0; rt < row_tiles(a, s.rows); ++rt) n += own_tiles(a, s, rt, prefix_tiles);
+      n *= a.Nk;
+    }
+    long long sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sum64[warp] = sum;
+    __syncthreads();
+    long long before = base;
+    for (int i = 0; i < 4; ++i) {
+      if (i < warp) before += warp_sum64[i];
+      base += warp_sum64[i];
+    }
+    if (b < a.B) w.first[b] = before + sum - n;
+  }
+  if (threadIdx.x == 0) {
+    w.first[a.B] = base;
+    w.plan->prefix_tiles = prefix_tiles;
+    w.plan->prefix_row = first_row == 0x7fffffff ? 0 : first_row;
+    w.plan->total = base + static_cast<long long>(row_tiles(a, last_row(a))) * a.Nk * prefix_tiles;
+  }
+}
+
+// Step 1: one CTA (or, for few tokens, several) per token and one more for the plan.  VEC: whole heads rotated in halves or not
+// at all, every address a multiple of 16 bytes: a thread moves 2 x 16 bytes; otherwise one element.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefix_attn_args a) {
+  const Work w = work_of(a);
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  if (blockIdx.x == a.T) {
+    if (blockIdx.y == 0) make_plan(a, w);
+    return;
+  }
+  const int t = blockIdx.x, H = a.H, heads = a.N + 2 * a.Nk, G = a.N / a.Nk;
+  if (t >= last_row(a)) return;
+  long long slot, pos;
+  if (a.positions) {
+    pos = a.positions[t];
+    slot = a.slot_mapping[t];
+  } else {
+    const int b = sequence_of(a.cu_seqlens, a.B, t);
+    pos = static_cast<long long>(a.past_seqlens[b]) + (t - a.cu_seqlens[b]);
+    const long long j = pos / a.block_size;
+    slot = pos >= 0 && j < a.max_blocks ? static_cast<long long>(a.block_table[static_cast<long long>(b) * a.max_blocks + j]) * a.block_size + pos % a.block_size : -1;
+  }
+  const bool keep = slot >= 0 && slot < static_cast<long long>(a.num_blocks) * a.block_size;
+  if (!keep && threadIdx.x == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
+  const int half = a.rot_dim / 2;
+  pos = pos < 0 ? 0 : pos >= a.cos_rows ? a.cos_rows - 1 : pos;   // never past the rotary tables
+  const T* cosr = a.cos_cache ? static_cast<const T*>(a.cos_cache) + pos * half : nullptr;
+  const T* sinr = a.cos_cache ? static_cast<const T*>(a.sin_cache) + pos * half : nullptr;
+  const int per_block = (heads + gridDim.y - 1) / gridDim.y;
+  const int lo = blockIdx.y * per_block, hi = min(heads, lo + per_block), items = VEC ? H / 16 : H;
+  for (int idx = lo * items + threadIdx.x; idx < hi * items; idx += 128) {
+    const int head = idx / items, d = VEC ? idx % items * 8 : idx % items;
+    const int kind = head < a.N ? 0 : head < a.N + a.Nk ? 1 : 2, kh = head - (kind == 1 ? a.N : a.N + a.Nk);
+    const T* src;
+    if (a.k == nullptr) src = static_cast<const T*>(a.qkv) + (static_cast<long long>(t) * heads + head) * H;
+    else if (kind == 0) src = static_cast<const T*>(a.qkv) + (static_cast<long long>(t) * a.N + head) * H;
+    else src = static_cast<const T*>(kind == 1 ? a.k : a.v) + (static_cast<long long>(t) * a.Nk + kh) * H;
+    T* dst;
+    if (kind == 0) {
+      dst = reinterpret_cast<T*>(w.q) + ((static_cast<long long>(head / G) * a.T + t) * G + head % G) * H;
+    } else {
+      if (!keep) continue;
+      dst = static_cast<T*>(kind == 1 ? a.k_cache : a.v_cache) + (slot * a.Nk + kh) * H;
+    }
+    const bool turn = kind < 2 && cosr;
+    if (VEC) {
+      const int far = H / 2;
+      const uint4 u4 = *reinterpret_cast<const uint4*>(src + d), v4 = *reinterpret_cast<const uint4*>(src + d + far);
+      if (!turn) {
+        *reinterpret_cast<uint4*>(dst + d) = u4;
+        *reinterpret_cast<uint4*>(dst + d + far) = v4;
+        continue;
+      }
+      const uint4 c4 = *reinterpret_cast<const uint4*>(cosr + d), s4 = *reinterpret_cast<const uint4*>(sinr + d);
+      const T *u = reinterpret_cast<const T*>(&u4), *v = reinterpret_cast<const T*>(&v4), *c = reinterpret_cast<const T*>(&c4), *s = reinterpret_cast<const T*>(&s4);
+      __align__(16) T y0[8], y1[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x0 = to_float<T>(u[e]), x1 = to_float<T>(v[e]), cc = to_float<T>(c[e]), ss = to_float<T>(s[e]);
+        y0[e] = from_float<T>(x0 * cc - x1 * ss);
+        y1[e] = from_float<T>(x1 * cc + x0 * ss);
+      }
+      *reinterpret_cast<uint4*>(dst + d) = *reinterpret_cast<const uint4*>(y0);
+      *reinterpret_cast<uint4*>(dst + d + far) = *reinterpret_cast<const uint4*>(y1);
+    } else {
+      T y = src[d];
+      if (turn && d < a.rot_dim) {
+        const int i = a.interleaved ? d >> 1 : d % half;
+        const bool upper = a.interleaved ? d & 1 : d >= half;
+        const float c = to_float<T>(cosr[i]), s = to_float<T>(sinr[i]), own = to_float<T>(src[d]);
+        const float other = to_float<T>(src[a.interleaved ? d ^ 1 : upper ? d - half : d + half]);
+        y = from_float<T>(upper ? own * c + other * s : own * c - other * s);
+      }
+      dst[d] = y;
+    }
+  }
+}
+
+template <int HD>
+struct TcSmem {
+  static constexpr int kStages = HD == 64 ? 3 : 2;
+  static constexpr int kBoxes = HD / 64;                  // boxes of 64 elements per row
+  static constexpr int kQBox = kQT * 128, kBox = kKT * 128;
+  static constexpr int kStageBytes = 2 * kBoxes * kBox;   // K, then V
+  static constexpr int kOffKV = kBoxes * kQBox;
+  static constexpr int kOffBar = kOffKV + kStages * kStageBytes;
+  static constexpr int kOffFirst = kOffBar + 256;
+  static constexpr int kTotal = kOffFirst + 8 * (kPlanInSmem + 1) + 1024;
+};
+enum { BAR_Q = 0, BAR_Q_FREE, BAR_K_FULL, BAR_K_EMPTY = BAR_K_FULL + 3, BAR_V_FULL = BAR_K_EMPTY + 3, BAR_V_EMPTY = BAR_V_FULL + 3, BAR_S = BAR_V_EMPTY + 3,
+       BAR_P = BAR_S + 2, BAR_O = BAR_P + 2, BAR_END, BAR_O_FREE, BAR_COUNT };
+static_assert(BAR_COUNT * 8 + 4 <= 256, "barriers do not fit");
+
+// A CTA's share of one unit.
+struct Segment {
+  int kvh, seq;          // key head; sequence, -1 for the prefix
+  int q_row;             // first row of the unit among the T G rows of its key head
+  int rows, tiles;       // rows of the unit, tiles of the segment
+  int key0, end;         // first key of the segment, end of the unit's keys
+  int past, in_seq;      // own units: tokens in front of the sequence's rows, first row of the unit among the sequence's rows x G
+  int table_row;
+  long long slot;
+};
+struct Walk {
+  const ortb200_prefix_attn_args& a;
+  const long long* first;   // running sums, in shared memory when they fit
+  long long total, cur, stop, prefix_total;
+  int prefix_tiles, prefix_row, all_rows;
+  __device__ bool next(Segment& g) {
+    if (cur >= stop) return false;
+    const int G = a.N / a.Nk;
+    long long left;         // tiles of the unit from `cur` on
+    if (cur < prefix_total) {
+      const long long u = cur / prefix_tiles;
+      const int t0 = static_cast<int>(cur - u * prefix_tiles), rt = static_cast<int>(u / a.Nk);
+      g.kvh = static_cast<int>(u % a.Nk);
+      g.seq = -1;
+      g.q_row = rt * kQT;
+      g.rows = min(kQT, all_rows * G - g.q_row);
+      g.key0 = t0 * kKT;
+      g.end = prefix_tiles * kKT;
+      g.past = g.in_seq = 0;
+      g.table_row = prefix_row;
+      g.slot = prefix_slot(a, rt, g.kvh, g.rows);
+      left = prefix_tiles - t0;
+    } else {
+      long long x = cur - prefix_total;
+      int lo = 0, hi = a.B;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= x) lo = mid; else hi = mid;
+      }
+      x -= first[lo];
+      const Span s = span_of(a, lo);
+      int rt = 0, n = own_tiles(a, s, 0, prefix_tiles);
+      while (x >= static_cast<long long>(n) * a.Nk) {
+        x -= static_cast<long long>(n) * a.Nk;
+        n = own_tiles(a, s, ++rt, prefix_tiles);
+      }
+      g.kvh = static_cast<int>(x / n);
+      const int t0 = static_cast<int>(x % n);
+      g.seq = lo;
+      g.in_seq = rt * kQT;
+      g.q_row = s.row0 * G + g.in_seq;
+      g.rows = min(kQT, s.rows * G - g.in_seq);
+      g.key0 = (prefix_tiles + t0) * kKT;
+      g.end = own_end(a, s, rt);
+      g.past = s.past;
+      g.table_row = lo;
+      g.slot = own_slot(a, s.row0, rt, g.kvh, g.rows);
+      left = n - t0;
+    }
+    g.tiles = static_cast<int>(min(left, stop - cur));
+    cur += g.tiles;
+    return true;
+  }
+};
+
+__device__ __forceinline__ void store8(float* p, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]),
+               "f"(v[7])
+               : "memory");
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 2)
+prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                   const ortb200_prefix_attn_args a, const float scale) {
+  using L = TcSmem<HD>;
+  constexpr int STAGES = L::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BAR_COUNT);
+  long long* first_sm = reinterpret_cast<long long*>(smem + L::kOffFirst);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool bf16 = a.dtype == ORTB200_BF16;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+    for (int i = 0; i < BAR_COUNT; ++i) mbar_init(&bars[i], i == BAR_P || i == BAR_P + 1 || i == BAR_O_FREE ? 128 : 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  const Work w = work_of(a);
+  const bool kept = a.B <= kPlanInSmem;
+  if (kept)
+    for (int b = threadIdx.x; b <= a.B; b += kThreads) first_sm[b] = w.first[b];
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_s = *tmem_slot;          // S / P: two buffers of 64 columns
+  const uint32_t tmem_o = tmem_s + 2 * kKT;
+
+  Walk walk{a, kept ? first_sm : w.first};
+  walk.total = w.plan->total;
+  walk.prefix_tiles = w.plan->prefix_tiles;
+  walk.prefix_row = w.plan->prefix_row;
+  walk.all_rows = last_row(a);
+  walk.prefix_total = static_cast<long long>(row_tiles(a, walk.all_rows)) * a.Nk * walk.prefix_tiles;
+  walk.cur = share(walk.total, blockIdx.x);
+  walk.stop = share(walk.total, blockIdx.x + 1);
+  Segment g;
+  bool ok = true;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------------------------------------------- loads
+    const int piece = min(a.block_size, kKT), pieces = kKT / piece;   // rows that one block gives a tile
+    int s = 0, seg = 0, k_tiles = 0, v_tiles = 0;
+    uint32_t parity = 1;   // the first round over the stages waits for nothing
+    while (ok && walk.next(g)) {
+      const int* table = a.block_table + static_cast<long long>(g.table_row) * a.max_blocks;
+      if (seg > 0 && !mbar_wait_warp(&bars[BAR_Q_FREE], (seg - 1) & 1)) { ok = false; break; }
+      if (lane == 0) {
+        mbar_expect_tx(&bars[BAR_Q], L::kBoxes * L::kQBox);
+        for (int bx = 0; bx < L::kBoxes; ++bx) tma_load_3d(smem + bx * L::kQBox, &tm_q, &bars[BAR_Q], bx * 64, g.q_row, g.kvh);
+      }
+      ++seg;
+      auto block_at = [&](int key) { return min(max(table[min(key / a.block_size, a.max_blocks - 1)], 0), a.num_blocks - 1); };
+      int block = lane < pieces ? block_at(g.key0 + lane * piece) : 0;
+      for (int t = 0; t < g.tiles; ++t) {
+        const int key = g.key0 + t * kKT + lane * piece, in_block = key % a.block_size;
+        uint8_t* st = smem + L::kOffKV + s * L::kStageBytes + lane * piece * 128;
+        if (!mbar_wait_warp(&bars[BAR_K_EMPTY + s], parity)) { ok = false; break; }
+        if (lane == 0) mbar_expect_tx(&bars[BAR_K_FULL + s], L::kBoxes * L::kBox);
+        __syncwarp();
+        ++k_tiles;
+        if (lane < pieces)
+          for (int bx = 0; bx < L::kBoxes; ++bx) tma_load_4d(st + bx * L::kBox, &tm_k, &bars[BAR_K_FULL + s], bx * 64, in_block, g.kvh, block);
+        if (!mbar_wait_warp(&bars[BAR_V_EMPTY + s], parity)) { ok = false; break; }
+        if (lane == 0) mbar_expect_tx(&bars[BAR_V_FULL + s], L::kBoxes * L::kBox);
+        __syncwarp();
+        ++v_tiles;
+        if (lane < pieces)
+          for (int bx = 0; bx < L::kBoxes; ++bx) tma_load_4d(st + (L::kBoxes + bx) * L::kBox, &tm_v, &bars[BAR_V_FULL + s], bx * 64, in_block, g.kvh, block);
+        if (t + 1 < g.tiles && lane < pieces) block = block_at(key + kKT);
+        if (++s == STAGES) { s = 0; parity ^= 1u; }
+      }
+    }
+    // whoever gave up: no copy may be on its way when the CTA ends
+    if (seg > 0 && !mbar_wait_warp(&bars[BAR_Q], (seg - 1) & 1)) ok = false;
+    for (int i = 0; i < STAGES; ++i) {
+      const int k = (k_tiles - i + STAGES - 1) / STAGES, v = (v_tiles - i + STAGES - 1) / STAGES;   // loads into stage i
+      if (k > 0 && !mbar_wait_warp(&bars[BAR_K_FULL + i], (k - 1) & 1)) ok = false;
+      if (v > 0 && !mbar_wait_warp(&bars[BAR_V_FULL + i], (v - 1) & 1)) ok = false;
+    }
+    if (!ok && lane == 0 && a.status) atomicExch(a.status, kStatusTimeoutProducer);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------------------------------------- products
+    const uint32_t idesc_s = umma_idesc_f16(bf16, kQT, kKT);
+    const uint32_t idesc_o = umma_idesc_f16_bmn(bf16, kQT, HD);
+    const uint32_t q_addr = smem_u32(smem);
+    int s = 0, seg = 0, it = 0;   // stage, segment and tile of this CTA
+    uint32_t parity = 0;
+    auto issue_s = [&](int tile, int stage, bool last) {
+      if (lane == 0) {
+        const uint32_t k_addr = smem_u32(smem + L::kOffKV + stage * L::kStageBytes);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          umma_f16(tmem_s + (tile & 1) * kKT, umma_desc_sw128(q_addr + (kk / 4) * L::kQBox + (kk % 4) * 32),
+                   umma_desc_sw128(k_addr + (kk / 4) * L::kBox + (kk % 4) * 32), idesc_s, kk > 0 ? 1u : 0u);
+        umma_commit(&bars[BAR_S + (tile & 1)]);
+        umma_commit(&bars[BAR_K_EMPTY + stage]);
+        if (last) umma_commit(&bars[BAR_Q_FREE]);
+      }
+      __syncwarp();
+    };
+    while (ok && walk.next(g)) {
+      // scores go over the weights of two tiles before; the products that read those are behind the last tile's, which are over
+      if (it > 0 && !mbar_wait_warp(&bars[BAR_O], (it - 1) & 1)) { ok = false; break; }
+      if (!mbar_wait_warp(&bars[BAR_Q], seg & 1) || !mbar_wait_warp(&bars[BAR_K_FULL + s], parity)) { ok = false; break; }
+      tcgen05_fence_after();
+      issue_s(it, s, g.tiles == 1);
+      for (int t = 0; t < g.tiles; ++t, ++it) {
+        const int s1 = s + 1 == STAGES ? 0 : s + 1;
+        const uint32_t parity1 = s1 == 0 ? parity ^ 1u : parity;
+        if (t + 1 < g.tiles) {
+          if (it > 0 && !mbar_wait_warp(&bars[BAR_O], (it - 1) & 1)) { ok = false; break; }
+          if (!mbar_wait_warp(&bars[BAR_K_FULL + s1], parity1)) { ok = false; break; }
+          tcgen05_fence_after();
+          issue_s(it + 1, s1, t + 2 == g.tiles);
+        }
+        uint8_t* v = smem + L::kOffKV + s * L::kStageBytes + L::kBoxes * L::kBox;
+        if (!mbar_wait_warp(&bars[BAR_V_FULL + s], parity)) { ok = false; break; }
+        const int live = g.end - (g.key0 + t * kKT);
+        if (live < kKT) {
+          // what lies behind the last key may be anything, and 0 * NaN would reach the product
+          const uint4 zero = make_uint4(0, 0, 0, 0);
+          for (int i = lane; i < (kKT - live) * 8; i += 32)
+            for (int bx = 0; bx < L::kBoxes; ++bx) *reinterpret_cast<uint4*>(v + bx * L::kBox + live * 128 + i * 16) = zero;
+          fence_proxy_async();
+          __syncwarp();
+        }
+        if (!mbar_wait_warp(&bars[BAR_P + (it & 1)], (it >> 1) & 1)) { ok = false; break; }
+        if (t == 0 && seg > 0 && !mbar_wait_warp(&bars[BAR_O_FREE], (seg - 1) & 1)) { ok = false; break; }
+        tcgen05_fence_after();
+        if (lane == 0) {
+          const uint32_t v_addr = smem_u32(v), tmem_p = tmem_s + (it & 1) * kKT;
+#pragma unroll
+          for (int kk = 0; kk < kKT / 16; ++kk)
+            umma_f16_ts(tmem_o, tmem_p + kk * 8, umma_desc_mn_sw128(v_addr + kk * 2048, L::kBox, 1024), idesc_o, t > 0 || kk > 0 ? 1u : 0u);
+          umma_commit(&bars[BAR_O]);
+          umma_commit(&bars[BAR_V_EMPTY + s]);
+          if (t == g.tiles - 1) umma_commit(&bars[BAR_END]);
+        }
+        __syncwarp();
+        s = s1;
+        parity = parity1;
+      }
+      ++seg;
+    }
+    if (!ok && lane == 0 && a.status) atomicExch(a.status, kStatusTimeoutMma);
+  } else {
+    // --------------------------------------------------------------------------------- softmax, one thread per row
+    const int qw = warp & 3, r = qw * 32 + lane, G = a.N / a.Nk;
+    const uint32_t lane_addr = static_cast<uint32_t>(qw * 32) << 16;
+    const float scale_log2 = scale * 1.4426950408889634f;
+    // The reference maximum of a row is raised only when a tile exceeds it by 2^8 (weights stay below 256), so that O in tensor
+    // memory is rescaled a few times per row.
+    constexpr float kRaise = 8.f;
+    int seg = 0, it = 0;
+    while (ok && walk.next(g)) {
+      const bool idle = qw * 32 >= g.rows;   // a warp without rows keeps the barriers going
+      const int pos = g.seq < 0 ? 0x7fffffff : g.past + (g.in_seq + r) / G;
+      const int first_pos = g.seq < 0 ? 0x7fffffff : g.past + g.in_seq / G;
+      float m = -INFINITY, l = 0.f;
+      for (int t = 0; t < g.tiles; ++t, ++it) {
+        const int key0 = g.key0 + t * kKT;
+        if (ok && !mbar_wait_warp(&bars[BAR_S + (it & 1)], (it >> 1) & 1)) ok = false;
+        tcgen05_fence_after();
+        if (!idle) {
+          const uint32_t s_addr = tmem_s + (it & 1) * kKT + lane_addr;
+          float sv[kKT];
+          tmem_ld_x32(s_addr, sv);
+          tmem_ld_x32(s_addr + 32, sv + 32);
+          tmem_ld_wait();
+          float fs = scale_log2;   // scores stay unscaled: the scale is part of the exponent's multiply-add; a cap leaves base-2 exponents
+          if (a.softcap > 0.f) {
+            fs = 1.f;
+#pragma unroll
+            for (int j = 0; j < kKT; ++j) sv[j] = a.softcap * tanhf(sv[j] * scale / a.softcap) * 1.4426950408889634f;
+          }
+          if (key0 + kKT > g.end || key0 + kKT - 1 > first_pos) {
+            const int hi = min(g.end - key0, pos - key0 + 1);   // keys of this tile that the row sees
+#pragma unroll
+            for (int j = 0; j < kKT; ++j) sv[j] = j < hi ? sv[j] : -INFINITY;
+          }
+          float m_raw = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < kKT; j += 2) m_raw = fmax3(m_raw, sv[j], sv[j + 1]);
+          const float m_tile = m_raw * fs;
+          const bool raise = m_tile > m + kRaise;   // also the first finite maximum of a row
+          if (__any_sync(0xffffffffu, raise)) {
+            const float corr = raise ? (m == -INFINITY ? 0.f : ex2_approx(m - m_tile)) : 1.f;
+            if (t > 0) {
+              if (ok && !mbar_wait_warp(&bars[BAR_O], (it - 1) & 1)) ok = false;
+              tcgen05_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < HD; c += 32) {
+                float v[32];
+                tmem_ld_x32(tmem_o + lane_addr + c, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] *= corr;
+                tmem_st_x32(tmem_o + lane_addr + c, v);
+              }
+            }
+            l *= corr;
+            if (raise) m = m_tile;
+          }
+          const float neg_m = m == -INFINITY ? 0.f : -m;
+          float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+          for (int c = 0; c < kKT; c += 32) {
+            uint32_t packed[16];
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float p0 = ex2_approx(fmaf(sv[c + j], fs, neg_m)), p1 = ex2_approx(fmaf(sv[c + j + 1], fs, neg_m));
+              sum0 += p0;
+              sum1 += p1;
+              if (bf16) {
+                __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
+                packed[j / 2] = *reinterpret_cast<uint32_t*>(&h);
+              } else {
+                __half2 h = __floats2half2_rn(p0, p1);
+                packed[j / 2] = *reinterpret_cast<uint32_t*>(&h);
+              }
+            }
+            tmem_st_x16_u32(s_addr + c / 2, packed);
+          }
+          l += sum0 + sum1;
+          tmem_st_wait();
+        }
+        tcgen05_fence_before();
+        mbar_arrive(&bars[BAR_P + (it & 1)]);
+      }
+      if (ok && !mbar_wait_warp(&bars[BAR_END], seg & 1)) ok = false;
+      tcgen05_fence_after();
+      if (!idle) {
+        const long long row = g.slot + static_cast<long long>(blockIdx.x) * kQT + r;
+        const bool mine = ok && r < g.rows;
+        if (mine) w.ml[row] = make_float2(m, l);
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+          float v[32];
+          tmem_ld_x32(tmem_o + lane_addr + c, v);
+          tmem_ld_wait();
+          if (mine)
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) store8(w.o + row * HD + c + j, v + j);
+        }
+      }
+      tcgen05_fence_before();
+      mbar_arrive(&bars[BAR_O_FREE]);
+      ++seg;
+    }
+    if (!ok && lane == 0 && a.status) atomicExch(a.status, kStatusTimeoutEpilogue);
+  }
+
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_dealloc(tmem_s, kTmemCols);
+  }
+}
+
+// Step 3: one warp per token and query head.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_attn_args a) {
+  constexpr int E = HD / 32;
+  const int lane = threadIdx.x & 31;
+  const long long item = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  pdl_wait_prior_grids();
+  if (item >= a.T * a.N) return;
+  const Work w = work_of(a);
+  const int t = static_cast<int>(item / a.N), head = static_cast<int>(item % a.N), G = a.N / a.Nk, kvh = head / G, all_rows = last_row(a);
+  float o[E], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  if (t < all_rows) {
+    const int b = sequence_of(a.cu_seqlens, a.B, t);
+    const Span s = span_of(a, b);
+    const bool owned = t >= s.row0 && t < s.row0 + s.rows;   // cumulative lengths that start behind 0 leave rows to nobody
+    const long long total = owned ? w.plan->total : 0;
+    const int prefix_tiles = owned ? w.plan->prefix_tiles : 0;
+    // the row's two units: first tile, tiles, first slot, row within the unit
+    const int pr = t * G + head % G, prt = pr / kQT, orow = owned ? (t - s.row0) * G + head % G : 0, ort = orow / kQT;
+    long long tile[2], slot[2];
+    int tiles[2];
+    tile[0] = (static_cast<long long>(prt) * a.Nk + kvh) * prefix_tiles;
+    tiles[0] = prefix_tiles;
+    slot[0] = prefix_slot(a, prt, kvh, min(kQT, all_rows * G - prt * kQT)) + pr % kQT;
+    tile[1] = static_cast<long long>(row_tiles(a, all_rows)) * a.Nk * prefix_tiles + w.first[b];
+    for (int rt = 0; rt < ort; ++rt) tile[1] += static_cast<long long>(own_tiles(a, s, rt, prefix_tiles)) * a.Nk;
+    tiles[1] = owned ? own_tiles(a, s, ort, prefix_tiles) : 0;
+    tile[1] += static_cast<long long>(kvh) * tiles[1];
+    slot[1] = own_slot(a, s.row0, ort, kvh, min(kQT, s.rows * G - ort * kQT)) + orow % kQT;
+    for (int u = 0; u < 2; ++u) {
+      if (tiles[u] == 0) continue;
+      const long long from = tile[u], to = from + tiles[u];
+      const int i0 = owner(total, from), i1 = owner(total, to - 1);
+      for (int c = i0; c <= i1; c += 32) {
+        // lane j: the segment of CTA c + j, if that has a share of the unit
+        const int i = c + lane;
+        const bool has = i <= i1 && max(from, share(total, i)) < min(to, share(total, i + 1));
+        const float2 ml = has ? w.ml[slot[u] + static_cast<long long>(i) * kQT] : make_float2(-INFINITY, 0.f);
+        const float mm = fmaxf(m, warp_max(ml.x));
+        const float keep = m == -INFINITY ? 0.f : exp2f(m - mm), mine = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mm);
+        // a row whose scores are all NaN has no maximum; its sum carries the NaN on
+        l = l * keep + warp_sum(ml.x == -INFINITY ? ml.y : ml.y * mine);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] *= keep;
+        for (unsigned left = __ballot_sync(0xffffffffu, has); left != 0; left &= left - 1) {
+          const int j = __ffs(left) - 1;
+          const float f = __shfl_sync(0xffffffffu, mine, j);
+          const float* p = w.o + (slot[u] + static_cast<long long>(c + j) * kQT) * HD + lane * E;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] += f * p[e];
+        }
+        m = mm;
+      }
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* out = static_cast<T*>(a.out) + item * HD + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[e] = from_float<T>(o[e] * inv);
+}
+
+template <typename T>
+bool vectorised(const ortb200_prefix_attn_args* a) {
+  if (a->cos_cache && (a->interleaved || a->rot_dim != a->H)) return false;
+  uintptr_t p = reinterpret_cast<uintptr_t>(a->qkv) | reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v);
+  if (a->cos_cache) p |= reinterpret_cast<uintptr_t>(a->cos_cache) | reinterpret_cast<uintptr_t>(a->sin_cache);
+  return (p & 15) == 0;
+}
+
+template <typename T, int HD>
+int launch_tc(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
+  using L = TcSmem<HD>;
+  const CUtensorMapDataType dt = a->dtype == ORTB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const int64_t rows = a->T * (a->N / a->Nk), entry = static_cast<int64_t>(a->Nk) * HD * 2;
+  CUtensorMap tq, tk, tv;
+  if (make_tensor_map_3d(&tq, work_of(*a).q, dt, 2, HD, rows, a->Nk, HD * 2, rows * HD * 2, 64, kQT) != 0) return -6;
+  const int64_t dims[4] = {HD, a->block_size, a->Nk, a->num_blocks}, strides[3] = {entry, HD * 2, entry * a->block_size};
+  const int box = a->block_size < kKT ? a->block_size : kKT;
+  if (make_tensor_map_4d(&tk, a->k_cache, dt, 2, dims, strides, 64, box) != 0) return -6;
+  if (make_tensor_map_4d(&tv, a->v_cache, dt, 2, dims, strides, 64, box) != 0) return -6;
+  auto kern = prefix_attn_kernel<HD>;
+  static bool attr_set = false;
+  if (!attr_set) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) != cudaSuccess) return -10;
+    attr_set = true;
+  }
+  const int heads = a->N + 2 * a->Nk;
+  const long long spread = 2 * kGrid / (a->T + 1), most = (heads + 15) / 16;   // few tokens: several CTAs per token, 16 heads at least to each
+  const dim3 prep_grid(static_cast<unsigned>(a->T + 1), static_cast<unsigned>(spread < 1 ? 1 : spread > most ? most : spread));
+  int rc = vectorised<T>(a) ? launch_kernel(prefix_prep_tc_kernel<T, true>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a)
+                            : launch_kernel(prefix_prep_tc_kernel<T, false>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a);
+  if (rc != 0) return rc;
+  const float scale = a->scale != 0.f ? a->scale : 1.f / sqrtf(static_cast<float>(HD));
+  // the two later steps may set up while the step before them ends: they wait for it before they read
+  rc = launch_kernel(kern, dim3(kGrid), kThreads, L::kTotal, stream, true, tq, tk, tv, *a, scale);
+  if (rc != 0) return rc;
+  return launch_kernel(prefix_join_kernel<T, HD>, dim3(static_cast<unsigned>((a->T * a->N + 3) / 4)), 128, 0, stream, true, *a);
+}
+
 template <typename T>
 int launch_rows(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
   T* q = static_cast<T*>(a->workspace);
@@ -131,7 +796,8 @@ int launch_rows(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
 using namespace ortb200;
 
 extern "C" int64_t ortb200_prefix_attn_workspace_bytes(int64_t T, int B, int N, int Nk, int H, int tensor_cores) {
-  return T * N * H * 4;
+  if (!tensor_cores) return up256(T * N * H * 4);
+  return up256(sizeof(Plan) + 8ll * (B + 1)) + up256(T * N * H * 2) + up256(segment_rows(T, N) * 8) + segment_rows(T, N) * H * 4;
 }
 
 extern "C" int ortb200_prefix_attn(const ortb200_prefix_attn_args* a, ortb200_stream_t stream_) {
@@ -145,6 +811,14 @@ extern "C" int ortb200_prefix_attn(const ortb200_prefix_attn_args* a, ortb200_st
   if (a->cos_cache && (!a->sin_cache || a->cos_rows <= 0 || a->rot_dim <= 0 || a->rot_dim % 2 != 0 || a->rot_dim > a->H)) return -1;
   if (a->H > kMaxHead || a->T * a->N > 0x7fffffffll) return -2;
   if (a->workspace_bytes < ortb200_prefix_attn_workspace_bytes(a->T, a->B, a->N, a->Nk, a->H, a->tensor_cores)) return -1;
+  if (a->tensor_cores) {
+    const bool blocks = a->block_size % kKT == 0 || a->block_size == 8 || a->block_size == 16 || a->block_size == 32;
+    if ((a->H != 64 && a->H != 128) || !blocks || a->N / a->Nk > kQT) return -2;
+    if (((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & 15) || (reinterpret_cast<uintptr_t>(a->workspace) & 255)) return -3;
+    if (a->dtype == ORTB200_BF16) return a->H == 128 ? launch_tc<__nv_bfloat16, 128>(a, stream) : launch_tc<__nv_bfloat16, 64>(a, stream);
+    if (a->dtype == ORTB200_F16) return a->H == 128 ? launch_tc<__half, 128>(a, stream) : launch_tc<__half, 64>(a, stream);
+    return -4;
+  }
   switch (a->dtype) {
     case ORTB200_F16: return launch_rows<__half>(a, stream);
     case ORTB200_BF16: return launch_rows<__nv_bfloat16>(a, stream);
