@@ -175,7 +175,7 @@ class TokenLogProbsKernel final : public WithGeneric {
     WantOnGpu(ctx);
     at::Tensor x = ctx.Input(0).contiguous(), tokens = ctx.Input(1).to(at::kLong).contiguous();
     const int dt = DtypeCode(x.scalar_type());
-    if (dt < 0 || z.rows > 0x7fffffffll) {
+    if (dt < 0 || z.rows > 0x0fffffffll) {
       Generic(ctx);
       return;
     }
@@ -215,7 +215,7 @@ class TokenLogProbsGradKernel final : public WithGeneric {
     WantOnGpu(ctx);
     at::Tensor x = ctx.Input(0).contiguous(), tokens = ctx.Input(1).to(at::kLong).contiguous();
     const int dt = DtypeCode(x.scalar_type());
-    if (dt < 0 || z.rows > 0x7fffffffll) {
+    if (dt < 0 || z.rows > 0x0fffffffll) {
       Generic(ctx);
       return;
     }
