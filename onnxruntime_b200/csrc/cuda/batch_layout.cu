@@ -13,7 +13,11 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxRequests = 16384;   // 8 bytes of shared memory each
 
-__device__ __forceinline__ int blocks_of(long long tokens, int s) { return static_cast<int>((tokens + s - 1) / s); }
+// (past and new each fit 31 bits: their sum fits 32)
+__device__ __forceinline__ long long blocks_of(long long tokens, int s) {
+  const unsigned t = static_cast<unsigned>(tokens), q = t / static_cast<unsigned>(s);
+  return static_cast<long long>(q) + (q * static_cast<unsigned>(s) != t);
+}
 
 // exclusive running sums over the block of two values per thread; the totals of all threads in tot_a, tot_b
 __device__ __forceinline__ void scan2(int& a, int& b, int& tot_a, int& tot_b, int (*sm)[2]) {
@@ -51,40 +55,48 @@ __global__ void __launch_bounds__(kThreads) batch_layout_kernel(const ortb200_ba
     totals[0] = totals[1] = 0;
   }
   __syncthreads();
-  const int s = a.block_size;
-  int base_a = 0, base_b = 0, worst = 0;
+  const int s = a.block_size, each = (a.B + kThreads - 1) / kThreads;
+  // a thread's requests follow one another: their sums first, the running sums of the threads, then every request's
+  const int b0 = min(static_cast<int>(threadIdx.x) * each, a.B), b1 = min(b0 + each, a.B);
+  int worst = 0, run_a = 0, run_b = 0;
   unsigned long long sum_a = 0, sum_b = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-    const int b = b0 + threadIdx.x;
-    int n = 0, need = 0;
-    if (b < a.B) {
-      const int past = a.past_seqlens[b];
-      n = a.new_tokens[b];
-      if (past < 0 || n < 0) {
-        worst = 4;
-        n = 0;
-      } else {
-        const int held = blocks_of(past, s), all = blocks_of(static_cast<long long>(past) + n, s);
-        need = all - held;
-        if (need > 0 && all > a.max_blocks && worst < 2) worst = 2;
-        if (n > 0 && held > a.max_blocks && worst < 2) worst = 2;
-      }
+  auto request = [&](int b, int& n, int& need) {
+    const int past = a.past_seqlens[b];
+    n = a.new_tokens[b];
+    need = 0;
+    if (past < 0 || n < 0) {
+      worst = 4;
+      n = 0;
+      return;
     }
+    const long long held = blocks_of(past, s), all = blocks_of(static_cast<long long>(past) + n, s);
+    need = static_cast<int>(all - held);
+    if (n > 0 && all > a.max_blocks && worst < 2) worst = 2;
+  };
+#pragma unroll 4
+  for (int b = b0; b < b1; ++b) {
+    int n, need;
+    request(b, n, need);
     sum_a += n;
     sum_b += need;
-    int ta, tb;
-    scan2(n, need, ta, tb, sm);
-    if (b < a.B) {
-      cum[b] = base_a + n;
-      first[b] = base_b + need;
-    }
-    base_a += ta;
-    base_b += tb;
+  }
+  run_a = static_cast<int>(sum_a);
+  run_b = static_cast<int>(sum_b);
+  int base_a, base_b;
+  scan2(run_a, run_b, base_a, base_b, sm);
+#pragma unroll 4
+  for (int b = b0; b < b1; ++b) {
+    int n, need;
+    request(b, n, need);
+    cum[b] = run_a;
+    first[b] = run_b;
+    run_a += n;
+    run_b += need;
   }
   // 64-bit totals: what overflows 32 bits in the running sums is refused here
-  atomicAdd(&totals[0], sum_a);
-  atomicAdd(&totals[1], sum_b);
-  atomicMax(&refused_sm, worst);
+  if (sum_a) atomicAdd(&totals[0], sum_a);
+  if (sum_b) atomicAdd(&totals[1], sum_b);
+  if (worst) atomicMax(&refused_sm, worst);
   if (threadIdx.x == 0) {
     cum[a.B] = base_a;
     first[a.B] = base_b;
@@ -106,23 +118,71 @@ __global__ void __launch_bounds__(kThreads) batch_layout_kernel(const ortb200_ba
         const int mid = (lo + hi) >> 1;
         if (cum[mid] <= t) lo = mid; else hi = mid;
       }
-      const int past = a.past_seqlens[lo], held = blocks_of(past, s);
+      const int past = a.past_seqlens[lo];
+      const long long held = blocks_of(past, s);
       pos = static_cast<long long>(past) + (t - cum[lo]);
-      const int j = static_cast<int>(pos / s);
+      const unsigned j = static_cast<unsigned>(pos) / static_cast<unsigned>(s), offset = static_cast<unsigned>(pos) - j * static_cast<unsigned>(s);
       // a block that this call hands out is not read from the table, which another CTA may be writing
       const int block = j < held ? a.table_in[static_cast<long long>(lo) * a.max_blocks + j] : a.free_blocks[first[lo] + j - held];
-      slot = static_cast<long long>(block) * s + pos % s;
+      slot = static_cast<long long>(block) * s + offset;
     }
     a.positions[t] = pos;
     a.slot_mapping[t] = slot;
   }
+  // the table: what the requests hold, and the blocks that they are given
+  const int used = refused ? 0 : base_b;
+  if (a.table_out == a.table_in) {
+    for (int i = static_cast<int>(tid); i < used; i += static_cast<int>(stride)) {
+      int lo = 0, hi = a.B;   // the request that block i goes to
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= i) lo = mid; else hi = mid;
+      }
+      a.table_out[static_cast<long long>(lo) * a.max_blocks + blocks_of(a.past_seqlens[lo], s) + i - first[lo]] = a.free_blocks[i];
+    }
+    return;
+  }
   const long long entries = static_cast<long long>(a.B) * a.max_blocks;
+  auto entry = [&](int old, int b, int j) {
+    const int fresh = refused ? 0 : first[b + 1] - first[b];
+    if (fresh == 0) return old;
+    const long long k = j - blocks_of(a.past_seqlens[b], s);
+    return k >= 0 && k < fresh ? a.free_blocks[first[b] + k] : old;
+  };
+  if (((reinterpret_cast<uintptr_t>(a.table_in) | reinterpret_cast<uintptr_t>(a.table_out)) & 15) == 0 && a.max_blocks % 4 == 0) {
+    // rows of whole vectors; four of them on their way per thread
+    const unsigned per_row = static_cast<unsigned>(a.max_blocks) / 4;
+    const long long vectors = entries / 4;
+    const int4* in = reinterpret_cast<const int4*>(a.table_in);
+    int4* out = reinterpret_cast<int4*>(a.table_out);
+    for (long long i = tid; i < vectors; i += 4 * stride) {
+      int4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i + u * stride < vectors) v[u] = __ldcs(in + i + u * stride);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const long long at = i + u * stride;
+        if (at >= vectors) break;
+        const int b = static_cast<int>(at <= 0xffffffffll ? static_cast<unsigned>(at) / per_row : at / per_row), j = 4 * static_cast<int>(at - static_cast<long long>(b) * per_row);
+        const int fresh = refused ? 0 : first[b + 1] - first[b];
+        if (fresh > 0) {
+          const long long k = j - blocks_of(a.past_seqlens[b], s);
+          if (k > -4 && k < fresh) {
+            int* e = reinterpret_cast<int*>(&v[u]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (k + c >= 0 && k + c < fresh) e[c] = a.free_blocks[first[b] + k + c];
+          }
+        }
+        __stcs(out + at, v[u]);
+      }
+    }
+    return;
+  }
   for (long long i = tid; i < entries; i += stride) {
     const int b = static_cast<int>(i / a.max_blocks), j = static_cast<int>(i % a.max_blocks);
-    const int fresh = refused ? 0 : first[b + 1] - first[b];
-    const int held = fresh > 0 ? blocks_of(a.past_seqlens[b], s) : 0;
-    if (j >= held && j < held + fresh) a.table_out[i] = a.free_blocks[first[b] + j - held];
-    else if (a.table_out != a.table_in) a.table_out[i] = a.table_in[i];
+    a.table_out[i] = entry(a.table_in[i], b, j);
   }
 }
 
