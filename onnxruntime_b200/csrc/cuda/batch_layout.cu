@@ -19,47 +19,23 @@ __device__ __forceinline__ long long blocks_of(long long tokens, int s) {
   return static_cast<long long>(q) + (q * static_cast<unsigned>(s) != t);
 }
 
-// exclusive running sums over the block of two values per thread; the totals of all threads in tot_a, tot_b
-__device__ __forceinline__ void scan2(int& a, int& b, int& tot_a, int& tot_b, int (*sm)[2]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int own_a = a, own_b = b;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
-    if (lane >= o) { a += x; b += y; }
-  }
-  __syncthreads();
-  if (lane == 31) { sm[warp][0] = a; sm[warp][1] = b; }
-  __syncthreads();
-  tot_a = tot_b = 0;
-  int before_a = 0, before_b = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w == warp) { before_a = tot_a; before_b = tot_b; }
-    tot_a += sm[w][0];
-    tot_b += sm[w][1];
-  }
-  a += before_a - own_a;
-  b += before_b - own_b;
-}
+// What a warp knows of its requests: tokens, blocks to hand out, the largest refusal code.
+struct Totals {
+  long long tokens, blocks;
+  int worst;
+};
 
 __global__ void __launch_bounds__(kThreads) batch_layout_kernel(const ortb200_batch_layout_args a) {
   extern __shared__ int sums[];
   int* cum = sums;              // [B + 1]
   int* first = sums + a.B + 1;  // [B + 1]
-  __shared__ int sm[kThreads / 32][2];
-  __shared__ int refused_sm;
-  __shared__ unsigned long long totals[2];
-  if (threadIdx.x == 0) {
-    refused_sm = 0;
-    totals[0] = totals[1] = 0;
-  }
-  __syncthreads();
+  __shared__ Totals sm[kThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int s = a.block_size, each = (a.B + kThreads - 1) / kThreads;
   // a thread's requests follow one another: their sums first, the running sums of the threads, then every request's
   const int b0 = min(static_cast<int>(threadIdx.x) * each, a.B), b1 = min(b0 + each, a.B);
-  int worst = 0, run_a = 0, run_b = 0;
-  unsigned long long sum_a = 0, sum_b = 0;
+  int worst = 0;
+  long long sum_a = 0, sum_b = 0;   // 64 bits: what would overflow the 32 of the outputs is refused
   auto request = [&](int b, int& n, int& need) {
     const int past = a.past_seqlens[b];
     n = a.new_tokens[b];
@@ -80,34 +56,49 @@ __global__ void __launch_bounds__(kThreads) batch_layout_kernel(const ortb200_ba
     sum_a += n;
     sum_b += need;
   }
-  run_a = static_cast<int>(sum_a);
-  run_b = static_cast<int>(sum_b);
-  int base_a, base_b;
-  scan2(run_a, run_b, base_a, base_b, sm);
+  long long up_a = sum_a, up_b = sum_b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, up_a, o), y = __shfl_up_sync(0xffffffffu, up_b, o);
+    if (lane >= o) {
+      up_a += x;
+      up_b += y;
+    }
+  }
+  worst = __reduce_max_sync(0xffffffffu, worst);
+  if (lane == 31) sm[warp] = {up_a, up_b, worst};
+  __syncthreads();
+  long long run_a = up_a - sum_a, run_b = up_b - sum_b, all_a = 0, all_b = 0;
+  int refused = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) {
+      run_a += sm[w].tokens;
+      run_b += sm[w].blocks;
+    }
+    all_a += sm[w].tokens;
+    all_b += sm[w].blocks;
+    refused = max(refused, sm[w].worst);
+  }
+  if (refused < 4 && all_a > a.rows) refused = 3;
+  if (refused < 2 && all_b > a.num_free) refused = 1;
 #pragma unroll 4
   for (int b = b0; b < b1; ++b) {
     int n, need;
     request(b, n, need);
-    cum[b] = run_a;
-    first[b] = run_b;
+    cum[b] = static_cast<int>(run_a);
+    first[b] = static_cast<int>(run_b);
     run_a += n;
     run_b += need;
   }
-  // 64-bit totals: what overflows 32 bits in the running sums is refused here
-  if (sum_a) atomicAdd(&totals[0], sum_a);
-  if (sum_b) atomicAdd(&totals[1], sum_b);
-  if (worst) atomicMax(&refused_sm, worst);
   if (threadIdx.x == 0) {
-    cum[a.B] = base_a;
-    first[a.B] = base_b;
+    cum[a.B] = static_cast<int>(all_a);
+    first[a.B] = static_cast<int>(all_b);
   }
   __syncthreads();
-  int refused = refused_sm;
-  if (refused < 4 && totals[0] > static_cast<unsigned long long>(a.rows)) refused = 3;
-  if (refused < 2 && totals[1] > static_cast<unsigned long long>(a.num_free)) refused = 1;
 
   const long long tid = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x, stride = static_cast<long long>(gridDim.x) * kThreads;
-  if (tid == 0) a.blocks_used[0] = refused ? -refused : base_b;
+  if (tid == 0) a.blocks_used[0] = refused ? -refused : static_cast<int>(all_b);
   for (long long b = tid; b <= a.B; b += stride) a.cum[b] = refused ? 0 : cum[b];
   const int end = refused ? 0 : cum[a.B];
   for (long long t = tid; t < a.rows; t += stride) {
@@ -130,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) batch_layout_kernel(const ortb200_ba
     a.slot_mapping[t] = slot;
   }
   // the table: what the requests hold, and the blocks that they are given
-  const int used = refused ? 0 : base_b;
+  const int used = refused ? 0 : static_cast<int>(all_b);
   if (a.table_out == a.table_in) {
     for (int i = static_cast<int>(tid); i < used; i += static_cast<int>(stride)) {
       int lo = 0, hi = a.B;   // the request that block i goes to
