@@ -3,7 +3,7 @@
 //
 // One pass over a row.  A thread keeps a running maximum m, S = sum exp(x - m) and W = sum exp(x - m) (x - m) of the logits it has
 // seen; when the maximum moves from m to m', W becomes (W + S (m - m')) c and S becomes S c with c = exp(m - m').  Joined over
-// the row: log_sum_exp = m + log S and entropy = log S - W / S.  All of it is held in 32 bits.
+// the row: log_sum_exp = m + log S and entropy = log S - W / S.  All of it is held in 32 bits, and to the base 2.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -16,14 +16,15 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256;
-constexpr int kMaxTop = 32;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxTop = 32, kMaxParts = 16;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float exp_fast(float d) {   // relative error 2^-22 + |d| 2^-23: what is far below the maximum weighs little
+__device__ __forceinline__ float exp2_fast(float t) {   // relative error 2^-22
   float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * kLog2e));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
   return e;
 }
+__device__ __forceinline__ float exp_fast(float d) { return exp2_fast(d * kLog2e); }   // and |d| 2^-23: what is far below 1 weighs little
 
 // A row as its first elements up to a 16-byte boundary, whole vectors, and the rest.
 template <typename T>
@@ -45,37 +46,59 @@ __device__ __forceinline__ void unpack(const uint4& v, float* f) {
   for (int i = 0; i < Row<T>::E; ++i) f[i] = to_float<T>(t[i]);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {   // NaN if one of them is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// With t = x log2(e): m the largest t, s = sum 2^(t - m), w = sum 2^(t - m) (t - m).  The exponent is one multiply-add whose only
+// rounding is that of its result, so that the reference m is no source of error; two logits go through one instruction.
 struct Stats {
   float m, s, w;
+  static __device__ __forceinline__ Stats none() { return {-INFINITY, 0.f, 0.f}; }
   __device__ __forceinline__ void raise(float to) {   // to >= m
     if (s != 0.f) {
-      const float d = m - to, c = expf(d);
+      const float d = m - to, c = exp2f(d);
       w = d == 0.f ? w : (w + s * d) * c;
       s *= c;
     }
     m = to;
   }
+  // N logits whose largest is `top` (NaN if one of them is)
   template <int N>
-  __device__ __forceinline__ void add(const float* x) {
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
-    if (top > m) raise(top);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float s0 = 0.f, s1 = 0.f, w0 = 0.f, w1 = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float d0 = x[i] - ref, e0 = exp_fast(d0);
-      s0 += e0;
-      w0 = fmaf(e0, fmaxf(d0, -1e30f), w0);   // an impossible token: 0 times -inf counts as 0
-      if (i + 1 < N) {
-        const float d1 = x[i + 1] - ref, e1 = exp_fast(d1);
-        s1 += e1;
-        w1 = fmaf(e1, fmaxf(d1, -1e30f), w1);
-      }
+  __device__ __forceinline__ void add(const float* x, float top) {
+    if (top * kLog2e > m) raise(top * kLog2e);
+    const float ref = m == -INFINITY ? 0.f : -m;
+    if (N == 1) {
+      const float t = max_nan(fmaf(x[0], kLog2e, ref), -1e30f), e = exp2_fast(t);
+      s += e;
+      w = fmaf(e, t, w);
+      return;
     }
-    s += s0 + s1;
-    w += w0 + w1;
+    const f32x2 scale = pack2(kLog2e, kLog2e), ref2 = pack2(ref, ref), one = pack2(1.f, 1.f);
+    f32x2 s2 = pack2(0.f, 0.f), w2 = s2;
+#pragma unroll
+    for (int i = 0; i + 1 < N; i += 2) {
+      float t0, t1;
+      unpack2(fma2(pack2(x[i], x[i + 1]), scale, ref2), t0, t1);
+      // an impossible token has t = -inf: 0 times that has to count as 0
+      t0 = max_nan(t0, -1e30f);
+      t1 = max_nan(t1, -1e30f);
+      const f32x2 e = pack2(exp2_fast(t0), exp2_fast(t1));
+      s2 = fma2(e, one, s2);
+      w2 = fma2(e, pack2(t0, t1), w2);
+    }
+    float a, b;
+    unpack2(s2, a, b);
+    s += a + b;
+    unpack2(w2, a, b);
+    w += a + b;
   }
   __device__ __forceinline__ void join(Stats b) {
     const float to = fmaxf(m, b.m);
@@ -84,31 +107,35 @@ struct Stats {
     s += b.s;
     w += b.w;
   }
+  __device__ __forceinline__ Stats shuffle_xor(int o) const {
+    Stats r;
+    r.m = __shfl_xor_sync(0xffffffffu, m, o);
+    r.s = __shfl_xor_sync(0xffffffffu, s, o);
+    r.w = __shfl_xor_sync(0xffffffffu, w, o);
+    return r;
+  }
 };
 
-// The 32 best (value, index) pairs a warp has seen, lane i the i-th best.  A key orders by value, then by lower index; zeros of both
-// signs are equal, NaN is the largest.
-__device__ __forceinline__ unsigned long long key_of(float f, int index) {
+// A key orders (value, index) pairs by value, then by lower index; zeros of both signs are equal, NaN is the largest.
+__device__ __forceinline__ unsigned order_of(float f) {
   f += 0.f;
   const unsigned u = __float_as_uint(f);
-  const unsigned order = f != f ? 0xffffffffu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
-  return (static_cast<unsigned long long>(order) << 32) | (0xffffffffu - static_cast<unsigned>(index));
+  return f != f ? 0xffffffffu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float value_of(unsigned long long key) {
-  const unsigned order = static_cast<unsigned>(key >> 32);
-  return __uint_as_float((order & 0x80000000u) ? order & 0x7fffffffu : ~order);
-}
+__device__ __forceinline__ float ordered(unsigned order) { return __uint_as_float((order & 0x80000000u) ? order & 0x7fffffffu : ~order); }
+__device__ __forceinline__ unsigned long long key_of(float f, int index) { return (static_cast<unsigned long long>(order_of(f)) << 32) | (0xffffffffu - static_cast<unsigned>(index)); }
+__device__ __forceinline__ float value_of(unsigned long long key) { return ordered(static_cast<unsigned>(key >> 32)); }
+
+// The 32 best pairs a warp has seen, lane i the i-th best.
 struct Best {
   unsigned long long mine = 0;     // this lane's pair; 0: none
   unsigned long long last = 0;     // the top_k-th: what is not above it is no alternative
-  float limit = -INFINITY;         // its value
   __device__ __forceinline__ void insert(unsigned long long key, int lane, int top_k) {
     const int above = __popc(__ballot_sync(0xffffffffu, mine > key));
     const unsigned long long up = __shfl_up_sync(0xffffffffu, mine, 1);
     if (lane > above) mine = up;
     if (lane == above) mine = key;
     last = __shfl_sync(0xffffffffu, mine, top_k - 1);
-    limit = value_of(last);
   }
   // one pair of every lane (0: none)
   __device__ __forceinline__ void offer(unsigned long long key, int lane, int top_k) {
@@ -117,30 +144,74 @@ struct Best {
       if (k > last) insert(k, lane, top_k);
     }
   }
-  // x[0 .. N) of every lane, of which those below `count` exist, at index, index + 1 ...; all of them come behind what was offered before, so that a
-  // value equal to the limit is no alternative
-  template <int N>
-  __device__ __forceinline__ void offer_all(const float* x, int index, int count, int lane, int top_k) {
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < N; ++i) any |= i < count && !(x[i] <= limit);
-    if (!__any_sync(0xffffffffu, any || (last == 0 && count > 0))) return;
-#pragma unroll
-    for (int i = 0; i < N; ++i) offer(i < count ? key_of(x[i], index + i) : 0, lane, top_k);
-  }
+  __device__ __forceinline__ void offer_one(bool has, float x, int index, int lane, int top_k) { offer(has ? key_of(x, index) : 0, lane, top_k); }
 };
+// The k largest of n different keys (0: none) in shared memory, in order, to out[0 .. k), which holds zeros: a key's place is the
+// number of larger ones.
+__device__ __forceinline__ void select_best(const unsigned long long* keys, int n, unsigned long long* out, int k) {
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const unsigned long long mine = keys[i];
+    if (mine == 0) continue;
+    int larger = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) larger += keys[j] > mine;
+    if (larger < k) out[larger] = mine;
+  }
+}
 
 struct Shared {
   Stats stats[kThreads / 32];
-  unsigned long long best[kThreads / 32][kMaxTop];
-  Stats joined;                        // of the CTA
-  unsigned long long joined_best[kMaxTop];
+  Stats part_stats[kMaxParts];                            // the first CTA's: what the cluster's CTAs found
+  unsigned bound, kth[2];                                 // values (order_of) that top_k of the CTA's reach: of a warp's list, of the threads' largest
+  __align__(16) unsigned tops[kThreads];
+  unsigned long long best[kThreads / 32 * kMaxTop];
+  unsigned long long part_best[kMaxParts * kMaxTop];      // the first CTA's
+  unsigned long long chosen[kMaxTop];
 };
 
+// order_of the top_k-th largest of what the threads hold.  `turn` counts the calls: what the last call found may still be read.
+__device__ __forceinline__ unsigned kth_of_threads(Shared& sm, float top, int turn, int lane, int top_k) {
+  unsigned sorted = order_of(top);
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int o = size / 2; o > 0; o >>= 1) {   // a bitonic sort of the warp's, the largest first
+      const unsigned other = __shfl_xor_sync(0xffffffffu, sorted, o);
+      sorted = ((lane & o) == 0) == ((lane & size) == 0) ? max(sorted, other) : min(sorted, other);
+    }
+  if (lane < top_k) sm.tops[(threadIdx.x >> 5) * top_k + lane] = sorted;
+  if (threadIdx.x == 0) {
+    sm.kth[turn & 1] = 0xffffffffu;
+    if (turn == 0) sm.bound = 0;
+  }
+  __syncthreads();
+  const int n = kThreads / 32 * top_k;
+  if (static_cast<int>(threadIdx.x & ~31u) >= n) {   // (whole warps)
+    __syncthreads();
+    return sm.kth[turn & 1];
+  }
+  const unsigned mine = static_cast<int>(threadIdx.x) < n ? sm.tops[threadIdx.x] : 0;
+  int larger = static_cast<int>(threadIdx.x) < n ? 0 : top_k;
+  for (int i = 0; i < n; i += 4) {   // (8 lists: a multiple of 4)
+    const uint4 t = *reinterpret_cast<const uint4*>(sm.tops + i);
+    larger += (t.x > mine) + (t.y > mine) + (t.z > mine) + (t.w > mine);
+  }
+  const unsigned least = __reduce_min_sync(0xffffffffu, larger < top_k ? mine : 0xffffffffu);
+  if (lane == 0) atomicMin(&sm.kth[turn & 1], least);
+  __syncthreads();
+  return sm.kth[turn & 1];
+}
+
 // A cluster of CTAs per row, each with a share of its vectors; the first CTA puts the shares together over distributed shared memory.
+//
+// Without alternatives the row is one stream: 2000 rows of 50257 fp32 logits take 70 us (402 MB, 61 at the copy rate), 2000 of bf16
+// 50 (201 MB, 31: the exponentials, 16 a clock and SM, take 27 by themselves), 6 rows of 128256 bf16 4.6, which is latency: begin, one
+// round of loads, two barriers of the cluster.  With the best 1 / 5 / 20: 84 / 96 / 136, 70 / 85 / 124 and 7.5 / 9.0 / 16 us.  What costs
+// there is not the insertions alone: bounds from one warp each (110 us for bf16 with one alternative), lists merged one by
+// one (13 us for 6 rows with five) and ranks counted among all 256 threads' values (120) were slower.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, TOP ? 3 : 4) token_log_probs_kernel(const ortb200_token_log_probs_args a) {
-  constexpr int E = Row<T>::E, U = TOP ? 2 : 4;
+__global__ void __launch_bounds__(kThreads, TOP && sizeof(T) == 4 ? 3 : 4) token_log_probs_kernel(const ortb200_token_log_probs_args a) {
+  constexpr int E = Row<T>::E, U = TOP && E == 8 ? 2 : 4;
   __shared__ Shared sm;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
@@ -154,86 +225,124 @@ __global__ void __launch_bounds__(kThreads, TOP ? 3 : 4) token_log_probs_kernel(
     token = a.tokens[row];
     if (token >= 0 && token < a.vocab) chosen = to_float<T>(x.x[token]);
   }
-  Stats st = {-INFINITY, 0.f, 0.f};
+  Stats st = Stats::none();
   Best best;
+  if (parts > 1) cluster.barrier_arrive();   // (waited for before anything goes to another CTA's memory: that one has begun then)
   if (part == 0) {   // the elements in front of the first vector: fewer than a warp
     const bool has = static_cast<int>(threadIdx.x) < x.head;
     const float f = has ? to_float<T>(x.x[threadIdx.x]) : 0.f;
-    if (has) st.add<1>(&f);
-    if (TOP && warp == 0) best.offer_all<1>(&f, threadIdx.x, has ? 1 : 0, lane, top_k);
+    if (has) st.add<1>(&f, f);
+    if (TOP && warp == 0) best.offer_one(has, f, threadIdx.x, lane, top_k);
   }
   const int from = static_cast<int>(static_cast<long long>(x.vectors) * part / parts), to = static_cast<int>(static_cast<long long>(x.vectors) * (part + 1) / parts);
   const uint4* body = x.body();
-  int v = from + threadIdx.x;
-  const int whole = from + (to - from) / (kThreads * U) * (kThreads * U);
-  for (; v < whole; v += kThreads * U) {
-    uint4 raw[U];
+  // U vectors at a time, the next ones on their way; behind the share's end stand impossible tokens that are no alternatives
+  const int rounds = (to - from + kThreads * U - 1) / (kThreads * U);
+  uint4 raw[U];
+  float highest = -INFINITY;
+  unsigned bound = 0;
+  int turn = 0;
+  auto fetch = [&](int v) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = __ldcs(body + v + u * kThreads);
+    for (int u = 0; u < U; ++u)
+      if (v + u * kThreads < to) raw[u] = __ldcs(body + v + u * kThreads);
+  };
+  int v = from + threadIdx.x;
+  fetch(v);
+  for (int i = 0; i < rounds; ++i, v += kThreads * U) {
+    const int count = min(U, (to - v + kThreads - 1) / kThreads);   // vectors of this thread (may be negative: none)
+    float f[U * E];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float f[E];
-      unpack<T>(raw[u], f);
-      st.add<E>(f);
-      if (TOP) best.offer_all<E>(f, x.head + (v + u * kThreads) * E, E, lane, top_k);
+      unpack<T>(raw[u], f + u * E);
+      if (u >= count)
+#pragma unroll
+        for (int j = 0; j < E; ++j) f[u * E + j] = -INFINITY;
     }
-  }
-  for (int v0 = whole; v0 < to; v0 += kThreads) {   // (all threads: alternatives are offered by whole warps)
-    v = v0 + threadIdx.x;
-    float f[E];
-    if (v < to) {
-      unpack<T>(__ldcs(body + v), f);
-      st.add<E>(f);
+    if (i + 1 < rounds) fetch(v + kThreads * U);
+    float top = max_nan(f[0], f[1]);
+#pragma unroll
+    for (int j = 2; j < U * E; j += 2) top = max3(top, f[j], f[j + 1]);
+    st.add<U * E>(f, top);
+    if (TOP) {
+      // what is below the top_k-th of the threads' largest so far is no alternative; it is found anew when the number of rounds
+      // has become fourfold: by then some 3 top_k values have passed the old one
+      highest = max_nan(highest, top);
+      if ((i & (i + 1)) == 0 && ((i + 1) & 0x55555555)) bound = max(bound, kth_of_threads(sm, highest, turn++, lane, top_k));
+      const float limit = ordered(max(bound, *static_cast<volatile unsigned*>(&sm.bound)));
+      if (__any_sync(0xffffffffu, !(top < limit))) {   // (NaN is the largest)
+        unsigned may = 0;
+#pragma unroll
+        for (int j = 0; j < U * E; ++j) may |= j / E < count && !(f[j] < limit) ? 1u << j : 0u;
+        const unsigned any = __reduce_or_sync(0xffffffffu, may);
+        const unsigned long long before = best.last;
+#pragma unroll
+        for (int j = 0; j < U * E; ++j)
+          if (any >> j & 1) best.offer_one(may >> j & 1, f[j], x.head + (v + j / E * kThreads) * E + j % E, lane, top_k);
+        if (best.last != before && lane == 0) atomicMax(&sm.bound, static_cast<unsigned>(best.last >> 32));
+      }
     }
-    if (TOP) best.offer_all<E>(f, x.head + v * E, v < to ? E : 0, lane, top_k);
   }
   if (part == parts - 1) {
     const int i = x.tail() + threadIdx.x;
     const float f = i < x.n ? to_float<T>(x.x[i]) : 0.f;
-    if (i < x.n) st.add<1>(&f);
-    if (TOP && warp == 0) best.offer_all<1>(&f, i, i < x.n ? 1 : 0, lane, top_k);
+    if (i < x.n) st.add<1>(&f, f);
+    if (TOP && warp == 0) best.offer_one(i < x.n, f, i, lane, top_k);
   }
   // the warp's, the CTA's, the cluster's
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) st.join({__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.w, o)});
+  for (int o = 16; o > 0; o >>= 1) st.join(st.shuffle_xor(o));
   if (lane == 0) sm.stats[warp] = st;
-  if (TOP) sm.best[warp][lane] = lane < top_k ? best.mine : 0;
+  if (TOP) {
+    if (lane < top_k) sm.best[warp * top_k + lane] = best.mine;
+    if (warp == 0) sm.chosen[lane] = 0;
+  }
   __syncthreads();
+  if (TOP) {
+    select_best(sm.best, kThreads / 32 * top_k, sm.chosen, top_k);
+    __syncthreads();
+  }
   if (warp == 0) {
-    st = sm.stats[0];
-    for (int i = 1; i < kThreads / 32; ++i) st.join(sm.stats[i]);
-    if (TOP)
-      for (int i = 1; i < kThreads / 32; ++i) best.offer(sm.best[i][lane], lane, top_k);
-    if (parts > 1) {
-      if (lane == 0) sm.joined = st;
-      if (TOP) sm.joined_best[lane] = lane < top_k ? best.mine : 0;
-    }
+    st = lane < kThreads / 32 ? sm.stats[lane] : Stats::none();
+#pragma unroll
+    for (int o = kThreads / 64; o > 0; o >>= 1) st.join(st.shuffle_xor(o));
   }
   if (parts > 1) {
+    cluster.barrier_wait();
+    Shared* to_first = cluster.map_shared_rank(&sm, 0);
+    if (threadIdx.x == 0) to_first->part_stats[part] = st;
+    if (TOP && static_cast<int>(threadIdx.x) < top_k) to_first->part_best[part * top_k + threadIdx.x] = sm.chosen[threadIdx.x];
     cluster.sync();
-    if (part == 0 && warp == 0) {
-      for (int c = 1; c < parts; ++c) {
-        const Shared* other = cluster.map_shared_rank(&sm, c);
-        st.join(other->joined);
-        if (TOP) best.offer(other->joined_best[lane], lane, top_k);
-      }
+    if (part != 0) return;
+    if (TOP) {
+      if (warp == 0) sm.chosen[lane] = 0;
+      __syncthreads();
+      select_best(sm.part_best, parts * top_k, sm.chosen, top_k);
+      __syncthreads();
+    }
+    if (warp == 0) {
+      st = lane < parts ? sm.part_stats[lane] : Stats::none();
+#pragma unroll
+      for (int o = kMaxParts / 2; o > 0; o >>= 1) st.join(st.shuffle_xor(o));
     }
   }
-  if (part == 0 && warp == 0) {
+  if (warp == 0) {   // (lane 0 has the sums of all)
+    st.m = __shfl_sync(0xffffffffu, st.m, 0);
+    st.s = __shfl_sync(0xffffffffu, st.s, 0);
+    st.w = __shfl_sync(0xffffffffu, st.w, 0);
     const bool empty = st.s == 0.f;   // nothing in the row is possible
-    const float log_s = logf(st.s), lse = empty ? -INFINITY : st.m + log_s;
+    const float log_s = log2f(st.s), lse = empty ? -INFINITY : (st.m + log_s) * kLn2;
     if (lane == 0) {
       if (a.log_sum_exp) a.log_sum_exp[row] = lse;
-      if (a.entropy) a.entropy[row] = empty ? 0.f : log_s - st.w / st.s;
+      if (a.entropy) a.entropy[row] = empty ? 0.f : (log_s - st.w / st.s) * kLn2;
       if (a.log_prob) a.log_prob[row] = token < 0 || token >= a.vocab ? 0.f : empty ? -INFINITY : chosen - lse;
     }
     if (TOP && lane < top_k) {
-      const unsigned index = 0xffffffffu - static_cast<unsigned>(best.mine);
-      if (a.top_tokens) a.top_tokens[row * top_k + lane] = index;
-      if (a.top_log_probs) a.top_log_probs[row * top_k + lane] = empty ? -INFINITY : value_of(best.mine) - lse;
+      const unsigned long long key = sm.chosen[lane];
+      if (a.top_tokens) a.top_tokens[row * top_k + lane] = 0xffffffffu - static_cast<unsigned>(key);
+      if (a.top_log_probs) a.top_log_probs[row * top_k + lane] = empty ? -INFINITY : value_of(key) - lse;
     }
   }
-  if (parts > 1) cluster.sync();   // no CTA leaves while its shared memory is read
 }
 
 // One CTA per share of a row.  The token and the alternatives are few: their logits are read before anything is written (the
@@ -315,16 +424,26 @@ __global__ void __launch_bounds__(kThreads, 4) token_log_probs_grad_kernel(const
   if (own) dx[at[threadIdx.x]] = from_float<T>(kept);
 }
 
-// CTAs per row: enough for four on each SM while a share keeps some thousand logits
-int parts_of(int64_t rows, int vocab, int most) {
-  int parts = 1;
-  while (parts < most && rows * parts < 4 * 148 && vocab / (2 * parts) >= 2048) parts *= 2;
-  return parts;
+// CTAs per row, a power of two: the least of waves x (3 us to begin and to join + the share at 16 KB a microsecond), which is what a
+// CTA with its loads in flight reads when four of them share an SM.
+int parts_of(int64_t rows, int64_t row_bytes) {
+  int best = 1;
+  double least = 1e30;
+  for (int parts = 1; parts <= kMaxParts; parts *= 2) {
+    const double waves = static_cast<double>((rows * parts + 4 * 148 - 1) / (4 * 148));
+    const double t = waves * (3.0 + static_cast<double>(row_bytes) / parts / 16384.0);
+    if (t < 0.98 * least) {
+      least = t;
+      best = parts;
+    }
+  }
+  return best;
 }
 
 template <typename T, bool TOP>
 int launch_log_probs(const ortb200_token_log_probs_args* a, cudaStream_t stream) {
-  const int parts = parts_of(a->rows, a->vocab, 8);
+  const int parts = parts_of(a->rows, static_cast<int64_t>(a->vocab) * sizeof(T));
+  if (parts > 8 && cudaFuncSetAttribute(token_log_probs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return -10;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a->rows * parts));
   cfg.blockDim = dim3(kThreads);
@@ -373,7 +492,10 @@ extern "C" int ortb200_token_log_probs_grad(const ortb200_token_log_probs_grad_a
   if (a.rows == 0) return 0;
   if (!a.logits || !a.tokens || !a.log_sum_exp || !a.d_logits || (a.d_entropy && !a.entropy) || (a.d_top_log_probs && !a.top_tokens)) return -1;
   if (!a.d_top_log_probs) a.top_k = 0;
-  const int parts = parts_of(a.rows, a.vocab, 8);
+  // shares of 8 KB at least, until there are eight CTAs for each SM
+  const int64_t row_bytes = static_cast<int64_t>(a.vocab) * (a.dtype == ORTB200_F32 ? 4 : 2);
+  const int64_t most = row_bytes / 8192 < 1 ? 1 : row_bytes / 8192, wanted = (8 * 148 + a.rows - 1) / a.rows;
+  const int parts = static_cast<int>(wanted < most ? wanted : most);
   const dim3 grid(static_cast<unsigned>(a.rows * parts));
   switch (a.dtype) {
     case ORTB200_F16: return launch_kernel(token_log_probs_grad_kernel<__half>, grid, kThreads, 0, stream, a.use_pdl != 0, a, parts);
