@@ -555,14 +555,14 @@ std::vector<Value> InferenceSession::RunImpl(const RunOptions& ro, const std::ve
   // memory pattern of this set of input shapes: traced on its first eager run, planned afterwards
   std::string pattern;
   bool trace_memory = false;
-  if (so_.enable_mem_pattern) {
-    std::ostringstream key;
-    for (size_t i = 0; i < inputs.size(); ++i)
-      if (inputs[i].t.defined()) key << input_names_[i] << inputs[i].t.sizes() << ";";
-    pattern = key.str();
-    trace_memory = memory_plans_.count(pattern) == 0 && memory_plans_.size() < 16;
-  }
   auto run_eager = [&]() {
+    if (so_.enable_mem_pattern) {
+      std::ostringstream key;
+      for (size_t i = 0; i < inputs.size(); ++i)
+        if (inputs[i].t.defined()) key << input_names_[i] << inputs[i].t.sizes() << ";";
+      pattern = key.str();
+      trace_memory = memory_plans_.count(pattern) == 0 && memory_plans_.size() < 16;
+    }
     if (trace_memory) ex->BeginMemoryTrace();
     std::vector<Value> r;
     try {
