@@ -118,7 +118,8 @@ void SharedPrefixPagedAttentionImpl(Ctx& ctx) {
                      "SharedPrefixPagedAttention: lengths of sequence ", b, " do not fit the batch or the block table");
     if (S == 0) continue;
     at::Tensor pos = z.placed ? given_pos.narrow(0, t0, S) : at::arange(S, at::kLong) + pl;
-    if (z.rotary) pos = pos.clamp(0, ctx.Input(9).size(0) - 1);
+    ORTB_ENFORCE_ARG(!z.rotary || (pos.min().item<int64_t>() >= 0 && pos.max().item<int64_t>() < ctx.Input(9).size(0)),
+                     "SharedPrefixPagedAttention: a position of sequence ", b, " lies outside the rotary tables");
     at::Tensor qb = rotate(q.narrow(0, t0, S), pos), kb = rotate(k.narrow(0, t0, S), pos), vb = v.narrow(0, t0, S);
     const int64_t nblk = BlocksOf(L, z.block_size);
     at::Tensor blocks = table[b].narrow(0, 0, nblk);

@@ -60,7 +60,10 @@ __global__ void __launch_bounds__(128) prefix_prep_kernel(const ortb200_prefix_a
   }
   const bool keep = slot >= 0 && slot < static_cast<long long>(a.num_blocks) * a.block_size;
   if (!keep && threadIdx.x == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
-  pos = pos < 0 ? 0 : pos >= a.cos_rows ? a.cos_rows - 1 : pos;   // never past the rotary tables
+  if (a.cos_cache && (pos < 0 || pos >= a.cos_rows)) {   // never past the rotary tables
+    if (threadIdx.x == 0 && a.status) atomicExch(a.status, kStatusBadLength);
+    pos = pos < 0 ? 0 : a.cos_rows - 1;
+  }
   const T* cosr = a.cos_cache ? static_cast<const T*>(a.cos_cache) + pos * half : nullptr;
   const T* sinr = a.cos_cache ? static_cast<const T*>(a.sin_cache) + pos * half : nullptr;
   for (int idx = threadIdx.x; idx < heads * H; idx += blockDim.x) {
@@ -304,7 +307,10 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
   const bool keep = slot >= 0 && slot < static_cast<long long>(a.num_blocks) * a.block_size;
   if (!keep && threadIdx.x == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
   const int half = a.rot_dim / 2;
-  pos = pos < 0 ? 0 : pos >= a.cos_rows ? a.cos_rows - 1 : pos;   // never past the rotary tables
+  if (a.cos_cache && (pos < 0 || pos >= a.cos_rows)) {   // never past the rotary tables
+    if (threadIdx.x == 0 && a.status) atomicExch(a.status, kStatusBadLength);
+    pos = pos < 0 ? 0 : a.cos_rows - 1;
+  }
   const T* cosr = a.cos_cache ? static_cast<const T*>(a.cos_cache) + pos * half : nullptr;
   const T* sinr = a.cos_cache ? static_cast<const T*>(a.sin_cache) + pos * half : nullptr;
   const int per_block = (heads + gridDim.y - 1) / gridDim.y;

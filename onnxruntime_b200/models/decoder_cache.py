@@ -4,12 +4,13 @@ A model declares what it keeps per sequence as a list of ``CacheTensor``: "paged
 live in blocks of ``block_size`` tokens named by a block table; "slot" tensors have a fixed size per sequence (recurrent
 state) and live in one slot.  ``CachePool`` owns the device tensors and hands blocks and slots to sequences; the graph
 updates both in place.  Slots are not cleared between owners: an operator starts from the zero state when a sequence's
-past length is 0.
+past length is 0.  Sequences that begin with the same tokens share the blocks that these fill (``fork``); a block goes back
+to the pool with its last owner.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, Hashable, List, Sequence, Tuple
+from typing import Dict, Hashable, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -45,6 +46,7 @@ class CachePool:
         self.free_blocks = list(range(num_blocks - 1, -1, -1))   # popped from the end: block 0 first, freed blocks first
         self.free_slots = list(range(num_slots - 1, -1, -1))
         self.sequences: Dict[Hashable, SequenceEntry] = {}
+        self.owners: Dict[int, int] = {}                         # blocks of more than one sequence: how many
 
     def open(self, seq: Hashable) -> SequenceEntry:
         if seq in self.sequences:
@@ -54,6 +56,45 @@ class CachePool:
         entry = SequenceEntry(self.free_slots.pop())
         self.sequences[seq] = entry
         return entry
+
+    def fork(self, seq: Hashable, source: Hashable, tokens: Optional[int] = None) -> SequenceEntry:
+        """Opens ``seq`` as a continuation of the first ``tokens`` (default: all) tokens of ``source``.  Blocks that these fill are
+        shared, a block that they fill in part is copied; state in slots is copied, and has no memory of fewer tokens than all."""
+        if seq in self.sequences:
+            raise ValueError(f"sequence {seq!r} is already open")
+        src = self.sequences[source]
+        tokens = src.length if tokens is None else tokens
+        if not 0 <= tokens <= src.length:
+            raise ValueError(f"sequence {source!r} holds {src.length} tokens, not {tokens}")
+        if tokens < src.length and any(c.kind == "slot" for c in self.spec):
+            raise ValueError(f"the state of sequence {source!r} is that of all its {src.length} tokens")
+        whole, rest = divmod(tokens, self.block_size)
+        if rest and not self.free_blocks:
+            raise CacheFull(f"sequence {seq!r} needs a cache block for a copy, none is free")
+        entry = self.open(seq)
+        entry.length = tokens
+        entry.blocks = src.blocks[:whole]
+        for block in entry.blocks:
+            self.owners[block] = self.owners.get(block, 1) + 1
+        if rest:
+            entry.blocks.append(self.free_blocks.pop())
+        for c in self.spec:
+            t = self.tensors[c.input]
+            if c.kind == "slot":
+                t[entry.slot].copy_(t[src.slot])
+            elif rest:
+                t[entry.blocks[-1]].copy_(t[src.blocks[whole]])
+        return entry
+
+    def common_tokens(self, seqs: Sequence[Hashable]) -> int:
+        """How many leading tokens of all ``seqs`` lie in the same blocks."""
+        entries = [self.sequences[s] for s in seqs]
+        blocks = 0
+        for column in zip(*(e.blocks for e in entries)):
+            if any(b != column[0] for b in column):
+                break
+            blocks += 1
+        return min([blocks * self.block_size] + [e.length for e in entries]) if entries else 0
 
     def reserve(self, seq: Hashable, tokens: int) -> bool:
         """Room for ``tokens`` more tokens of ``seq``; True when blocks were added.  All or nothing."""
@@ -70,12 +111,19 @@ class CachePool:
 
     def close(self, seq: Hashable) -> None:
         entry = self.sequences.pop(seq)
-        self.free_blocks.extend(reversed(entry.blocks))
+        for block in reversed(entry.blocks):
+            left = self.owners.pop(block, 1) - 1
+            if left == 0:
+                self.free_blocks.append(block)
+            elif left > 1:
+                self.owners[block] = left
         self.free_slots.append(entry.slot)
 
     def copy_sequence_state(self, sources: Sequence[Hashable], targets: Sequence[Hashable]) -> None:
         """Content of ``targets[i]`` becomes that of ``sources[i]`` (beam search); all open, with equally many blocks."""
         src, dst = [self.sequences[s] for s in sources], [self.sequences[t] for t in targets]
+        if any(b in self.owners for e in dst for b in e.blocks):
+            raise ValueError("blocks that several sequences share are not written")
         src_blocks = [b for e in src for b in e.blocks]
         dst_blocks = [b for e in dst for b in e.blocks]
         if any(len(a.blocks) != len(b.blocks) for a, b in zip(src, dst)):

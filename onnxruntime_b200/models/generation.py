@@ -10,10 +10,12 @@ session captures it on the first step and replays it afterwards.
 """
 from __future__ import annotations
 
+from dataclasses import dataclass, field
 from typing import Dict, Hashable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
+from .. import onnx_lite as ol
 from ..capi import InferenceSession, RunOptions
 from .decoder_cache import CacheFull, CachePool
 from .llama import LlamaConfig, empty_kv_cache
@@ -155,7 +157,11 @@ class PagedDecoderRunner:
     ``step`` runs one batch of any composition - whole prompts, portions of prompts, single tokens - for sequences named
     by the caller and returns the wanted logits; ``release`` gives a sequence's blocks and slot back.  ``prefill`` /
     ``decode_step`` drive a fixed batch of ``batch`` rows on top of the same pool.  A step that brings one token per
-    sequence has fixed shapes and addresses and is captured as one CUDA graph per batch size."""
+    sequence has fixed shapes and addresses and is captured as one CUDA graph per batch size.
+
+    ``fork`` opens a sequence behind the tokens of another one, with the blocks that these fill in common.  A model built with
+    ``shared_prefix`` attends to what all sequences of a batch have in common once for all of them, and extends its block
+    tables on the device."""
 
     def __init__(self, session: InferenceSession, cfg, batch: int, max_len: int, block_size: int = 256,
                  tp_size: int = 1, device: Optional[torch.device] = None, graph_id: int = 1, num_blocks: Optional[int] = None,
@@ -172,6 +178,7 @@ class PagedDecoderRunner:
         self.has_argmax = "next_tokens" in out_info
         self.has_slots = "state_slots" in in_names
         self.has_key_starts = "key_starts" in in_names
+        self.has_layout = "free_blocks" in in_names
         self.logits_dtype = {"tensor(float)": torch.float32, "tensor(float16)": torch.float16,
                              "tensor(bfloat16)": torch.bfloat16}[out_info["logits"].type]
         self._steps: Dict[int, "_DecodeBuffers"] = {}
@@ -211,9 +218,24 @@ class PagedDecoderRunner:
     def _slots(self, seqs) -> torch.Tensor:
         return torch.tensor([self.pool.sequences[s].slot for s in seqs], dtype=torch.int32)
 
-    def _bind(self, binding, ids, cum, past, table, slots, key_starts, rows, logits, nxt) -> None:
+    def _granted(self, seqs, new) -> List[int]:
+        """The blocks that the batch enters with these new tokens, in its order."""
+        got = []
+        for s, n in zip(seqs, new):
+            e = self.pool.sequences[s]
+            got += e.blocks[-(-e.length // self.block_size):-(-(e.length + n) // self.block_size)]
+        return got
+
+    def _bind(self, binding, ids, cum, past, table, slots, key_starts, rows, logits, nxt, free=None, shared=None, used=None) -> None:
         binding.bind_torch_input("input_ids", ids)
-        binding.bind_torch_input("cumulative_sequence_length", cum)
+        if self.has_layout:      # `cum` holds the new tokens of every sequence, the table is extended in place
+            binding.bind_torch_input("new_tokens", cum)
+            binding.bind_torch_input("free_blocks", free)
+            binding.bind_torch_input("shared_prefix", shared)
+            binding.bind_torch_output("block_table_out", table)
+            binding.bind_torch_output("blocks_used", used)
+        else:
+            binding.bind_torch_input("cumulative_sequence_length", cum)
         binding.bind_torch_input("past_seqlens", past)
         binding.bind_torch_input("block_table", table)
         binding.bind_torch_input("logits_indices", rows)
@@ -265,6 +287,10 @@ class PagedDecoderRunner:
         logits, _ = self._run_packed(ids, starts, seqs, rows or [0])
         return logits if rows else logits[:0]
 
+    def fork(self, seq: Hashable, source: Hashable, tokens: Optional[int] = None) -> None:
+        """Opens ``seq`` behind the first ``tokens`` (default: all) tokens that ``source`` holds."""
+        self.pool.fork(seq, source, tokens)
+
     def release(self, seq: Hashable) -> None:
         """The sequence is finished: its blocks and slot go back to the pool."""
         self.pool.close(seq)
@@ -278,8 +304,13 @@ class PagedDecoderRunner:
         logits = torch.empty(len(rows), self.cfg.vocab_size, dtype=self.logits_dtype, device=dev)
         nxt = torch.empty(len(rows), dtype=torch.int64, device=dev)
         binding = self.sess.io_binding()
-        self._bind(binding, ids.to(dev), torch.tensor(starts, dtype=torch.int32).to(dev), past.to(dev), self._table(seqs).to(dev),
-                   self._slots(seqs).to(dev), key_starts, torch.tensor(rows, dtype=torch.int64).to(dev), logits, nxt)
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32).to(dev)  # noqa: E731
+        cum, layout = starts, {}
+        if self.has_layout:
+            cum = [starts[b + 1] - starts[b] for b in range(len(seqs))]
+            layout = dict(free=i32(self._granted(seqs, cum)), shared=i32([self.pool.common_tokens(seqs)]), used=i32([0]))
+        self._bind(binding, ids.to(dev), i32(cum), past.to(dev), self._table(seqs).to(dev),
+                   self._slots(seqs).to(dev), key_starts, torch.tensor(rows, dtype=torch.int64).to(dev), logits, nxt, **layout)
         self.sess.run_with_iobinding(binding, self._ro_prefill)
         for b, s in enumerate(seqs):
             self.pool.advance(s, starts[b + 1] - starts[b])
@@ -291,18 +322,34 @@ class PagedDecoderRunner:
         if rows not in self._steps:
             buf = _DecodeBuffers(rows, self.blocks_per_seq, self.cfg.vocab_size, self.logits_dtype, self.device)
             buf.binding = self.sess.io_binding()
-            self._bind(buf.binding, buf.ids, buf.cum, buf.past, buf.table, buf.slots, buf.key_starts, buf.rows, buf.logits, buf.next)
+            self._bind(buf.binding, buf.ids, buf.new if self.has_layout else buf.cum, buf.past, buf.table, buf.slots, buf.key_starts, buf.rows, buf.logits, buf.next,
+                       buf.free, buf.shared, buf.used)
             buf.options.add_run_config_entry("gpu_graph_id", str(self._graph_id + len(self._steps)))
             self._steps[rows] = buf
         return self._steps[rows]
 
     def _run_decode(self, buf: "_DecodeBuffers", seqs) -> None:
         """One token per sequence, ids already in ``buf.ids``; room has been reserved."""
-        layout = [(s, self.pool.sequences[s].slot, tuple(self.pool.sequences[s].blocks)) for s in seqs]
-        if layout != buf.layout:
-            buf.table.copy_(self._table(seqs))
-            buf.slots.copy_(self._slots(seqs))
-            buf.layout = layout
+        entries = [self.pool.sequences[s] for s in seqs]
+        if self.has_layout:
+            # New blocks reach the table in the step that enters them; another batch, or one that has moved since, has its table
+            # sent.  (A sequence that was closed and opened again has another entry.)
+            granted = self._granted(seqs, [1] * len(seqs))
+            if granted:
+                buf.free[:len(granted)].copy_(torch.tensor(granted, dtype=torch.int32))
+            found = [e.length for e in entries]
+            if buf.layout is None or any(a is not b for a, b in zip(buf.layout, entries)) or buf.tokens != found:
+                buf.table.copy_(self._table(seqs))
+                buf.slots.copy_(self._slots(seqs))
+                buf.shared.fill_(self.pool.common_tokens(seqs))
+                buf.layout = entries
+            buf.tokens = [n + 1 for n in found]
+        else:
+            layout = [(s, e.slot, tuple(e.blocks)) for s, e in zip(seqs, entries)]
+            if layout != buf.layout:
+                buf.table.copy_(self._table(seqs))
+                buf.slots.copy_(self._slots(seqs))
+                buf.layout = layout
         lengths = [self.pool.sequences[s].length for s in seqs]
         if lengths.count(lengths[0]) == len(lengths):
             buf.past.fill_(lengths[0])
@@ -381,7 +428,12 @@ class _DecodeBuffers:
         self.rows = torch.arange(rows, dtype=torch.int64, device=device)
         self.logits = torch.zeros(rows, vocab, dtype=logits_dtype, device=device)
         self.next = torch.zeros(rows, dtype=torch.int64, device=device)
+        self.new = torch.ones(rows, dtype=torch.int32, device=device)
+        self.free = torch.zeros(rows, dtype=torch.int32, device=device)     # a token enters one new block at most
+        self.shared = torch.zeros(1, dtype=torch.int32, device=device)
+        self.used = torch.zeros(1, dtype=torch.int32, device=device)
         self.layout = None
+        self.tokens = None       # lengths that the next step of the same batch finds
         self.binding = None
         self.options = RunOptions()
 
@@ -396,7 +448,8 @@ class GenerationConfig:
                  pad_token_id: int = 0, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
                  repetition_penalty: float = 1.0, no_repeat_ngram_size: int = 0, num_beams: int = 1,
                  length_penalty: float = 1.0, early_stopping: bool = False, num_return_sequences: int = 1,
-                 vocab_mask: Optional[torch.Tensor] = None, seed: Optional[int] = None):
+                 vocab_mask: Optional[torch.Tensor] = None, seed: Optional[int] = None, logprobs: Optional[int] = None):
+        """``logprobs``: report log probabilities, entropies and that many best alternatives (``generate_requests``)."""
         self.__dict__.update(locals())
         del self.__dict__["self"]
 
@@ -478,19 +531,123 @@ def generate(runner: Union[DecoderRunner, PagedDecoderRunner], input_ids: torch.
     return seqs
 
 
-def generate_requests(runner: PagedDecoderRunner, prompts: Sequence[Sequence[int]], cfg: GenerationConfig) -> List[List[int]]:
+class TokenScorer:
+    """Log probabilities of chosen tokens, entropies and the ``top_k`` best alternatives out of logits:
+    ``com.ortb200.TokenLogProbs`` as a session of its own on the provider of the logits' device."""
+
+    def __init__(self, vocab_size: int, top_k: int, dtype: torch.dtype, device: torch.device):
+        T = ol.TensorProto
+        kind = {torch.float32: T.FLOAT, torch.float16: T.FLOAT16, torch.bfloat16: T.BFLOAT16}[dtype]
+        info = ol.make_tensor_value_info
+        outs = [info("log_prob", T.FLOAT, ["rows"]), info("entropy", T.FLOAT, ["rows"]), info("top_log_probs", T.FLOAT, ["rows", top_k]),
+                info("top_tokens", T.INT64, ["rows", top_k])]
+        graph = ol.make_graph([ol.make_node("TokenLogProbs", ["logits", "tokens"], [o.name for o in outs], domain="com.ortb200", top_k=top_k)], "scores",
+                              [info("logits", kind, ["rows", vocab_size]), info("tokens", T.INT64, ["rows"])], outs)
+        gpu = device.type == "cuda"
+        self.sess = InferenceSession(ol.make_model(graph, opset=17, extra_opsets={"com.ortb200": 1}).serialize(),
+                                     providers=[("CUDAExecutionProvider", {"device_id": str(device.index or 0)}) if gpu else "CPUExecutionProvider"])
+        self.top_k, self.device = top_k, device
+
+    def __call__(self, logits: torch.Tensor, tokens: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+        """logits [rows, vocab], tokens [rows] -> log probabilities [rows], entropies [rows], and of the alternatives log
+        probabilities and tokens [rows, top_k], the best first."""
+        rows = logits.shape[0]
+        outs = [torch.empty(s, dtype=d, device=self.device) for s, d in
+                (((rows,), torch.float32), ((rows,), torch.float32), ((rows, self.top_k), torch.float32), ((rows, self.top_k), torch.int64))]
+        binding = self.sess.io_binding()
+        binding.bind_torch_input("logits", logits)
+        binding.bind_torch_input("tokens", tokens.to(self.device))
+        for name, t in zip(("log_prob", "entropy", "top_log_probs", "top_tokens"), outs):
+            binding.bind_torch_output(name, t)
+        self.sess.run_with_iobinding(binding)
+        return tuple(outs)
+
+
+@dataclass
+class Generated:
+    """A request's tokens and, for each, what the model thought of it: its log probability and the entropy of the distribution it
+    comes from (before any logits processor), and the best alternatives."""
+    tokens: List[int] = field(default_factory=list)
+    log_probs: List[float] = field(default_factory=list)
+    entropies: List[float] = field(default_factory=list)
+    top_tokens: List[List[int]] = field(default_factory=list)
+    top_log_probs: List[List[float]] = field(default_factory=list)
+
+
+def score_requests(runner: PagedDecoderRunner, texts: Sequence[Sequence[int]], top_k: int = 0, shared_prompt: Sequence[int] = (),
+                   rows: int = 1024) -> List[Generated]:
+    """Log probabilities that the model gives to every token of ``texts`` but the first (with ``shared_prompt`` in front of all
+    of them: to every token).  A text runs in portions of ``rows`` tokens at most, alone, behind the shared prompt's blocks."""
+    scorer = TokenScorer(runner.cfg.vocab_size, top_k, runner.logits_dtype, runner.device)
+    results = []
+    prompt_logits = None
+    try:
+        if len(shared_prompt):
+            prompt_logits = runner.step([(("shared prompt",), shared_prompt, [len(shared_prompt) - 1])]).clone()
+        for i, text in enumerate(texts):
+            text, seq, got = [int(t) for t in text], ("text", i), Generated()
+            results.append(got)
+            if not text:
+                continue
+
+            def note(logits: torch.Tensor, tokens: List[int]) -> None:
+                lp, h, top_lp, top = (t.tolist() for t in scorer(logits, torch.tensor(tokens, dtype=torch.int64)))
+                got.tokens += tokens
+                got.log_probs += lp
+                got.entropies += h
+                got.top_log_probs += top_lp
+                got.top_tokens += top
+            if prompt_logits is not None:
+                runner.fork(seq, ("shared prompt",))
+                note(prompt_logits, text[:1])
+            try:
+                for start in range(0, len(text) - 1, rows):
+                    portion = text[start:min(start + rows, len(text) - 1)]
+                    note(runner.step([(seq, portion, range(len(portion)))]), text[start + 1:start + 1 + len(portion)])
+            finally:
+                if seq in runner.pool.sequences:
+                    runner.release(seq)
+    finally:
+        if ("shared prompt",) in runner.pool.sequences:
+            runner.release(("shared prompt",))
+    return results
+
+
+def generate_requests(runner: PagedDecoderRunner, prompts: Sequence[Sequence[int]], cfg: GenerationConfig,
+                      shared_prompt: Sequence[int] = ()) -> Union[List[List[int]], List[Generated]]:
     """Greedy or sampled continuations of prompts of any lengths, with the processors and knobs of ``generate``.  At most
     ``runner.batch`` requests run at a time; a finished one frees its blocks and slot, and the next waiting prompt joins
-    the running batch in a step of its own.  Returns the generated tokens of every request (end token included)."""
+    the running batch in a step of its own.  Returns the generated tokens of every request (end token included).
+
+    ``shared_prompt`` stands in front of every prompt: it runs once, the requests share the cache blocks that it fills, and it
+    takes one of the runner's sequences.  With ``cfg.logprobs`` the requests come back as ``Generated``."""
+    if len(shared_prompt):
+        if any(len(p) == 0 for p in prompts):
+            raise ValueError("a request behind a shared prompt has a token of its own at least")
+        if len(shared_prompt) > runner.max_len:
+            raise CacheFull(f"the shared prompt exceeds {runner.max_len} tokens")
+        key = ("shared prompt",)
+        runner.step([(key, shared_prompt, [])])
+        try:
+            return _generate_requests(runner, prompts, cfg, [int(t) for t in shared_prompt], key)
+        finally:
+            runner.release(key)
+    return _generate_requests(runner, prompts, cfg, [], None)
+
+
+def _generate_requests(runner: PagedDecoderRunner, prompts, cfg: GenerationConfig, shared: List[int], key):
     if cfg.num_beams > 1:
         raise ValueError("beam search needs a fixed batch: use generate()")
     sampling = cfg.top_k > 0 or cfg.top_p < 1.0 or cfg.seed is not None
     gen = torch.Generator(device=runner.device)
     if cfg.seed is not None:
         gen.manual_seed(cfg.seed)
-    texts = [[int(t) for t in p] for p in prompts]
+    texts = [shared + [int(t) for t in p] for p in prompts]
     done: List[Optional[List[int]]] = [None] * len(texts)
     new: Dict[int, List[int]] = {}
+    held_by_all = len(shared) // runner.block_size     # blocks that a request does not need for itself
+    scorer = TokenScorer(runner.cfg.vocab_size, cfg.logprobs, runner.logits_dtype, runner.device) if cfg.logprobs is not None else None
+    details = [Generated() for _ in texts]
     waiting, running = list(range(len(texts))), []
 
     def pick(i: int, logits: torch.Tensor) -> None:
@@ -501,23 +658,34 @@ def generate_requests(runner: PagedDecoderRunner, prompts: Sequence[Sequence[int
         else:
             tok = int(scores.argmax(-1))
         new[i].append(tok)
+        if scorer is not None:
+            lp, h, top_lp, top = (t.tolist() for t in scorer(logits.reshape(1, -1), torch.tensor([tok], dtype=torch.int64)))
+            d = details[i]
+            d.tokens.append(tok)
+            d.log_probs += lp
+            d.entropies += h
+            d.top_log_probs += top_lp
+            d.top_tokens += top
         if len(new[i]) >= cfg.max_new_tokens or tok == cfg.eos_token_id:
             done[i] = new.pop(i)
             running.remove(i)
             runner.release(("request", i))
 
     while waiting or running:
-        joining = waiting[:runner.batch - len(running)]
+        joining = waiting[:min(runner.batch - len(running), len(runner.pool.free_slots))]
         while joining:   # prompts that fit into the free blocks together with the tokens they will generate
             room = len(runner.pool.free_blocks)
-            need = [(len(texts[i]) + cfg.max_new_tokens + runner.block_size - 1) // runner.block_size for i in joining]
+            need = [(len(texts[i]) + cfg.max_new_tokens + runner.block_size - 1) // runner.block_size - held_by_all for i in joining]
             held = sum(max(0, (len(texts[i]) + cfg.max_new_tokens + runner.block_size - 1) // runner.block_size
                            - len(runner.pool.sequences[("request", i)].blocks)) for i in running)
             if sum(need) + held <= room:
                 break
             joining.pop()
         if joining:
-            logits = runner.step([(("request", i), texts[i], [len(texts[i]) - 1]) for i in joining])
+            if key is not None:
+                for i in joining:
+                    runner.fork(("request", i), key)
+            logits = runner.step([(("request", i), texts[i][len(shared):], [len(texts[i]) - len(shared) - 1]) for i in joining])
             waiting = waiting[len(joining):]
             running += joining
             for i in joining:
@@ -529,7 +697,7 @@ def generate_requests(runner: PagedDecoderRunner, prompts: Sequence[Sequence[int
             raise CacheFull(f"request {waiting[0]} does not fit into the cache")
         for row, i in enumerate(joining):
             pick(i, logits[row])
-    return done
+    return done if scorer is None else details
 
 
 def _last_logits(runner: DecoderRunner, prefill: bool) -> torch.Tensor:

@@ -368,6 +368,22 @@ def _sce(b, n, dy, needs):
     b.add_grad(n.inputs[0], b.one("SoftmaxCrossEntropyLossGrad", ins, MS, **_copy_attrs(n, ("reduction", "ignore_index"))))
 
 
+@_rule("TokenLogProbs")
+def _token_log_probs(b, n, dy, needs):
+    if not needs[0]:
+        return
+    while len(n.outputs) < 5:                          # the backward half reads the saved sums and what was chosen
+        n.outputs.append("")
+    for i, want in ((1, dy[1:2]), (3, dy[2:3]), (4, ["always"])):
+        if any(want) and not n.outputs[i]:
+            n.outputs[i] = b.name("saved_log_prob")
+    g = [d or "" for d in dy] + [""] * (5 - len(dy))
+    ins = [n.inputs[0], n.inputs[1], n.outputs[4], n.outputs[1] if g[1] else "", g[0], g[1], n.outputs[3] if g[2] else "", g[2], g[4]]
+    while not ins[-1]:
+        ins.pop()
+    b.add_grad(n.inputs[0], b.one("TokenLogProbsGrad", ins, OWN))
+
+
 # ---- fallback: differentiate the node itself -------------------------------------------------------------------
 _NODE_SESSIONS: Dict[bytes, object] = {}
 
@@ -488,7 +504,7 @@ def build_gradient_graph(model: ol.Model, requires_grad: Sequence[str], loss: st
                 raise NotImplementedError(f"no gradient rule for operator '{n.op_type}' (node '{n.name}')")
             _fallback_rule(b, n, dy, needs, model)
             continue
-        if dy[0] is None and n.op_type not in ("Split",):
+        if dy[0] is None and n.op_type not in ("Split", "TokenLogProbs"):
             continue
         rule(b, n, dy, needs)
     known = {v.name: v for v in g.inputs}
