@@ -13,10 +13,24 @@
 // segments of a row.  Which CTA wrote what follows from the same arithmetic: nothing is counted, nothing waited for.
 //
 // Within a CTA (192 threads, two per SM): warp 0 loads tiles by TMA through the block table, warp 1 issues the products
-// (S = Q K^T into tensor memory, O += P V with P in tensor memory over the scores), warps 2 to 5 hold one row per thread.
+// (S = Q K^T into tensor memory, O += P V with P in tensor memory over the scores), warps 2 to 5 hold one row per thread.  Units of
+// up to eight rows, which sequences with single tokens have, leave tensor memory out: those four warps multiply themselves, out of
+// the same tiles (few_rows).
+//
+// What bounds it.  Many rows (24 prompts of up to 150 tokens behind 6000, 28 heads of 128): the tensor pipe, which has half as much
+// again to do as the formula because weights count as two 16-bit values; a tile of 128 rows and 64 keys takes 768 clocks of it and
+// a CTA is done with one in about 2000, two CTAs side by side; 512 clocks of exponentials per tile run beside it.  284 us in all, of
+// which the product kernel has 234 and the join 37.  Single tokens behind a long prefix: segments and their hand-overs; 180 sequences of 16
+// heads of 64 behind 20011 tokens take 114 us, 64 of 64 heads of 128 behind 8192 tokens 64 us, where the bytes need 37 and 23.
+// Slower, each against the form of its time at (180 behind 20011, 64 behind 8192): 128-key tiles with one score buffer 164 and 82 us
+// instead of 149 and 70; eight softmax warps with half a row each 150 and 80; rows held four times with a quarter of the keys to each
+// warp 162 and 78; the next tiles asked into L2 ahead of their loads 198 and 81 instead of 132 and 65; one thread for loads and
+// scores and one for the products with V 147 and 72 instead of 140 and 67; few rows through tensor memory like all others 139 and 68
+// instead of 115 and 64.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <math.h>
+#include <algorithm>
 #include <type_traits>
 #include "attn_internal.h"
 #include "launch_util.cuh"
@@ -137,9 +151,12 @@ __global__ void __launch_bounds__(128) prefix_rows_kernel(const ortb200_prefix_a
 // Weights reach the product with V as the sum of two 16-bit values.  Rounded once they would be off by as much as the rounded
 // queries are, and the result by 1.7 times the rounding of a 32-bit one instead of 1.4; it costs half a product more, 7 % of the
 // time where sequences bring single tokens and 12 % where the tensor pipe is full.
-constexpr bool kSplit = true;
+// The reference maximum of a row is raised only when a tile exceeds it by 2^8 (weights stay below 256), so that O is rescaled a few
+// times per row.
+constexpr float kRaise = 8.f;
 constexpr int kQT = 128;          // query rows of a unit
 constexpr int kKT = 64;           // keys of a tile
+constexpr int kFew = 8;           // units of so few rows go another way through the same tiles
 constexpr int kThreads = 192;
 constexpr int kGrid = 296;        // two CTAs on each of 148 SMs
 constexpr int kTmemCols = 256;    // two score buffers of 64 columns, O in up to 128
@@ -179,13 +196,17 @@ __host__ __device__ inline Work work_of(const ortb200_prefix_attn_args& a) {
 }
 
 // A unit of n tiles takes n + extra(rows) places in the numbering, the tiles behind the others: beginning and ending a segment
-// costs a CTA as much time as some tiles, the more the more rows are written, and a share of many short units has to be worth as
-// much as one of a long unit.
-__device__ __forceinline__ int extra(int rows) { return rows > 32 ? 5 : 2; }
+// costs a CTA as much time as some tiles, and a share of many short units has to be worth as much as one of a long unit.  For 24
+// prompts of up to 150 tokens behind 6000 (28 heads) 1, 2, 3 and 5 places took 303, 257, 234 and 238 us where rows are many; with
+// few rows 0, 1 and 2 make 108, 104 and 112 us (180 single tokens behind 20011), 54, 52 and 52 us (64 behind 8192).
+__device__ __forceinline__ int extra(int rows) { return rows > 32 ? 4 : 1; }
 __device__ __forceinline__ int places(int tiles, int rows) { return tiles > 0 ? tiles + extra(rows) : 0; }
 // The share of CTA i of `total` places starts at share(i); place x belongs to CTA owner(x).
 __device__ __forceinline__ long long share(long long total, int i) { return total * i / kGrid; }
-__device__ __forceinline__ int owner(long long total, long long x) { return static_cast<int>(((x + 1) * kGrid - 1) / total); }
+__device__ __forceinline__ int owner(long long total, long long x) {
+  if (total < 0x7fffffffll / kGrid) return static_cast<int>((static_cast<unsigned>(x + 1) * kGrid - 1) / static_cast<unsigned>(total));   // a 64-bit quotient costs five times as much
+  return static_cast<int>(((x + 1) * kGrid - 1) / total);
+}
 
 // Unit `rt` (rows [128 rt, 128 rt + 128) of the sequence's rows x G) of a sequence: its keys [prefix keys, end) in tiles of 64.
 __device__ __forceinline__ int own_end(const ortb200_prefix_attn_args& a, const Span& s, int rt) {
@@ -376,7 +397,7 @@ struct TcSmem {
   static constexpr int kTotal = kOffFirst + 8 * (kPlanInSmem + 1) + 1024;
 };
 enum { BAR_Q = 0, BAR_Q_FREE = BAR_Q + 2, BAR_K_FULL = BAR_Q_FREE + 2, BAR_K_EMPTY = BAR_K_FULL + 3, BAR_V_FULL = BAR_K_EMPTY + 3, BAR_V_EMPTY = BAR_V_FULL + 3, BAR_S = BAR_V_EMPTY + 3,
-       BAR_P = BAR_S + 2, BAR_O = BAR_P + 2, BAR_END, BAR_O_FREE, BAR_COUNT };
+       BAR_P = BAR_S + 2, BAR_O = BAR_P + 2, BAR_END, BAR_O_FREE, BAR_FEW, BAR_FEW_END = BAR_FEW + 4, BAR_COUNT = BAR_FEW_END + 2 };
 static_assert(BAR_COUNT * 8 + 4 <= 256, "barriers do not fit");
 
 // A CTA's share of one unit.
@@ -389,71 +410,120 @@ struct Segment {
   int table_row;
   long long slot;
 };
+// The segments of a CTA one after the other: its first unit is searched for, the others follow from the one before.
 struct Walk {
   const ortb200_prefix_attn_args& a;
-  const long long* first;
-  Plan plan;
-  int all_rows;
-  long long prefix_total, cur, stop;
-  __device__ Walk(const ortb200_prefix_attn_args& args, const long long* f, const Plan& p, int cta) : a(args), first(f), plan(p) {
+  int prefix_tiles, prefix_row, all_rows;
+  long long left;        // places of the share that are left
+  int seq, rt, kvh, at;  // the unit and the place within it
+  int tiles, before;     // its tiles and the places in front of them
+  Span s;
+  Segment unit;          // what all key heads' segments of the unit have in common
+  __device__ Walk(const ortb200_prefix_attn_args& args, const long long* first, const Plan& p, int cta) : a(args), prefix_tiles(p.prefix_tiles), prefix_row(p.prefix_row) {
     all_rows = last_row(a);
-    prefix_total = prefix_places(a, all_rows, p.prefix_tiles);
-    cur = share(p.total, cta);
-    stop = share(p.total, cta + 1);
+    const long long prefix_total = prefix_places(a, all_rows, prefix_tiles);
+    long long x = share(p.total, cta);
+    left = share(p.total, cta + 1) - x;
+    seq = -1;
+    rt = kvh = at = 0;
+    if (left == 0) return;
+    if (x < prefix_total) {
+      prefix_unit();
+      const int all = tiles + before;
+      const long long u = x / all;
+      at = static_cast<int>(x - u * all);
+      rt = static_cast<int>(u / a.Nk);
+      kvh = static_cast<int>(u - static_cast<long long>(rt) * a.Nk);
+      prefix_unit();
+    } else {
+      x -= prefix_total;
+      int lo = 0, hi = a.B;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= x) lo = mid; else hi = mid;
+      }
+      x -= first[lo];
+      seq = lo;
+      s = span_of(a, seq);
+      own_unit();
+      while (x >= static_cast<long long>(tiles + before) * a.Nk) {
+        x -= static_cast<long long>(tiles + before) * a.Nk;
+        ++rt;
+        own_unit();
+      }
+      kvh = static_cast<int>(x) / (tiles + before);
+      at = static_cast<int>(x) - kvh * (tiles + before);
+    }
+  }
+  __device__ void prefix_unit() {
+    tiles = prefix_tiles;
+    before = extra(unit_rows(a, all_rows, 0));
+    unit.seq = -1;
+    unit.q_row = rt * kQT;
+    unit.rows = unit_rows(a, all_rows, rt);
+    unit.key0 = 0;
+    unit.end = tiles * kKT;
+    unit.past = unit.in_seq = 0;
+    unit.table_row = prefix_row;
+    unit.slot = prefix_slot(a, rt, 0, unit.rows);
+  }
+  __device__ void own_unit() {
+    tiles = own_tiles(a, s, rt, prefix_tiles);
+    unit.rows = unit_rows(a, s.rows, rt);
+    before = tiles > 0 ? extra(unit.rows) : 0;
+    unit.seq = unit.table_row = seq;
+    unit.in_seq = rt * kQT;
+    unit.q_row = s.row0 * (a.N / a.Nk) + unit.in_seq;
+    unit.key0 = prefix_tiles * kKT;
+    unit.end = own_end(a, s, rt);
+    unit.past = s.past;
+    unit.slot = own_slot(a, s.row0, rt, 0, unit.rows);
+  }
+  __device__ void step() {   // to the next unit that has tiles; there is one while places are left
+    at = 0;
+    if (++kvh < a.Nk) return;
+    kvh = 0;
+    ++rt;
+    if (seq < 0) {
+      if (rt < row_tiles(a, all_rows)) {
+        prefix_unit();
+        return;
+      }
+      s.rows = 0;
+    }
+    do {
+      if (rt < row_tiles(a, s.rows) && seq >= 0) {
+        own_unit();
+        if (tiles > 0) return;
+        ++rt;
+      } else {
+        if (++seq >= a.B) {
+          left = 0;
+          return;
+        }
+        s = span_of(a, seq);
+        rt = 0;
+      }
+    } while (true);
   }
   __device__ bool next(Segment& g) {
-    const int G = a.N / a.Nk;
-    while (cur < stop) {
-      int n, at, before;    // the unit's tiles, the place within it, and the places in front of its tiles
-      if (cur < prefix_total) {
-        n = plan.prefix_tiles;
-        before = extra(unit_rows(a, all_rows, 0));
-        const long long u = cur / (n + before);
-        at = static_cast<int>(cur - u * (n + before));
-        const int rt = static_cast<int>(u / a.Nk);
-        g.kvh = static_cast<int>(u % a.Nk);
-        g.seq = -1;
-        g.q_row = rt * kQT;
-        g.rows = unit_rows(a, all_rows, rt);
-        g.key0 = 0;
-        g.end = n * kKT;
-        g.past = g.in_seq = 0;
-        g.table_row = plan.prefix_row;
-        g.slot = prefix_slot(a, rt, g.kvh, g.rows);
-      } else {
-        long long x = cur - prefix_total;
-        int lo = 0, hi = a.B;
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (first[mid] <= x) lo = mid; else hi = mid;
-        }
-        x -= first[lo];
-        const Span s = span_of(a, lo);
-        int rt = 0, all = own_places(a, s, 0, plan.prefix_tiles);
-        while (x >= static_cast<long long>(all) * a.Nk) {
-          x -= static_cast<long long>(all) * a.Nk;
-          all = own_places(a, s, ++rt, plan.prefix_tiles);
-        }
-        g.kvh = static_cast<int>(x) / all;
-        at = static_cast<int>(x) % all;
-        g.seq = lo;
-        g.in_seq = rt * kQT;
-        g.q_row = s.row0 * G + g.in_seq;
-        g.rows = unit_rows(a, s.rows, rt);
-        before = extra(g.rows);
-        n = all - before;
-        g.key0 = plan.prefix_tiles * kKT;
-        g.end = own_end(a, s, rt);
-        g.past = s.past;
-        g.table_row = lo;
-        g.slot = own_slot(a, s.row0, rt, g.kvh, g.rows);
+    while (left > 0) {
+      if (at == tiles + before) {
+        step();
+        if (left == 0) break;
       }
-      const int upto = static_cast<int>(min(static_cast<long long>(n + before), at + (stop - cur)));
-      cur += upto - at;
-      const int t0 = max(at - before, 0);
+      const int upto = static_cast<int>(min(static_cast<long long>(tiles + before), at + left)), t0 = max(at - before, 0);
+      left -= upto - at;
+      at = upto;
       g.tiles = max(upto - before, 0) - t0;
+      if (g.tiles == 0) continue;
+      const int n = g.tiles;
+      g = unit;
+      g.tiles = n;
+      g.kvh = kvh;
       g.key0 += t0 * kKT;
-      if (g.tiles > 0) return true;
+      g.slot += static_cast<long long>(kvh) * g.rows;
+      return true;
     }
     return false;
   }
@@ -533,7 +603,216 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
   return done != 0;
 }
 
+__device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_bar(bar, parity)); }
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <bool BF16>
+__device__ __forceinline__ void mma_warp(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float x, float y) {
+  if (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Two weights as 16-bit values, and what that leaves of them.
+template <bool BF16>
+__device__ __forceinline__ void split2(float p0, float p1, uint32_t& high, uint32_t& rest) {
+  high = pack16<BF16>(p0, p1);
+  if (BF16) {
+    const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&high);
+    rest = pack16<BF16>(p0 - __low2float(h), p1 - __high2float(h));
+  } else {
+    const __half2 h = *reinterpret_cast<const __half2*>(&high);
+    rest = pack16<BF16>(p0 - __low2float(h), p1 - __high2float(h));
+  }
+}
+__device__ __forceinline__ float max_over_keys(float x) {   // lanes that hold the same row
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+__device__ __forceinline__ float sum_over_keys(float x) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// A segment of up to eight rows.  In tensor memory they would fill 8 of 128 lanes, and a tile would still take the whole chain of
+// S, softmax and O with its hand-overs; so each of the four warps multiplies a quarter of a tile's keys itself, keys and dims as
+// the 16 rows of a product and the queries as its 8 columns: S^T = K Q^T, O^T += V^T P^T.  A warp has its own running maximum and
+// sums; they meet once per segment, in the place of the queries.
+template <int HD, bool BF16, bool CAP>
+__device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, const Work& w, const Segment& g, uint8_t* smem, uint64_t* bars, float2 (*part)[kFew],
+                                         const QueryPlace& qp, float scale, int qw, int lane, int& stage, uint32_t& parity, int& few_tiles, int few_segments, bool& ok) {
+  using L = TcSmem<HD>;
+  const int G = a.N / a.Nk, n0 = (lane & 3) * 2;
+  float fs = scale * 1.4426950408889634f;
+  const float cap_scale = CAP ? scale / a.softcap : 0.f;
+  if (CAP) fs = 1.f;
+  const int seen0 = g.seq < 0 ? g.end : min(g.end, g.past + (g.in_seq + n0) / G + 1), seen1 = g.seq < 0 ? g.end : min(g.end, g.past + (g.in_seq + n0 + 1) / G + 1);
+  if (ok && !wait_warp(&bars[BAR_Q + qp.place], qp.fills() & 1)) ok = false;
+  uint32_t q[HD / 16][2];
+  const uint32_t q_row = smem_u32(smem + qp.place * L::kHalf) + (lane & 7) * 128;
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i) {
+    const int chunk = 4 * i + (lane >> 3);
+    ldmatrix4(q_row + (chunk >> 3) * L::kQBox + (((chunk & 7) ^ (lane & 7)) << 4), q[2 * i][0], q[2 * i][1], q[2 * i + 1][0], q[2 * i + 1][1]);
+  }
+  // (the rows of a warp's matrices start at a multiple of eight, so that the swizzle's row is the lane's)
+  const uint32_t kv0 = smem_u32(smem + L::kOffKV), k_row = kv0 + (qw * 16 + (lane & 15)) * 128;
+  const uint32_t v_row = kv0 + L::kBoxes * L::kBox + (qw * 16 + (lane & 7) + ((lane >> 4) << 3)) * 128;
+  float o[HD / 16][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+  for (int d = 0; d < HD / 16; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+  for (int t = 0; t < g.tiles; ++t) {
+    const int first = g.key0 + t * kKT + qw * 16, key = first + (lane >> 2);
+    if (first < g.end) {
+      if (ok && !wait_warp(&bars[BAR_K_FULL + stage], parity)) ok = false;
+      float c[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        const int chunk = 2 * kk + (lane >> 4);
+        uint32_t k[4];
+        ldmatrix4(k_row + stage * L::kStageBytes + (kk / 4) * L::kBox + (((chunk & 7) ^ (lane & 7)) << 4), k[0], k[1], k[2], k[3]);
+        mma_warp<BF16>(kk & 1 ? e : c, k, q[kk][0], q[kk][1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[i] += e[i];
+        if (CAP) c[i] = a.softcap * tanhf(c[i] * cap_scale) * 1.4426950408889634f;
+      }
+      if (key >= seen0) c[0] = -INFINITY;
+      if (key >= seen1) c[1] = -INFINITY;
+      if (key + 8 >= seen0) c[2] = -INFINITY;
+      if (key + 8 >= seen1) c[3] = -INFINITY;
+      float t0 = fmaxf(c[0], c[2]) * fs, t1 = fmaxf(c[1], c[3]) * fs;
+      if (__any_sync(0xffffffffu, t0 > m0 + kRaise || t1 > m1 + kRaise)) {
+        t0 = max_over_keys(t0);
+        t1 = max_over_keys(t1);
+        const bool raise0 = t0 > m0 + kRaise, raise1 = t1 > m1 + kRaise;
+        const float corr0 = raise0 ? (m0 == -INFINITY ? 0.f : ex2_approx(m0 - t0)) : 1.f, corr1 = raise1 ? (m1 == -INFINITY ? 0.f : ex2_approx(m1 - t1)) : 1.f;
+        if (raise0) m0 = t0;
+        if (raise1) m1 = t1;
+        l0 *= corr0;
+        l1 *= corr1;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) {
+          o[d][0] *= corr0;
+          o[d][1] *= corr1;
+          o[d][2] *= corr0;
+          o[d][3] *= corr1;
+        }
+      }
+      const float neg0 = m0 == -INFINITY ? 0.f : -m0, neg1 = m1 == -INFINITY ? 0.f : -m1;
+      const float p00 = ex2_approx(fmaf(c[0], fs, neg0)), p01 = ex2_approx(fmaf(c[1], fs, neg1));
+      const float p80 = ex2_approx(fmaf(c[2], fs, neg0)), p81 = ex2_approx(fmaf(c[3], fs, neg1));
+      l0 += p00 + p80;
+      l1 += p01 + p81;
+      uint32_t h0, h1, r0, r1;
+      split2<BF16>(p00, p01, h0, r0);
+      split2<BF16>(p80, p81, h1, r1);
+      h0 = transpose8(h0);
+      h1 = transpose8(h1);
+      r0 = transpose8(r0);
+      r1 = transpose8(r1);
+      if (ok && !wait_warp(&bars[BAR_V_FULL + stage], parity)) ok = false;
+      const int live = g.end - first;
+      if (live < 16) {   // what lies behind the last key may be anything, and 0 * NaN would reach the product: these rows of V become 0
+        uint8_t* v = smem + L::kOffKV + stage * L::kStageBytes + L::kBoxes * L::kBox + (qw * 16 + live) * 128;
+        for (int i = lane; i < (16 - live) * 8; i += 32)
+#pragma unroll
+          for (int bx = 0; bx < L::kBoxes; ++bx) *reinterpret_cast<uint4*>(v + bx * L::kBox + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+        __syncwarp();
+      }
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) {
+        const int chunk = 2 * d + ((lane >> 3) & 1);
+        uint32_t v[4];
+        ldmatrix4_trans(v_row + stage * L::kStageBytes + (d / 4) * L::kBox + (((chunk & 7) ^ (lane & 7)) << 4), v[0], v[1], v[2], v[3]);
+        mma_warp<BF16>(o[d], v, h0, h1);
+        mma_warp<BF16>(o[d], v, r0, r1);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars[BAR_FEW + (few_tiles & 3)]);
+    ++few_tiles;
+    if (++stage == L::kStages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+  l0 = sum_over_keys(l0);
+  l1 = sum_over_keys(l1);
+  named_barrier(1, 128);   // all have read the queries, and the sums of the segment before
+  if (lane < 4) {
+    part[qw][n0] = make_float2(m0, l0);
+    part[qw][n0 + 1] = make_float2(m1, l1);
+  }
+  // [box of 64 dims][warp][row][dim], the dims in groups of eight exchanged by row so that the stores meet different banks
+  auto sums = [&](int warp, int row, int dim) {
+    return reinterpret_cast<float*>(smem + qp.place * L::kHalf + (dim >> 6) * L::kQBox) + (warp * kFew + row) * 64 + ((dim & 63) ^ ((row >> 1) << 3));
+  };
+#pragma unroll
+  for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *sums(qw, n0 + (i & 1), d * 16 + (lane >> 2) + (i >> 1) * 8) = o[d][i];
+  named_barrier(1, 128);
+  constexpr int E = HD / 16;
+  const int n = (qw * 32 + lane) >> 4, d0 = (lane & 15) * E;
+  if (n < g.rows && ok) {
+    float m = -INFINITY, l = 0.f, v[E];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, part[i][n].x);
+#pragma unroll
+    for (int x = 0; x < E; ++x) v[x] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 ml = part[i][n];
+      const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - m);
+      l += ml.x == -INFINITY ? ml.y : ml.y * f;   // (a sum without a maximum is 0 or NaN)
+      const float* from = sums(i, n, d0);
+#pragma unroll
+      for (int x = 0; x < E; x += 4) {
+        const float4 y = *reinterpret_cast<const float4*>(from + x);
+        v[x] += f * y.x;
+        v[x + 1] += f * y.y;
+        v[x + 2] += f * y.z;
+        v[x + 3] += f * y.w;
+      }
+    }
+    const long long row = g.slot + static_cast<long long>(blockIdx.x) * kQT + n;
+    if ((lane & 15) == 0) w.ml[row] = make_float2(m, l);
+#pragma unroll
+    for (int x = 0; x < E; x += 4) *reinterpret_cast<float4*>(w.o + row * HD + d0 + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+  }
+  fence_proxy_async();   // the next queries arrive where the sums were
+  __syncwarp();
+  if (lane == 0) mbar_arrive(&bars[BAR_FEW_END + (few_segments & 1)]);
+}
 
 template <int HD, bool BF16, bool CAP>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -547,12 +826,13 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BAR_COUNT);
   long long* first_sm = reinterpret_cast<long long*>(smem + L::kOffFirst);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float2 part[4][kFew];
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
-    for (int i = 0; i < BAR_COUNT; ++i) mbar_init(&bars[i], i == BAR_P || i == BAR_P + 1 || i == BAR_O_FREE ? 4 : 1);
+    for (int i = 0; i < BAR_COUNT; ++i) mbar_init(&bars[i], i == BAR_P || i == BAR_P + 1 || i >= BAR_O_FREE ? 4 : 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -669,7 +949,25 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           if (qp.both) umma_commit(&bars[BAR_Q_FREE + 1]);
         }
       };
+      int few_tiles = 0, few_segments = 0;
       while (ok && walk.next(g)) {
+        if (g.rows <= kFew) {   // the other warps do these; what they have read goes back in the order of the tiles
+          qp.take(g.rows);
+          for (int t = 0; t < g.tiles; ++t, ++few_tiles) {
+            if (!wait_bar(&bars[BAR_FEW + (few_tiles & 3)], (few_tiles >> 2) & 1)) { ok = false; break; }
+            mbar_arrive(&bars[BAR_K_EMPTY + s]);
+            mbar_arrive(&bars[BAR_V_EMPTY + s]);
+            if (++s == STAGES) {
+              s = 0;
+              parity ^= 1u;
+            }
+          }
+          if (ok && !wait_bar(&bars[BAR_FEW_END + (few_segments & 1)], (few_segments >> 1) & 1)) ok = false;
+          mbar_arrive(&bars[BAR_Q_FREE + qp.place]);
+          ++few_segments;
+          qp.done();
+          continue;
+        }
         // scores go over the weights of two tiles before; the products that read those are behind the last tile's, which are over
         if (it > 0 && !wait_bar(&bars[BAR_O], (it - 1) & 1)) { ok = false; break; }
         qp.take(g.rows);
@@ -691,9 +989,8 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           const uint32_t low = v_low + s * (L::kStageBytes >> 4), p = tmem_s + (it & 1) * kKT;
 #pragma unroll
           for (int kk = 0; kk < kKT / 16; ++kk) mma_ts(tmem_o, p + kk * 8, low + kk * (2048 >> 4), idesc_o, t > 0 || kk > 0 ? 1u : 0u);
-          if (kSplit)
 #pragma unroll
-            for (int kk = 0; kk < kKT / 16; ++kk) mma_ts(tmem_o, p + kKT / 2 + kk * 8, low + kk * (2048 >> 4), idesc_o, 1u);
+          for (int kk = 0; kk < kKT / 16; ++kk) mma_ts(tmem_o, p + kKT / 2 + kk * 8, low + kk * (2048 >> 4), idesc_o, 1u);
           umma_commit(&bars[BAR_O]);
           umma_commit(&bars[BAR_V_EMPTY + s]);
           if (t == g.tiles - 1) umma_commit(&bars[BAR_END]);
@@ -711,11 +1008,18 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const int qw = warp & 3, r = qw * 32 + lane, G = a.N / a.Nk;
     const uint32_t lane_addr = static_cast<uint32_t>(qw * 32) << 16;
     const float scale_log2 = scale * 1.4426950408889634f;
-    // The reference maximum of a row is raised only when a tile exceeds it by 2^8 (weights stay below 256), so that O in tensor
-    // memory is rescaled a few times per row.
-    constexpr float kRaise = 8.f;
-    int seg = 0, it = 0;
-    while (ok && walk.next(g)) {
+    int seg = 0, it = 0, few_tiles = 0, few_segments = 0, stage = 0;
+    uint32_t parity = 0;
+    QueryPlace qp;
+    while (walk.next(g)) {   // to the end even when a wait gave up: the four warps meet at barriers
+      qp.take(g.rows);
+      if (g.rows <= kFew) {
+        few_rows<HD, BF16, CAP>(a, w, g, smem, bars, part, qp, scale, qw, lane, stage, parity, few_tiles, few_segments, ok);
+        ++few_segments;
+        qp.done();
+        continue;
+      }
+      qp.done();
       const bool idle = qw * 32 >= g.rows;   // a warp without rows keeps the barriers going
       const int pos = g.seq < 0 ? 0x7fffffff : g.past + (g.in_seq + r) / G;
       const int first_pos = g.seq < 0 ? 0x7fffffff : g.past + g.in_seq / G;
@@ -765,42 +1069,45 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             if (raise) m = m_tile;
           }
           const float neg_m = m == -INFINITY ? 0.f : -m;
-          float sum0 = 0.f, sum1 = 0.f;
+          f32x2 sum = pack2(0.f, 0.f);
+          const f32x2 fs2 = pack2(fs, fs), neg2 = pack2(neg_m, neg_m), one = pack2(1.f, 1.f), minus = pack2(-1.f, -1.f);
 #pragma unroll
           for (int c = 0; c < kKT; c += 32) {
             uint32_t packed[16], rest[16];
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
-              const float p0 = ex2_approx(fmaf(sv[c + j], fs, neg_m)), p1 = ex2_approx(fmaf(sv[c + j + 1], fs, neg_m));
-              sum0 += p0;
-              sum1 += p1;
-              if (BF16) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
-                packed[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
-                if (kSplit) {
-                  const __nv_bfloat162 d = __floats2bfloat162_rn(p0 - __low2float(h), p1 - __high2float(h));
-                  rest[j / 2] = *reinterpret_cast<const uint32_t*>(&d);
-                }
+              float p0, p1, h0, h1;
+              unpack2(fma2(pack2(sv[c + j], sv[c + j + 1]), fs2, neg2), p0, p1);
+              const f32x2 p = pack2(ex2_approx(p0), ex2_approx(p1));
+              sum = fma2(p, one, sum);
+              unpack2(p, p0, p1);
+              if (BF16) {   // the upper halves of the two, not rounded, and what is left
+                h0 = __uint_as_float(__float_as_uint(p0) & 0xffff0000u);
+                h1 = __uint_as_float(__float_as_uint(p1) & 0xffff0000u);
+                packed[j / 2] = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
               } else {
                 const __half2 h = __floats2half2_rn(p0, p1);
                 packed[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
-                if (kSplit) {
-                  const __half2 d = __floats2half2_rn(p0 - __low2float(h), p1 - __high2float(h));
-                  rest[j / 2] = *reinterpret_cast<const uint32_t*>(&d);
-                }
+                h0 = __low2float(h);
+                h1 = __high2float(h);
               }
+              float d0, d1;
+              unpack2(fma2(pack2(h0, h1), minus, p), d0, d1);
+              rest[j / 2] = pack16<BF16>(d0, d1);
             }
             tmem_st_x16_u32(s_addr + c / 2, packed);
-            if (kSplit) tmem_st_x16_u32(s_addr + kKT / 2 + c / 2, rest);
+            tmem_st_x16_u32(s_addr + kKT / 2 + c / 2, rest);
           }
+          float sum0, sum1;
+          unpack2(sum, sum0, sum1);
           l += sum0 + sum1;
           tmem_st_wait();
         }
         const int live = g.end - key0;
         if (live < kKT && ok) {
           // what lies behind the last key may be anything, and 0 * NaN would reach the product: these rows of V become 0
-          if (!wait_warp(&bars[BAR_V_FULL + it % STAGES], (it / STAGES) & 1)) ok = false;
-          uint8_t* v = smem + L::kOffKV + it % STAGES * L::kStageBytes + L::kBoxes * L::kBox + live * 128;
+          if (!wait_warp(&bars[BAR_V_FULL + stage], parity)) ok = false;
+          uint8_t* v = smem + L::kOffKV + stage * L::kStageBytes + L::kBoxes * L::kBox + live * 128;
           for (int i = r; i < (kKT - live) * 8; i += 128)
 #pragma unroll
             for (int bx = 0; bx < L::kBoxes; ++bx) *reinterpret_cast<uint4*>(v + bx * L::kBox + i * 16) = make_uint4(0, 0, 0, 0);
@@ -809,6 +1116,10 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[BAR_P + (it & 1)]);
+        if (++stage == STAGES) {
+          stage = 0;
+          parity ^= 1u;
+        }
       }
       if (ok && !wait_warp(&bars[BAR_END], seg & 1)) ok = false;
       tcgen05_fence_after();
@@ -852,93 +1163,159 @@ __device__ __forceinline__ void load_cg(const float* p, float* v) {
     v[0] = x.x; v[1] = x.y;
   }
 }
-// Step 3: one warp per token and query head.
+// Step 3: a warp joins `per` neighbouring rows of a key head (32 at most).  Each lane looks one row's sequence up; where the
+// segments of a unit are is worked out once for all of its rows.
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_attn_args a) {
+__global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_attn_args a, const int per) {
   constexpr int E = HD / 32;
-  const int lane = threadIdx.x & 31;
-  const long long item = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (item >= a.T * a.N) return;
+  const int lane = threadIdx.x & 31, G = a.N / a.Nk, all_rows = last_row(a);
+  const unsigned item = blockIdx.x * 4 + (threadIdx.x >> 5), rows = static_cast<unsigned>(a.T) * G;
+  const int kvh = static_cast<int>(item % a.Nk);
+  const unsigned row0 = item / a.Nk * per;
+  if (row0 >= rows) return;
+  const int count = static_cast<int>(min(rows - row0, static_cast<unsigned>(per)));
   const Work w = work_of(a);
-  const int t = static_cast<int>(item / a.N), head = static_cast<int>(item % a.N), G = a.N / a.Nk, kvh = head / G, all_rows = last_row(a);
-  float o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
   // (step 1 has ended when this step begins: only the segments are waited for)
-  const int4 tok = __ldcg(&w.token[t]);
   const Plan plan = {__ldcg(&w.plan->total), __ldcg(&w.plan->prefix_tiles), 0};
-  const bool live = t < all_rows && t >= tok.y && t < tok.y + tok.z && plan.total > 0;   // lengths that start behind 0 leave rows to nobody
-  // the row's two units, 0 of the prefix and 1 of its own keys: first tile in the numbering, tiles, first slot
-  long long from0 = 0, from1 = 0, slot0 = 0, slot1 = 0;
-  int tiles0 = 0, tiles1 = 0;
-  if (live) {
-    const Span s = {tok.y, tok.z, tok.w};
-    const int pr = t * G + head % G, prt = pr / kQT, orow = (t - s.row0) * G + head % G, ort = orow / kQT;
-    tiles0 = plan.prefix_tiles;
-    const int before0 = extra(unit_rows(a, all_rows, 0));
-    from0 = (static_cast<long long>(prt) * a.Nk + kvh) * (tiles0 + before0) + before0;
-    slot0 = prefix_slot(a, prt, kvh, unit_rows(a, all_rows, prt)) + pr % kQT;
-    long long start = prefix_places(a, all_rows, tiles0) + __ldcg(&w.first[tok.x]);
-    for (int rt = 0; rt < ort; ++rt) start += static_cast<long long>(own_places(a, s, rt, tiles0)) * a.Nk;
-    tiles1 = own_tiles(a, s, ort, tiles0);
-    const int rows1 = unit_rows(a, s.rows, ort);
-    from1 = start + static_cast<long long>(kvh) * places(tiles1, rows1) + extra(rows1);
-    slot1 = own_slot(a, s.row0, ort, kvh, rows1) + orow % kQT;
-  }
+  const int my_t = static_cast<int>((row0 + min(lane, count - 1)) / G);
+  const int4 my_tok = __ldcg(&w.token[my_t]);
+  const bool my_live = my_t < all_rows && my_t >= my_tok.y && my_t < my_tok.y + my_tok.z && plan.total > 0;   // lengths that start behind 0 leave rows to nobody
+  // where the own units of the row's sequence start
+  const long long my_start = my_live ? prefix_places(a, all_rows, plan.prefix_tiles) + __ldcg(&w.first[my_tok.x]) : 0;
+  // the units of a row, 0 of the prefix and 1 of its own keys: first tile in the numbering, tiles, first slot
+  int prt = -1, ort = -1, seq = -1, tiles0 = 0, tiles1 = 0, first0 = 0, first1 = 0, count0 = 0, count1 = 0;
+  long long from0 = 0, from1 = 0, slot0 = 0, slot1 = 0, start = 0;
   // segment k of the row, over both units: CTA first0 + k of the one or first1 + k - count0 of the other
-  const int first0 = tiles0 > 0 ? owner(plan.total, from0) : 0, count0 = tiles0 > 0 ? owner(plan.total, from0 + tiles0 - 1) - first0 + 1 : 0;
-  const int first1 = tiles1 > 0 ? owner(plan.total, from1) : 0, count1 = tiles1 > 0 ? owner(plan.total, from1 + tiles1 - 1) - first1 + 1 : 0;
-  pdl_wait_prior_grids();
-  for (int k0 = 0; k0 < count0 + count1; k0 += 32) {
-    const int k = k0 + lane;
-    const bool own = k >= count0;
+  bool has = false, own = false;
+  long long base = 0;
+  auto segment = [&](int k) {
+    own = k >= count0;
     const int i = own ? first1 + k - count0 : first0 + k;
     const long long from = own ? from1 : from0;
-    const bool has = k < count0 + count1 && max(from, share(plan.total, i)) < min(from + (own ? tiles1 : tiles0), share(plan.total, i + 1));
-    const long long row = (own ? slot1 : slot0) + static_cast<long long>(i) * kQT;
-    const float2 ml = has ? __ldcg(&w.ml[row]) : make_float2(-INFINITY, 0.f);
-    unsigned left = __ballot_sync(0xffffffffu, has);
-    // the segments' values are on their way while the weights are formed
-    constexpr int R = 8;
-    float v[R][E];
-    int at[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      at[r] = left != 0 ? __ffs(left) - 1 : -1;
-      left &= left - 1;
-      const long long rw = __shfl_sync(0xffffffffu, row, max(at[r], 0));
-      if (at[r] >= 0) load_cg<E>(w.o + rw * HD + lane * E, v[r]);
+    has = k < count0 + count1 && max(from, share(plan.total, i)) < min(from + (own ? tiles1 : tiles0), share(plan.total, i + 1));
+    base = (own ? slot1 : slot0) + static_cast<long long>(i) * kQT;
+  };
+  // rows of up to four segments, the usual ones: their places, the same in all lanes
+  constexpr int kShort = 4;
+  int n = 0, places4[kShort] = {0, 0, 0, 0};
+  int t = -1;
+  bool live = false;
+  int4 tok = {0, 0, 0, 0};
+  for (int r = 0; r < count; ++r) {
+    const int pr = static_cast<int>(row0) + r;
+    if (r == 0 || pr == (t + 1) * G) {
+      t = __shfl_sync(0xffffffffu, my_t, r);
+      live = __shfl_sync(0xffffffffu, my_live, r);
+      tok = {__shfl_sync(0xffffffffu, my_tok.x, r), __shfl_sync(0xffffffffu, my_tok.y, r), __shfl_sync(0xffffffffu, my_tok.z, r), __shfl_sync(0xffffffffu, my_tok.w, r)};
     }
-    const float mm = fmaxf(m, warp_max(ml.x));
-    const float keep = m == -INFINITY ? 0.f : exp2f(m - mm), mine = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mm);
-    // a row whose scores are all NaN has no maximum; its sum carries the NaN on
-    l = l * keep + warp_sum(ml.x == -INFINITY ? ml.y : ml.y * mine);
+    const int orow = pr - tok.y * G;
+    if (!live) {
+      count0 = count1 = n = 0;
+      prt = -1;
+    } else if (pr / kQT != prt || tok.x != seq || orow / kQT != ort) {
+      const Span s = {tok.y, tok.z, tok.w};
+      prt = pr / kQT;
+      tiles0 = plan.prefix_tiles;
+      const int before0 = extra(unit_rows(a, all_rows, 0));
+      from0 = (static_cast<long long>(prt) * a.Nk + kvh) * (tiles0 + before0) + before0;
+      slot0 = prefix_slot(a, prt, kvh, unit_rows(a, all_rows, prt));
+      if (tok.x != seq || ort < 0) {
+        seq = tok.x;
+        ort = 0;
+        start = __shfl_sync(0xffffffffu, my_start, r);
+      }
+      for (; ort < orow / kQT; ++ort) start += static_cast<long long>(own_places(a, s, ort, tiles0)) * a.Nk;
+      tiles1 = own_tiles(a, s, ort, tiles0);
+      const int rows1 = unit_rows(a, s.rows, ort);
+      from1 = start + static_cast<long long>(kvh) * places(tiles1, rows1) + extra(rows1);
+      slot1 = own_slot(a, s.row0, ort, kvh, rows1);
+      first0 = tiles0 > 0 ? owner(plan.total, from0) : 0;
+      first1 = tiles1 > 0 ? owner(plan.total, from1) : 0;
+      count0 = tiles0 > 0 ? owner(plan.total, from0 + tiles0 - 1) - first0 + 1 : 0;
+      count1 = tiles1 > 0 ? owner(plan.total, from1 + tiles1 - 1) - first1 + 1 : 0;
+      segment(lane);
+      unsigned left = __ballot_sync(0xffffffffu, has);
+      n = count0 + count1 > 32 ? kShort + 1 : __popc(left);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] *= keep;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const float f = __shfl_sync(0xffffffffu, mine, max(at[r], 0));
-      if (at[r] >= 0)
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += f * v[r][e];
+      for (int i = 0; i < kShort; ++i) {
+        const int from = max(__ffs(left) - 1, 0);
+        places4[i] = static_cast<int>(__shfl_sync(0xffffffffu, base, from)) * 2 + (from >= count0);
+        left &= left - 1;
+      }
     }
-    for (; left != 0; left &= left - 1) {
-      const int j = __ffs(left) - 1;
-      const float f = __shfl_sync(0xffffffffu, mine, j);
-      float x[E];
-      load_cg<E>(w.o + __shfl_sync(0xffffffffu, row, j) * HD + lane * E, x);
+    if (r == 0) pdl_wait_prior_grids();
+    float o[E], m = -INFINITY, l = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] += f * x[e];
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    if (n <= kShort) {
+      float2 ml[kShort];
+      float v[kShort][E];
+#pragma unroll
+      for (int i = 0; i < kShort; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.f);
+        if (i < n) {
+          const unsigned row = (places4[i] >> 1) + static_cast<unsigned>(places4[i] & 1 ? orow : pr) % kQT;
+          ml[i] = __ldcg(&w.ml[row]);
+          load_cg<E>(w.o + static_cast<unsigned long long>(row) * HD + lane * E, v[i]);
+        }
+      }
+      m = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+#pragma unroll
+      for (int i = 0; i < kShort; ++i)
+        if (i < n) {
+          const float f = ml[i].x == -INFINITY ? 0.f : exp2f(ml[i].x - m);
+          l += ml[i].x == -INFINITY ? ml[i].y : ml[i].y * f;   // a row whose scores are all NaN has no maximum; its sum carries the NaN on
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] += f * v[i][e];
+        }
     }
-    m = mm;
+    for (int k0 = 0; n > kShort && k0 < count0 + count1; k0 += 32) {
+      segment(k0 + lane);
+      const long long row = base + (own ? orow : pr) % kQT;
+      const float2 ml = has ? __ldcg(&w.ml[row]) : make_float2(-INFINITY, 0.f);
+      unsigned left = __ballot_sync(0xffffffffu, has);
+      // the segments' values are on their way while the weights are formed
+      constexpr int R = 4;
+      float v[R][E];
+      int at[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        at[r] = left != 0 ? __ffs(left) - 1 : -1;
+        left &= left - 1;
+        const long long rw = __shfl_sync(0xffffffffu, row, max(at[r], 0));
+        if (at[r] >= 0) load_cg<E>(w.o + rw * HD + lane * E, v[r]);
+      }
+      const float mm = fmaxf(m, warp_max(ml.x));
+      const float keep = m == -INFINITY ? 0.f : exp2f(m - mm), mine = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mm);
+      // a row whose scores are all NaN has no maximum; its sum carries the NaN on
+      l = l * keep + warp_sum(ml.x == -INFINITY ? ml.y : ml.y * mine);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] *= keep;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float f = __shfl_sync(0xffffffffu, mine, max(at[r], 0));
+        if (at[r] >= 0)
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] += f * v[r][e];
+      }
+      for (; left != 0; left &= left - 1) {
+        const int j = __ffs(left) - 1;
+        const float f = __shfl_sync(0xffffffffu, mine, j);
+        float x[E];
+        load_cg<E>(w.o + __shfl_sync(0xffffffffu, row, j) * HD + lane * E, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += f * x[e];
+      }
+      m = mm;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* out = static_cast<T*>(a.out) + (static_cast<long long>(t) * a.N + kvh * G + (pr - t * G)) * HD + lane * E;
+    __align__(8) T y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = from_float<T>(o[e] * inv);
+    if (E == 4) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(y);
+    else *reinterpret_cast<uint32_t*>(out) = *reinterpret_cast<const uint32_t*>(y);
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* out = static_cast<T*>(a.out) + item * HD + lane * E;
-  __align__(8) T y[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) y[e] = from_float<T>(o[e] * inv);
-  if (E == 4) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(y);
-  else *reinterpret_cast<uint32_t*>(out) = *reinterpret_cast<const uint32_t*>(y);
 }
 
 template <typename T>
@@ -973,7 +1350,12 @@ int launch_tc(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
   // the two later steps may set up while the step before them ends: they wait for it before they read
   rc = launch_kernel(kern, dim3(kGrid), kThreads, L::kTotal, stream, true, tq, tk, tv, *a, scale);
   if (rc != 0) return rc;
-  return launch_kernel(prefix_join_kernel<T, HD>, dim3(static_cast<unsigned>((a->T * a->N + 3) / 4)), 128, 0, stream, true, *a);
+  // one row per warp until there are rows for 16 warps on each SM, which is what fits at once: warps that come later would look their
+  // segments up when the others have ended (24 prompts of up to 150 tokens: 37 us behind the product kernel instead of 80)
+  const long long fit = 16 * kGrid / 2;
+  const int per = static_cast<int>(std::min<long long>(32, (a->T * a->N + fit - 1) / fit));
+  const long long warps = (rows + per - 1) / per * a->Nk;
+  return launch_kernel(prefix_join_kernel<T, HD>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0, stream, true, *a, per);
 }
 
 template <typename T>
@@ -1004,7 +1386,7 @@ extern "C" int ortb200_prefix_attn(const ortb200_prefix_attn_args* a, ortb200_st
   if ((a->k != nullptr) != (a->v != nullptr) || (a->positions != nullptr) != (a->slot_mapping != nullptr)) return -1;
   if (a->block_size <= 0 || a->max_blocks <= 0 || a->num_blocks <= 0) return -1;
   if (a->cos_cache && (!a->sin_cache || a->cos_rows <= 0 || a->rot_dim <= 0 || a->rot_dim % 2 != 0 || a->rot_dim > a->H)) return -1;
-  if (a->H > kMaxHead || a->T * a->N > 0x7fffffffll) return -2;
+  if (a->H > kMaxHead || a->T * a->N > (a->tensor_cores ? 1ll << 29 : 0x7fffffffll)) return -2;   // (places of segment rows, doubled, pass in 32 bits)
   if (a->workspace_bytes < ortb200_prefix_attn_workspace_bytes(a->T, a->B, a->N, a->Nk, a->H, a->tensor_cores)) return -1;
   if (a->tensor_cores) {
     const bool blocks = a->block_size % kKT == 0 || a->block_size == 8 || a->block_size == 16 || a->block_size == 32;

@@ -293,6 +293,29 @@ def test_prefix_sizes_of_models(dt, N, Nk, H, prefix, held, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N,Nk,H,size", [(8, 2, 64, 16), (8, 2, 128, 64), (4, 4, 128, 8)])
+def test_prefix_units_of_few_and_of_many_rows(dt, N, Nk, H, size):
+    """Sequences of 1 to 40 tokens by turns: units of up to eight rows and of more follow one another on every SM."""
+    new = [(1, 2, 3, 40, 1, 0, 2, 8, 9)[i % 9] for i in range(130)]
+    PrefixCase(dt, N, Nk, H, size, 100, [(29 * i) % 83 for i in range(130)], new, seed=4).run(GPU)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new", [[1], [5, 4]])
+def test_prefix_of_one_key_head_in_hundreds_of_parts(dt, new):
+    PrefixCase(dt, 1, 1, 64, 64, 22000, [5, 70][:len(new)], new, seed=6, stale=0.0).run(GPU)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", [1, 2, 3])
+def test_prefix_scores_far_apart_within_a_tile(kind, rows):
+    """Each quarter of a tile has a maximum of its own, and most weights vanish beside one."""
+    PrefixCase(kind[1], 4, 2, 128, 16, 70, [60, 0, 190], [rows, 1, rows], scale=2.0, seed=rows).run(kind[0])
+
+
+@pytest.mark.gpu
 def test_prefix_captured_graph_follows_the_lengths():
     """One captured step is replayed for other lengths, another shared prefix and other queries."""
     a = PrefixCase(torch.bfloat16, 8, 2, 128, 64, 192, [5, 70, 200], [1, 1, 1], seed=1)
