@@ -649,6 +649,18 @@ __device__ __forceinline__ void split2(float p0, float p1, uint32_t& high, uint3
     rest = pack16<BF16>(p0 - __low2float(h), p1 - __high2float(h));
   }
 }
+// cap tanh(x / cap) with its scores' exponents to the base 2, as c - 2 c / (1 + e^(2 x / cap)): off by some 2^-22 of the cap, which
+// an exponent feels as little as the rounding of a score.  (tanhf, which is exact for small x too: 50 us instead of 20 for 15 single
+// tokens of 16 heads behind 514 tokens.)
+struct Cap {
+  float in, out;
+  __device__ Cap(float scale, float cap) : in(2.f * 1.4426950408889634f * scale / cap), out(cap * 1.4426950408889634f) {}
+  __device__ float operator()(float x) const {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2_approx(x * in)));
+    return fmaf(-2.f * out, r, out);
+  }
+};
 __device__ __forceinline__ float max_over_keys(float x) {   // lanes that hold the same row
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
@@ -670,7 +682,7 @@ __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, cons
   using L = TcSmem<HD>;
   const int G = a.N / a.Nk, n0 = (lane & 3) * 2;
   float fs = scale * 1.4426950408889634f;
-  const float cap_scale = CAP ? scale / a.softcap : 0.f;
+  const Cap cap(scale, a.softcap);
   if (CAP) fs = 1.f;
   const int seen0 = g.seq < 0 ? g.end : min(g.end, g.past + (g.in_seq + n0) / G + 1), seen1 = g.seq < 0 ? g.end : min(g.end, g.past + (g.in_seq + n0 + 1) / G + 1);
   if (ok && !wait_warp(&bars[BAR_Q + qp.place], qp.fills() & 1)) ok = false;
@@ -702,7 +714,7 @@ __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, cons
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         c[i] += e[i];
-        if (CAP) c[i] = a.softcap * tanhf(c[i] * cap_scale) * 1.4426950408889634f;
+        if (CAP) c[i] = cap(c[i]);
       }
       if (key >= seen0) c[0] = -INFINITY;
       if (key >= seen1) c[1] = -INFINITY;
@@ -1037,8 +1049,9 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           float fs = scale_log2;   // scores stay unscaled: the scale is part of the exponent's multiply-add; a cap leaves base-2 exponents
           if (CAP) {
             fs = 1.f;
+            const Cap cap(scale, a.softcap);
 #pragma unroll
-            for (int j = 0; j < kKT; ++j) sv[j] = a.softcap * tanhf(sv[j] * scale / a.softcap) * 1.4426950408889634f;
+            for (int j = 0; j < kKT; ++j) sv[j] = cap(sv[j]);
           }
           if (key0 + kKT > g.end || key0 + kKT - 1 > first_pos) {
             const int hi = min(g.end - key0, pos - key0 + 1);   // keys of this tile that the row sees
@@ -1164,12 +1177,16 @@ __device__ __forceinline__ void load_cg(const float* p, float* v) {
   }
 }
 // Step 3: a warp joins `per` neighbouring rows of a key head (32 at most).  Each lane looks one row's sequence up; where the
-// segments of a unit are is worked out once for all of its rows.
-template <typename T, int HD>
+// segments of a unit are is worked out once for all of its rows.  SPLIT: few rows, whose segments may be hundreds; the four warps of
+// a CTA share one row's.
+template <typename T, int HD, bool SPLIT>
 __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_attn_args a, const int per) {
   constexpr int E = HD / 32;
   const int lane = threadIdx.x & 31, G = a.N / a.Nk, all_rows = last_row(a);
-  const unsigned item = blockIdx.x * 4 + (threadIdx.x >> 5), rows = static_cast<unsigned>(a.T) * G;
+  const int warp = threadIdx.x >> 5;
+  __shared__ float part_o[SPLIT ? 4 : 1][HD];
+  __shared__ float2 part_ml[4];
+  const unsigned item = SPLIT ? blockIdx.x : blockIdx.x * 4 + warp, rows = static_cast<unsigned>(a.T) * G;
   const int kvh = static_cast<int>(item % a.Nk);
   const unsigned row0 = item / a.Nk * per;
   if (row0 >= rows) return;
@@ -1269,44 +1286,61 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
           for (int e = 0; e < E; ++e) o[e] += f * v[i][e];
         }
     }
-    for (int k0 = 0; n > kShort && k0 < count0 + count1; k0 += 32) {
+    for (int k0 = SPLIT ? warp * 32 : 0; n > kShort && k0 < count0 + count1; k0 += SPLIT ? 128 : 32) {
       segment(k0 + lane);
       const long long row = base + (own ? orow : pr) % kQT;
       const float2 ml = has ? __ldcg(&w.ml[row]) : make_float2(-INFINITY, 0.f);
       unsigned left = __ballot_sync(0xffffffffu, has);
-      // the segments' values are on their way while the weights are formed
-      constexpr int R = 4;
-      float v[R][E];
-      int at[R];
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        at[r] = left != 0 ? __ffs(left) - 1 : -1;
-        left &= left - 1;
-        const long long rw = __shfl_sync(0xffffffffu, row, max(at[r], 0));
-        if (at[r] >= 0) load_cg<E>(w.o + rw * HD + lane * E, v[r]);
-      }
       const float mm = fmaxf(m, warp_max(ml.x));
       const float keep = m == -INFINITY ? 0.f : exp2f(m - mm), mine = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mm);
-      // a row whose scores are all NaN has no maximum; its sum carries the NaN on
       l = l * keep + warp_sum(ml.x == -INFINITY ? ml.y : ml.y * mine);
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] *= keep;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const float f = __shfl_sync(0xffffffffu, mine, max(at[r], 0));
-        if (at[r] >= 0)
-#pragma unroll
-          for (int e = 0; e < E; ++e) o[e] += f * v[r][e];
-      }
-      for (; left != 0; left &= left - 1) {
-        const int j = __ffs(left) - 1;
-        const float f = __shfl_sync(0xffffffffu, mine, j);
-        float x[E];
-        load_cg<E>(w.o + __shfl_sync(0xffffffffu, row, j) * HD + lane * E, x);
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += f * x[e];
-      }
       m = mm;
+      while (left != 0) {   // R segments' values on their way at a time
+        constexpr int R = 8;
+        float v[R][E], f[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const bool some = left != 0;
+          const int at = some ? __ffs(left) - 1 : 0;
+          left &= left - 1;
+          const long long from = __shfl_sync(0xffffffffu, row, at);
+          f[i] = __shfl_sync(0xffffffffu, mine, at);
+          if (some) {
+            load_cg<E>(w.o + from * HD + lane * E, v[i]);
+          } else {
+            f[i] = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[i][e] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] += f[i] * v[i][e];
+      }
+    }
+    if (SPLIT) {
+      if (n > kShort) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) part_o[warp][lane * E + e] = o[e];
+        if (lane == 0) part_ml[warp] = make_float2(m, l);
+        __syncthreads();
+        m = fmaxf(fmaxf(part_ml[0].x, part_ml[1].x), fmaxf(part_ml[2].x, part_ml[3].x));
+        l = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 ml = part_ml[i];
+          const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+          l += ml.x == -INFINITY ? ml.y : ml.y * f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] += f * part_o[i][lane * E + e];
+        }
+      }
+      if (warp != 0) return;   // (a CTA has one row)
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T* out = static_cast<T*>(a.out) + (static_cast<long long>(t) * a.N + kvh * G + (pr - t * G)) * HD + lane * E;
@@ -1350,12 +1384,15 @@ int launch_tc(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
   // the two later steps may set up while the step before them ends: they wait for it before they read
   rc = launch_kernel(kern, dim3(kGrid), kThreads, L::kTotal, stream, true, tq, tk, tv, *a, scale);
   if (rc != 0) return rc;
-  // one row per warp until there are rows for 16 warps on each SM, which is what fits at once: warps that come later would look their
-  // segments up when the others have ended (24 prompts of up to 150 tokens: 37 us behind the product kernel instead of 80)
+  // Up to four rows per SM: a CTA each (one token of 32 heads over two key heads behind 18529 tokens: 20 us instead of 74 with one
+  // warp a row).  Then one row per warp until there are rows for 16 warps on each SM, which is what fits at once: warps that come
+  // later would look their segments up when the others have ended (24 prompts of up to 150 tokens: 37 us behind the product kernel
+  // instead of 80).
+  if (a->T * a->N <= 2 * kGrid) return launch_kernel(prefix_join_kernel<T, HD, true>, dim3(static_cast<unsigned>(a->T * a->N)), 128, 0, stream, true, *a, 1);
   const long long fit = 16 * kGrid / 2;
   const int per = static_cast<int>(std::min<long long>(32, (a->T * a->N + fit - 1) / fit));
   const long long warps = (rows + per - 1) / per * a->Nk;
-  return launch_kernel(prefix_join_kernel<T, HD>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0, stream, true, *a, per);
+  return launch_kernel(prefix_join_kernel<T, HD, false>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0, stream, true, *a, per);
 }
 
 template <typename T>

@@ -347,6 +347,10 @@ __global__ void __launch_bounds__(kThreads, TOP && sizeof(T) == 4 ? 3 : 4) token
 
 // One CTA per share of a row.  The token and the alternatives are few: their logits are read before anything is written (the
 // gradient may lie over the logits), and their elements written once more at the end.
+//
+// d x_i = p_i (sum of what does not go to single tokens - d_entropy (log p_i + entropy)) + what goes to token i.  A stream of one read
+// and one write: 4096 rows of 128256 bf16 logits take 354 us (2.1 GB, 321 at the copy rate), 300 of 32000 fp16 10 us, of
+// which beginning and ending are half.  Both kernels together 568 us, 1673 when they went element by element.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) token_log_probs_grad_kernel(const ortb200_token_log_probs_grad_args a, int parts) {
   constexpr int E = Row<T>::E, U = 2;
