@@ -631,6 +631,9 @@ def generate_requests(runner: PagedDecoderRunner, prompts: Sequence[Sequence[int
         try:
             return _generate_requests(runner, prompts, cfg, [int(t) for t in shared_prompt], key)
         finally:
+            for i in range(len(prompts)):   # of a call that was given up
+                if ("request", i) in runner.pool.sequences:
+                    runner.release(("request", i))
             runner.release(key)
     return _generate_requests(runner, prompts, cfg, [], None)
 

@@ -205,6 +205,16 @@ def test_a_shared_prompt_needs_room_and_prompts():
     assert not shared.pool.sequences
 
 
+def test_a_call_that_is_given_up_leaves_nothing_open():
+    """The second request outgrows the longest sequence when it joins; the first is under way."""
+    shared = decoders(CPU, 16, 2, 64)[2]
+    free = len(shared.pool.free_blocks)
+    with pytest.raises(CacheFull):
+        generate_requests(shared, [[3], [4] * 60], GenerationConfig(max_new_tokens=5), shared_prompt=[1] * 20)
+    assert shared.pool.sequences == {} and len(shared.pool.free_blocks) == free and shared.pool.owners == {}
+    assert [len(r) for r in generate_requests(shared, [[3], [4]], GenerationConfig(max_new_tokens=5), shared_prompt=[1] * 20)] == [5, 5]
+
+
 def test_registry_and_tool(tmp_path, capsys):
     from onnxruntime_b200.safetensors_lite import save_file
     from onnxruntime_b200.tools.generate import main
