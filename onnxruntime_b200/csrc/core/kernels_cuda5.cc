@@ -151,7 +151,7 @@ class SharedPrefixPagedAttentionKernel final : public WithGeneric {
       // 16-bit heads of 64 or 128 over blocks that a tile of 64 keys divides, or that divide it
       const bool blocks = z.block_size % 64 == 0 || z.block_size == 8 || z.block_size == 16 || z.block_size == 32;
       const bool aligned = ((reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache)) & 15) == 0;
-      a.tensor_cores = dt != ORTB200_F32 && (z.H == 64 || z.H == 128) && blocks && aligned && z.N / z.Nk <= 128 ? 1 : 0;
+      a.tensor_cores = dt != ORTB200_F32 && (z.H == 64 || z.H == 128) && blocks && aligned && z.N / z.Nk <= 128 && z.T * z.N <= (1 << 29) ? 1 : 0;
       a.use_pdl = Pdl(ctx);
       a.status = ctx.session()->StatusWord().data_ptr<int>();
       const int64_t bytes = ortb200_prefix_attn_workspace_bytes(a.T, a.B, a.N, a.Nk, a.H, a.tensor_cores);

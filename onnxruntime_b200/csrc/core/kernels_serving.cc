@@ -233,7 +233,8 @@ SharedPrefixSizes CheckSharedPrefix(Ctx& ctx) {
   const at::Tensor &q = ctx.RequiredInput(0), &kc = ctx.RequiredInput(3), &vc = ctx.RequiredInput(4);
   ORTB_ENFORCE_ARG(n.attr_i("local_window_size", -1) <= 0, op, ": a window excludes the shared tokens; use PagedAttention");
   ORTB_ENFORCE_ARG(z.N > 0 && z.Nk > 0 && z.N % z.Nk == 0, op, ": num_heads must be a multiple of kv_num_heads");
-  ORTB_ENFORCE_ARG(z.softcap >= 0.f, op, ": softcap must not be negative");
+  ORTB_ENFORCE_ARG(z.softcap >= 0.f && std::isfinite(z.softcap), op, ": softcap must be finite and not negative");
+  ORTB_ENFORCE_ARG(z.scale >= 0.f && std::isfinite(z.scale), op, ": scale must be finite and not negative");
   ORTB_ENFORCE_ARG(q.dim() == 2 && kc.dim() == 4 && vc.sizes() == kc.sizes() && kc.size(2) == z.Nk, op, ": query must be [tokens, width] and the caches [blocks, block size, ",
                    z.Nk, ", head size]");
   ORTB_ENFORCE_ARG(q.is_floating_point() && kc.scalar_type() == q.scalar_type() && vc.scalar_type() == q.scalar_type(), op, ": query and caches must have one floating type");
@@ -258,6 +259,7 @@ SharedPrefixSizes CheckSharedPrefix(Ctx& ctx) {
   z.B = ctx.Input(6).size(0);
   z.max_blocks = ctx.Input(7).size(1);
   ORTB_ENFORCE_ARG(ctx.Input(5).size(0) == z.B + 1 && ctx.Input(7).size(0) == z.B, op, ": lengths and block table disagree about the number of sequences");
+  ORTB_ENFORCE_ARG(z.T == 0 || z.B == 0 || z.max_blocks > 0, op, ": a block table without columns");
   ORTB_ENFORCE_ARG(ctx.Input(8).numel() == 1, op, ": shared_prefix is one number");
   if (z.rotary) {
     const at::Tensor &c = ctx.RequiredInput(9), &s = ctx.RequiredInput(10);

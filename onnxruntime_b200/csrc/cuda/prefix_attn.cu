@@ -649,13 +649,15 @@ __device__ __forceinline__ void split2(float p0, float p1, uint32_t& high, uint3
     rest = pack16<BF16>(p0 - __low2float(h), p1 - __high2float(h));
   }
 }
-// cap tanh(x / cap) with its scores' exponents to the base 2, as c - 2 c / (1 + e^(2 x / cap)): off by some 2^-22 of the cap, which
-// an exponent feels as little as the rounding of a score.  (tanhf, which is exact for small x too: 50 us instead of 20 for 15 single
-// tokens of 16 heads behind 514 tokens.)
+// cap tanh(scale x / cap) as an exponent to the base 2.  CAP 1, caps up to 64: c - 2 c / (1 + e^(2 scale x / cap)), off by some 2^-22 of
+// the cap, so a weight by 2^-15 at most.  CAP 2, larger ones: tanhf, which is as exact where x is small beside the cap (50 us instead of
+// 18.5 for 15 single tokens of 16 heads behind 514 tokens).
+template <int CAP>
 struct Cap {
   float in, out;
-  __device__ Cap(float scale, float cap) : in(2.f * 1.4426950408889634f * scale / cap), out(cap * 1.4426950408889634f) {}
+  __device__ Cap(float scale, float cap) : in(CAP == 2 ? scale / cap : 2.f * 1.4426950408889634f * scale / cap), out(cap * 1.4426950408889634f) {}
   __device__ float operator()(float x) const {
+    if (CAP == 2) return out * tanhf(x * in);
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2_approx(x * in)));
     return fmaf(-2.f * out, r, out);
@@ -676,13 +678,13 @@ __device__ __forceinline__ float sum_over_keys(float x) {
 // S, softmax and O with its hand-overs; so each of the four warps multiplies a quarter of a tile's keys itself, keys and dims as
 // the 16 rows of a product and the queries as its 8 columns: S^T = K Q^T, O^T += V^T P^T.  A warp has its own running maximum and
 // sums; they meet once per segment, in the place of the queries.
-template <int HD, bool BF16, bool CAP>
+template <int HD, bool BF16, int CAP>
 __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, const Work& w, const Segment& g, uint8_t* smem, uint64_t* bars, float2 (*part)[kFew],
                                          const QueryPlace& qp, float scale, int qw, int lane, int& stage, uint32_t& parity, int& few_tiles, int few_segments, bool& ok) {
   using L = TcSmem<HD>;
   const int G = a.N / a.Nk, n0 = (lane & 3) * 2;
   float fs = scale * 1.4426950408889634f;
-  const Cap cap(scale, a.softcap);
+  const Cap<CAP> cap(scale, a.softcap);
   if (CAP) fs = 1.f;
   const int seen0 = g.seq < 0 ? g.end : min(g.end, g.past + (g.in_seq + n0) / G + 1), seen1 = g.seq < 0 ? g.end : min(g.end, g.past + (g.in_seq + n0 + 1) / G + 1);
   if (ok && !wait_warp(&bars[BAR_Q + qp.place], qp.fills() & 1)) ok = false;
@@ -826,7 +828,7 @@ __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, cons
   if (lane == 0) mbar_arrive(&bars[BAR_FEW_END + (few_segments & 1)]);
 }
 
-template <int HD, bool BF16, bool CAP>
+template <int HD, bool BF16, int CAP>
 __global__ void __launch_bounds__(kThreads, 2)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                    const ortb200_prefix_attn_args a, const float scale) {
@@ -1049,7 +1051,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           float fs = scale_log2;   // scores stay unscaled: the scale is part of the exponent's multiply-add; a cap leaves base-2 exponents
           if (CAP) {
             fs = 1.f;
-            const Cap cap(scale, a.softcap);
+            const Cap<CAP> cap(scale, a.softcap);
 #pragma unroll
             for (int j = 0; j < kKT; ++j) sv[j] = cap(sv[j]);
           }
@@ -1372,7 +1374,7 @@ int launch_tc(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
   if (make_tensor_map_4d(&tk, a->k_cache, dt, 2, dims, strides, 64, box) != 0) return -6;
   if (make_tensor_map_4d(&tv, a->v_cache, dt, 2, dims, strides, 64, box) != 0) return -6;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  auto kern = a->softcap > 0.f ? prefix_attn_kernel<HD, kBf16, true> : prefix_attn_kernel<HD, kBf16, false>;
+  auto kern = a->softcap > 64.f ? prefix_attn_kernel<HD, kBf16, 2> : a->softcap > 0.f ? prefix_attn_kernel<HD, kBf16, 1> : prefix_attn_kernel<HD, kBf16, 0>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) != cudaSuccess) return -10;   // per device
   const int heads = a->N + 2 * a->Nk;
   const long long spread = 2 * kGrid / (a->T + 1), most = (heads + 15) / 16;   // few tokens: several CTAs per token, 16 heads at least to each

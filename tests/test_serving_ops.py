@@ -96,6 +96,12 @@ def test_layout_of_many_requests(provider, B):
 
 
 @pytest.mark.parametrize("provider", PROVIDERS)
+def test_layout_of_more_requests_than_one_launch_takes(provider):
+    B = 16400
+    check_layout(provider, [i % 5 for i in range(B)], [(i + 1) % 2 for i in range(B)], torch.arange(3 * B, dtype=torch.int32).reshape(B, 3), list(range(7, 3 * B)), B, 2)
+
+
+@pytest.mark.parametrize("provider", PROVIDERS)
 @pytest.mark.parametrize("past,new,free,rows,code", [
     ([4, 9], [1, 4], 1, 5, -1),                 # two blocks wanted, one free
     ([4, 29], [1, 4], 9, 5, -2),                # the second request outgrows its eight blocks of four
@@ -309,6 +315,13 @@ def test_prefix_of_one_key_head_in_hundreds_of_parts(dt, new):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("cap", [0.5, 30.0, 64.0, 65.0, 1e6])
+def test_prefix_caps(kind, cap):
+    """Caps below the scores, near them, and so large that they change nothing."""
+    PrefixCase(kind[1], 4, 1, 64, 16, 70, [60, 0, 190], [3, 1, 1], spread=2.0, cap=cap, seed=2).run(kind[0])
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("rows", [1, 2, 3])
 def test_prefix_scores_far_apart_within_a_tile(kind, rows):
     """Each quarter of a tile has a maximum of its own, and most weights vanish beside one."""
@@ -369,6 +382,10 @@ def test_prefix_argument_checks(provider):
     broken(lambda c: setattr(c, "pos", c.pos[:0]))
     broken(lambda c: setattr(c, "qkv", c.qkv[:, :-1]))
     broken(lambda c: setattr(c, "cap", -1.0))
+    broken(lambda c: setattr(c, "cap", math.inf))
+    broken(lambda c: setattr(c, "scale", -0.5))
+    broken(lambda c: setattr(c, "scale", math.nan))
+    broken(lambda c: setattr(c, "table", c.table[:, :0]))
     broken(lambda c: setattr(c, "caches", [c.caches[0], c.caches[1][:-1]]))
 
 
