@@ -3,6 +3,11 @@
 //
 // Two running sums over the requests (tokens, blocks to hand out) decide everything; every CTA forms them for itself in shared
 // memory, so that one launch does it all and no CTA waits for another.
+//
+// What bounds it: the launch where requests are few (24 requests 3.5 us on the device, 160 with 27000 rows 4.1), the table where
+// it is large: 1000 requests of 4096 blocks, 33 MB there and back, take 10.3 us, 5.1 at the copy rate.  Slower per call: one 64-bit
+// atomic in shared memory per request for the totals (14 and 27 us instead of 9 and 13), and an entry of the table per thread
+// instead of four times 16 bytes (45).
 #include <cuda_runtime.h>
 #include "launch_util.cuh"
 #include "serving_ops.h"
