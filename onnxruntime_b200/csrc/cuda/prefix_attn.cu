@@ -160,7 +160,7 @@ constexpr int kFew = 8;           // units of so few rows go another way through
 constexpr int kThreads = 192;
 constexpr int kGrid = 296;        // two CTAs on each of 148 SMs
 constexpr int kTmemCols = 256;    // two score buffers of 64 columns, O in up to 128
-constexpr int kPlanInSmem = 1024; // sequences whose running sums a CTA keeps in shared memory
+constexpr int kPlanInSmem = 768;  // row tiles whose running sums a CTA keeps in shared memory
 
 // What follows from the lengths.
 struct Plan {
@@ -171,20 +171,27 @@ struct Plan {
 
 struct Work {            // the workspace's parts
   Plan* plan;
-  long long* first;      // [B + 1]: where the own units of each sequence start, behind the prefix's
+  long long* first;      // [row tiles of all sequences + 1]: where the own units of each start, behind the prefix's
+  int* tile0;            // [B + 1]: which of those row tiles are a sequence's
   int4* token;           // [T]: the token's sequence, that sequence's first row, rows and past
   uint16_t* q;           // [Nk, T G, H]
   float2* ml;            // per row of a segment: m (in units of log 2) and l
   float* o;              // per row of a segment: H values
 };
 __host__ __device__ inline long long up256(long long n) { return (n + 255) / 256 * 256; }
+// row tiles of all sequences, at most
+__host__ __device__ inline long long most_row_tiles(long long T, int B, int N, int Nk) { return T * (N / Nk) / kQT + B; }
+__host__ __device__ inline long long plan_bytes(long long T, int B, int N, int Nk) {
+  return up256(sizeof(Plan) + 8 * (most_row_tiles(T, B, N, Nk) + 1) + 4ll * (B + 1));
+}
 __host__ __device__ inline long long segment_rows(long long T, int N) { return 2 * T * N + static_cast<long long>(kGrid) * kQT; }
 __host__ __device__ inline Work work_of(const ortb200_prefix_attn_args& a) {
   char* p = static_cast<char*>(a.workspace);
   Work w;
   w.plan = reinterpret_cast<Plan*>(p);
   w.first = reinterpret_cast<long long*>(p + sizeof(Plan));
-  p += up256(sizeof(Plan) + 8ll * (a.B + 1));
+  w.tile0 = reinterpret_cast<int*>(w.first + most_row_tiles(a.T, a.B, a.N, a.Nk) + 1);
+  p += plan_bytes(a.T, a.B, a.N, a.Nk);
   w.token = reinterpret_cast<int4*>(p);
   p += up256(a.T * 16);
   w.q = reinterpret_cast<uint16_t*>(p);
@@ -209,44 +216,57 @@ __device__ __forceinline__ int owner(long long total, long long x) {
 }
 
 // Unit `rt` (rows [128 rt, 128 rt + 128) of the sequence's rows x G) of a sequence: its keys [prefix keys, end) in tiles of 64.
-__device__ __forceinline__ int own_end(const ortb200_prefix_attn_args& a, const Span& s, int rt) {
-  const int G = a.N / a.Nk, last = min(rt * kQT + kQT, s.rows * G) - 1;
+__device__ __forceinline__ int own_end(const ortb200_prefix_attn_args& a, int G, const Span& s, int rt) {
+  const int last = min(rt * kQT + kQT, s.rows * G) - 1;
   return static_cast<int>(min(static_cast<long long>(s.past) + last / G + 1, static_cast<long long>(a.max_blocks) * a.block_size));
 }
-__device__ __forceinline__ int own_tiles(const ortb200_prefix_attn_args& a, const Span& s, int rt, int prefix_tiles) {
-  return max((own_end(a, s, rt) + kKT - 1) / kKT - prefix_tiles, 0);
+__device__ __forceinline__ int own_tiles(const ortb200_prefix_attn_args& a, int G, const Span& s, int rt, int prefix_tiles) {
+  return max((own_end(a, G, s, rt) + kKT - 1) / kKT - prefix_tiles, 0);
 }
-__device__ __forceinline__ int row_tiles(const ortb200_prefix_attn_args& a, int rows) { return (rows * (a.N / a.Nk) + kQT - 1) / kQT; }
-__device__ __forceinline__ int unit_rows(const ortb200_prefix_attn_args& a, int rows, int rt) { return min(kQT, rows * (a.N / a.Nk) - rt * kQT); }
-__device__ __forceinline__ int own_places(const ortb200_prefix_attn_args& a, const Span& s, int rt, int prefix_tiles) {
-  return places(own_tiles(a, s, rt, prefix_tiles), unit_rows(a, s.rows, rt));
+__device__ __forceinline__ int row_tiles(int G, int rows) { return (rows * G + kQT - 1) / kQT; }
+__device__ __forceinline__ int unit_rows(int G, int rows, int rt) { return min(kQT, rows * G - rt * kQT); }
+__device__ __forceinline__ int own_places(const ortb200_prefix_attn_args& a, int G, const Span& s, int rt, int prefix_tiles) {
+  return places(own_tiles(a, G, s, rt, prefix_tiles), unit_rows(G, s.rows, rt));
 }
 // all units of the prefix are numbered like the first
-__device__ __forceinline__ long long prefix_places(const ortb200_prefix_attn_args& a, int all_rows, int prefix_tiles) {
-  return static_cast<long long>(row_tiles(a, all_rows)) * a.Nk * places(prefix_tiles, unit_rows(a, all_rows, 0));
+__device__ __forceinline__ long long prefix_places(const ortb200_prefix_attn_args& a, int G, int all_rows, int prefix_tiles) {
+  return static_cast<long long>(row_tiles(G, all_rows)) * a.Nk * places(prefix_tiles, unit_rows(G, all_rows, 0));
 }
 // first row that the segments of a unit may use, before 128 rows per CTA number: units follow one another without a gap
 __device__ __forceinline__ long long prefix_slot(const ortb200_prefix_attn_args& a, int rt, int kvh, int rows) {
   return static_cast<long long>(rt) * kQT * a.Nk + static_cast<long long>(kvh) * rows;
 }
-__device__ __forceinline__ long long own_slot(const ortb200_prefix_attn_args& a, int row0, int rt, int kvh, int rows) {
-  return a.T * a.N + static_cast<long long>(a.Nk) * (static_cast<long long>(row0) * (a.N / a.Nk) + static_cast<long long>(rt) * kQT) + static_cast<long long>(kvh) * rows;
+__device__ __forceinline__ long long own_slot(const ortb200_prefix_attn_args& a, int G, int row0, int rt, int kvh, int rows) {
+  return a.T * a.N + static_cast<long long>(a.Nk) * (static_cast<long long>(row0) * G + static_cast<long long>(rt) * kQT) + static_cast<long long>(kvh) * rows;
 }
 
-// All THREADS of a CTA: how many tokens all sequences share, and where the own units of each sequence start (`first`, written
-// for all to read after the next barrier).
+// the last of n ascending places that is not behind x
+template <typename I>
+__device__ __forceinline__ int sequence_with(const I* places, int n, I x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (places[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+// All THREADS of a CTA: how many tokens all sequences share, and where the own units of each row tile start (`first` and `tile0`,
+// written for all to read after the next barrier).
 template <int THREADS>
-__device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, long long* first, int* status) {
+__device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, long long* first, int* tile0, int* status) {
   __shared__ int least_sm[THREADS / 32], row_sm[THREADS / 32];
   __shared__ long long sum_sm[THREADS / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int least = 0x7fffffff, row = 0x7fffffff;
+  __shared__ int tiles_sm[THREADS / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.N / a.Nk;
+  int least = 0x7fffffff, row = 0x7fffffff, several = 0;
   const int promised = *a.shared_prefix, all_rows = last_row(a);
   for (int b = threadIdx.x; b < a.B; b += THREADS) {
     const Span s = span_of(a, b);
+    if (status && (a.cu_seqlens[b] < 0 || a.cu_seqlens[b + 1] < a.cu_seqlens[b] || a.cu_seqlens[b + 1] > a.T)) atomicExch(status, kStatusBadLength);
     if (s.rows == 0) continue;
     least = min(least, s.past);
     row = min(row, b);
+    several |= s.rows * G > kQT;
     if (status && (a.past_seqlens[b] != s.past || s.past + static_cast<long long>(s.rows) > static_cast<long long>(a.max_blocks) * a.block_size))
       atomicExch(status, kStatusBadLength);
   }
@@ -256,7 +276,7 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
     least_sm[warp] = least;
     row_sm[warp] = row;
   }
-  __syncthreads();
+  several = __syncthreads_or(several);
 #pragma unroll
   for (int i = 0; i < THREADS / 32; ++i) {
     least = min(least, least_sm[i]);
@@ -265,22 +285,15 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
   Plan p;
   p.prefix_tiles = least == 0x7fffffff ? 0 : max(min(promised, least), 0) / kKT;
   p.prefix_row = row == 0x7fffffff ? 0 : row;
-  long long base = 0;
-  for (int b0 = 0; b0 < a.B; b0 += THREADS) {
-    const int b = b0 + threadIdx.x;
-    long long n = 0;
-    if (b < a.B) {
-      const Span s = span_of(a, b);
-      for (int rt = 0; rt < row_tiles(a, s.rows); ++rt) n += own_places(a, s, rt, p.prefix_tiles);
-      n *= a.Nk;
-    }
+  // running sums of the threads' values, behind `base`, which then includes them
+  auto running = [&](long long n, long long& base, bool again) {
     long long sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long x = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += x;
     }
-    if (b0 > 0) __syncthreads();
+    if (again) __syncthreads();
     if (lane == 31) sum_sm[warp] = sum;
     __syncthreads();
     long long before = base;
@@ -289,10 +302,57 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
       if (i < warp) before += sum_sm[i];
       base += sum_sm[i];
     }
-    if (b < a.B) first[b] = before + sum - n;
+    return before + sum - n;
+  };
+  if (!several) {   // no sequence has more than one row tile: one pass instead of two (0.5 us of a step of two sequences)
+    long long base = 0;
+    int tiles = 0;
+    for (int b0 = 0; b0 < a.B; b0 += THREADS) {
+      const int b = b0 + threadIdx.x;
+      const Span s = b < a.B ? span_of(a, b) : Span{0, 0, 0};
+      const bool some = s.rows > 0;
+      const unsigned with = __ballot_sync(0xffffffffu, some);
+      if (b0 > 0) __syncthreads();
+      if (lane == 31) tiles_sm[warp] = __popc(with);   // read behind the next barrier, as sum_sm is
+      const long long at = running(some ? static_cast<long long>(own_places(a, G, s, 0, p.prefix_tiles)) * a.Nk : 0, base, false);
+      int tile = tiles + __popc(with & ((1u << lane) - 1));
+#pragma unroll
+      for (int i = 0; i < THREADS / 32; ++i) {
+        if (i < warp) tile += tiles_sm[i];
+        tiles += tiles_sm[i];
+      }
+      if (b < a.B) tile0[b] = tile;
+      if (some) first[tile] = at;
+    }
+    if (threadIdx.x == 0) {
+      tile0[a.B] = tiles;
+      first[tiles] = base;
+    }
+    p.total = base + prefix_places(a, G, all_rows, p.prefix_tiles);
+    return p;
   }
-  if (threadIdx.x == 0) first[a.B] = base;
-  p.total = base + prefix_places(a, all_rows, p.prefix_tiles);
+  const long long most = most_row_tiles(a.T, a.B, a.N, a.Nk);   // more than these only lengths that overlap have: the rest is left out
+  long long tiles = 0, base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += THREADS) {
+    const int b = b0 + threadIdx.x;
+    const long long at = running(b < a.B ? row_tiles(G, span_of(a, b).rows) : 0, tiles, b0 > 0);
+    if (b < a.B) tile0[b] = static_cast<int>(min(at, most));
+  }
+  tiles = min(tiles, most);
+  if (threadIdx.x == 0) tile0[a.B] = static_cast<int>(tiles);
+  __syncthreads();
+  for (int r0 = 0; r0 < tiles; r0 += THREADS) {
+    const int r = r0 + threadIdx.x;
+    long long n = 0;
+    if (r < tiles) {
+      const int b = sequence_with(tile0, a.B, r);
+      n = static_cast<long long>(own_places(a, G, span_of(a, b), r - tile0[b], p.prefix_tiles)) * a.Nk;
+    }
+    const long long at = running(n, base, r0 > 0);
+    if (r < tiles) first[r] = at;
+  }
+  if (threadIdx.x == 0) first[tiles] = base;
+  p.total = base + prefix_places(a, G, all_rows, p.prefix_tiles);
   return p;
 }
 
@@ -305,7 +365,7 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
   pdl_launch_dependents();   // behind the wait: when step 2 begins, everything in front of this step has ended
   if (blockIdx.x == a.T) {
     if (blockIdx.y != 0) return;
-    const Plan p = make_plan<128>(a, w.first, a.status);
+    const Plan p = make_plan<128>(a, w.first, w.tile0, a.status);
     if (threadIdx.x == 0) *w.plan = p;
     return;
   }
@@ -394,7 +454,8 @@ struct TcSmem {
   static constexpr int kOffBar = kOffKV + kStages * kStageBytes;
   static constexpr int kOffFirst = kOffBar + 256;
   static constexpr int kHalf = kQT / 2 * 128;             // the second of two places for queries of up to 64 rows
-  static constexpr int kTotal = kOffFirst + 8 * (kPlanInSmem + 1) + 1024;
+  static constexpr int kOffTile0 = kOffFirst + 8 * (kPlanInSmem + 1);
+  static constexpr int kTotal = kOffTile0 + 4 * (kPlanInSmem + 1) + 1024;
 };
 enum { BAR_Q = 0, BAR_Q_FREE = BAR_Q + 2, BAR_K_FULL = BAR_Q_FREE + 2, BAR_K_EMPTY = BAR_K_FULL + 3, BAR_V_FULL = BAR_K_EMPTY + 3, BAR_V_EMPTY = BAR_V_FULL + 3, BAR_S = BAR_V_EMPTY + 3,
        BAR_P = BAR_S + 2, BAR_O = BAR_P + 2, BAR_END, BAR_O_FREE, BAR_FEW, BAR_FEW_END = BAR_FEW + 4, BAR_COUNT = BAR_FEW_END + 2 };
@@ -413,15 +474,17 @@ struct Segment {
 // The segments of a CTA one after the other: its first unit is searched for, the others follow from the one before.
 struct Walk {
   const ortb200_prefix_attn_args& a;
-  int prefix_tiles, prefix_row, all_rows;
+  const int* tile0;
+  int G, prefix_tiles, prefix_row, all_rows;
   long long left;        // places of the share that are left
   int seq, rt, kvh, at;  // the unit and the place within it
   int tiles, before;     // its tiles and the places in front of them
   Span s;
   Segment unit;          // what all key heads' segments of the unit have in common
-  __device__ Walk(const ortb200_prefix_attn_args& args, const long long* first, const Plan& p, int cta) : a(args), prefix_tiles(p.prefix_tiles), prefix_row(p.prefix_row) {
+  __device__ Walk(const ortb200_prefix_attn_args& args, const long long* first, const int* tiles_of, const Plan& p, int cta)
+      : a(args), tile0(tiles_of), G(args.N / args.Nk), prefix_tiles(p.prefix_tiles), prefix_row(p.prefix_row) {
     all_rows = last_row(a);
-    const long long prefix_total = prefix_places(a, all_rows, prefix_tiles);
+    const long long prefix_total = prefix_places(a, G, all_rows, prefix_tiles);
     long long x = share(p.total, cta);
     left = share(p.total, cta + 1) - x;
     seq = -1;
@@ -437,30 +500,22 @@ struct Walk {
       prefix_unit();
     } else {
       x -= prefix_total;
-      int lo = 0, hi = a.B;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (first[mid] <= x) lo = mid; else hi = mid;
-      }
-      x -= first[lo];
-      seq = lo;
+      const int r = sequence_with(first, tile0[a.B], x);
+      x -= first[r];
+      seq = sequence_with(tile0, a.B, r);
+      rt = r - tile0[seq];
       s = span_of(a, seq);
       own_unit();
-      while (x >= static_cast<long long>(tiles + before) * a.Nk) {
-        x -= static_cast<long long>(tiles + before) * a.Nk;
-        ++rt;
-        own_unit();
-      }
       kvh = static_cast<int>(x) / (tiles + before);
       at = static_cast<int>(x) - kvh * (tiles + before);
     }
   }
   __device__ void prefix_unit() {
     tiles = prefix_tiles;
-    before = extra(unit_rows(a, all_rows, 0));
+    before = extra(unit_rows(G, all_rows, 0));
     unit.seq = -1;
     unit.q_row = rt * kQT;
-    unit.rows = unit_rows(a, all_rows, rt);
+    unit.rows = unit_rows(G, all_rows, rt);
     unit.key0 = 0;
     unit.end = tiles * kKT;
     unit.past = unit.in_seq = 0;
@@ -468,16 +523,16 @@ struct Walk {
     unit.slot = prefix_slot(a, rt, 0, unit.rows);
   }
   __device__ void own_unit() {
-    tiles = own_tiles(a, s, rt, prefix_tiles);
-    unit.rows = unit_rows(a, s.rows, rt);
+    tiles = own_tiles(a, G, s, rt, prefix_tiles);
+    unit.rows = unit_rows(G, s.rows, rt);
     before = tiles > 0 ? extra(unit.rows) : 0;
     unit.seq = unit.table_row = seq;
     unit.in_seq = rt * kQT;
-    unit.q_row = s.row0 * (a.N / a.Nk) + unit.in_seq;
+    unit.q_row = s.row0 * G + unit.in_seq;
     unit.key0 = prefix_tiles * kKT;
-    unit.end = own_end(a, s, rt);
+    unit.end = own_end(a, G, s, rt);
     unit.past = s.past;
-    unit.slot = own_slot(a, s.row0, rt, 0, unit.rows);
+    unit.slot = own_slot(a, G, s.row0, rt, 0, unit.rows);
   }
   __device__ void step() {   // to the next unit that has tiles; there is one while places are left
     at = 0;
@@ -485,14 +540,13 @@ struct Walk {
     kvh = 0;
     ++rt;
     if (seq < 0) {
-      if (rt < row_tiles(a, all_rows)) {
+      if (rt < row_tiles(G, all_rows)) {
         prefix_unit();
         return;
       }
-      s.rows = 0;
     }
     do {
-      if (rt < row_tiles(a, s.rows) && seq >= 0) {
+      if (seq >= 0 && rt < tile0[seq + 1] - tile0[seq]) {
         own_unit();
         if (tiles > 0) return;
         ++rt;
@@ -839,6 +893,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BAR_COUNT);
   long long* first_sm = reinterpret_cast<long long*>(smem + L::kOffFirst);
+  int* tile0_sm = reinterpret_cast<int*>(smem + L::kOffTile0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ float2 part[4][kFew];
 
@@ -857,9 +912,9 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   // once.  Only the loading warp waits for step 1, in front of the first query or new key that it fetches.
   const Work w = work_of(a);
   Plan plan;
-  const bool kept = a.B <= kPlanInSmem;
+  const bool kept = most_row_tiles(a.T, a.B, a.N, a.Nk) <= kPlanInSmem;
   if (kept) {
-    plan = make_plan<kThreads>(a, first_sm, nullptr);
+    plan = make_plan<kThreads>(a, first_sm, tile0_sm, nullptr);
   } else {
     pdl_wait_prior_grids();
     plan = *w.plan;
@@ -870,7 +925,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   const uint32_t tmem_s = __reduce_or_sync(0xffffffffu, *tmem_slot);   // S / P: two buffers of 64 columns; the same for all, and known to be
   const uint32_t tmem_o = tmem_s + 2 * kKT;
 
-  Walk walk(a, kept ? first_sm : w.first, plan, blockIdx.x);
+  Walk walk(a, kept ? first_sm : w.first, kept ? tile0_sm : w.tile0, plan, blockIdx.x);
   Segment g;
   bool ok = true;
 
@@ -1199,8 +1254,10 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
   const int my_t = static_cast<int>((row0 + min(lane, count - 1)) / G);
   const int4 my_tok = __ldcg(&w.token[my_t]);
   const bool my_live = my_t < all_rows && my_t >= my_tok.y && my_t < my_tok.y + my_tok.z && plan.total > 0;   // lengths that start behind 0 leave rows to nobody
-  // where the own units of the row's sequence start
-  const long long my_start = my_live ? prefix_places(a, all_rows, plan.prefix_tiles) + __ldcg(&w.first[my_tok.x]) : 0;
+  // where the own units of the row's row tile start
+  const int my_ort = my_live ? (static_cast<int>(row0) + min(lane, count - 1) - my_tok.y * G) / kQT : 0, my_tile = my_live ? __ldcg(&w.tile0[my_tok.x]) + my_ort : 0;
+  const bool counted = my_live && my_tile < __ldcg(&w.tile0[my_tok.x + 1]);
+  const long long my_start = counted ? prefix_places(a, G, all_rows, plan.prefix_tiles) + __ldcg(&w.first[my_tile]) : 0;
   // the units of a row, 0 of the prefix and 1 of its own keys: first tile in the numbering, tiles, first slot
   int prt = -1, ort = -1, seq = -1, tiles0 = 0, tiles1 = 0, first0 = 0, first1 = 0, count0 = 0, count1 = 0;
   long long from0 = 0, from1 = 0, slot0 = 0, slot1 = 0, start = 0;
@@ -1224,7 +1281,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
     const int pr = static_cast<int>(row0) + r;
     if (r == 0 || pr == (t + 1) * G) {
       t = __shfl_sync(0xffffffffu, my_t, r);
-      live = __shfl_sync(0xffffffffu, my_live, r);
+      live = __shfl_sync(0xffffffffu, counted, r);
       tok = {__shfl_sync(0xffffffffu, my_tok.x, r), __shfl_sync(0xffffffffu, my_tok.y, r), __shfl_sync(0xffffffffu, my_tok.z, r), __shfl_sync(0xffffffffu, my_tok.w, r)};
     }
     const int orow = pr - tok.y * G;
@@ -1235,19 +1292,16 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
       const Span s = {tok.y, tok.z, tok.w};
       prt = pr / kQT;
       tiles0 = plan.prefix_tiles;
-      const int before0 = extra(unit_rows(a, all_rows, 0));
+      const int before0 = extra(unit_rows(G, all_rows, 0));
       from0 = (static_cast<long long>(prt) * a.Nk + kvh) * (tiles0 + before0) + before0;
-      slot0 = prefix_slot(a, prt, kvh, unit_rows(a, all_rows, prt));
-      if (tok.x != seq || ort < 0) {
-        seq = tok.x;
-        ort = 0;
-        start = __shfl_sync(0xffffffffu, my_start, r);
-      }
-      for (; ort < orow / kQT; ++ort) start += static_cast<long long>(own_places(a, s, ort, tiles0)) * a.Nk;
-      tiles1 = own_tiles(a, s, ort, tiles0);
-      const int rows1 = unit_rows(a, s.rows, ort);
+      slot0 = prefix_slot(a, prt, kvh, unit_rows(G, all_rows, prt));
+      seq = tok.x;
+      ort = orow / kQT;
+      start = __shfl_sync(0xffffffffu, my_start, r);
+      tiles1 = own_tiles(a, G, s, ort, tiles0);
+      const int rows1 = unit_rows(G, s.rows, ort);
       from1 = start + static_cast<long long>(kvh) * places(tiles1, rows1) + extra(rows1);
-      slot1 = own_slot(a, s.row0, ort, kvh, rows1);
+      slot1 = own_slot(a, G, s.row0, ort, kvh, rows1);
       first0 = tiles0 > 0 ? owner(plan.total, from0) : 0;
       first1 = tiles1 > 0 ? owner(plan.total, from1) : 0;
       count0 = tiles0 > 0 ? owner(plan.total, from0 + tiles0 - 1) - first0 + 1 : 0;
@@ -1413,7 +1467,7 @@ using namespace ortb200;
 
 extern "C" int64_t ortb200_prefix_attn_workspace_bytes(int64_t T, int B, int N, int Nk, int H, int tensor_cores) {
   if (!tensor_cores) return up256(T * N * H * 4);
-  return up256(sizeof(Plan) + 8ll * (B + 1)) + up256(T * 16) + up256(T * N * H * 2) + up256(segment_rows(T, N) * 8) + segment_rows(T, N) * H * 4;
+  return plan_bytes(T, B, N, Nk) + up256(T * 16) + up256(T * N * H * 2) + up256(segment_rows(T, N) * 8) + segment_rows(T, N) * H * 4;
 }
 
 extern "C" int ortb200_prefix_attn(const ortb200_prefix_attn_args* a, ortb200_stream_t stream_) {

@@ -9,7 +9,7 @@ import torch
 import onnxruntime_b200 as ort
 import serving_oracle as oracle
 from onnxruntime_b200 import onnx_lite as ol
-from onnxruntime_b200.capi import InvalidArgument
+from onnxruntime_b200.capi import EPFail, InvalidArgument
 
 CPU, GPU = "CPUExecutionProvider", "CUDAExecutionProvider"
 PROVIDERS = [pytest.param(CPU, id="cpu"), pytest.param(GPU, marks=pytest.mark.gpu, id="gpu")]
@@ -305,6 +305,22 @@ def test_prefix_units_of_few_and_of_many_rows(dt, N, Nk, H, size):
     """Sequences of 1 to 40 tokens by turns: units of up to eight rows and of more follow one another on every SM."""
     new = [(1, 2, 3, 40, 1, 0, 2, 8, 9)[i % 9] for i in range(130)]
     PrefixCase(dt, N, Nk, H, size, 100, [(29 * i) % 83 for i in range(130)], new, seed=4).run(GPU)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,H,held,new", [(128, 64, [5] * 8, [100] * 8), (2, 128, [i % 7 for i in range(780)], [1] * 780), (64, 128, [0, 3, 0], [900, 1, 700])])
+def test_prefix_batches_of_many_row_tiles(N, H, held, new):
+    """More row tiles than a CTA keeps the running sums of: long prompts, and many sequences."""
+    PrefixCase(torch.bfloat16, N, 1, H, 16, 70, held, new, seed=7).run(GPU)
+
+
+@pytest.mark.parametrize("provider", PROVIDERS)
+@pytest.mark.parametrize("cum", [[0, 4, 2], [0, 2, 9], [-1, 2, 5]])
+def test_prefix_lengths_that_fit_no_batch_are_an_error(provider, cum):
+    c = PrefixCase(torch.float32 if provider == CPU else torch.bfloat16, 4, 2, 64, 16, 70, [5, 30], [2, 3])
+    c.cum = i32(*cum)
+    with pytest.raises((InvalidArgument, EPFail)):
+        c.call(provider)()
 
 
 @pytest.mark.gpu
