@@ -314,6 +314,25 @@ def test_prefix_batches_of_many_row_tiles(N, H, held, new):
     PrefixCase(torch.bfloat16, N, 1, H, 16, 70, held, new, seed=7).run(GPU)
 
 
+@pytest.mark.gpu
+def test_prefix_of_a_cache_beyond_32_bit_offsets():
+    """The same blocks behind 2^31 elements of cache give the same bits."""
+    a = PrefixCase(torch.bfloat16, 4, 2, 128, 64, 100, [5, 70], [1, 3], stale=0.0)
+    near = a.call(GPU)()
+    first, used = 2 ** 31 // (64 * 2 * 128) + 3, len(a.caches[0])
+    caches = [torch.zeros(first + used, 64, 2, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for c, mine in zip(caches, a.caches):
+        c[first:].copy_(mine)
+    a.caches, a.table, a.slot = caches, a.table + first, a.slot + first * 64
+    call = a.call(GPU)
+    call.sess.run_with_iobinding(call.binding)
+    torch.cuda.synchronize()
+    call.sess.check_device_status()
+    assert torch.equal(call.outs["out"].cpu(), near["out"])
+    for name in ("kc_out", "vc_out"):
+        assert torch.equal(call.outs[name][first:].cpu(), near[name]) and not call.outs[name][:first].any()
+
+
 @pytest.mark.parametrize("provider", PROVIDERS)
 @pytest.mark.parametrize("cum", [[0, 4, 2], [0, 2, 9], [-1, 2, 5]])
 def test_prefix_lengths_that_fit_no_batch_are_an_error(provider, cum):
@@ -368,6 +387,45 @@ def test_prefix_captured_graph_follows_the_lengths():
         got = dict(out=got["out"], kc_out=got["kc_out"][:len(b.caches[0])], vc_out=got["vc_out"][:len(b.caches[1])])
         b.check(got)
     assert call.sess.num_captured_graphs() == 1
+
+
+@pytest.mark.gpu
+def test_prefix_two_captured_graphs_of_one_session_by_turns():
+    a = PrefixCase(torch.bfloat16, 8, 2, 128, 64, 192, [5, 70], [1, 1], seed=1)
+    b = PrefixCase(torch.bfloat16, 8, 2, 128, 64, 320, [300, 9, 64, 0, 31], [1, 1, 1, 1, 1], seed=2)
+    first, second = a.call(GPU, graph=True), b.call(GPU, graph=True)
+    second.sess = first.sess
+    second.binding = first.sess.io_binding()
+    for n, t in second.ins.items():
+        second.binding.bind_torch_input(n, t)
+    for n, t in second.outs.items():
+        second.binding.bind_torch_output(n, t)
+    for _ in range(3):
+        for i, (case, call) in enumerate(((a, first), (b, second))):
+            call.outs["out"].fill_(3.0)
+            options = ort.RunOptions()
+            options.add_run_config_entry("gpu_graph_id", str(i + 1))
+            call.sess.run_with_iobinding(call.binding, options)
+            torch.cuda.synchronize()
+            call.sess.check_device_status()
+            case.check({n: t.cpu() for n, t in call.outs.items()})
+    assert first.sess.num_captured_graphs() == 2
+
+
+@pytest.mark.gpu
+def test_prefix_two_sessions_at_once():
+    cases = [PrefixCase(torch.float16, 16, 4, 64, 16, 700, [(31 * i) % 290 for i in range(40)], [1] * 40, seed=s, stale=0.0) for s in (1, 2)]
+    calls = [c.call(GPU) for c in cases]
+    alone = [call()["out"] for call in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(20):
+        for call, stream in zip(calls, streams):
+            with torch.cuda.stream(stream):
+                call.sess.run_with_iobinding(call.binding)
+    torch.cuda.synchronize()
+    for call, want in zip(calls, alone):
+        call.sess.check_device_status()
+        assert torch.equal(call.outs["out"].cpu(), want)
 
 
 @pytest.mark.gpu
@@ -510,6 +568,28 @@ def test_log_probs_sizes_of_models(dt, rows, V):
     # p carries the error of lse (tol) as a factor; the output is rounded once (fp16: also below its normal range)
     bound = half_step(dt) * want.abs() + tol * (p * (grads["g_lp"].abs() + 40 * grads["g_h"].abs())[:, None]) + torch.finfo(dt).tiny * half_step(dt) + 1e-9
     assert ((got["dx"].double() - want).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+def test_log_probs_beyond_32_bit_offsets():
+    """The last of so many rows that their logits are more than 2^31; tolerances as above."""
+    rows, V = 2 ** 31 // 50257 + 7, 50257
+    g = torch.Generator().manual_seed(1)
+    last = (2.5 * torch.randn(V, generator=g)).bfloat16()
+    x = torch.zeros(rows, V, dtype=torch.bfloat16, device="cuda")
+    x[-1] = last.cuda()
+    grads = dict(g_lp=torch.ones(rows), g_h=torch.zeros(rows))
+    call = score_call(GPU, x, torch.full((rows,), 5), 3, grads)
+    call.sess.run_with_iobinding(call.binding)
+    torch.cuda.synchronize()
+    logp = torch.log_softmax(last.double(), -1)
+    tol = 4e-6 * 20
+    assert abs(float(call.outs["lp"][-1]) - float(logp[5])) < tol and abs(float(call.outs["h"][-1]) + float((logp.exp() * logp).sum())) < tol
+    assert (call.outs["lse"][:-1].cpu().double() - math.log(V)).abs().max() < tol and (call.outs["index"][:-1].cpu() == torch.arange(3)).all()
+    assert torch.equal(call.outs["index"][-1].cpu(), torch.sort(last.float(), descending=True, stable=True)[1][:3])
+    want = -logp.exp()
+    want[5] += 1
+    assert ((call.outs["dx"][-1].cpu().double() - want).abs() <= half_step(torch.bfloat16) * want.abs() + tol * logp.exp() + 1e-9).all()
 
 
 GRADS = ["g_lp", "g_h", "g_top", "g_lse"]
