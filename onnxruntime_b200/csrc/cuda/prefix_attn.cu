@@ -19,8 +19,8 @@
 //
 // What bounds it.  Many rows (24 prompts of up to 150 tokens behind 6000, 28 heads of 128): the tensor pipe, which has half as much
 // again to do as the formula because weights count as two 16-bit values; a tile of 128 rows and 64 keys takes 768 clocks of it and
-// a CTA is done with one in about 2000, two CTAs side by side; 512 clocks of exponentials per tile run beside it.  284 us in all, of
-// which the product kernel has 234 and the join 37.  Single tokens behind a long prefix: segments and their hand-overs; 180 sequences of 16
+// a CTA is done with one in 2000 to 2500, two CTAs side by side; 512 clocks of exponentials per tile run beside it.  284 us in all on
+// one GPU, of which the product kernel has 234 and the join 37, and up to 330 on others, whose clocks settle lower.  Single tokens behind a long prefix: segments and their hand-overs; 180 sequences of 16
 // heads of 64 behind 20011 tokens take 114 us, 64 of 64 heads of 128 behind 8192 tokens 64 us, where the bytes need 37 and 23.
 // Slower, each against the form of its time at (180 behind 20011, 64 behind 8192): 128-key tiles with one score buffer 164 and 82 us
 // instead of 149 and 70; eight softmax warps with half a row each 150 and 80; rows held four times with a quarter of the keys to each
@@ -1440,7 +1440,7 @@ int launch_tc(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
   // the two later steps may set up while the step before them ends: they wait for it before they read
   rc = launch_kernel(kern, dim3(kGrid), kThreads, L::kTotal, stream, true, tq, tk, tv, *a, scale);
   if (rc != 0) return rc;
-  // Up to four rows per SM: a CTA each (one token of 32 heads over two key heads behind 18529 tokens: 20 us instead of 74 with one
+  // Up to four rows per SM: a CTA each (one token of 32 heads over two key heads behind 18529 tokens: 23 us instead of 74 with one
   // warp a row).  Then one row per warp until there are rows for 16 warps on each SM, which is what fits at once: warps that come
   // later would look their segments up when the others have ended (24 prompts of up to 150 tokens: 37 us behind the product kernel
   // instead of 80).
