@@ -1466,6 +1466,7 @@ int launch_rows(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
 using namespace ortb200;
 
 extern "C" int64_t ortb200_prefix_attn_workspace_bytes(int64_t T, int B, int N, int Nk, int H, int tensor_cores) {
+  if (T < 0 || B < 0 || N <= 0 || Nk <= 0 || H <= 0) return -1;
   if (!tensor_cores) return up256(T * N * H * 4);
   return plan_bytes(T, B, N, Nk) + up256(T * 16) + up256(T * N * H * 2) + up256(segment_rows(T, N) * 8) + segment_rows(T, N) * H * 4;
 }

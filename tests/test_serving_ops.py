@@ -1,5 +1,6 @@
 """The operators around one step of a serving batch against serving_oracle.py: PagedBatchLayout, SharedPrefixPagedAttention,
 TokenLogProbs and its gradient, each on the CPU provider and (marked gpu) on the GPU."""
+import ctypes
 import math
 
 import numpy as np
@@ -746,3 +747,16 @@ def test_layout_attention_and_log_probs_in_one_graph(kind):
         ins["past"].add_(1)
         ins["free"].copy_(i32(*free))
         ins["q"].copy_(torch.randn(2, (N + 2 * Nk) * H, generator=g).to(dt))
+
+
+# ------------------------------------------------------------------------------------------------------------- the C interface
+def test_c_entries_refuse_what_is_missing():
+    """A return code, on a machine without a GPU too."""
+    from onnxruntime_b200.ops import _kernels as K
+    lib = ctypes.CDLL(K.lib_path())
+    for name in ("ortb200_batch_layout", "ortb200_prefix_attn", "ortb200_token_log_probs", "ortb200_token_log_probs_grad"):
+        assert getattr(lib, name)(None, None) == -1, name
+    size = lib.ortb200_prefix_attn_workspace_bytes
+    size.restype, size.argtypes = ctypes.c_int64, [ctypes.c_int64] + [ctypes.c_int] * 5
+    assert size(10, 2, 8, 0, 64, 1) == size(-1, 2, 8, 2, 64, 1) == size(10, 2, 8, 2, 0, 0) == -1
+    assert size(10, 2, 8, 2, 64, 1) > size(10, 2, 8, 2, 64, 0) > 0
