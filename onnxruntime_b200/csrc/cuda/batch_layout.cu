@@ -197,7 +197,7 @@ extern "C" int ortb200_batch_layout(const ortb200_batch_layout_args* a, ortb200_
   if (a->num_free > 0 && !a->free_blocks) return -1;
   if (a->B > kMaxRequests || a->rows > 0x7fffffffll) return -2;
   const int smem = 8 * (a->B + 1);
-  if (smem > 48 * 1024) {
+  if (smem > 47 * 1024) {   // (the kernel has some shared memory of its own, which counts towards the 48 KB that need no leave)
     if (cudaFuncSetAttribute(batch_layout_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * (kMaxRequests + 1)) != cudaSuccess) return -10;
   }
   const long long most = a->rows > static_cast<long long>(a->B) * a->max_blocks ? a->rows : static_cast<long long>(a->B) * a->max_blocks;

@@ -97,6 +97,12 @@ def test_layout_of_many_requests(provider, B):
 
 
 @pytest.mark.parametrize("provider", PROVIDERS)
+@pytest.mark.parametrize("B", [6119, 6120, 6143, 6144, 16384])
+def test_layout_around_48_kb_of_running_sums(provider, B):
+    check_layout(provider, [i % 5 for i in range(B)], [(i + 1) % 2 for i in range(B)], torch.arange(3 * B, dtype=torch.int32).reshape(B, 3), list(range(7, 3 * B)), B, 2)
+
+
+@pytest.mark.parametrize("provider", PROVIDERS)
 def test_layout_of_more_requests_than_one_launch_takes(provider):
     B = 16400
     check_layout(provider, [i % 5 for i in range(B)], [(i + 1) % 2 for i in range(B)], torch.arange(3 * B, dtype=torch.int32).reshape(B, 3), list(range(7, 3 * B)), B, 2)
