@@ -315,9 +315,11 @@ def test_prefix_units_of_few_and_of_many_rows(dt, N, Nk, H, size):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("N,H,held,new", [(128, 64, [5] * 8, [100] * 8), (2, 128, [i % 7 for i in range(780)], [1] * 780), (64, 128, [0, 3, 0], [900, 1, 700])])
+@pytest.mark.parametrize("N,H,held,new", [(128, 64, [5] * 8, [100] * 8), (2, 128, [i % 7 for i in range(780)], [1] * 780), (64, 128, [0, 3, 0], [900, 1, 700]),
+                                          (2, 128, [i % 7 for i in range(400)], [(1, 1, 0, 2)[i % 4] for i in range(400)]),
+                                          (16, 64, [i % 9 for i in range(300)], [(1, 9, 0, 2)[i % 4] for i in range(300)])])
 def test_prefix_batches_of_many_row_tiles(N, H, held, new):
-    """More row tiles than a CTA keeps the running sums of: long prompts, and many sequences."""
+    """More row tiles than a CTA keeps the running sums of (long prompts, many sequences), and more than it has threads."""
     PrefixCase(torch.bfloat16, N, 1, H, 16, 70, held, new, seed=7).run(GPU)
 
 
