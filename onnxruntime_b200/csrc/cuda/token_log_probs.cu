@@ -3,7 +3,8 @@
 //
 // One pass over a row.  A thread keeps a running maximum m, S = sum exp(x - m) and W = sum exp(x - m) (x - m) of the logits it has
 // seen; when the maximum moves from m to m', W becomes (W + S (m - m')) c and S becomes S c with c = exp(m - m').  Joined over
-// the row: log_sum_exp = m + log S and entropy = log S - W / S.  All of it is held in 32 bits, and to the base 2.
+// the row: log_sum_exp = m + log S and entropy = log S - W / S.  All of it is held in 32 bits; m is a logit as it is, exponents
+// and W are to the base 2.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -57,14 +58,18 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// With t = x log2(e): m the largest t, s = sum 2^(t - m), w = sum 2^(t - m) (t - m).  The exponent is one multiply-add whose only
-// rounding is that of its result, so that the reference m is no source of error; two logits go through one instruction.
+constexpr float kFar = -1e30f;   // an exponent below all that count: 0 times it is 0, where 0 times -inf would be NaN
+
+// m the largest logit, s = sum 2^t, w = sum 2^t t with t = (x - m) log2(e).  The difference comes first: the maximum's own exponent is
+// 0 whatever its size.  (One multiply-add x log2(e) - m log2(e) is off by 2^-24 of |m|, which for masks of -1e10 and beyond is more
+// than a 32-bit exponent holds; it took 592 instead of 601 us for 4096 rows of 128256 bf16 logits and their gradient.)  Two logits go
+// through one instruction.
 struct Stats {
   float m, s, w;
   static __device__ __forceinline__ Stats none() { return {-INFINITY, 0.f, 0.f}; }
   __device__ __forceinline__ void raise(float to) {   // to >= m
     if (s != 0.f) {
-      const float d = m - to, c = exp2f(d);
+      const float d = fmaxf((m - to) * kLog2e, kFar), c = exp2f(d);
       w = d == 0.f ? w : (w + s * d) * c;
       s *= c;
     }
@@ -73,10 +78,10 @@ struct Stats {
   // N logits whose largest is `top` (NaN if one of them is)
   template <int N>
   __device__ __forceinline__ void add(const float* x, float top) {
-    if (top * kLog2e > m) raise(top * kLog2e);
+    if (top > m) raise(top);
     const float ref = m == -INFINITY ? 0.f : -m;
     if (N == 1) {
-      const float t = max_nan(fmaf(x[0], kLog2e, ref), -1e30f), e = exp2_fast(t);
+      const float t = max_nan((x[0] + ref) * kLog2e, kFar), e = exp2_fast(t);
       s += e;
       w = fmaf(e, t, w);
       return;
@@ -86,10 +91,9 @@ struct Stats {
 #pragma unroll
     for (int i = 0; i + 1 < N; i += 2) {
       float t0, t1;
-      unpack2(fma2(pack2(x[i], x[i + 1]), scale, ref2), t0, t1);
-      // an impossible token has t = -inf: 0 times that has to count as 0
-      t0 = max_nan(t0, -1e30f);
-      t1 = max_nan(t1, -1e30f);
+      unpack2(mul2(fma2(pack2(x[i], x[i + 1]), one, ref2), scale), t0, t1);
+      t0 = max_nan(t0, kFar);   // (an impossible token has -inf, and so has one beyond 32 bits below the largest)
+      t1 = max_nan(t1, kFar);
       const f32x2 e = pack2(exp2_fast(t0), exp2_fast(t1));
       s2 = fma2(e, one, s2);
       w2 = fma2(e, pack2(t0, t1), w2);
@@ -331,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, TOP && sizeof(T) == 4 ? 3 : 4) token
     st.s = __shfl_sync(0xffffffffu, st.s, 0);
     st.w = __shfl_sync(0xffffffffu, st.w, 0);
     const bool empty = st.s == 0.f;   // nothing in the row is possible
-    const float log_s = log2f(st.s), lse = empty ? -INFINITY : (st.m + log_s) * kLn2;
+    const float log_s = log2f(st.s), lse = empty ? -INFINITY : fmaf(log_s, kLn2, st.m);
     if (lane == 0) {
       if (a.log_sum_exp) a.log_sum_exp[row] = lse;
       if (a.entropy) a.entropy[row] = empty ? 0.f : (log_s - st.w / st.s) * kLn2;
@@ -377,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_log_probs_grad_kernel(const
   const bool empty = lse == -INFINITY;   // nothing in the row is possible, and nothing changes that
   auto slope = [&](float v) {
     const float lp = v - lse;
-    return empty ? 0.f : exp_fast(lp) * (all - g_h * (fmaxf(lp, -1e30f) + h));   // an impossible token: 0 times -inf counts as 0
+    return empty ? 0.f : exp_fast(lp) * (all - g_h * (fmaxf(lp, kFar) + h));   // an impossible token: 0 times -inf counts as 0
   };
   // this share's elements: vectors [from, to), the head in the first and the tail in the last
   const int from = static_cast<int>(static_cast<long long>(x.vectors) * part / parts), to = static_cast<int>(static_cast<long long>(x.vectors) * (part + 1) / parts);
