@@ -156,12 +156,13 @@ void TokenLogProbsImpl(Ctx& ctx) {
   const double inf = std::numeric_limits<double>::infinity();
   at::Tensor m = z.rows > 0 ? x.amax(1, true) : x.narrow(1, 0, 1);
   at::Tensor empty = m.eq(-inf);                                     // nothing in the row is possible
-  at::Tensor d = x - at::where(empty, at::zeros_like(m), m), e = at::exp(d), s = e.sum(1, true);
+  at::Tensor from = at::where(empty, at::zeros_like(m), m), d = x - from, e = at::exp(d), s = e.sum(1, true);
   at::Tensor log_s = at::log(s), lse = at::where(empty, m, m + log_s);
   at::Tensor w = at::where(x.eq(-inf), at::zeros_like(e), e * d).sum(1, true);
   at::Tensor entropy = at::where(empty, at::zeros_like(s), log_s - w / s);
   at::Tensor in = tokens.ge(0).logical_and(tokens.lt(z.vocab));
-  auto log_prob_of = [&](const at::Tensor& idx) { return at::where(empty, at::full_like(lse, -inf), x.gather(1, idx) - lse); };
+  // (from the largest logit: m + log S is rounded by 2^-24 of m)
+  auto log_prob_of = [&](const at::Tensor& idx) { return at::where(empty, at::full_like(lse, -inf), x.gather(1, idx) - from - log_s); };
   at::Tensor lp = log_prob_of(at::where(in, tokens, at::zeros_like(tokens)).unsqueeze(1)).squeeze(1);
   std::vector<int64_t> top = z.lead;
   top.push_back(z.top_k);

@@ -68,7 +68,7 @@ int ortb200_prefix_attn(const ortb200_prefix_attn_args* args, ortb200_stream_t s
 int64_t ortb200_prefix_attn_workspace_bytes(int64_t T, int B, int N, int Nk, int H, int tensor_cores);
 
 // Row by row over logits x [rows, vocab], with m the largest and S = sum exp(x - m):
-//   log_sum_exp = m + log S;  log_prob = x[token] - log_sum_exp;  entropy = log S - sum exp(x - m) (x - m) / S
+//   log_sum_exp = m + log S;  log_prob = (x[token] - m) - log S;  entropy = log S - sum exp(x - m) (x - m) / S
 // and the top_k largest, equal ones by the lower index.  A token outside [0, vocab) is padding: log_prob 0.
 typedef struct {
   const void* logits;         // [rows, vocab] dtype

@@ -336,15 +336,17 @@ __global__ void __launch_bounds__(kThreads, TOP && sizeof(T) == 4 ? 3 : 4) token
     st.w = __shfl_sync(0xffffffffu, st.w, 0);
     const bool empty = st.s == 0.f;   // nothing in the row is possible
     const float log_s = log2f(st.s), lse = empty ? -INFINITY : fmaf(log_s, kLn2, st.m);
+    // from the largest logit, not from m + log S, whose rounding is 2^-24 of m: log S is never below 0, so this is never above it
+    auto log_prob_of = [&](float f) { return empty ? -INFINITY : (f - st.m) - log_s * kLn2; };
     if (lane == 0) {
       if (a.log_sum_exp) a.log_sum_exp[row] = lse;
       if (a.entropy) a.entropy[row] = empty ? 0.f : (log_s - st.w / st.s) * kLn2;
-      if (a.log_prob) a.log_prob[row] = token < 0 || token >= a.vocab ? 0.f : empty ? -INFINITY : chosen - lse;
+      if (a.log_prob) a.log_prob[row] = token < 0 || token >= a.vocab ? 0.f : log_prob_of(chosen);
     }
     if (TOP && lane < top_k) {
       const unsigned long long key = sm.chosen[lane];
       if (a.top_tokens) a.top_tokens[row * top_k + lane] = 0xffffffffu - static_cast<unsigned>(key);
-      if (a.top_log_probs) a.top_log_probs[row * top_k + lane] = empty ? -INFINITY : value_of(key) - lse;
+      if (a.top_log_probs) a.top_log_probs[row * top_k + lane] = log_prob_of(value_of(key));
     }
   }
 }

@@ -81,9 +81,38 @@ def masked_rows(V, mask, dtype):
 @pytest.mark.parametrize("mask", [1e4, 6e4, 1e6, 1e9, 2e9, 1e10, 1e15, 1e20, 1e30, 1e37, 1e38, 2.5e38, math.inf])
 def test_log_probs_with_finite_masks(kind, V, k, times, mask):
     """Masks of every size up to the type's lowest value (``inf`` stands for that)."""
-    most = torch.finfo(kind[1]).max
+    most, times = torch.finfo(kind[1]).max, times if kind[0] == GPU else 1   # (many rows are another division of the work on a GPU alone)
     if mask > most and mask != math.inf:
         pytest.skip("beyond the type")
     x = masked_rows(V, min(mask, most), kind[1]).repeat(times, 1)
     tokens = torch.tensor([0, V - 1, 1, V // 3, V - 1, 3, 9, 2, 0, V // 5, 7, V - 1]).repeat(times)
     check_rows(kind, x, tokens, k, relative=False)
+
+
+@pytest.mark.parametrize("kind", SCORE_KINDS)
+@pytest.mark.parametrize("V,times", [(40, 1), (50257, 1), (20000, 60)])
+@pytest.mark.parametrize("mask", [1e4, 1e6, 1e10, 1e30, math.inf])
+def test_log_probs_relative_to_the_largest_logit(kind, V, times, mask):
+    """A row of equal logits has the log probability -log V whatever their size."""
+    most, times = torch.finfo(kind[1]).max, times if kind[0] == GPU else 1   # (many rows are another division of the work on a GPU alone)
+    if mask > most and mask != math.inf:
+        pytest.skip("beyond the type")
+    x = masked_rows(V, min(mask, most), kind[1]).repeat(times, 1)
+    tokens = torch.tensor([0, V - 1, 1, V // 3, V - 1, 3, 9, 2, 0, V // 5, 7, V - 1]).repeat(times)
+    got = check_rows(kind, x, tokens, 3)
+    assert (got["lp"][::12] + math.log(V)).abs().max() < 1e-4
+
+
+@pytest.mark.parametrize("kind", SCORE_KINDS)
+@pytest.mark.parametrize("base", [0.0, 5.0, 23.7, 60.0, 333.3, 1000.0, -1000.0, 30000.0])
+def test_log_probs_of_confident_rows(kind, base):
+    """Tokens of nearly all the probability: no log probability above 0, and each as near as the difference to the largest logit allows."""
+    V, rows = 3001, 200
+    g = torch.Generator().manual_seed(int(abs(base)))
+    x = base + torch.randn(rows, V, generator=g)
+    tokens = torch.randint(0, V, (rows,), generator=g)
+    margin = torch.linspace(5, 40, rows)
+    x[torch.arange(rows), tokens] = base + margin + torch.rand(rows, generator=g)
+    x = x.to(kind[1])
+    got = check_rows(kind, x, tokens, 4)
+    assert (got["lp"] <= 0).all() and (got["top"] <= 0).all()
