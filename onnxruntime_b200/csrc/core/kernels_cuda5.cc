@@ -182,8 +182,8 @@ class TokenLogProbsKernel final : public WithGeneric {
     std::vector<int64_t> top = z.lead;
     top.push_back(z.top_k);
     const auto wanted = [&](int i) { return i < ctx.OutputCount() && ctx.OutputNeeded(i); };
-    at::Tensor out[5];
-    for (int i : {0, 1, 4})
+    at::Tensor out[6];
+    for (int i : {0, 1, 4, 5})
       if (wanted(i)) out[i] = Output(ctx, i, z.lead, at::kFloat, x);
     if (wanted(2)) out[2] = Output(ctx, 2, top, at::kFloat, x);
     if (wanted(3)) out[3] = Output(ctx, 3, top, at::kLong, x);
@@ -195,6 +195,7 @@ class TokenLogProbsKernel final : public WithGeneric {
     a.log_sum_exp = wanted(4) ? out[4].data_ptr<float>() : nullptr;
     a.top_log_probs = wanted(2) ? out[2].data_ptr<float>() : nullptr;
     a.top_tokens = wanted(3) ? out[3].data_ptr<int64_t>() : nullptr;
+    a.log_sum_exp_rest = wanted(5) ? out[5].data_ptr<float>() : nullptr;
     a.rows = z.rows;
     a.vocab = static_cast<int>(z.vocab);
     a.top_k = wanted(2) || wanted(3) ? static_cast<int>(z.top_k) : 0;
@@ -202,7 +203,7 @@ class TokenLogProbsKernel final : public WithGeneric {
     a.use_pdl = Pdl(ctx);
     CheckLaunch(ortb200_token_log_probs(&a, ctx.cuda_stream()), "ortb200_token_log_probs");
     ctx.session()->AddLaunches(z.rows > 0 ? 1 : 0);
-    for (int i = 0; i < 5; ++i)
+    for (int i = 0; i < 6; ++i)
       if (out[i].defined()) ctx.SetOutput(i, out[i]);
   }
 };
@@ -219,7 +220,7 @@ class TokenLogProbsGradKernel final : public WithGeneric {
       Generic(ctx);
       return;
     }
-    at::Tensor keep[9];
+    at::Tensor keep[10];
     auto floats = [&](int i) -> const float* {
       if (!ctx.HasInput(i)) return nullptr;
       keep[i] = ctx.Input(i).to(at::kFloat).contiguous();
@@ -239,6 +240,7 @@ class TokenLogProbsGradKernel final : public WithGeneric {
       a.top_k = static_cast<int>(z.top_k);
     }
     a.d_log_sum_exp = floats(8);
+    a.log_sum_exp_rest = floats(9);
     at::Tensor dx = Output(ctx, 0, ctx.Input(0).sizes(), x.scalar_type(), x, 0);
     a.d_logits = dx.data_ptr();
     a.rows = z.rows;

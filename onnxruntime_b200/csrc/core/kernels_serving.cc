@@ -174,6 +174,10 @@ void TokenLogProbsImpl(Ctx& ctx) {
     if (ctx.OutputCount() > 3) ctx.SetOutput(3, order.reshape(top).contiguous());
   }
   if (ctx.OutputCount() > 4) ctx.SetOutput(4, F32(lse).reshape(z.lead));
+  if (ctx.OutputCount() > 5) {   // what rounding to 32 bits takes from m + log S
+    at::Tensor sum = lse.to(at::kFloat).to(at::kDouble), rest = (m.to(at::kDouble) - sum) + log_s.to(at::kDouble);
+    ctx.SetOutput(5, F32(at::where(at::isfinite(sum), rest, at::zeros_like(rest))).reshape(z.lead));
+  }
 }
 
 void TokenLogProbsGradImpl(Ctx& ctx) {
@@ -182,7 +186,7 @@ void TokenLogProbsGradImpl(Ctx& ctx) {
   const double inf = std::numeric_limits<double>::infinity();
   auto column = [&](int i) { return ctx.HasInput(i) ? ctx.Input(i).to(x.scalar_type()).reshape({z.rows, 1}) : at::zeros({z.rows, 1}, x.options()); };
   at::Tensor lse = column(2), empty = lse.eq(-inf);
-  at::Tensor lp = x - at::where(empty, at::zeros_like(lse), lse), gone = x.eq(-inf);
+  at::Tensor lp = x - at::where(empty, at::zeros_like(lse), lse) - column(9), gone = x.eq(-inf);
   at::Tensor in = tokens.ge(0).logical_and(tokens.lt(z.vocab));
   at::Tensor g = at::where(in, column(4), at::zeros_like(lse)), all = column(8) - g, h = column(5);
   at::Tensor top;
@@ -307,7 +311,7 @@ TokenLogProbsSizes CheckTokenLogProbsGrad(Ctx& ctx) {
   TokenLogProbsSizes z = LogitsAndTokens(ctx);
   ctx.RequiredInput(2);
   ORTB_ENFORCE_ARG(!ctx.HasInput(5) || ctx.HasInput(3), "TokenLogProbsGrad: the gradient of the entropy needs the entropy");
-  for (int i : {2, 3, 4, 5, 8})
+  for (int i : {2, 3, 4, 5, 8, 9})
     ORTB_ENFORCE_ARG(!ctx.HasInput(i) || (ctx.Input(i).is_floating_point() && ctx.Input(i).numel() == z.rows), "TokenLogProbsGrad: input ", i, " must hold one floating value per row");
   if (ctx.HasInput(7)) {
     const at::Tensor& k = ctx.RequiredInput(6);

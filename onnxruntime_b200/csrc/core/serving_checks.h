@@ -24,7 +24,7 @@ struct BatchLayoutSizes {
 BatchLayoutSizes CheckBatchLayout(OpKernelContext& ctx);
 
 // com.ortb200 TokenLogProbs: logits, tokens.  com.ortb200 TokenLogProbsGrad: logits, tokens, log_sum_exp, entropy?, d_log_prob?,
-// d_entropy?, top_tokens?, d_top_log_probs?, d_log_sum_exp?
+// d_entropy?, top_tokens?, d_top_log_probs?, d_log_sum_exp?, log_sum_exp_rest?
 struct TokenLogProbsSizes {
   int64_t rows = 0, vocab = 0, top_k = 0;
   std::vector<int64_t> lead;   // shape of one value per row

@@ -704,11 +704,11 @@ void RegisterBuiltinSchemas(std::map<std::string, OpSchema>& t) {
     lead.pop_back();
     Dims top = lead;
     top.push_back(Known(c.node.attr_i("top_k", 0)));
-    for (size_t i : {0, 1, 4}) c.SetOutput(i, pb::FLOAT, lead);
+    for (size_t i : {0, 1, 4, 5}) c.SetOutput(i, pb::FLOAT, lead);
     c.SetOutput(2, pb::FLOAT, top);
     c.SetOutput(3, pb::INT64, top);
   });
-  Reg(t, FUSED, "TokenLogProbsGrad", 3, 9, Same);
+  Reg(t, FUSED, "TokenLogProbsGrad", 3, 10, Same);
   Reg(t, FUSED, "SwiGLU", 1, 1, [](Ctx& c) {
     if (!c.HasShape(0) || c.Rank(0) < 1) return;
     Dims out = c.Dims(0);

@@ -70,6 +70,8 @@ int64_t ortb200_prefix_attn_workspace_bytes(int64_t T, int B, int N, int Nk, int
 // Row by row over logits x [rows, vocab], with m the largest and S = sum exp(x - m):
 //   log_sum_exp = m + log S;  log_prob = (x[token] - m) - log S;  entropy = log S - sum exp(x - m) (x - m) / S
 // and the top_k largest, equal ones by the lower index.  A token outside [0, vocab) is padding: log_prob 0.
+// log_sum_exp_rest is what rounding took from log_sum_exp (2^-24 of m, which may be more than log S): x - log_sum_exp - log_sum_exp_rest
+// is the log probability of every x.
 typedef struct {
   const void* logits;         // [rows, vocab] dtype
   const int64_t* tokens;      // [rows]
@@ -78,6 +80,7 @@ typedef struct {
   float* log_sum_exp;         // [rows]
   float* top_log_probs;       // [rows, top_k]
   int64_t* top_tokens;        // [rows, top_k]
+  float* log_sum_exp_rest;    // [rows]
   int64_t rows;
   int vocab, top_k;           // 0 <= top_k <= min(32, vocab)
   int dtype;
@@ -87,7 +90,8 @@ int ortb200_token_log_probs(const ortb200_token_log_probs_args* args, ortb200_st
 
 //   d_logits[v] = p_v (d_log_sum_exp - d_log_prob - sum_k d_top[k] - d_entropy (log p_v + entropy))
 //                 + d_log_prob [v = token] + sum_k d_top[k] [v = top_tokens[k]]
-// d_logits may be logits.  Of the gradients any may be null; a padding token has no d_log_prob.
+// with log p_v = logits[v] - log_sum_exp - log_sum_exp_rest.  d_logits may be logits.  Of the gradients any may be null; a padding
+// token has no d_log_prob.
 typedef struct {
   const void* logits;
   const int64_t* tokens;
@@ -98,6 +102,7 @@ typedef struct {
   const int64_t* top_tokens;    // [rows, top_k], needed with d_top_log_probs
   const float* d_top_log_probs; // [rows, top_k]
   const float* d_log_sum_exp;   // [rows]
+  const float* log_sum_exp_rest;  // [rows], null: 0
   void* d_logits;               // [rows, vocab] dtype
   int64_t rows;
   int vocab, top_k;

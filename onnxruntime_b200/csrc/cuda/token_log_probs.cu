@@ -335,11 +335,15 @@ __global__ void __launch_bounds__(kThreads, TOP && sizeof(T) == 4 ? 3 : 4) token
     st.s = __shfl_sync(0xffffffffu, st.s, 0);
     st.w = __shfl_sync(0xffffffffu, st.w, 0);
     const bool empty = st.s == 0.f;   // nothing in the row is possible
-    const float log_s = log2f(st.s), lse = empty ? -INFINITY : fmaf(log_s, kLn2, st.m);
+    const float log_s = log2f(st.s), ln_s = __fmul_rn(log_s, kLn2), lse = empty ? -INFINITY : st.m + ln_s;
     // from the largest logit, not from m + log S, whose rounding is 2^-24 of m: log S is never below 0, so this is never above it
-    auto log_prob_of = [&](float f) { return empty ? -INFINITY : (f - st.m) - log_s * kLn2; };
+    auto log_prob_of = [&](float f) { return empty ? -INFINITY : (f - st.m) - ln_s; };
     if (lane == 0) {
       if (a.log_sum_exp) a.log_sum_exp[row] = lse;
+      if (a.log_sum_exp_rest) {   // the error of the sum m + ln_s, exact
+        const float added = lse - st.m;
+        a.log_sum_exp_rest[row] = isfinite(lse) ? (st.m - (lse - added)) + (ln_s - added) : 0.f;
+      }
       if (a.entropy) a.entropy[row] = empty ? 0.f : (log_s - st.w / st.s) * kLn2;
       if (a.log_prob) a.log_prob[row] = token < 0 || token >= a.vocab ? 0.f : log_prob_of(chosen);
     }
@@ -367,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_log_probs_grad_kernel(const
   pdl_wait_prior_grids();
   const Row<T> x(static_cast<const T*>(a.logits) + row * a.vocab, a.vocab);
   T* dx = static_cast<T*>(a.d_logits) + row * a.vocab;
-  const float lse = a.log_sum_exp[row];
+  const float lse = a.log_sum_exp[row], rest = a.log_sum_exp_rest ? a.log_sum_exp_rest[row] : 0.f;
   const float g_h = a.d_entropy ? a.d_entropy[row] : 0.f, h = a.d_entropy ? a.entropy[row] : 0.f;
   const int special = 1 + a.top_k;
   if (static_cast<int>(threadIdx.x) < special) {
@@ -382,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_log_probs_grad_kernel(const
   for (int k = 0; k < special; ++k) all -= gain[k];
   const bool empty = lse == -INFINITY;   // nothing in the row is possible, and nothing changes that
   auto slope = [&](float v) {
-    const float lp = v - lse;
+    const float lp = (v - lse) - rest;
     return empty ? 0.f : exp_fast(lp) * (all - g_h * (fmaxf(lp, kFar) + h));   // an impossible token: 0 times -inf counts as 0
   };
   // this share's elements: vectors [from, to), the head in the first and the tail in the last

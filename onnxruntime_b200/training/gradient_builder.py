@@ -372,15 +372,13 @@ def _sce(b, n, dy, needs):
 def _token_log_probs(b, n, dy, needs):
     if not needs[0]:
         return
-    while len(n.outputs) < 5:                          # the backward half reads the saved sums and what was chosen
+    while len(n.outputs) < 6:                          # the backward half reads the saved sums and what was chosen
         n.outputs.append("")
-    for i, want in ((1, dy[1:2]), (3, dy[2:3]), (4, ["always"])):
+    for i, want in ((1, dy[1:2]), (3, dy[2:3]), (4, ["always"]), (5, ["always"])):
         if any(want) and not n.outputs[i]:
             n.outputs[i] = b.name("saved_log_prob")
     g = [d or "" for d in dy] + [""] * (5 - len(dy))
-    ins = [n.inputs[0], n.inputs[1], n.outputs[4], n.outputs[1] if g[1] else "", g[0], g[1], n.outputs[3] if g[2] else "", g[2], g[4]]
-    while not ins[-1]:
-        ins.pop()
+    ins = [n.inputs[0], n.inputs[1], n.outputs[4], n.outputs[1] if g[1] else "", g[0], g[1], n.outputs[3] if g[2] else "", g[2], g[4], n.outputs[5]]
     b.add_grad(n.inputs[0], b.one("TokenLogProbsGrad", ins, OWN))
 
 

@@ -5,7 +5,11 @@ import math
 import pytest
 import torch
 
-from test_serving_ops import GPU, SCORE_KINDS, score_call
+import onnxruntime_b200 as ort
+import serving_oracle as oracle
+from onnxruntime_b200 import onnx_lite as ol
+from onnxruntime_b200.training.gradient_builder import build_gradient_graph
+from test_serving_ops import FUSED, GPU, ONNX, SCORE_KINDS, half_step, score_call
 
 
 # ---------------------------------------------------------------------------------------------------- token log probabilities
@@ -116,3 +120,55 @@ def test_log_probs_of_confident_rows(kind, base):
     x = x.to(kind[1])
     got = check_rows(kind, x, tokens, 4)
     assert (got["lp"] <= 0).all() and (got["top"] <= 0).all()
+
+
+@pytest.mark.parametrize("kind", SCORE_KINDS)
+@pytest.mark.parametrize("outputs", [["lp"], ["", "h"], ["", "", "top"], ["", "", "", "", "lse"], ["lp", "h", "top", "index", "lse"]])
+@pytest.mark.parametrize("base", [0.0, 30.0, -2000.0, 60000.0, 1e7, -1e30, -math.inf])
+def test_gradient_graph_of_log_probs_far_from_zero(kind, outputs, base):
+    """The probabilities that a gradient is made of do not depend on where the logits lie (``-inf`` stands for the type's lowest value)."""
+    rows, V, k, dt = 6, 333, 3, kind[1]
+    g = torch.Generator().manual_seed(1)
+    base = torch.finfo(dt).min if base == -math.inf else base
+    if abs(base) > torch.finfo(dt).max:
+        pytest.skip("beyond the type")
+    x, tokens = base + 2 * torch.randn(rows, V, generator=g), torch.tensor([1, 332, 0, 7, -1, 200])
+    x[1] = base
+    x[2, ::3] = torch.finfo(dt).min
+    x[3] = torch.finfo(dt).min
+    x[4, 1::2] = -math.inf
+    x = x.clamp(min=torch.finfo(dt).min).to(dt) if base > -1e30 else x.double().clamp(min=torch.finfo(dt).min).to(dt)
+    x[4, 1::2] = -math.inf
+    weights = {n: torch.randn(rows, *([k] if n == "top" else []), generator=g) for n in ("lp", "h", "top", "lse")}
+    T = ol.TensorProto
+    nodes, parts = [ol.make_node("TokenLogProbs", ["x", "tokens"], outputs, domain=FUSED, top_k=k)], []
+    for o in outputs:
+        if o in weights:
+            nodes += [ol.make_node("Mul", [o, "c_" + o], [o + "_c"]), ol.make_node("ReduceSum", [o + "_c"], [o + "_sum"], keepdims=0)]
+            parts.append(o + "_sum")
+    nodes.append(ol.make_node("Sum", parts, ["loss"]))
+    info = ol.make_tensor_value_info
+    used = [o for o in outputs if o in weights]
+    graph = ol.make_graph(nodes, "g", [info("x", ONNX[dt], [rows, V]), info("tokens", T.INT64, [rows])] + [info("c_" + o, T.FLOAT, list(weights[o].shape)) for o in used],
+                          [info("loss", T.FLOAT, [])])
+    model = build_gradient_graph(ol.make_model(graph, opset=17, extra_opsets={FUSED: 1}), ["x"], "loss", recompute_fallback=False)
+    sess = ort.InferenceSession(model.serialize(), providers=[kind[0]])
+    dev = "cuda" if kind[0] == GPU else "cpu"
+    binding, dx = sess.io_binding(), torch.full((rows, V), 7.0, dtype=dt, device=dev)
+    for n, t in dict(x=x, tokens=tokens, **{"c_" + o: weights[o] for o in used}).items():
+        binding.bind_torch_input(n, t.to(dev))
+    binding.bind_torch_output("x_grad", dx)
+    binding.bind_torch_output("loss", torch.zeros((), device=dev))
+    sess.run_with_iobinding(binding)
+    c = {n: w.double() if n in used else torch.zeros_like(w).double() for n, w in weights.items()}
+    index = torch.sort(x.float(), dim=-1, descending=True, stable=True)[1][:, :k]
+    want = oracle.token_log_probs_grad(x.double(), tokens, c["lp"], c["h"], index, c["top"], c["lse"])
+    _, h, _, logp, r, _ = exact_rows(x, tokens)
+    # p carries r, and its exponent (formed from a difference, rounded three times) 2^-22 |log p|; its factor is a sum of the coefficients and, with the
+    # entropy, of |log p| + h; the result is rounded once
+    size = sum(w.abs().reshape(rows, -1).sum(1) for w in c.values())[:, None]
+    p, far = logp.exp(), logp.clamp(min=-1e4).abs()
+    off = (r[:, None] + 2.0 ** -22 * (1 + far)) * p * (size + c["h"].abs()[:, None] * (far + h[:, None]) * 2) + 2.0 ** -21 * p * size * (1 + far)
+    bound = half_step(dt) * want.abs() + off + 2.0 ** -22 * size * (want.abs() > 0) + torch.finfo(dt).tiny
+    got = dx.cpu().double()
+    assert torch.isfinite(got).all() and ((got - want).abs() <= bound).all(), "%g of the bound" % float(((got - want).abs() / bound).max())
