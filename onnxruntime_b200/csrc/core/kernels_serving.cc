@@ -158,7 +158,7 @@ void TokenLogProbsImpl(Ctx& ctx) {
   at::Tensor empty = m.eq(-inf);                                     // nothing in the row is possible
   at::Tensor from = at::where(empty, at::zeros_like(m), m), d = x - from, e = at::exp(d), s = e.sum(1, true);
   at::Tensor log_s = at::log(s), lse = at::where(empty, m, m + log_s);
-  at::Tensor w = at::where(x.eq(-inf), at::zeros_like(e), e * d).sum(1, true);
+  at::Tensor w = (e * d.clamp_min(-1000.0)).sum(1, true);             // (exp(-1000) is 0, and 0 times -inf has to count as 0)
   at::Tensor entropy = at::where(empty, at::zeros_like(s), log_s - w / s);
   at::Tensor in = tokens.ge(0).logical_and(tokens.lt(z.vocab));
   // (from the largest logit: m + log S is rounded by 2^-24 of m)
@@ -195,7 +195,7 @@ void TokenLogProbsGradImpl(Ctx& ctx) {
     all = all - top.sum(1, true);
   }
   at::Tensor dx = at::exp(lp) * all;
-  if (ctx.HasInput(5)) dx = dx - at::exp(lp) * h * (lp + column(3));
+  if (ctx.HasInput(5)) dx = dx - at::exp(lp) * h * (lp.clamp_min(-1000.0) + column(3));   // (exp(-1000) is 0: the factor needs no more than a finite value)
   dx = at::where(gone, at::zeros_like(dx), dx);
   dx = dx.scatter_add(1, at::where(in, tokens, at::zeros_like(tokens)), g);
   if (top.defined() && z.top_k > 0) dx = dx.scatter_add(1, ctx.Input(6).to(at::kLong).reshape({z.rows, z.top_k}), top);

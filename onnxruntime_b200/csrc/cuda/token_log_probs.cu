@@ -387,7 +387,8 @@ __global__ void __launch_bounds__(kThreads, 4) token_log_probs_grad_kernel(const
   const bool empty = lse == -INFINITY;   // nothing in the row is possible, and nothing changes that
   auto slope = [&](float v) {
     const float lp = (v - lse) - rest;
-    return empty ? 0.f : exp_fast(lp) * (all - g_h * (fmaxf(lp, kFar) + h));   // an impossible token: 0 times -inf counts as 0
+    // exp(-200) is 0 in 32 bits: below, the factor needs no more than a finite value (an impossible token has lp = -inf)
+    return empty ? 0.f : exp_fast(lp) * (all - g_h * (fmaxf(lp, -200.f) + h));
   };
   // this share's elements: vectors [from, to), the head in the first and the tail in the last
   const int from = static_cast<int>(static_cast<long long>(x.vectors) * part / parts), to = static_cast<int>(static_cast<long long>(x.vectors) * (part + 1) / parts);

@@ -172,3 +172,25 @@ def test_gradient_graph_of_log_probs_far_from_zero(kind, outputs, base):
     bound = half_step(dt) * want.abs() + off + 2.0 ** -22 * size * (want.abs() > 0) + torch.finfo(dt).tiny
     got = dx.cpu().double()
     assert torch.isfinite(got).all() and ((got - want).abs() <= bound).all(), "%g of the bound" % float(((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("kind", SCORE_KINDS)
+def test_log_probs_gradient_of_an_excluded_token_by_a_large_factor(kind):
+    """An impossible token has no part in the entropy, however large the entropy's gradient."""
+    x = torch.tensor([[0.0, 1.0, -math.inf, 2.0]]).to(kind[1])
+    got = score_call(kind[0], x, torch.tensor([3]), 0, dict(g_h=torch.tensor([1e9])))()["dx"]
+    want = oracle.token_log_probs_grad(x.double(), torch.tensor([3]), torch.zeros(1), torch.tensor([1e9]), torch.zeros(1, 0), torch.zeros(1, 0), torch.zeros(1))
+    assert got[0, 2] == 0
+    if kind[1] != torch.float16:
+        assert ((got.double() - want).abs() <= (half_step(kind[1]) + 2.0 ** -19) * 1e9).all()
+
+
+@pytest.mark.parametrize("kind", SCORE_KINDS)
+def test_log_probs_gradient_of_logits_as_far_apart_as_the_type_allows(kind):
+    most = torch.finfo(kind[1]).max
+    x = torch.tensor([[most, -most, 0.0, most], [-most, most, -math.inf, -most]]).to(kind[1])
+    tokens, grads = torch.tensor([0, 1]), dict(g_lp=torch.tensor([1.0, 2.0]), g_h=torch.tensor([3.0, -1.0]))
+    every = score_call(kind[0], x, tokens, 0, grads)()
+    got = every["dx"]
+    assert abs(float(every["h"][0]) - math.log(2)) < 1e-6 and every["h"][1] == 0
+    assert torch.isfinite(got).all() and (got[:, 1:3] == 0).all()      # no possible token there, or the only one
