@@ -194,3 +194,28 @@ def test_log_probs_gradient_of_logits_as_far_apart_as_the_type_allows(kind):
     got = every["dx"]
     assert abs(float(every["h"][0]) - math.log(2)) < 1e-6 and every["h"][1] == 0
     assert torch.isfinite(got).all() and (got[:, 1:3] == 0).all()      # no possible token there, or the only one
+
+
+@pytest.mark.parametrize("kind", SCORE_KINDS)
+@pytest.mark.parametrize("V,k", [(40, 12), (1031, 32), (5000, 7)])
+def test_log_probs_of_hard_rows_row_by_row(kind, V, k):
+    """Ties, zeros of both signs, impossible tokens, one certain token, steep and flat rows, rows of extreme values: each row against a bound from its
+    own differences, which a large logit of another row does not widen."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(14, V, generator=g)
+    x[0] = 0.0
+    x[1] = torch.randint(-2, 3, (V,), generator=g).float()
+    x[2, ::2], x[2, 1::2] = 0.0, -0.0
+    x[3, 1:] = -math.inf
+    x[4, :-1] = -math.inf
+    x[5, 5:] = -math.inf
+    x[6] = torch.arange(V).float()
+    x[7] = -torch.arange(V).float() - 1000
+    x[8] = -torch.finfo(torch.float16).max
+    x[9] = -torch.finfo(torch.float16).max
+    x[9, 7] = torch.finfo(torch.float16).max
+    x[10] = torch.where(torch.arange(V) % 3 == 0, -math.inf, 5.0)
+    x[11] = torch.linspace(-1e-3, 1e-3, V)
+    x[12] = torch.linspace(20, -20, V) ** 3
+    tokens = torch.tensor([0, 1, V - 1, 0, V - 1, 3, V - 1, 0, 2, 7, 4, 5, 0, 6])
+    check_rows(kind, x.to(kind[1]), tokens, k)
