@@ -54,7 +54,9 @@ __device__ __forceinline__ Span span_of(const ortb200_prefix_attn_args& a, int b
   s.past = min(max(a.past_seqlens[b], 0), cap);
   return s;
 }
-__device__ __forceinline__ int last_row(const ortb200_prefix_attn_args& a) { return min(max(a.cu_seqlens[a.B], 0), static_cast<int>(a.T)); }
+__device__ __forceinline__ int last_row(const ortb200_prefix_attn_args& a) {
+  return a.B == 0 ? 0 : min(max(a.cu_seqlens[a.B], 0), static_cast<int>(a.T));   // (without sequences there are no lengths and no table to read)
+}
 
 // Row t: rotate its query heads into `q_out` [T, N, H], its key heads into the cache beside the values.
 template <typename T>

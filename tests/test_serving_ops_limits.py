@@ -9,7 +9,7 @@ import onnxruntime_b200 as ort
 import serving_oracle as oracle
 from onnxruntime_b200 import onnx_lite as ol
 from onnxruntime_b200.training.gradient_builder import build_gradient_graph
-from test_serving_ops import FUSED, GPU, ONNX, SCORE_KINDS, half_step, score_call
+from test_serving_ops import FUSED, GPU, KINDS, ONNX, SCORE_KINDS, PrefixCase, half_step, i32, score_call
 
 
 # ---------------------------------------------------------------------------------------------------- token log probabilities
@@ -219,3 +219,19 @@ def test_log_probs_of_hard_rows_row_by_row(kind, V, k):
     x[12] = torch.linspace(20, -20, V) ** 3
     tokens = torch.tensor([0, 1, V - 1, 0, V - 1, 3, V - 1, 0, 2, 7, 4, 5, 0, 6])
     check_rows(kind, x.to(kind[1]), tokens, k)
+
+
+# ---------------------------------------------------------------------------------------------------- shared prefix attention
+def unchanged(case, got):
+    """What the caches held before the call, NaN among it, is there still."""
+    return all(torch.equal(got[n].nan_to_num(77.0), c.nan_to_num(77.0)) for n, c in zip(("kc_out", "vc_out"), case.caches))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("first", [0, 2])
+def test_prefix_without_sequences(kind, first):
+    """Tokens that no sequence has, whatever the only cumulative length says: zeros, and no access to lengths or tables that are empty."""
+    c = PrefixCase(kind[1], 4, 2, 64, 16, 20, [3], [3])
+    c.lengths, c.cum, c.table = [], i32(first), torch.zeros(0, 4, dtype=torch.int32)
+    got = c.call(kind[0])()
+    assert (got["out"] == 0).all() and unchanged(c, got)
