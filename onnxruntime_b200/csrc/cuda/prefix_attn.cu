@@ -58,6 +58,9 @@ __device__ __forceinline__ int last_row(const ortb200_prefix_attn_args& a) {
   return a.B == 0 ? 0 : min(max(a.cu_seqlens[a.B], 0), static_cast<int>(a.T));   // (without sequences there are no lengths and no table to read)
 }
 
+// Rows in front of the first sequence, and those between lengths that run backwards, are nobody's: nothing of them is cached.
+__device__ __forceinline__ bool owned(const ortb200_prefix_attn_args& a, int b, int t) { return t >= a.cu_seqlens[b] && t < a.cu_seqlens[b + 1]; }
+
 // Row t: rotate its query heads into `q_out` [T, N, H], its key heads into the cache beside the values.
 template <typename T>
 __global__ void __launch_bounds__(128) prefix_prep_kernel(const ortb200_prefix_attn_args a, T* q_out) {
@@ -65,6 +68,7 @@ __global__ void __launch_bounds__(128) prefix_prep_kernel(const ortb200_prefix_a
   pdl_wait_prior_grids();
   if (t >= last_row(a)) return;
   const int b = sequence_of(a.cu_seqlens, a.B, t);
+  if (!owned(a, b, t)) return;
   const long long place = static_cast<long long>(a.past_seqlens[b]) + (t - a.cu_seqlens[b]);
   long long slot, pos = place;
   if (a.positions) {
@@ -116,9 +120,9 @@ __global__ void __launch_bounds__(128) prefix_rows_kernel(const ortb200_prefix_a
   float o[R], qv[R], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int r = 0; r < R; ++r) o[r] = 0.f;
-  if (t < last_row(a)) {
-    const int b = sequence_of(a.cu_seqlens, a.B, t);
-    const Span s = span_of(a, b);   // (cumulative lengths that start behind 0 leave rows to nobody: no keys)
+  const int b = t < last_row(a) ? sequence_of(a.cu_seqlens, a.B, t) : -1;
+  if (b >= 0 && owned(a, b, t)) {
+    const Span s = span_of(a, b);
     const long long cap = static_cast<long long>(a.max_blocks) * a.block_size;
     const int keys = static_cast<int>(min(static_cast<long long>(s.past) + (t - s.row0) + 1, cap));
     const float scale = a.scale != 0.f ? a.scale : 1.f / sqrtf(static_cast<float>(H));
@@ -378,6 +382,7 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
     const Span sp = span_of(a, b);
     w.token[t] = make_int4(b, sp.row0, sp.rows, sp.past);
   }
+  if (!owned(a, b, t)) return;   // (its queries stay what the workspace holds; no row's result reaches another's)
   long long slot, pos;
   if (a.positions) {
     pos = a.positions[t];

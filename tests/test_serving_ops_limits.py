@@ -235,3 +235,20 @@ def test_prefix_without_sequences(kind, first):
     c.lengths, c.cum, c.table = [], i32(first), torch.zeros(0, 4, dtype=torch.int32)
     got = c.call(kind[0])()
     assert (got["out"] == 0).all() and unchanged(c, got)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("placed", [False, True])
+@pytest.mark.parametrize("H", [64, 24])
+@pytest.mark.parametrize("first", [1, 2, 40])
+def test_prefix_rows_in_front_of_the_first_sequence(kind, placed, H, first):
+    """They are nobody's, like those behind the last one: zeros, and neither the cache nor the other rows feel them, whatever their slots say."""
+    base, c = (PrefixCase(kind[1], 4, 2, H, 16, 70, [30, 5, 0], [1, 3, 12], placed=placed, seed=first, behind=2) for _ in range(2))
+    lead = torch.full((first, 4 + 2 * 2, H), math.nan, dtype=kind[1])
+    c.qkv, c.cum = torch.cat([lead, c.qkv]), c.cum + first
+    # with slots of the first sequence's oldest tokens, and a position of no table
+    c.pos = torch.cat([torch.arange(first) - 1, c.pos])
+    c.slot = torch.cat([c.table[0, 0].long() * 16 + torch.arange(first) % 16, c.slot])
+    got = c.call(kind[0])()
+    assert (got["out"][:first] == 0).all()
+    base.check(dict(got, out=got["out"][first:]))
