@@ -58,14 +58,26 @@ __device__ __forceinline__ int last_row(const ortb200_prefix_attn_args& a) {
   return a.B == 0 ? 0 : min(max(a.cu_seqlens[a.B], 0), static_cast<int>(a.T));   // (without sequences there are no lengths and no table to read)
 }
 
+// Lengths of sequence b that fit neither the batch nor the table are cut, and reported.
+__device__ __forceinline__ void check_lengths(const ortb200_prefix_attn_args& a, int b, const Span& s, int* status) {
+  const bool batch = a.cu_seqlens[b] >= 0 && a.cu_seqlens[b + 1] >= a.cu_seqlens[b] && a.cu_seqlens[b + 1] <= a.T;
+  const bool table = s.rows == 0 || (a.past_seqlens[b] == s.past && s.past + static_cast<long long>(s.rows) <= static_cast<long long>(a.max_blocks) * a.block_size);
+  if (!batch || !table) atomicExch(status, kStatusBadLength);
+}
+
 // Rows in front of the first sequence, and those between lengths that run backwards, are nobody's: nothing of them is cached.
 __device__ __forceinline__ bool owned(const ortb200_prefix_attn_args& a, int b, int t) { return t >= a.cu_seqlens[b] && t < a.cu_seqlens[b + 1]; }
 
-// Row t: rotate its query heads into `q_out` [T, N, H], its key heads into the cache beside the values.
+// CTA t: rotate row t's query heads into `q_out` [T, N, H], its key heads into the cache beside the values.
 template <typename T>
 __global__ void __launch_bounds__(128) prefix_prep_kernel(const ortb200_prefix_attn_args a, T* q_out) {
   const int t = blockIdx.x, H = a.H, heads = a.N + 2 * a.Nk, half = a.rot_dim / 2;
   pdl_wait_prior_grids();
+  if (t == a.T) {   // one more CTA for the lengths
+    if (a.status)
+      for (int b = threadIdx.x; b < a.B; b += blockDim.x) check_lengths(a, b, span_of(a, b), a.status);
+    return;
+  }
   if (t >= last_row(a)) return;
   const int b = sequence_of(a.cu_seqlens, a.B, t);
   if (!owned(a, b, t)) return;
@@ -268,13 +280,11 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
   const int promised = *a.shared_prefix, all_rows = last_row(a);
   for (int b = threadIdx.x; b < a.B; b += THREADS) {
     const Span s = span_of(a, b);
-    if (status && (a.cu_seqlens[b] < 0 || a.cu_seqlens[b + 1] < a.cu_seqlens[b] || a.cu_seqlens[b + 1] > a.T)) atomicExch(status, kStatusBadLength);
+    if (status) check_lengths(a, b, s, status);
     if (s.rows == 0) continue;
     least = min(least, s.past);
     row = min(row, b);
     several |= s.rows * G > kQT;
-    if (status && (a.past_seqlens[b] != s.past || s.past + static_cast<long long>(s.rows) > static_cast<long long>(a.max_blocks) * a.block_size))
-      atomicExch(status, kStatusBadLength);
   }
   least = __reduce_min_sync(0xffffffffu, least);
   row = __reduce_min_sync(0xffffffffu, row);
@@ -1461,7 +1471,7 @@ int launch_tc(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
 template <typename T>
 int launch_rows(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
   T* q = static_cast<T*>(a->workspace);
-  int rc = launch_kernel(prefix_prep_kernel<T>, dim3(static_cast<unsigned>(a->T)), 128, 0, stream, a->use_pdl != 0, *a, q);
+  int rc = launch_kernel(prefix_prep_kernel<T>, dim3(static_cast<unsigned>(a->T + 1)), 128, 0, stream, a->use_pdl != 0, *a, q);
   if (rc != 0) return rc;
   const long long items = a->T * a->N;
   return launch_kernel(prefix_rows_kernel<T>, dim3(static_cast<unsigned>((items + 3) / 4)), 128, 0, stream, a->use_pdl != 0, *a, static_cast<const T*>(q));
@@ -1487,7 +1497,7 @@ extern "C" int ortb200_prefix_attn(const ortb200_prefix_attn_args* a, ortb200_st
   if ((a->k != nullptr) != (a->v != nullptr) || (a->positions != nullptr) != (a->slot_mapping != nullptr)) return -1;
   if (a->block_size <= 0 || a->max_blocks <= 0 || a->num_blocks <= 0) return -1;
   if (a->cos_cache && (!a->sin_cache || a->cos_rows <= 0 || a->rot_dim <= 0 || a->rot_dim % 2 != 0 || a->rot_dim > a->H)) return -1;
-  if (a->H > kMaxHead || a->T * a->N > (a->tensor_cores ? 1ll << 29 : 0x7fffffffll)) return -2;   // (places of segment rows, doubled, pass in 32 bits)
+  if (a->H > kMaxHead || a->T * a->N > (a->tensor_cores ? 1ll << 29 : 0x7ffffffell)) return -2;   // (places of segment rows, doubled, pass in 32 bits)
   if (a->workspace_bytes < ortb200_prefix_attn_workspace_bytes(a->T, a->B, a->N, a->Nk, a->H, a->tensor_cores)) return -1;
   if (a->tensor_cores) {
     const bool blocks = a->block_size % kKT == 0 || a->block_size == 8 || a->block_size == 16 || a->block_size == 32;

@@ -8,6 +8,7 @@ import torch
 import onnxruntime_b200 as ort
 import serving_oracle as oracle
 from onnxruntime_b200 import onnx_lite as ol
+from onnxruntime_b200.capi import EPFail, InvalidArgument
 from onnxruntime_b200.training.gradient_builder import build_gradient_graph
 from test_serving_ops import FUSED, GPU, KINDS, ONNX, SCORE_KINDS, PrefixCase, half_step, i32, score_call
 
@@ -252,3 +253,18 @@ def test_prefix_rows_in_front_of_the_first_sequence(kind, placed, H, first):
     got = c.call(kind[0])()
     assert (got["out"][:first] == 0).all()
     base.check(dict(got, out=got["out"][first:]))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("form", [dict(H=64), dict(H=24), dict(H=64, size=10)])
+@pytest.mark.parametrize("cum,past", [([0, 4, 2], None), ([0, 2, 9], None), ([-1, 2, 5], None), ([0, 2, 5], [75, 190]), ([0, 2, 5], [75, -1])])
+@pytest.mark.parametrize("placed", [False, True])
+def test_prefix_lengths_that_fit_no_batch_or_table_are_an_error_in_every_form(kind, form, cum, past, placed):
+    """Cumulative lengths that run backwards, beyond the tokens or below 0, and tokens beyond the table, with slots given and without."""
+    c = PrefixCase(kind[1], 4, 2, form["H"], form.get("size", 16), 70, [5, 30], [2, 3], placed=placed)
+    c.cum = i32(*cum)
+    if past:
+        c.lengths = [(p, 1) for p in past]
+        assert max(past) > c.table.shape[1] * c.size - 3 or min(past) < 0
+    with pytest.raises((InvalidArgument, EPFail)):
+        c.call(kind[0])()
