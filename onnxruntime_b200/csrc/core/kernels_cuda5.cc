@@ -109,6 +109,7 @@ class SharedPrefixPagedAttentionKernel final : public WithGeneric {
       return;
     }
     at::Tensor out = Output(ctx, 0, {z.T, z.N * z.H}, q.scalar_type(), q);
+    if (reinterpret_cast<uintptr_t>(out.data_ptr()) & 15) out = at::empty_like(out);   // rows are written by vectors
     if (z.T > 0 && z.max_blocks == 0) out.zero_();
     if (z.T > 0 && z.max_blocks > 0) {
       at::Tensor cum = ctx.Input(5).contiguous(), past = ctx.Input(6).contiguous(), table = ctx.Input(7).contiguous(), cos, sin, pos, slot;

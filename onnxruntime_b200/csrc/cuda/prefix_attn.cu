@@ -1502,7 +1502,8 @@ extern "C" int ortb200_prefix_attn(const ortb200_prefix_attn_args* a, ortb200_st
   if (a->tensor_cores) {
     const bool blocks = a->block_size % kKT == 0 || a->block_size == 8 || a->block_size == 16 || a->block_size == 32;
     if ((a->H != 64 && a->H != 128) || !blocks || a->N / a->Nk > kQT) return -2;
-    if (((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & 15) || (reinterpret_cast<uintptr_t>(a->workspace) & 255)) return -3;
+    if ((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache) | reinterpret_cast<uintptr_t>(a->out)) & 15) return -3;
+    if (reinterpret_cast<uintptr_t>(a->workspace) & 255) return -3;
     if (a->dtype == ORTB200_BF16) return a->H == 128 ? launch_tc<__nv_bfloat16, 128>(a, stream) : launch_tc<__nv_bfloat16, 64>(a, stream);
     if (a->dtype == ORTB200_F16) return a->H == 128 ? launch_tc<__half, 128>(a, stream) : launch_tc<__half, 64>(a, stream);
     return -4;

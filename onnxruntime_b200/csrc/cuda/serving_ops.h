@@ -35,7 +35,8 @@ int ortb200_batch_layout_max_requests(void);
 // Attention of packed queries over a paged cache whose sequences share their first *shared_prefix tokens: rotary embedding and
 // cache append, then the keys of the prefix (rounded down to whole tiles of 64, cut to the shortest past) once for the rows of
 // all sequences and every sequence's own keys for its own rows, joined by their softmax maxima and sums.
-// workspace: ortb200_prefix_attn_workspace_bytes(), 256-byte aligned, any content.
+// workspace: ortb200_prefix_attn_workspace_bytes(), 256-byte aligned, any content.  With tensor_cores the caches and out are 16-byte
+// aligned.
 typedef struct {
   const void* qkv;            // [T, (N + 2 Nk) H], or queries alone [T, N H] when k and v are given
   const void* k;              // [T, Nk H]
@@ -50,7 +51,7 @@ typedef struct {
   const void* sin_cache;
   const int64_t* positions;   // [T] and
   const int64_t* slot_mapping;  // [T]: rotary position and cache slot of every row; both null: from the lengths and the table
-  void* out;                  // [T, N H]; rows behind the last sequence become 0
+  void* out;                  // [T, N H]; rows of no sequence become 0
   void* workspace;
   int64_t workspace_bytes;
   int64_t T;

@@ -1,5 +1,6 @@
 """The operators around a serving step at the ends of their ranges: masks of any size, logits far from zero, confident rows, lengths that fit no batch,
 sizes next to 32 bits, buffers on odd addresses, and the paths of the decoder that use them on a GPU."""
+import ctypes
 import math
 
 import pytest
@@ -9,6 +10,7 @@ import onnxruntime_b200 as ort
 import serving_oracle as oracle
 from onnxruntime_b200 import onnx_lite as ol
 from onnxruntime_b200.capi import EPFail, InvalidArgument
+from onnxruntime_b200.ops import _kernels as kernels
 from onnxruntime_b200.training.gradient_builder import build_gradient_graph
 from test_serving_ops import FUSED, GPU, KINDS, ONNX, SCORE_KINDS, PrefixCase, half_step, i32, score_call
 
@@ -268,3 +270,41 @@ def test_prefix_lengths_that_fit_no_batch_or_table_are_an_error_in_every_form(ki
         assert max(past) > c.table.shape[1] * c.size - 3 or min(past) < 0
     with pytest.raises((InvalidArgument, EPFail)):
         c.call(kind[0])()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("H,new", [(64, [1, 3]), (128, [1, 3]), (128, [40, 1]), (24, [1, 3])])
+@pytest.mark.parametrize("shift", [1, 2, 4])
+def test_prefix_buffers_on_odd_addresses(kind, H, new, shift):
+    """Queries and the bound result start ``shift`` elements behind an aligned address."""
+    c = PrefixCase(kind[1], 4, 2, H, 16, 70, [5, 30], new)
+    call = c.call(kind[0])
+    for n, bind in (("q", call.binding.bind_torch_input), ("out", call.binding.bind_torch_output)):
+        t = (call.ins if n == "q" else call.outs)[n]
+        moved = torch.empty(t.numel() + shift, dtype=t.dtype, device=t.device)[shift:].view(t.shape)
+        moved.copy_(t)
+        (call.ins if n == "q" else call.outs)[n] = moved
+        bind(n, moved)
+    c.check(call())
+
+
+class PrefixArgs(ctypes.Structure):
+    """ortb200_prefix_attn_args"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("qkv", "k", "v", "k_cache", "v_cache", "cu_seqlens", "past_seqlens", "block_table", "shared_prefix", "cos_cache", "sin_cache",
+                                               "positions", "slot_mapping", "out", "workspace")] + [("workspace_bytes", ctypes.c_int64), ("T", ctypes.c_int64)] + [
+        (n, ctypes.c_int) for n in ("B", "N", "Nk", "H", "block_size", "max_blocks", "num_blocks", "cos_rows", "rot_dim", "interleaved")] + [
+        ("scale", ctypes.c_float), ("softcap", ctypes.c_float)] + [(n, ctypes.c_int) for n in ("dtype", "tensor_cores", "use_pdl")] + [("status", ctypes.c_void_p)]
+
+
+def refused(name, args):
+    """What a C entry answers to arguments that it has to refuse on the host: the addresses are none, so a call that were let through would fault."""
+    if torch.cuda.is_available():
+        pytest.skip("never launched with addresses that are none")
+    return getattr(ctypes.CDLL(kernels.lib_path()), name)(ctypes.byref(args), None)
+
+
+@pytest.mark.parametrize("field", ["out", "k_cache", "v_cache", "workspace"])
+def test_prefix_c_entry_refuses_addresses_that_vectors_do_not_take(field):
+    place = {n: 1 << 20 for n in ("qkv", "k_cache", "v_cache", "cu_seqlens", "past_seqlens", "block_table", "shared_prefix", "out", "workspace")}
+    place[field] += 4
+    assert refused("ortb200_prefix_attn", PrefixArgs(**place, workspace_bytes=1 << 40, T=2, B=1, N=2, Nk=1, H=64, block_size=16, max_blocks=4, num_blocks=9, dtype=1, tensor_cores=1)) == -3
