@@ -176,7 +176,7 @@ class TokenLogProbsKernel final : public WithGeneric {
     WantOnGpu(ctx);
     at::Tensor x = ctx.Input(0).contiguous(), tokens = ctx.Input(1).to(at::kLong).contiguous();
     const int dt = DtypeCode(x.scalar_type());
-    if (dt < 0 || z.rows > 0x0fffffffll) {
+    if (dt < 0 || z.rows > 0x0fffffffll || z.vocab > ortb200_token_log_probs_max_vocab()) {
       Generic(ctx);
       return;
     }
@@ -217,7 +217,7 @@ class TokenLogProbsGradKernel final : public WithGeneric {
     WantOnGpu(ctx);
     at::Tensor x = ctx.Input(0).contiguous(), tokens = ctx.Input(1).to(at::kLong).contiguous();
     const int dt = DtypeCode(x.scalar_type());
-    if (dt < 0 || z.rows > 0x0fffffffll) {
+    if (dt < 0 || z.rows > 0x0fffffffll || z.vocab > ortb200_token_log_probs_max_vocab()) {
       Generic(ctx);
       return;
     }

@@ -88,6 +88,7 @@ typedef struct {
   int use_pdl;
 } ortb200_token_log_probs_args;
 int ortb200_token_log_probs(const ortb200_token_log_probs_args* args, ortb200_stream_t stream);
+int ortb200_token_log_probs_max_vocab(void);
 
 //   d_logits[v] = p_v (d_log_sum_exp - d_log_prob - sum_k d_top[k] - d_entropy (log p_v + entropy))
 //                 + d_log_prob [v = token] + sum_k d_top[k] [v = top_tokens[k]]

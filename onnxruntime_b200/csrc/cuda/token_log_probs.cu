@@ -18,6 +18,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256;
 constexpr int kMaxTop = 32, kMaxParts = 16;
+constexpr int kMaxVocab = 0x7fff0000;   // an index plus the threads of a CTA fits 31 bits
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float exp2_fast(float t) {   // relative error 2^-22
@@ -484,10 +485,12 @@ int launch_log_probs(const ortb200_token_log_probs_args* a, cudaStream_t stream)
 
 using namespace ortb200;
 
+extern "C" int ortb200_token_log_probs_max_vocab(void) { return kMaxVocab; }
+
 extern "C" int ortb200_token_log_probs(const ortb200_token_log_probs_args* a, ortb200_stream_t stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (!a || a->rows < 0 || a->vocab <= 0 || a->top_k < 0 || a->top_k > a->vocab) return -1;
-  if (a->top_k > kMaxTop || a->rows > 0x0fffffffll) return -2;
+  if (a->top_k > kMaxTop || a->rows > 0x0fffffffll || a->vocab > kMaxVocab) return -2;
   if (a->rows == 0) return 0;
   if (!a->logits || !a->tokens) return -1;
   switch (a->dtype) {
@@ -503,7 +506,7 @@ extern "C" int ortb200_token_log_probs_grad(const ortb200_token_log_probs_grad_a
   if (!a_) return -1;
   ortb200_token_log_probs_grad_args a = *a_;
   if (a.rows < 0 || a.vocab <= 0 || a.top_k < 0 || a.top_k > a.vocab) return -1;
-  if (a.top_k > kMaxTop || a.rows > 0x0fffffffll) return -2;
+  if (a.top_k > kMaxTop || a.rows > 0x0fffffffll || a.vocab > kMaxVocab) return -2;
   if (a.rows == 0) return 0;
   if (!a.logits || !a.tokens || !a.log_sum_exp || !a.d_logits || (a.d_entropy && !a.entropy) || (a.d_top_log_probs && !a.top_tokens)) return -1;
   if (!a.d_top_log_probs) a.top_k = 0;

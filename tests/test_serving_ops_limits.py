@@ -308,3 +308,22 @@ def test_prefix_c_entry_refuses_addresses_that_vectors_do_not_take(field):
     place = {n: 1 << 20 for n in ("qkv", "k_cache", "v_cache", "cu_seqlens", "past_seqlens", "block_table", "shared_prefix", "out", "workspace")}
     place[field] += 4
     assert refused("ortb200_prefix_attn", PrefixArgs(**place, workspace_bytes=1 << 40, T=2, B=1, N=2, Nk=1, H=64, block_size=16, max_blocks=4, num_blocks=9, dtype=1, tensor_cores=1)) == -3
+
+
+# ------------------------------------------------------------------------------------------------------ sizes next to 32 bits
+class LogProbsArgs(ctypes.Structure):
+    """ortb200_token_log_probs_args"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "tokens", "log_prob", "entropy", "log_sum_exp", "top_log_probs", "top_tokens", "log_sum_exp_rest")] + [
+        ("rows", ctypes.c_int64)] + [(n, ctypes.c_int) for n in ("vocab", "top_k", "dtype", "use_pdl")]
+
+
+class LogProbsGradArgs(ctypes.Structure):
+    """ortb200_token_log_probs_grad_args"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "tokens", "log_sum_exp", "entropy", "d_log_prob", "d_entropy", "top_tokens", "d_top_log_probs", "d_log_sum_exp",
+                                               "log_sum_exp_rest", "d_logits")] + [("rows", ctypes.c_int64)] + [(n, ctypes.c_int) for n in ("vocab", "top_k", "dtype", "use_pdl")]
+
+
+@pytest.mark.parametrize("name,args", [("ortb200_token_log_probs", LogProbsArgs), ("ortb200_token_log_probs_grad", LogProbsGradArgs)])
+def test_log_probs_c_entry_refuses_vocabularies_next_to_32_bits(name, args):
+    place = {n: 1 << 20 for n, t in args._fields_ if t is ctypes.c_void_p}
+    assert refused(name, args(**place, rows=1, vocab=2 ** 31 - 1, top_k=0, dtype=1)) == -2
