@@ -65,7 +65,7 @@ class PagedBatchLayoutKernel final : public WithGeneric {
   void Compute(Ctx& ctx) const override {
     const BatchLayoutSizes z = CheckBatchLayout(ctx);
     WantOnGpu(ctx);
-    if (z.B > ortb200_batch_layout_max_requests()) {
+    if (z.B > ortb200_batch_layout_max_requests() || z.rows > ortb200_batch_layout_max_rows()) {
       Generic(ctx);
       return;
     }

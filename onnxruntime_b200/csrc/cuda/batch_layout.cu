@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxRequests = 16384;   // 8 bytes of shared memory each
+constexpr long long kMaxRows = 0x7ff00000;   // a row or block plus the threads of the grid fits 31 bits
 
 // (past and new each fit 31 bits: their sum fits 32)
 __device__ __forceinline__ long long blocks_of(long long tokens, int s) {
@@ -188,6 +189,7 @@ __global__ void __launch_bounds__(kThreads) batch_layout_kernel(const ortb200_ba
 using namespace ortb200;
 
 extern "C" int ortb200_batch_layout_max_requests(void) { return kMaxRequests; }
+extern "C" int64_t ortb200_batch_layout_max_rows(void) { return kMaxRows; }
 
 extern "C" int ortb200_batch_layout(const ortb200_batch_layout_args* a, ortb200_stream_t stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
@@ -195,7 +197,7 @@ extern "C" int ortb200_batch_layout(const ortb200_batch_layout_args* a, ortb200_
   if (a->B > 0 && (!a->past_seqlens || !a->new_tokens || (a->max_blocks > 0 && (!a->table_in || !a->table_out)))) return -1;
   if (a->rows > 0 && (!a->positions || !a->slot_mapping)) return -1;
   if (a->num_free > 0 && !a->free_blocks) return -1;
-  if (a->B > kMaxRequests || a->rows > 0x7fffffffll) return -2;
+  if (a->B > kMaxRequests || a->rows > kMaxRows) return -2;
   const int smem = 8 * (a->B + 1);
   if (smem > 47 * 1024) {   // (the kernel has some shared memory of its own, which counts towards the 48 KB that need no leave)
     if (cudaFuncSetAttribute(batch_layout_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * (kMaxRequests + 1)) != cudaSuccess) return -10;

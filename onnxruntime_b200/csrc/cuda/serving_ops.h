@@ -31,6 +31,7 @@ typedef struct {
 } ortb200_batch_layout_args;
 int ortb200_batch_layout(const ortb200_batch_layout_args* args, ortb200_stream_t stream);
 int ortb200_batch_layout_max_requests(void);
+int64_t ortb200_batch_layout_max_rows(void);
 
 // Attention of packed queries over a paged cache whose sequences share their first *shared_prefix tokens: rotary embedding and
 // cache append, then the keys of the prefix (rounded down to whole tiles of 64, cut to the shortest past) once for the rows of

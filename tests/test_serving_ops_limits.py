@@ -327,3 +327,14 @@ class LogProbsGradArgs(ctypes.Structure):
 def test_log_probs_c_entry_refuses_vocabularies_next_to_32_bits(name, args):
     place = {n: 1 << 20 for n, t in args._fields_ if t is ctypes.c_void_p}
     assert refused(name, args(**place, rows=1, vocab=2 ** 31 - 1, top_k=0, dtype=1)) == -2
+
+
+class LayoutArgs(ctypes.Structure):
+    """ortb200_batch_layout_args"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("past_seqlens", "new_tokens", "table_in", "free_blocks", "table_out", "cum", "positions", "slot_mapping", "blocks_used")] + [
+        (n, ctypes.c_int) for n in ("B", "max_blocks", "block_size")] + [("num_free", ctypes.c_int64), ("rows", ctypes.c_int64)]
+
+
+def test_layout_c_entry_refuses_rows_next_to_32_bits():
+    place = {n: 1 << 20 for n, t in LayoutArgs._fields_ if t is ctypes.c_void_p}
+    assert refused("ortb200_batch_layout", LayoutArgs(**place, B=1, max_blocks=2 ** 31 - 1, block_size=1, num_free=2 ** 31 - 1, rows=2 ** 31 - 1)) == -2
