@@ -104,7 +104,8 @@ class SharedPrefixPagedAttentionKernel final : public WithGeneric {
     at::Tensor q = ctx.Input(0).contiguous(), k, v;
     const at::Tensor &kc = ctx.Input(3), &vc = ctx.Input(4);
     const int dt = DtypeCode(q.scalar_type());
-    if (dt < 0 || z.H > 256 || z.T * z.N > 0x7ffffffell || !kc.is_contiguous() || !vc.is_contiguous()) {
+    const bool wide = z.max_blocks * z.block_size > ortb200_prefix_attn_max_keys() || (z.N + 2 * z.Nk) * z.H > 0x7fffffffll || z.T * z.N > 0x7ffffffell;
+    if (dt < 0 || z.H > 256 || wide || !kc.is_contiguous() || !vc.is_contiguous()) {
       Generic(ctx);
       return;
     }

@@ -41,6 +41,7 @@ namespace ortb200 {
 namespace {
 
 constexpr int kMaxHead = 256;
+constexpr long long kMaxKeys = 0x7fff0000;
 
 // Lengths of sequence b, cut to what the buffers hold: rows [row0, row0 + rows) of the batch, keys [0, past + rows) of the cache.
 struct Span {
@@ -1482,6 +1483,8 @@ int launch_rows(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
 
 using namespace ortb200;
 
+extern "C" int64_t ortb200_prefix_attn_max_keys(void) { return kMaxKeys; }
+
 extern "C" int64_t ortb200_prefix_attn_workspace_bytes(int64_t T, int B, int N, int Nk, int H, int tensor_cores) {
   if (T < 0 || B < 0 || N <= 0 || Nk <= 0 || H <= 0) return -1;
   if (!tensor_cores) return up256(T * N * H * 4);
@@ -1498,6 +1501,8 @@ extern "C" int ortb200_prefix_attn(const ortb200_prefix_attn_args* a, ortb200_st
   if (a->block_size <= 0 || a->max_blocks <= 0 || a->num_blocks <= 0) return -1;
   if (a->cos_cache && (!a->sin_cache || a->cos_rows <= 0 || a->rot_dim <= 0 || a->rot_dim % 2 != 0 || a->rot_dim > a->H)) return -1;
   if (a->H > kMaxHead || a->T * a->N > (a->tensor_cores ? 1ll << 29 : 0x7ffffffell)) return -2;   // (places of segment rows, doubled, pass in 32 bits)
+  // what a sequence may hold, and the width of a token, pass in 32 bits
+  if (static_cast<long long>(a->max_blocks) * a->block_size > kMaxKeys || (a->N + 2ll * a->Nk) * a->H > 0x7fffffffll) return -2;
   if (a->workspace_bytes < ortb200_prefix_attn_workspace_bytes(a->T, a->B, a->N, a->Nk, a->H, a->tensor_cores)) return -1;
   if (a->tensor_cores) {
     const bool blocks = a->block_size % kKT == 0 || a->block_size == 8 || a->block_size == 16 || a->block_size == 32;

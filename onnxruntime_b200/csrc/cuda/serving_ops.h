@@ -67,6 +67,7 @@ typedef struct {
   int* status;
 } ortb200_prefix_attn_args;
 int ortb200_prefix_attn(const ortb200_prefix_attn_args* args, ortb200_stream_t stream);
+int64_t ortb200_prefix_attn_max_keys(void);   // of a sequence: max_blocks x block_size
 int64_t ortb200_prefix_attn_workspace_bytes(int64_t T, int B, int N, int Nk, int H, int tensor_cores);
 
 // Row by row over logits x [rows, vocab], with m the largest and S = sum exp(x - m):

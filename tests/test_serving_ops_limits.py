@@ -338,3 +338,11 @@ class LayoutArgs(ctypes.Structure):
 def test_layout_c_entry_refuses_rows_next_to_32_bits():
     place = {n: 1 << 20 for n, t in LayoutArgs._fields_ if t is ctypes.c_void_p}
     assert refused("ortb200_batch_layout", LayoutArgs(**place, B=1, max_blocks=2 ** 31 - 1, block_size=1, num_free=2 ** 31 - 1, rows=2 ** 31 - 1)) == -2
+
+
+@pytest.mark.parametrize("sizes", [dict(max_blocks=2 ** 23, block_size=256, N=2, Nk=1), dict(max_blocks=4, block_size=16, N=2 ** 25, Nk=1)])
+@pytest.mark.parametrize("tensor_cores", [0, 1])
+def test_prefix_c_entry_refuses_sizes_next_to_32_bits(sizes, tensor_cores):
+    """A table for 2^31 tokens of a sequence, and a token of 2^31 elements."""
+    place = {n: 1 << 20 for n in ("qkv", "k_cache", "v_cache", "cu_seqlens", "past_seqlens", "block_table", "shared_prefix", "out", "workspace")}
+    assert refused("ortb200_prefix_attn", PrefixArgs(**place, workspace_bytes=1 << 60, T=2, B=1, H=64, num_blocks=9, dtype=1, tensor_cores=tensor_cores, **sizes)) == -2
