@@ -85,6 +85,7 @@ class PagedBatchLayoutKernel final : public WithGeneric {
     a.blocks_used = used.data_ptr<int>();
     a.B = static_cast<int>(z.B); a.max_blocks = static_cast<int>(z.max_blocks); a.block_size = static_cast<int>(z.block_size);
     a.num_free = z.num_free; a.rows = z.rows;
+    a.status = z.strict ? ctx.session()->StatusWord().data_ptr<int>() : nullptr;
     CheckLaunch(ortb200_batch_layout(&a, ctx.cuda_stream()), "ortb200_batch_layout");
     ctx.session()->AddLaunches(1);
     ctx.SetOutput(0, table);

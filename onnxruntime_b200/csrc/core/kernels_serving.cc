@@ -50,6 +50,8 @@ void PagedBatchLayoutImpl(Ctx& ctx) {
   }
   if (refused < 4 && tokens > z.rows) refused = 3;
   if (refused < 2 && blocks > z.num_free) refused = 1;
+  ORTB_ENFORCE_ARG(!refused || !z.strict, "PagedBatchLayout: the batch cannot be laid out (", -refused, ": ",
+                   refused == 1 ? "too few free blocks" : refused == 2 ? "the table is too narrow" : refused == 3 ? "more tokens than rows" : "a negative length", ")");
   if (!refused) {
     int* tb = table.data_ptr<int>();
     int64_t row = 0, next = 0;
@@ -210,6 +212,7 @@ BatchLayoutSizes CheckBatchLayout(Ctx& ctx) {
   const char* op = "PagedBatchLayout";
   z.block_size = ctx.node().attr_i("block_size", 0);
   ORTB_ENFORCE_ARG(z.block_size > 0 && z.block_size <= (1 << 30), op, ": block_size must be positive");
+  z.strict = ctx.node().attr_i("strict", 0) != 0;
   WantInts(ctx, 0, at::kInt, 1, "past_seqlens");
   WantInts(ctx, 1, at::kInt, 1, "new_tokens");
   WantInts(ctx, 2, at::kInt, 2, "block_table");

@@ -20,6 +20,7 @@ SharedPrefixSizes CheckSharedPrefix(OpKernelContext& ctx);
 // com.ortb200 PagedBatchLayout: past_seqlens, new_tokens, block_table, free_blocks, rows
 struct BatchLayoutSizes {
   int64_t B = 0, max_blocks = 0, num_free = 0, rows = 0, block_size = 0;
+  bool strict = false;   // a batch that cannot be laid out is an error of the run, not of `blocks_used` alone
 };
 BatchLayoutSizes CheckBatchLayout(OpKernelContext& ctx);
 

@@ -104,7 +104,10 @@ __global__ void __launch_bounds__(kThreads) batch_layout_kernel(const ortb200_ba
   __syncthreads();
 
   const long long tid = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x, stride = static_cast<long long>(gridDim.x) * kThreads;
-  if (tid == 0) a.blocks_used[0] = refused ? -refused : static_cast<int>(all_b);
+  if (tid == 0) {
+    a.blocks_used[0] = refused ? -refused : static_cast<int>(all_b);
+    if (refused && a.status) atomicExch(a.status, kStatusBadLength);
+  }
   for (long long b = tid; b <= a.B; b += stride) a.cum[b] = refused ? 0 : cum[b];
   const int end = refused ? 0 : cum[a.B];
   for (long long t = tid; t < a.rows; t += stride) {

@@ -15,7 +15,7 @@ extern "C" {
 //   cum[b] = sum of new over the requests before b; row t of request b: position past_b + t - cum[b], slot = block * s + offset
 // Rows behind the last request get position and slot -1.  blocks_used: the sum of need, or, when the batch cannot be laid out,
 // -1 (too few free blocks), -2 (the table is too narrow), -3 (more tokens than rows) or -4 (a negative length): then the table
-// stays as it was, cum is 0 and every position and slot -1.
+// stays as it was, cum is 0 and every position and slot -1, and the status word, if there is one, says so too.
 typedef struct {
   const int* past_seqlens;    // [B]
   const int* new_tokens;      // [B]
@@ -28,6 +28,7 @@ typedef struct {
   int* blocks_used;           // [1]
   int B, max_blocks, block_size;
   int64_t num_free, rows;
+  int* status;                // null: blocks_used alone reports a refusal
 } ortb200_batch_layout_args;
 int ortb200_batch_layout(const ortb200_batch_layout_args* args, ortb200_stream_t stream);
 int ortb200_batch_layout_max_requests(void);

@@ -238,7 +238,7 @@ def build_llama(cfg: LlamaConfig, tp_rank: int = 0, tp_size: int = 1, external_w
             inputs += [ol.make_tensor_value_info("free_blocks", T.INT32, ["free"]), ol.make_tensor_value_info("shared_prefix", T.INT32, [1])]
             nodes.append(ol.make_node("PagedBatchLayout", ["past_seqlens", "new_tokens", "block_table", "free_blocks", "input_ids"],
                                       ["block_table_out", "cumulative_sequence_length", "positions", "slot_mapping", "blocks_used"],
-                                      name="layout", domain="com.ortb200", block_size=block_size))
+                                      name="layout", domain="com.ortb200", block_size=block_size, strict=1))
     else:
         inputs = [
             ol.make_tensor_value_info("input_ids", T.INT64, ["batch", "seq"]),

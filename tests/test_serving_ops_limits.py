@@ -12,7 +12,7 @@ from onnxruntime_b200 import onnx_lite as ol
 from onnxruntime_b200.capi import EPFail, InvalidArgument
 from onnxruntime_b200.ops import _kernels as kernels
 from onnxruntime_b200.training.gradient_builder import build_gradient_graph
-from test_serving_ops import FUSED, GPU, KINDS, ONNX, SCORE_KINDS, PrefixCase, half_step, i32, score_call
+from test_serving_ops import FUSED, GPU, KINDS, ONNX, PROVIDERS, SCORE_KINDS, Call, PrefixCase, half_step, i32, score_call
 
 
 # ---------------------------------------------------------------------------------------------------- token log probabilities
@@ -332,7 +332,7 @@ def test_log_probs_c_entry_refuses_vocabularies_next_to_32_bits(name, args):
 class LayoutArgs(ctypes.Structure):
     """ortb200_batch_layout_args"""
     _fields_ = [(n, ctypes.c_void_p) for n in ("past_seqlens", "new_tokens", "table_in", "free_blocks", "table_out", "cum", "positions", "slot_mapping", "blocks_used")] + [
-        (n, ctypes.c_int) for n in ("B", "max_blocks", "block_size")] + [("num_free", ctypes.c_int64), ("rows", ctypes.c_int64)]
+        (n, ctypes.c_int) for n in ("B", "max_blocks", "block_size")] + [("num_free", ctypes.c_int64), ("rows", ctypes.c_int64), ("status", ctypes.c_void_p)]
 
 
 def test_layout_c_entry_refuses_rows_next_to_32_bits():
@@ -346,3 +346,32 @@ def test_prefix_c_entry_refuses_sizes_next_to_32_bits(sizes, tensor_cores):
     """A table for 2^31 tokens of a sequence, and a token of 2^31 elements."""
     place = {n: 1 << 20 for n in ("qkv", "k_cache", "v_cache", "cu_seqlens", "past_seqlens", "block_table", "shared_prefix", "out", "workspace")}
     assert refused("ortb200_prefix_attn", PrefixArgs(**place, workspace_bytes=1 << 60, T=2, B=1, H=64, num_blocks=9, dtype=1, tensor_cores=tensor_cores, **sizes)) == -2
+
+
+# --------------------------------------------------------------------------------------------------------------- refused layouts
+LAYOUT_REFUSALS = [([4, 9], [1, 4], 1, 5), ([4, 29], [1, 4], 9, 5), ([4, 9], [1, 4], 9, 4), ([4, -1], [1, 4], 9, 5)]   # blocks, table, rows, a negative length
+
+
+@pytest.mark.parametrize("provider", PROVIDERS)
+@pytest.mark.parametrize("past,new,free,rows", LAYOUT_REFUSALS)
+def test_strict_layout_makes_a_refusal_an_error(provider, past, new, free, rows):
+    table = torch.arange(16, dtype=torch.int32).reshape(2, 8)
+    ins = dict(past=i32(*past), new=i32(*new), table=table, free=i32(*range(50, 50 + free)), rows=torch.zeros(rows, dtype=torch.int64))
+    outs = dict(block_table=table, cum=i32(0, 0, 0), positions=torch.zeros(rows, dtype=torch.int64), slots=torch.zeros(rows, dtype=torch.int64), used=i32(7))
+    call = Call(provider, [("PagedBatchLayout", list(ins), list(outs), dict(block_size=4, strict=1))], ins, outs)
+    with pytest.raises((InvalidArgument, EPFail)):
+        call()
+    call.ins["past"].copy_(i32(4, 9))
+    call.binding.bind_torch_input("new", i32(1, 1).to(call.ins["new"].device))
+    assert call()["used"].tolist() == [1]            # 4 and 9 tokens in blocks of 4: the first one enters a block; the session goes on
+
+
+@pytest.mark.parametrize("provider", PROVIDERS)
+def test_a_decoder_step_whose_layout_is_refused_is_an_error(provider):
+    """The shared-prefix form of the decoder with fewer blocks than its tokens need: not logits out of attention to nothing."""
+    from test_shared_prefix_generation import decoders
+    shared = decoders(provider, 16, 2, 64)[2]
+    shared._granted = lambda seqs, new: []
+    with pytest.raises((InvalidArgument, EPFail)):
+        shared.step([(0, [1, 2, 3], [2]), (1, [4], [0])])
+        shared.sess.check_device_status()
