@@ -63,7 +63,7 @@ constexpr float kFar = -1e30f;   // an exponent below all that count: 0 times it
 
 // m the largest logit, s = sum 2^t, w = sum 2^t t with t = (x - m) log2(e).  The difference comes first: the maximum's own exponent is
 // 0 whatever its size.  (One multiply-add x log2(e) - m log2(e) is off by 2^-24 of |m|, which for masks of -1e10 and beyond is more
-// than a 32-bit exponent holds; it took 592 instead of 601 us for 4096 rows of 128256 bf16 logits and their gradient.)  Two logits go
+// than a 32-bit exponent holds; it took 592 us instead of 601 in a call for 4096 rows of 128256 bf16 logits and their gradient.)  Two logits go
 // through one instruction.
 struct Stats {
   float m, s, w;
@@ -210,8 +210,8 @@ __device__ __forceinline__ unsigned kth_of_threads(Shared& sm, float top, int tu
 // A cluster of CTAs per row, each with a share of its vectors; the first CTA puts the shares together over distributed shared memory.
 //
 // Without alternatives the row is one stream: 2000 rows of 50257 fp32 logits take 70 us (402 MB, 61 at the copy rate), 2000 of bf16
-// 50 (201 MB, 31: the exponentials, 16 a clock and SM, take 27 by themselves), 6 rows of 128256 bf16 4.6, which is latency: begin, one
-// round of loads, two barriers of the cluster.  With the best 1 / 5 / 20: 84 / 96 / 136, 70 / 85 / 124 and 7.5 / 9.0 / 16 us.  What costs
+// 52 (201 MB, 31: the exponentials, 16 a clock and SM, take 27 by themselves), 6 rows of 128256 bf16 4.8, which is latency: begin, one
+// round of loads, two barriers of the cluster.  With the best 1 / 5 / 20: 84 / 98 / 139, 71 / 88 / 125 and 7.6 / 9.1 / 16 us.  What costs
 // there is not the insertions alone: bounds from one warp each (110 us for bf16 with one alternative), lists merged one by
 // one (13 us for 6 rows with five) and ranks counted among all 256 threads' values (120) were slower.
 template <typename T, bool TOP>
@@ -360,8 +360,8 @@ __global__ void __launch_bounds__(kThreads, TOP && sizeof(T) == 4 ? 3 : 4) token
 // gradient may lie over the logits), and their elements written once more at the end.
 //
 // d x_i = p_i (sum of what does not go to single tokens - d_entropy (log p_i + entropy)) + what goes to token i.  A stream of one read
-// and one write: 4096 rows of 128256 bf16 logits take 354 us (2.1 GB, 321 at the copy rate), 300 of 32000 fp16 10 us, of
-// which beginning and ending are half.  Both kernels together 568 us, 1673 when they went element by element.
+// and one write: 4096 rows of 128256 bf16 logits take 356 us (2.1 GB, 321 at the copy rate), 300 of 32000 fp16 10 us, of
+// which beginning and ending are half.  Both kernels together 561 us, 1673 when they went element by element.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) token_log_probs_grad_kernel(const ortb200_token_log_probs_grad_args a, int parts) {
   constexpr int E = Row<T>::E, U = 2;

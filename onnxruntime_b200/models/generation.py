@@ -228,7 +228,7 @@ class PagedDecoderRunner:
 
     def _bind(self, binding, ids, cum, past, table, slots, key_starts, rows, logits, nxt, free=None, shared=None, used=None) -> None:
         binding.bind_torch_input("input_ids", ids)
-        if self.has_layout:      # `cum` holds the new tokens of every sequence, the table is extended in place
+        if self.has_layout:      # `cum` holds the new tokens of every sequence; the extended table goes where the table is
             binding.bind_torch_input("new_tokens", cum)
             binding.bind_torch_input("free_blocks", free)
             binding.bind_torch_input("shared_prefix", shared)
