@@ -143,7 +143,10 @@ __global__ void __launch_bounds__(128) prefix_rows_kernel(const ortb200_prefix_a
     for (int r = 0; r < R; ++r) qv[r] = r * 32 + lane < H ? to_float<T>(q[item * H + r * 32 + lane]) : 0.f;
     for (int j = 0; j < keys; ++j) {
       const int block = a.block_table[static_cast<long long>(b) * a.max_blocks + j / a.block_size];
-      if (block < 0 || block >= a.num_blocks) continue;
+      if (block < 0 || block >= a.num_blocks) {
+        if (lane == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
+        continue;
+      }
       const long long at = ((static_cast<long long>(block) * a.block_size + j % a.block_size) * a.Nk + kvh) * H;
       float dot = 0.f;
 #pragma unroll
@@ -953,7 +956,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     int s = 0, k_tiles = 0, v_tiles = 0;
     uint32_t parity = 1;   // the first round over the stages waits for nothing
     QueryPlace qp;
-    bool waited = !kept;
+    bool waited = !kept, outside = false;
     auto wait_step1 = [&]() {
       if (waited) return;
       pdl_wait_prior_grids();
@@ -979,7 +982,12 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         return true;
       };
       bool q_asked = false;
-      auto block_at = [&](int key) { return min(max(table[min(key / a.block_size, a.max_blocks - 1)], 0), a.num_blocks - 1); };
+      // behind the unit's last key the table may hold anything; in front of it a block outside the cache is reported
+      auto block_at = [&](int key) {
+        const int named = table[min(key / a.block_size, a.max_blocks - 1)], block = min(max(named, 0), a.num_blocks - 1);
+        outside |= named != block && key < g.end;
+        return block;
+      };
       int block = lane < pieces ? block_at(g.key0 + lane * piece) : 0;
       for (int t = 0; t < g.tiles; ++t) {
         const int key = g.key0 + t * kKT + lane * piece, in_block = key % a.block_size;
@@ -1015,6 +1023,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       if (k > 0 && !wait_warp(&bars[BAR_K_FULL + i], (k - 1) & 1)) ok = false;
       if (v > 0 && !wait_warp(&bars[BAR_V_FULL + i], (v - 1) & 1)) ok = false;
     }
+    if (outside && a.status) atomicExch(a.status, kStatusBadArgument);
     if (!ok && lane == 0 && a.status) atomicExch(a.status, kStatusTimeoutProducer);
   } else if (warp == 1) {
     // ------------------------------------------------------------------------------------------------- products

@@ -375,3 +375,22 @@ def test_a_decoder_step_whose_layout_is_refused_is_an_error(provider):
     with pytest.raises((InvalidArgument, EPFail)):
         shared.step([(0, [1, 2, 3], [2]), (1, [4], [0])])
         shared.sess.check_device_status()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("form", [dict(), dict(H=24), dict(H=128, new=[40, 1]), dict(size=10), dict(size=128, H=128)])
+@pytest.mark.parametrize("bad", [-1, 10 ** 6])
+@pytest.mark.parametrize("placed", [False, True])
+def test_prefix_blocks_outside_the_cache(kind, form, bad, placed):
+    """Where a sequence has tokens they are an error, be it in the prefix or in its own keys; behind its end they may be anything."""
+    size, H, new = form.get("size", 16), form.get("H", 64), form.get("new", [2, 3])
+    make = lambda: PrefixCase(kind[1], 4, 2, H, size, 70, [5, 130], new, placed=placed)  # noqa: E731
+    c = make()
+    for b, (past, n) in enumerate(c.lengths):
+        c.table[b, oracle.blocks_of(past + n, size):] = bad
+    c.run(kind[0])
+    for b, column in ((0, 0), (1, (70 + 129) // size)):
+        c = make()
+        c.table[b, column] = bad
+        with pytest.raises((InvalidArgument, EPFail)):
+            c.call(kind[0])()
