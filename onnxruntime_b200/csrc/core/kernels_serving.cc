@@ -129,7 +129,7 @@ void SharedPrefixPagedAttentionImpl(Ctx& ctx) {
                      "SharedPrefixPagedAttention: the table of sequence ", b, " names a block outside the cache");
     for (int64_t s = 0; s < S; ++s) {
       const int64_t p = pl + s, slot = z.placed ? given_slot[t0 + s].item<int64_t>() : blocks[p / z.block_size].item<int64_t>() * z.block_size + p % z.block_size;
-      if (slot < 0 || slot >= z.num_blocks * z.block_size) continue;
+      ORTB_ENFORCE_ARG(slot >= 0 && slot < z.num_blocks * z.block_size, "SharedPrefixPagedAttention: the slot of a token of sequence ", b, " lies outside the cache");
       kc[slot / z.block_size][slot % z.block_size].copy_(kb[s]);
       vc[slot / z.block_size][slot % z.block_size].copy_(vb[s]);
     }

@@ -394,3 +394,23 @@ def test_prefix_blocks_outside_the_cache(kind, form, bad, placed):
         c.table[b, column] = bad
         with pytest.raises((InvalidArgument, EPFail)):
             c.call(kind[0])()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("H", [64, 24])
+@pytest.mark.parametrize("slot", [-1, 10 ** 7])
+def test_prefix_slots_outside_the_cache_are_an_error(kind, H, slot):
+    c = PrefixCase(kind[1], 4, 2, H, 16, 70, [5, 30], [2, 3])
+    c.slot[3] = slot
+    with pytest.raises((InvalidArgument, EPFail)):
+        c.call(kind[0])()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("H", [64, 24])
+@pytest.mark.parametrize("position", [-1, 10 ** 7])
+def test_prefix_positions_outside_the_rotary_tables_are_an_error(kind, H, position):
+    c = PrefixCase(kind[1], 4, 2, H, 16, 70, [5, 30], [2, 3])
+    c.pos[3] = position
+    with pytest.raises((InvalidArgument, EPFail)):
+        c.call(kind[0])()
