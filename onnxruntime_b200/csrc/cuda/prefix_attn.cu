@@ -21,7 +21,7 @@
 // again to do as the formula because weights count as two 16-bit values; a tile of 128 rows and 64 keys takes 768 clocks of it and
 // a CTA is done with one in 2000 to 2500, two CTAs side by side; 512 clocks of exponentials per tile run beside it.  284 us in all on
 // one GPU, of which the product kernel has 234 and the join 37, and up to 330 on others, whose clocks settle lower.  Single tokens behind a long prefix: segments and their hand-overs; 180 sequences of 16
-// heads of 64 behind 20011 tokens take 114 us, 64 of 64 heads of 128 behind 8192 tokens 64 us, where the bytes need 37 and 23.
+// heads of 64 behind 20011 tokens take 117 us, 64 of 64 heads of 128 behind 8192 tokens 61 to 63 us, where the bytes need 37 and 23.
 // Slower, each against the form of its time at (180 behind 20011, 64 behind 8192): 128-key tiles with one score buffer 164 and 82 us
 // instead of 149 and 70; eight softmax warps with half a row each 150 and 80; rows held four times with a quarter of the keys to each
 // warp 162 and 78; the next tiles asked into L2 ahead of their loads 198 and 81 instead of 132 and 65; one thread for loads and
