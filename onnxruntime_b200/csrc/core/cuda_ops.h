@@ -41,5 +41,6 @@ void RegisterMoreCudaKernels(KernelRegistry& r);
 void RegisterCudaKernels3(KernelRegistry& r);
 void RegisterCudaKernels4(KernelRegistry& r);
 void RegisterCudaKernels5(KernelRegistry& r);
+void RegisterCudaKernels6(KernelRegistry& r);
 
 }  // namespace ortb

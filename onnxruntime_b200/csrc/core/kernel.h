@@ -202,6 +202,7 @@ void RegisterControlFlowKernels(KernelRegistry& r);
 void RegisterCollectiveKernels(KernelRegistry& r);
 void RegisterHybridKernels(KernelRegistry& r);
 void RegisterServingKernels(KernelRegistry& r);
+void RegisterDraftKernels(KernelRegistry& r);
 void RegisterCudaKernels(KernelRegistry& r);
 void EnsureKernelsRegistered();
 

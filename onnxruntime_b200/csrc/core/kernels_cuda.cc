@@ -533,6 +533,7 @@ void RegisterCudaKernels(KernelRegistry& r) {
   RegisterCudaKernels3(r);
   RegisterCudaKernels4(r);
   RegisterCudaKernels5(r);
+  RegisterCudaKernels6(r);
 }
 
 }  // namespace ortb

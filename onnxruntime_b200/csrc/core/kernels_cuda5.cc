@@ -7,6 +7,7 @@
 #include "cuda_ops.h"
 #include "kernel.h"
 #include "serving_checks.h"
+#include "serving_cuda.h"
 #include "serving_ops.h"
 #include "session.h"
 
@@ -15,49 +16,6 @@ namespace ortb {
 namespace {
 
 using Ctx = OpKernelContext;
-constexpr const char* FUSED = "com.ortb200";
-
-int DtypeCode(at::ScalarType t) {
-  return t == at::kHalf ? ORTB200_F16 : t == at::kBFloat16 ? ORTB200_BF16 : t == at::kFloat ? ORTB200_F32 : -1;
-}
-int Pdl(Ctx& ctx) { return ctx.session()->config().Get("ortb200.pdl", "0") == "1" ? 1 : 0; }
-
-// The bound buffer of output i where it fits and is none of the inputs (but `in_place`), else a new tensor, which the executor
-// copies to whatever is bound.
-at::Tensor Output(Ctx& ctx, int i, at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like, int in_place = -1) {
-  if (i < ctx.OutputCount()) {
-    const at::Tensor& b = ctx.Preallocated(i);
-    if (b.defined() && b.device() == like.device() && b.scalar_type() == type && b.sizes() == sizes && b.is_contiguous()) {
-      bool apart = true;
-      for (int j = 0; j < ctx.InputCount(); ++j)
-        if (ctx.HasInput(j) && ctx.Input(j).is_alias_of(b) && !(j == in_place && ctx.Input(j).data_ptr() == b.data_ptr())) apart = false;
-      for (int j = 0; j < i; ++j)
-        if (ctx.Preallocated(j).defined() && ctx.Preallocated(j).is_alias_of(b)) apart = false;
-      if (apart) return b;
-    }
-  }
-  return at::empty(sizes, like.options().dtype(type));
-}
-
-// Operands that the kernels do not take run on the device-agnostic kernel.
-class WithGeneric : public OpKernel {
- public:
-  explicit WithGeneric(const OpKernelInfo& info) : OpKernel(info) {
-    if (const KernelDef* d = KernelRegistry::Generic().Find(info.node, info.graph)) generic_ = d->factory(info);
-  }
-
- protected:
-  void Generic(Ctx& ctx) const {
-    if (!generic_) ORTB_THROW(NOT_IMPLEMENTED, "no other kernel for ", node_.op_type);
-    generic_->Compute(ctx);
-  }
-  std::unique_ptr<OpKernel> generic_;
-};
-
-void WantOnGpu(Ctx& ctx) {
-  for (int i = 0; i < ctx.InputCount(); ++i)
-    ORTB_ENFORCE_ARG(!ctx.HasInput(i) || ctx.Input(i).device() == ctx.device(), ctx.node().op_type, ": input ", i, " must lie on the session's GPU");
-}
 
 class PagedBatchLayoutKernel final : public WithGeneric {
  public:
@@ -256,22 +214,13 @@ class TokenLogProbsGradKernel final : public WithGeneric {
   }
 };
 
-template <typename K>
-void Reg(KernelRegistry& r, const std::string& op) {
-  KernelDef d;
-  d.domain = FUSED;
-  d.op_type = op;
-  d.factory = [](const OpKernelInfo& info) { return std::make_unique<K>(info); };
-  r.Register(std::move(d));
-}
-
 }  // namespace
 
 void RegisterCudaKernels5(KernelRegistry& r) {
-  Reg<PagedBatchLayoutKernel>(r, "PagedBatchLayout");
-  Reg<SharedPrefixPagedAttentionKernel>(r, "SharedPrefixPagedAttention");
-  Reg<TokenLogProbsKernel>(r, "TokenLogProbs");
-  Reg<TokenLogProbsGradKernel>(r, "TokenLogProbsGrad");
+  RegFused<PagedBatchLayoutKernel>(r, "PagedBatchLayout");
+  RegFused<SharedPrefixPagedAttentionKernel>(r, "SharedPrefixPagedAttention");
+  RegFused<TokenLogProbsKernel>(r, "TokenLogProbs");
+  RegFused<TokenLogProbsGradKernel>(r, "TokenLogProbsGrad");
 }
 
 }  // namespace ortb

@@ -1,6 +1,6 @@
 // com.ortb200 operators around one step of a serving batch, device-agnostic versions (tensor library): PagedBatchLayout (block
 // table, positions and cache slots out of request lengths), SharedPrefixPagedAttention (sequences that begin with the same
-// tokens), TokenLogProbs and TokenLogProbsGrad (log probabilities, entropy and alternatives, and their gradient).  The GPU
+// tokens), TreePagedAttention (sequences that bring a tree of drafted tokens), TokenLogProbs and TokenLogProbsGrad (log probabilities, entropy and alternatives, and their gradient).  The GPU
 // provider has its own kernels (kernels_cuda5.cc).
 #include <ATen/ATen.h>
 
@@ -75,9 +75,29 @@ void PagedBatchLayoutImpl(Ctx& ctx) {
   ctx.SetOutput(4, used.to(dev));
 }
 
+// Of the rows of a sequence: which ones each sees, [S, S], and how deep each lies; undefined where the rows form a prompt.
+std::pair<at::Tensor, at::Tensor> TreeOf(const std::vector<int64_t>& parents, int64_t t0, int64_t S, int64_t b) {
+  for (int64_t i = 0; i < S; ++i) {
+    const int64_t p = parents[t0 + i];
+    ORTB_ENFORCE_ARG(p >= -1 && p < i && (S <= kMostTreeNodes || p == i - 1), "TreePagedAttention: the parent of row ", i, " of sequence ", b,
+                     S > kMostTreeNodes ? " must be the row before it: the sequence has more rows than a tree" : " must be a row in front of it, or -1");
+  }
+  if (S > kMostTreeNodes) return {};
+  at::Tensor sees = at::zeros({S, S}, at::kBool), depth = at::zeros({S}, at::kLong);
+  for (int64_t i = 0; i < S; ++i) {
+    const int64_t p = parents[t0 + i];
+    if (p >= 0) {
+      sees[i].copy_(sees[p]);
+      depth.data_ptr<int64_t>()[i] = depth.data_ptr<int64_t>()[p] + 1;
+    }
+    sees.data_ptr<bool>()[i * S + i] = true;
+  }
+  return {sees, depth};
+}
+
 // The promise about the first tokens changes nothing here: every sequence reads its own row of the table.
-void SharedPrefixPagedAttentionImpl(Ctx& ctx) {
-  const SharedPrefixSizes z = CheckSharedPrefix(ctx);
+void PagedQueries(Ctx& ctx, const SharedPrefixSizes& z) {
+  const std::string& op = ctx.node().op_type;
   at::Tensor q = ctx.Input(0), k, v;
   at::Tensor kc = ctx.Input(3), vc = ctx.Input(4);
   if (z.packed) {
@@ -93,6 +113,7 @@ void SharedPrefixPagedAttentionImpl(Ctx& ctx) {
   v = v.reshape({z.T, z.Nk, z.H});
   const std::vector<int64_t> cum = HostInts(ctx.Input(5)), past = HostInts(ctx.Input(6));
   const at::Tensor table = ctx.Input(7).to(at::kCPU, at::kLong);
+  const std::vector<int64_t> parents = z.tree ? HostInts(ctx.Input(8)) : std::vector<int64_t>();
   at::Tensor given_pos, given_slot;
   if (z.placed) {
     given_pos = ctx.Input(11).to(at::kCPU);
@@ -117,19 +138,21 @@ void SharedPrefixPagedAttentionImpl(Ctx& ctx) {
   for (int64_t b = 0; b < z.B; ++b) {
     const int64_t t0 = cum[b], S = cum[b + 1] - t0, pl = past[b], L = pl + S;
     ORTB_ENFORCE_ARG(t0 >= 0 && S >= 0 && t0 + S <= z.T && pl >= 0 && (S == 0 || L <= z.max_blocks * z.block_size),
-                     "SharedPrefixPagedAttention: lengths of sequence ", b, " do not fit the batch or the block table");
+                     op, ": lengths of sequence ", b, " do not fit the batch or the block table");
     if (S == 0) continue;
-    at::Tensor pos = z.placed ? given_pos.narrow(0, t0, S) : at::arange(S, at::kLong) + pl;
+    std::pair<at::Tensor, at::Tensor> tree;
+    if (z.tree) tree = TreeOf(parents, t0, S, b);
+    at::Tensor pos = z.placed ? given_pos.narrow(0, t0, S) : (tree.second.defined() ? tree.second : at::arange(S, at::kLong)) + pl;
     ORTB_ENFORCE_ARG(!z.rotary || (pos.min().item<int64_t>() >= 0 && pos.max().item<int64_t>() < ctx.Input(9).size(0)),
-                     "SharedPrefixPagedAttention: a position of sequence ", b, " lies outside the rotary tables");
+                     op, ": a position of sequence ", b, " lies outside the rotary tables");
     at::Tensor qb = rotate(q.narrow(0, t0, S), pos), kb = rotate(k.narrow(0, t0, S), pos), vb = v.narrow(0, t0, S);
     const int64_t nblk = BlocksOf(L, z.block_size);
     at::Tensor blocks = table[b].narrow(0, 0, nblk);
     ORTB_ENFORCE_ARG(blocks.min().item<int64_t>() >= 0 && blocks.max().item<int64_t>() < z.num_blocks,
-                     "SharedPrefixPagedAttention: the table of sequence ", b, " names a block outside the cache");
+                     op, ": the table of sequence ", b, " names a block outside the cache");
     for (int64_t s = 0; s < S; ++s) {
       const int64_t p = pl + s, slot = z.placed ? given_slot[t0 + s].item<int64_t>() : blocks[p / z.block_size].item<int64_t>() * z.block_size + p % z.block_size;
-      ORTB_ENFORCE_ARG(slot >= 0 && slot < z.num_blocks * z.block_size, "SharedPrefixPagedAttention: the slot of a token of sequence ", b, " lies outside the cache");
+      ORTB_ENFORCE_ARG(slot >= 0 && slot < z.num_blocks * z.block_size, op, ": the slot of a token of sequence ", b, " lies outside the cache");
       kc[slot / z.block_size][slot % z.block_size].copy_(kb[s]);
       vc[slot / z.block_size][slot % z.block_size].copy_(vb[s]);
     }
@@ -140,13 +163,18 @@ void SharedPrefixPagedAttentionImpl(Ctx& ctx) {
     at::Tensor s = at::matmul(F32(qb).permute({1, 0, 2}), gather(kc).transpose(1, 2)) * scale;   // [N, S, L]
     if (z.softcap > 0.f) s = at::tanh(s / z.softcap) * z.softcap;
     at::Tensor qpos = (at::arange(S, s.options().dtype(at::kLong)) + pl).unsqueeze(1), kpos = at::arange(L, s.options().dtype(at::kLong)).unsqueeze(0);
-    s = s.masked_fill(kpos.gt(qpos).unsqueeze(0), -std::numeric_limits<float>::infinity());
+    at::Tensor hidden = kpos.gt(qpos);
+    if (tree.first.defined()) hidden.narrow(1, pl, S).copy_(tree.first.logical_not());
+    s = s.masked_fill(hidden.unsqueeze(0), -std::numeric_limits<float>::infinity());
     out.narrow(0, t0, S).copy_(at::matmul(at::softmax(s, -1), gather(vc)).permute({1, 0, 2}));
   }
   ctx.SetOutput(0, out.reshape({z.T, z.N * z.H}));
   if (ctx.OutputCount() > 1) ctx.SetOutput(1, kc);
   if (ctx.OutputCount() > 2) ctx.SetOutput(2, vc);
 }
+
+void SharedPrefixPagedAttentionImpl(Ctx& ctx) { PagedQueries(ctx, CheckSharedPrefix(ctx)); }
+void TreePagedAttentionImpl(Ctx& ctx) { PagedQueries(ctx, CheckTreeAttention(ctx)); }
 
 at::Tensor WideLogits(const at::Tensor& x, const TokenLogProbsSizes& z) {
   return (x.scalar_type() == at::kDouble ? x : F32(x)).reshape({z.rows, z.vocab});
@@ -228,10 +256,11 @@ BatchLayoutSizes CheckBatchLayout(Ctx& ctx) {
   return z;
 }
 
-SharedPrefixSizes CheckSharedPrefix(Ctx& ctx) {
+namespace {
+SharedPrefixSizes PagedQuerySizes(Ctx& ctx, const char* no_window) {
   SharedPrefixSizes z;
   const Node& n = ctx.node();
-  const char* op = "SharedPrefixPagedAttention";
+  const std::string& op = n.op_type;
   z.N = n.attr_i("num_heads", 0);
   z.Nk = n.attr_i("kv_num_heads", 0);
   z.scale = n.attr_f("scale", 0.f);
@@ -239,7 +268,7 @@ SharedPrefixSizes CheckSharedPrefix(Ctx& ctx) {
   z.rotary = n.attr_i("do_rotary", 0) != 0;
   z.interleaved = n.attr_i("rotary_interleaved", 0) != 0;
   const at::Tensor &q = ctx.RequiredInput(0), &kc = ctx.RequiredInput(3), &vc = ctx.RequiredInput(4);
-  ORTB_ENFORCE_ARG(n.attr_i("local_window_size", -1) <= 0, op, ": a window excludes the shared tokens; use PagedAttention");
+  ORTB_ENFORCE_ARG(n.attr_i("local_window_size", -1) <= 0, op, no_window);
   ORTB_ENFORCE_ARG(z.N > 0 && z.Nk > 0 && z.N % z.Nk == 0, op, ": num_heads must be a multiple of kv_num_heads");
   ORTB_ENFORCE_ARG(z.softcap >= 0.f && std::isfinite(z.softcap), op, ": softcap must be finite and not negative");
   ORTB_ENFORCE_ARG(z.scale >= 0.f && std::isfinite(z.scale), op, ": scale must be finite and not negative");
@@ -263,12 +292,10 @@ SharedPrefixSizes CheckSharedPrefix(Ctx& ctx) {
   WantInts(ctx, 5, at::kInt, 1, "cumulative_sequence_length");
   WantInts(ctx, 6, at::kInt, 1, "past_seqlens");
   WantInts(ctx, 7, at::kInt, 2, "block_table");
-  WantInts(ctx, 8, at::kInt, -1, "shared_prefix");
   z.B = ctx.Input(6).size(0);
   z.max_blocks = ctx.Input(7).size(1);
   ORTB_ENFORCE_ARG(ctx.Input(5).size(0) == z.B + 1 && ctx.Input(7).size(0) == z.B, op, ": lengths and block table disagree about the number of sequences");
   ORTB_ENFORCE_ARG(z.T == 0 || z.B == 0 || z.max_blocks > 0, op, ": a block table without columns");
-  ORTB_ENFORCE_ARG(ctx.Input(8).numel() == 1, op, ": shared_prefix is one number");
   if (z.rotary) {
     const at::Tensor &c = ctx.RequiredInput(9), &s = ctx.RequiredInput(10);
     ORTB_ENFORCE_ARG(c.dim() == 2 && c.sizes() == s.sizes() && c.size(0) > 0 && c.size(1) > 0 && 2 * c.size(1) <= z.H && c.scalar_type() == q.scalar_type() &&
@@ -276,6 +303,23 @@ SharedPrefixSizes CheckSharedPrefix(Ctx& ctx) {
                      op, ": the rotary tables must be [positions, up to ", z.H / 2, "] of the query's type");
     z.rot_dim = 2 * c.size(1);
   }
+  return z;
+}
+}  // namespace
+
+SharedPrefixSizes CheckTreeAttention(Ctx& ctx) {
+  SharedPrefixSizes z = PagedQuerySizes(ctx, ": no window is known for trees; use PagedAttention");
+  WantInts(ctx, 8, at::kInt, 1, "parents");
+  ORTB_ENFORCE_ARG(ctx.Input(8).size(0) == z.T, "TreePagedAttention: parents have one entry per token");
+  z.tree = true;
+  return z;
+}
+
+SharedPrefixSizes CheckSharedPrefix(Ctx& ctx) {
+  const char* op = "SharedPrefixPagedAttention";
+  SharedPrefixSizes z = PagedQuerySizes(ctx, ": a window excludes the shared tokens; use PagedAttention");
+  WantInts(ctx, 8, at::kInt, -1, "shared_prefix");
+  ORTB_ENFORCE_ARG(ctx.Input(8).numel() == 1, op, ": shared_prefix is one number");
   z.placed = ctx.HasInput(11);
   ORTB_ENFORCE_ARG(z.placed == ctx.HasInput(12), op, ": positions and slot_mapping come together");
   for (int i : {11, 12})
@@ -329,6 +373,7 @@ TokenLogProbsSizes CheckTokenLogProbsGrad(Ctx& ctx) {
 void RegisterServingKernels(KernelRegistry& r) {
   r.RegisterFn(FUSED, "PagedBatchLayout", 1, kMax, PagedBatchLayoutImpl);
   r.RegisterFn(FUSED, "SharedPrefixPagedAttention", 1, kMax, SharedPrefixPagedAttentionImpl);
+  r.RegisterFn(FUSED, "TreePagedAttention", 1, kMax, TreePagedAttentionImpl);
   r.RegisterFn(FUSED, "TokenLogProbs", 1, kMax, TokenLogProbsImpl);
   r.RegisterFn(FUSED, "TokenLogProbsGrad", 1, kMax, TokenLogProbsGradImpl);
 }

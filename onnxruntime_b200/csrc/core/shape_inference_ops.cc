@@ -689,7 +689,7 @@ void RegisterBuiltinSchemas(std::map<std::string, OpSchema>& t) {
       if (c.Rank(4) >= 1) c.SetOutput(i, pb::INT64, {c.Dims(4)[0]});
     c.SetOutput(4, pb::INT32, {Known(1)});
   });
-  Reg(t, FUSED, "SharedPrefixPagedAttention", 9, 13, [](Ctx& c) {
+  const auto paged_queries = [](Ctx& c) {
     if (!c.HasShape(0) || c.Rank(0) != 2) return;
     Dims out = c.Dims(0);
     const int64_t N = c.node.attr_i("num_heads", 0), Nk = c.node.attr_i("kv_num_heads", 0);
@@ -697,6 +697,14 @@ void RegisterBuiltinSchemas(std::map<std::string, OpSchema>& t) {
     c.SetOutput(0, c.ElemType(0), out);
     c.PassThrough(3, 1);
     c.PassThrough(4, 2);
+  };
+  Reg(t, FUSED, "SharedPrefixPagedAttention", 9, 13, paged_queries);
+  Reg(t, FUSED, "TreePagedAttention", 9, 11, paged_queries);
+  Reg(t, FUSED, "PagedCacheMove", 3, 1 << 20, [](Ctx& c) {
+    for (size_t i = 2; i < c.node.inputs.size(); ++i) c.PassThrough(i, i - 2);
+  });
+  Reg(t, FUSED, "ProcessLogits", 1, 15, [](Ctx& c) {
+    if (c.HasShape(0)) c.SetOutput(0, pb::FLOAT, c.Dims(0));
   });
   Reg(t, FUSED, "TokenLogProbs", 2, 2, [](Ctx& c) {
     if (c.Rank(0) < 1) return;

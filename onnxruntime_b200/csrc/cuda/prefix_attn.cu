@@ -3,6 +3,10 @@
 // softmax(q K^T) V splits over any partition of the keys: with m the largest score of a part, l = sum exp(s - m) and
 // o = sum exp(s - m) v, two parts join as m = max(m1, m2), l = l1 e^(m1 - m) + l2 e^(m2 - m), o likewise; the result is o / l.
 //
+// Drafted tokens (com.ortb200.TreePagedAttention): the new rows of a sequence form a tree, in which a row sees its ancestors and itself beside
+// the cache.  Parents lie in front of their children, so that a tree is the causal mask with some of its bits taken out: all that
+// follows stays, and the tiles that hold new keys take a row's bits, which step 1 has worked out, instead of a bound.
+//
 // Step 1 rotates the queries and the new keys and appends keys and values to the cache; step 2 attends; step 3 joins the parts.
 //
 // Tensor-core form.  A unit of work is a tile of up to 128 query rows (a row is one token and one of the G query heads that
@@ -33,8 +37,8 @@
 #include <algorithm>
 #include <type_traits>
 #include "attn_internal.h"
+#include "draft_ops.h"
 #include "launch_util.cuh"
-#include "serving_ops.h"
 #include "tensor_map.h"
 
 namespace ortb200 {
@@ -69,9 +73,39 @@ __device__ __forceinline__ void check_lengths(const ortb200_prefix_attn_args& a,
 // Rows in front of the first sequence, and those between lengths that run backwards, are nobody's: nothing of them is cached.
 __device__ __forceinline__ bool owned(const ortb200_prefix_attn_args& a, int b, int t) { return t >= a.cu_seqlens[b] && t < a.cu_seqlens[b + 1]; }
 
+// Trees of drafted tokens: the rows of a sequence that a row sees, as bits, which step 1 works out.
+constexpr int kTreeWords = 8, kTreeNodes = 32 * kTreeWords;
+// All threads of row t's CTA, row i of the `rows` of its sequence: writes the row's bits, returns how deep it lies.  The walk from
+// parent to parent goes through shared memory; trees are a few levels deep.
+__device__ __forceinline__ int tree_row(const int* parents, int row0, int rows, int i, uint32_t* ancestors, int* status, bool write) {
+  __shared__ int parent_sm[kTreeNodes], depth_sm;
+  if (rows > kTreeNodes) {   // no tree: every row behind the one before it
+    if (threadIdx.x == 0 && status && parents[row0 + i] != i - 1) atomicExch(status, kStatusBadArgument);
+    return i;
+  }
+  for (int j = threadIdx.x; j <= i; j += blockDim.x) {
+    const int p = parents[row0 + j];
+    const bool none = p < -1 || p >= j;
+    if (none && j == i && status) atomicExch(status, kStatusBadArgument);
+    parent_sm[j] = none ? -1 : p;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {   // every lane walks, lane w keeps word w
+    uint32_t bits = 0;
+    int depth = -1;
+    for (int j = i; j >= 0; j = parent_sm[j], ++depth)
+      if (j >> 5 == static_cast<int>(threadIdx.x)) bits |= 1u << (j & 31);
+    if (write && threadIdx.x < kTreeWords) ancestors[threadIdx.x] = bits;
+    if (threadIdx.x == 0) depth_sm = depth;
+  }
+  __syncthreads();
+  return depth_sm;
+}
+__device__ __forceinline__ bool tree_sees(const uint32_t* ancestors, int j) { return j < kTreeNodes && (__ldcg(ancestors + (j >> 5)) >> (j & 31) & 1); }
+
 // CTA t: rotate row t's query heads into `q_out` [T, N, H], its key heads into the cache beside the values.
 template <typename T>
-__global__ void __launch_bounds__(128) prefix_prep_kernel(const ortb200_prefix_attn_args a, T* q_out) {
+__global__ void __launch_bounds__(128) prefix_prep_kernel(const ortb200_prefix_attn_args a, T* q_out, const int* parents, uint32_t* ancestors) {
   const int t = blockIdx.x, H = a.H, heads = a.N + 2 * a.Nk, half = a.rot_dim / 2;
   pdl_wait_prior_grids();
   if (t == a.T) {   // one more CTA for the lengths
@@ -90,6 +124,10 @@ __global__ void __launch_bounds__(128) prefix_prep_kernel(const ortb200_prefix_a
   } else {
     const long long j = place / a.block_size;
     slot = place >= 0 && j < a.max_blocks ? static_cast<long long>(a.block_table[static_cast<long long>(b) * a.max_blocks + j]) * a.block_size + place % a.block_size : -1;
+  }
+  if (parents) {
+    const Span s = span_of(a, b);
+    pos += tree_row(parents, s.row0, s.rows, t - s.row0, ancestors + static_cast<long long>(t) * kTreeWords, a.status, true) - (t - s.row0);
   }
   const bool keep = slot >= 0 && slot < static_cast<long long>(a.num_blocks) * a.block_size;
   if (!keep && threadIdx.x == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
@@ -122,7 +160,7 @@ __global__ void __launch_bounds__(128) prefix_prep_kernel(const ortb200_prefix_a
 // One warp per row and query head, any type and any head size up to 256: lane i holds the elements i, i + 32, ... of the head.
 // It reads the table row of its own sequence, which names the shared blocks too.
 template <typename T>
-__global__ void __launch_bounds__(128) prefix_rows_kernel(const ortb200_prefix_attn_args a, const T* q) {
+__global__ void __launch_bounds__(128) prefix_rows_kernel(const ortb200_prefix_attn_args a, const T* q, const uint32_t* ancestors) {
   constexpr int R = kMaxHead / 32;
   const int lane = threadIdx.x & 31, H = a.H;
   const long long item = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
@@ -141,7 +179,9 @@ __global__ void __launch_bounds__(128) prefix_rows_kernel(const ortb200_prefix_a
     const float scale = a.scale != 0.f ? a.scale : 1.f / sqrtf(static_cast<float>(H));
 #pragma unroll
     for (int r = 0; r < R; ++r) qv[r] = r * 32 + lane < H ? to_float<T>(q[item * H + r * 32 + lane]) : 0.f;
+    const bool tree = ancestors && s.rows <= kTreeNodes;
     for (int j = 0; j < keys; ++j) {
+      if (tree && j >= s.past && !tree_sees(ancestors + static_cast<long long>(t) * kTreeWords, j - s.past)) continue;
       const int block = a.block_table[static_cast<long long>(b) * a.max_blocks + j / a.block_size];
       if (block < 0 || block >= a.num_blocks) {
         if (lane == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
@@ -196,6 +236,7 @@ struct Work {            // the workspace's parts
   long long* first;      // [row tiles of all sequences + 1]: where the own units of each start, behind the prefix's
   int* tile0;            // [B + 1]: which of those row tiles are a sequence's
   int4* token;           // [T]: the token's sequence, that sequence's first row, rows and past
+  uint32_t* ancestors;   // [T, 8]: trees only
   uint16_t* q;           // [Nk, T G, H]
   float2* ml;            // per row of a segment: m (in units of log 2) and l
   float* o;              // per row of a segment: H values
@@ -207,6 +248,8 @@ __host__ __device__ inline long long plan_bytes(long long T, int B, int N, int N
   return up256(sizeof(Plan) + 8 * (most_row_tiles(T, B, N, Nk) + 1) + 4ll * (B + 1));
 }
 __host__ __device__ inline long long segment_rows(long long T, int N) { return 2 * T * N + static_cast<long long>(kGrid) * kQT; }
+__host__ __device__ inline long long tree_bytes(long long T) { return up256(T * kTreeWords * 4); }
+template <bool TREE>
 __host__ __device__ inline Work work_of(const ortb200_prefix_attn_args& a) {
   char* p = static_cast<char*>(a.workspace);
   Work w;
@@ -216,6 +259,8 @@ __host__ __device__ inline Work work_of(const ortb200_prefix_attn_args& a) {
   p += plan_bytes(a.T, a.B, a.N, a.Nk);
   w.token = reinterpret_cast<int4*>(p);
   p += up256(a.T * 16);
+  w.ancestors = reinterpret_cast<uint32_t*>(p);
+  if (TREE) p += tree_bytes(a.T);
   w.q = reinterpret_cast<uint16_t*>(p);
   p += up256(a.T * a.N * a.H * 2);
   w.ml = reinterpret_cast<float2*>(p);
@@ -281,7 +326,7 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
   __shared__ int tiles_sm[THREADS / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.N / a.Nk;
   int least = 0x7fffffff, row = 0x7fffffff, several = 0;
-  const int promised = *a.shared_prefix, all_rows = last_row(a);
+  const int promised = a.shared_prefix ? *a.shared_prefix : 0, all_rows = last_row(a);
   for (int b = threadIdx.x; b < a.B; b += THREADS) {
     const Span s = span_of(a, b);
     if (status) check_lengths(a, b, s, status);
@@ -378,9 +423,9 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
 
 // Step 1: one CTA (or, for few tokens, several) per token and one more for the plan.  VEC: whole heads rotated in halves or not
 // at all, every address a multiple of 16 bytes: a thread moves 2 x 16 bytes; otherwise one element.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefix_attn_args a) {
-  const Work w = work_of(a);
+template <typename T, bool VEC, bool TREE>
+__global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefix_attn_args a, const int* parents) {
+  const Work w = work_of<TREE>(a);
   pdl_wait_prior_grids();
   pdl_launch_dependents();   // behind the wait: when step 2 begins, everything in front of this step has ended
   if (blockIdx.x == a.T) {
@@ -405,6 +450,10 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
     pos = static_cast<long long>(a.past_seqlens[b]) + (t - a.cu_seqlens[b]);
     const long long j = pos / a.block_size;
     slot = pos >= 0 && j < a.max_blocks ? static_cast<long long>(a.block_table[static_cast<long long>(b) * a.max_blocks + j]) * a.block_size + pos % a.block_size : -1;
+  }
+  if (TREE) {
+    const Span s = span_of(a, b);
+    pos += tree_row(parents, s.row0, s.rows, t - s.row0, w.ancestors + static_cast<long long>(t) * kTreeWords, a.status, blockIdx.y == 0) - (t - s.row0);
   }
   const bool keep = slot >= 0 && slot < static_cast<long long>(a.num_blocks) * a.block_size;
   if (!keep && threadIdx.x == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
@@ -490,6 +539,7 @@ struct Segment {
   int key0, end;         // first key of the segment, end of the unit's keys
   int past, in_seq;      // own units: tokens in front of the sequence's rows, first row of the unit among the sequence's rows x G
   int table_row;
+  bool tree;             // own units: new keys are seen by the rows' bits
   long long slot;
 };
 // The segments of a CTA one after the other: its first unit is searched for, the others follow from the one before.
@@ -541,6 +591,7 @@ struct Walk {
     unit.end = tiles * kKT;
     unit.past = unit.in_seq = 0;
     unit.table_row = prefix_row;
+    unit.tree = false;
     unit.slot = prefix_slot(a, rt, 0, unit.rows);
   }
   __device__ void own_unit() {
@@ -553,6 +604,7 @@ struct Walk {
     unit.key0 = prefix_tiles * kKT;
     unit.end = own_end(a, G, s, rt);
     unit.past = s.past;
+    unit.tree = s.rows <= kTreeNodes;
     unit.slot = own_slot(a, G, s.row0, rt, 0, unit.rows);
   }
   __device__ void step() {   // to the next unit that has tiles; there is one while places are left
@@ -753,7 +805,7 @@ __device__ __forceinline__ float sum_over_keys(float x) {
 // S, softmax and O with its hand-overs; so each of the four warps multiplies a quarter of a tile's keys itself, keys and dims as
 // the 16 rows of a product and the queries as its 8 columns: S^T = K Q^T, O^T += V^T P^T.  A warp has its own running maximum and
 // sums; they meet once per segment, in the place of the queries.
-template <int HD, bool BF16, int CAP>
+template <int HD, bool BF16, int CAP, bool TREE>
 __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, const Work& w, const Segment& g, uint8_t* smem, uint64_t* bars, float2 (*part)[kFew],
                                          const QueryPlace& qp, float scale, int qw, int lane, int& stage, uint32_t& parity, int& few_tiles, int few_segments, bool& ok) {
   using L = TcSmem<HD>;
@@ -797,6 +849,15 @@ __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, cons
       if (key >= seen1) c[1] = -INFINITY;
       if (key + 8 >= seen0) c[2] = -INFINITY;
       if (key + 8 >= seen1) c[3] = -INFINITY;
+      if (TREE && g.tree && first + 16 > g.past) {   // (rows behind the unit's last take its bits)
+        const uint32_t* bits0 = w.ancestors + static_cast<long long>((g.q_row + min(n0, g.rows - 1)) / G) * kTreeWords;
+        const uint32_t* bits1 = w.ancestors + static_cast<long long>((g.q_row + min(n0 + 1, g.rows - 1)) / G) * kTreeWords;
+        const int j = key - g.past;
+        if (j >= 0 && !tree_sees(bits0, j)) c[0] = -INFINITY;
+        if (j >= 0 && !tree_sees(bits1, j)) c[1] = -INFINITY;
+        if (j + 8 >= 0 && !tree_sees(bits0, j + 8)) c[2] = -INFINITY;
+        if (j + 8 >= 0 && !tree_sees(bits1, j + 8)) c[3] = -INFINITY;
+      }
       float t0 = fmaxf(c[0], c[2]) * fs, t1 = fmaxf(c[1], c[3]) * fs;
       if (__any_sync(0xffffffffu, t0 > m0 + kRaise || t1 > m1 + kRaise)) {
         t0 = max_over_keys(t0);
@@ -903,7 +964,7 @@ __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, cons
   if (lane == 0) mbar_arrive(&bars[BAR_FEW_END + (few_segments & 1)]);
 }
 
-template <int HD, bool BF16, int CAP>
+template <int HD, bool BF16, int CAP, bool TREE>
 __global__ void __launch_bounds__(kThreads, 2)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                    const ortb200_prefix_attn_args a, const float scale) {
@@ -931,7 +992,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   }
   // Step 1 has begun when this step begins, and what came before has ended: lengths, table and old cache entries may be read at
   // once.  Only the loading warp waits for step 1, in front of the first query or new key that it fetches.
-  const Work w = work_of(a);
+  const Work w = work_of<TREE>(a);
   Plan plan;
   const bool kept = most_row_tiles(a.T, a.B, a.N, a.Nk) <= kPlanInSmem;
   if (kept) {
@@ -1110,7 +1171,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     while (walk.next(g)) {   // to the end even when a wait gave up: the four warps meet at barriers
       qp.take(g.rows);
       if (g.rows <= kFew) {
-        few_rows<HD, BF16, CAP>(a, w, g, smem, bars, part, qp, scale, qw, lane, stage, parity, few_tiles, few_segments, ok);
+        few_rows<HD, BF16, CAP, TREE>(a, w, g, smem, bars, part, qp, scale, qw, lane, stage, parity, few_tiles, few_segments, ok);
         ++few_segments;
         qp.done();
         continue;
@@ -1137,7 +1198,15 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 #pragma unroll
             for (int j = 0; j < kKT; ++j) sv[j] = cap(sv[j]);
           }
-          if (key0 + kKT > g.end || key0 + kKT - 1 > first_pos) {
+          if (TREE && g.tree && key0 + kKT > g.past) {   // 64 of the row's bits, the cache's all set (rows behind the unit's last take its bits)
+            const uint32_t* bits = w.ancestors + static_cast<long long>((g.q_row + min(r, g.rows - 1)) / G) * kTreeWords;
+            const int lo = key0 - g.past, w0 = lo >> 5;
+            auto word = [&](int i) { return i < 0 ? 0xffffffffu : i < kTreeWords ? __ldcg(bits + i) : 0u; };
+            const uint32_t b0 = word(w0), b1 = word(w0 + 1), b2 = word(w0 + 2);
+            const uint32_t low = __funnelshift_r(b0, b1, lo & 31), high = __funnelshift_r(b1, b2, lo & 31);
+#pragma unroll
+            for (int j = 0; j < kKT; ++j) sv[j] = (j < 32 ? low >> j : high >> (j - 32)) & 1 ? sv[j] : -INFINITY;
+          } else if (key0 + kKT > g.end || key0 + kKT - 1 > first_pos) {
             const int hi = min(g.end - key0, pos - key0 + 1);   // keys of this tile that the row sees
 #pragma unroll
             for (int j = 0; j < kKT; ++j) sv[j] = j < hi ? sv[j] : -INFINITY;
@@ -1263,7 +1332,7 @@ __device__ __forceinline__ void load_cg(const float* p, float* v) {
 // Step 3: a warp joins `per` neighbouring rows of a key head (32 at most).  Each lane looks one row's sequence up; where the
 // segments of a unit are is worked out once for all of its rows.  SPLIT: few rows, whose segments may be hundreds; the four warps of
 // a CTA share one row's.
-template <typename T, int HD, bool SPLIT>
+template <typename T, int HD, bool SPLIT, bool TREE>
 __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_attn_args a, const int per) {
   constexpr int E = HD / 32;
   const int lane = threadIdx.x & 31, G = a.N / a.Nk, all_rows = last_row(a);
@@ -1275,7 +1344,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
   const unsigned row0 = item / a.Nk * per;
   if (row0 >= rows) return;
   const int count = static_cast<int>(min(rows - row0, static_cast<unsigned>(per)));
-  const Work w = work_of(a);
+  const Work w = work_of<TREE>(a);
   // (step 1 has ended when this step begins: only the segments are waited for)
   const Plan plan = {__ldcg(&w.plan->total), __ldcg(&w.plan->prefix_tiles), 0};
   const int my_t = static_cast<int>((row0 + min(lane, count - 1)) / G);
@@ -1443,25 +1512,25 @@ bool vectorised(const ortb200_prefix_attn_args* a) {
   return (p & 15) == 0;
 }
 
-template <typename T, int HD>
-int launch_tc(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
+template <typename T, int HD, bool TREE>
+int launch_tc(const ortb200_prefix_attn_args* a, const int* parents, cudaStream_t stream) {
   using L = TcSmem<HD>;
   const CUtensorMapDataType dt = a->dtype == ORTB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const int64_t rows = a->T * (a->N / a->Nk), entry = static_cast<int64_t>(a->Nk) * HD * 2;
   CUtensorMap tq, tk, tv;
-  if (make_tensor_map_3d(&tq, work_of(*a).q, dt, 2, HD, rows, a->Nk, HD * 2, rows * HD * 2, 64, 16) != 0) return -6;
+  if (make_tensor_map_3d(&tq, work_of<TREE>(*a).q, dt, 2, HD, rows, a->Nk, HD * 2, rows * HD * 2, 64, 16) != 0) return -6;
   const int64_t dims[4] = {HD, a->block_size, a->Nk, a->num_blocks}, strides[3] = {entry, HD * 2, entry * a->block_size};
   const int box = a->block_size < kKT ? a->block_size : kKT;
   if (make_tensor_map_4d(&tk, a->k_cache, dt, 2, dims, strides, 64, box) != 0) return -6;
   if (make_tensor_map_4d(&tv, a->v_cache, dt, 2, dims, strides, 64, box) != 0) return -6;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  auto kern = a->softcap > 64.f ? prefix_attn_kernel<HD, kBf16, 2> : a->softcap > 0.f ? prefix_attn_kernel<HD, kBf16, 1> : prefix_attn_kernel<HD, kBf16, 0>;
+  auto kern = a->softcap > 64.f ? prefix_attn_kernel<HD, kBf16, 2, TREE> : a->softcap > 0.f ? prefix_attn_kernel<HD, kBf16, 1, TREE> : prefix_attn_kernel<HD, kBf16, 0, TREE>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) != cudaSuccess) return -10;   // per device
   const int heads = a->N + 2 * a->Nk;
   const long long spread = 2 * kGrid / (a->T + 1), most = (heads + 15) / 16;   // few tokens: several CTAs per token, 16 heads at least to each
   const dim3 prep_grid(static_cast<unsigned>(a->T + 1), static_cast<unsigned>(spread < 1 ? 1 : spread > most ? most : spread));
-  int rc = vectorised<T>(a) ? launch_kernel(prefix_prep_tc_kernel<T, true>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a)
-                            : launch_kernel(prefix_prep_tc_kernel<T, false>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a);
+  int rc = vectorised<T>(a) ? launch_kernel(prefix_prep_tc_kernel<T, true, TREE>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a, parents)
+                            : launch_kernel(prefix_prep_tc_kernel<T, false, TREE>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a, parents);
   if (rc != 0) return rc;
   const float scale = a->scale != 0.f ? a->scale : 1.f / sqrtf(static_cast<float>(HD));
   // the two later steps may set up while the step before them ends: they wait for it before they read
@@ -1471,20 +1540,53 @@ int launch_tc(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
   // warp a row).  Then one row per warp until there are rows for 16 warps on each SM, which is what fits at once: warps that come
   // later would look their segments up when the others have ended (24 prompts of up to 150 tokens: 37 us behind the product kernel
   // instead of 80).
-  if (a->T * a->N <= 2 * kGrid) return launch_kernel(prefix_join_kernel<T, HD, true>, dim3(static_cast<unsigned>(a->T * a->N)), 128, 0, stream, true, *a, 1);
+  if (a->T * a->N <= 2 * kGrid) return launch_kernel(prefix_join_kernel<T, HD, true, TREE>, dim3(static_cast<unsigned>(a->T * a->N)), 128, 0, stream, true, *a, 1);
   const long long fit = 16 * kGrid / 2;
   const int per = static_cast<int>(std::min<long long>(32, (a->T * a->N + fit - 1) / fit));
   const long long warps = (rows + per - 1) / per * a->Nk;
-  return launch_kernel(prefix_join_kernel<T, HD, false>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0, stream, true, *a, per);
+  return launch_kernel(prefix_join_kernel<T, HD, false, TREE>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0, stream, true, *a, per);
 }
 
 template <typename T>
-int launch_rows(const ortb200_prefix_attn_args* a, cudaStream_t stream) {
+int launch_rows(const ortb200_prefix_attn_args* a, const int* parents, cudaStream_t stream) {
   T* q = static_cast<T*>(a->workspace);
-  int rc = launch_kernel(prefix_prep_kernel<T>, dim3(static_cast<unsigned>(a->T + 1)), 128, 0, stream, a->use_pdl != 0, *a, q);
+  uint32_t* ancestors = parents ? reinterpret_cast<uint32_t*>(static_cast<char*>(a->workspace) + up256(a->T * a->N * a->H * 4)) : nullptr;
+  int rc = launch_kernel(prefix_prep_kernel<T>, dim3(static_cast<unsigned>(a->T + 1)), 128, 0, stream, a->use_pdl != 0, *a, q, parents, ancestors);
   if (rc != 0) return rc;
   const long long items = a->T * a->N;
-  return launch_kernel(prefix_rows_kernel<T>, dim3(static_cast<unsigned>((items + 3) / 4)), 128, 0, stream, a->use_pdl != 0, *a, static_cast<const T*>(q));
+  return launch_kernel(prefix_rows_kernel<T>, dim3(static_cast<unsigned>((items + 3) / 4)), 128, 0, stream, a->use_pdl != 0, *a, static_cast<const T*>(q),
+                       static_cast<const uint32_t*>(ancestors));
+}
+
+template <bool TREE>
+int launch_attn(const ortb200_prefix_attn_args* a, const int* parents, cudaStream_t stream) {
+  if (a->T == 0) return 0;
+  if (!a->qkv || !a->k_cache || !a->v_cache || !a->cu_seqlens || !a->out || !a->workspace) return -1;
+  if (a->B > 0 && (!a->past_seqlens || !a->block_table)) return -1;
+  if ((a->k != nullptr) != (a->v != nullptr) || (a->positions != nullptr) != (a->slot_mapping != nullptr)) return -1;
+  if (a->block_size <= 0 || a->max_blocks <= 0 || a->num_blocks <= 0) return -1;
+  if (a->cos_cache && (!a->sin_cache || a->cos_rows <= 0 || a->rot_dim <= 0 || a->rot_dim % 2 != 0 || a->rot_dim > a->H)) return -1;
+  if (a->H > kMaxHead || a->T * a->N > (a->tensor_cores ? 1ll << 29 : 0x7ffffffell)) return -2;   // (places of segment rows, doubled, pass in 32 bits)
+  // what a sequence may hold, and the width of a token, pass in 32 bits
+  if (static_cast<long long>(a->max_blocks) * a->block_size > kMaxKeys || (a->N + 2ll * a->Nk) * a->H > 0x7fffffffll) return -2;
+  const int64_t bytes = TREE ? ortb200_tree_attn_workspace_bytes(a->T, a->B, a->N, a->Nk, a->H, a->tensor_cores)
+                             : ortb200_prefix_attn_workspace_bytes(a->T, a->B, a->N, a->Nk, a->H, a->tensor_cores);
+  if (a->workspace_bytes < bytes) return -1;
+  if (a->tensor_cores) {
+    const bool blocks = a->block_size % kKT == 0 || a->block_size == 8 || a->block_size == 16 || a->block_size == 32;
+    if ((a->H != 64 && a->H != 128) || !blocks || a->N / a->Nk > kQT) return -2;
+    if ((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache) | reinterpret_cast<uintptr_t>(a->out)) & 15) return -3;
+    if (reinterpret_cast<uintptr_t>(a->workspace) & 255) return -3;
+    if (a->dtype == ORTB200_BF16) return a->H == 128 ? launch_tc<__nv_bfloat16, 128, TREE>(a, parents, stream) : launch_tc<__nv_bfloat16, 64, TREE>(a, parents, stream);
+    if (a->dtype == ORTB200_F16) return a->H == 128 ? launch_tc<__half, 128, TREE>(a, parents, stream) : launch_tc<__half, 64, TREE>(a, parents, stream);
+    return -4;
+  }
+  switch (a->dtype) {
+    case ORTB200_F16: return launch_rows<__half>(a, parents, stream);
+    case ORTB200_BF16: return launch_rows<__nv_bfloat16>(a, parents, stream);
+    case ORTB200_F32: return launch_rows<float>(a, parents, stream);
+  }
+  return -4;
 }
 
 }  // namespace
@@ -1501,31 +1603,22 @@ extern "C" int64_t ortb200_prefix_attn_workspace_bytes(int64_t T, int B, int N, 
 }
 
 extern "C" int ortb200_prefix_attn(const ortb200_prefix_attn_args* a, ortb200_stream_t stream_) {
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (!a || a->T < 0 || a->B < 0 || a->N <= 0 || a->Nk <= 0 || a->N % a->Nk != 0 || a->H <= 0) return -1;
-  if (a->T == 0) return 0;
-  if (!a->qkv || !a->k_cache || !a->v_cache || !a->cu_seqlens || !a->out || !a->shared_prefix || !a->workspace) return -1;
-  if (a->B > 0 && (!a->past_seqlens || !a->block_table)) return -1;
-  if ((a->k != nullptr) != (a->v != nullptr) || (a->positions != nullptr) != (a->slot_mapping != nullptr)) return -1;
-  if (a->block_size <= 0 || a->max_blocks <= 0 || a->num_blocks <= 0) return -1;
-  if (a->cos_cache && (!a->sin_cache || a->cos_rows <= 0 || a->rot_dim <= 0 || a->rot_dim % 2 != 0 || a->rot_dim > a->H)) return -1;
-  if (a->H > kMaxHead || a->T * a->N > (a->tensor_cores ? 1ll << 29 : 0x7ffffffell)) return -2;   // (places of segment rows, doubled, pass in 32 bits)
-  // what a sequence may hold, and the width of a token, pass in 32 bits
-  if (static_cast<long long>(a->max_blocks) * a->block_size > kMaxKeys || (a->N + 2ll * a->Nk) * a->H > 0x7fffffffll) return -2;
-  if (a->workspace_bytes < ortb200_prefix_attn_workspace_bytes(a->T, a->B, a->N, a->Nk, a->H, a->tensor_cores)) return -1;
-  if (a->tensor_cores) {
-    const bool blocks = a->block_size % kKT == 0 || a->block_size == 8 || a->block_size == 16 || a->block_size == 32;
-    if ((a->H != 64 && a->H != 128) || !blocks || a->N / a->Nk > kQT) return -2;
-    if ((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache) | reinterpret_cast<uintptr_t>(a->out)) & 15) return -3;
-    if (reinterpret_cast<uintptr_t>(a->workspace) & 255) return -3;
-    if (a->dtype == ORTB200_BF16) return a->H == 128 ? launch_tc<__nv_bfloat16, 128>(a, stream) : launch_tc<__nv_bfloat16, 64>(a, stream);
-    if (a->dtype == ORTB200_F16) return a->H == 128 ? launch_tc<__half, 128>(a, stream) : launch_tc<__half, 64>(a, stream);
-    return -4;
-  }
-  switch (a->dtype) {
-    case ORTB200_F16: return launch_rows<__half>(a, stream);
-    case ORTB200_BF16: return launch_rows<__nv_bfloat16>(a, stream);
-    case ORTB200_F32: return launch_rows<float>(a, stream);
-  }
-  return -4;
+  if (a->T > 0 && !a->shared_prefix) return -1;
+  return launch_attn<false>(a, nullptr, static_cast<cudaStream_t>(stream_));
+}
+
+extern "C" int ortb200_tree_attn_max_nodes(void) { return kTreeNodes; }
+
+extern "C" int64_t ortb200_tree_attn_workspace_bytes(int64_t T, int B, int N, int Nk, int H, int tensor_cores) {
+  const int64_t bytes = ortb200_prefix_attn_workspace_bytes(T, B, N, Nk, H, tensor_cores);
+  return bytes < 0 ? bytes : bytes + tree_bytes(T);
+}
+
+extern "C" int ortb200_tree_attn(const ortb200_tree_attn_args* args, ortb200_stream_t stream_) {
+  if (!args) return -1;
+  const ortb200_prefix_attn_args* a = &args->attn;
+  if (a->T < 0 || a->B < 0 || a->N <= 0 || a->Nk <= 0 || a->N % a->Nk != 0 || a->H <= 0) return -1;
+  if (a->shared_prefix || a->positions || a->slot_mapping || (a->T > 0 && !args->parents)) return -1;
+  return launch_attn<true>(a, args->parents, static_cast<cudaStream_t>(stream_));
 }
