@@ -5,7 +5,7 @@ live in blocks of ``block_size`` tokens named by a block table; "slot" tensors h
 state) and live in one slot.  ``CachePool`` owns the device tensors and hands blocks and slots to sequences; the graph
 updates both in place.  Slots are not cleared between owners: an operator starts from the zero state when a sequence's
 past length is 0.  Sequences that begin with the same tokens share the blocks that these fill (``fork``); a block goes back
-to the pool with its last owner.
+to the pool with its last owner.  Entries and blocks move in all paged tensors at once (``CacheMover``).
 """
 from __future__ import annotations
 
@@ -13,6 +13,9 @@ from dataclasses import dataclass, field
 from typing import Dict, Hashable, List, Optional, Sequence, Tuple
 
 import torch
+
+from .. import onnx_lite as ol
+from ..capi import InferenceSession
 
 
 @dataclass(frozen=True)
@@ -35,6 +38,40 @@ class SequenceEntry:
     length: int = 0
 
 
+class CacheMover:
+    """``com.ortb200.PagedCacheMove`` over given cache tensors, as a session of its own: one launch moves entries of tokens, or whole
+    blocks, in all of them.  All sources are read before any target is written."""
+
+    _TYPES = {torch.float32: ol.TensorProto.FLOAT, torch.float16: ol.TensorProto.FLOAT16, torch.bfloat16: ol.TensorProto.BFLOAT16, torch.float64: ol.TensorProto.DOUBLE,
+              torch.int8: ol.TensorProto.INT8, torch.uint8: ol.TensorProto.UINT8, torch.int32: ol.TensorProto.INT32, torch.int64: ol.TensorProto.INT64}
+
+    def __init__(self, tensors: Sequence[torch.Tensor], whole_blocks: bool):
+        self.device = tensors[0].device
+        info = ol.make_tensor_value_info
+        kinds = [self._TYPES[t.dtype] for t in tensors]
+        places = [info(n, ol.TensorProto.INT64, ["moves"]) for n in ("sources", "targets")]
+        names = ["cache.%d" % i for i in range(len(tensors))]
+        graph = ol.make_graph([ol.make_node("PagedCacheMove", ["sources", "targets"] + names, [n + ".out" for n in names], domain="com.ortb200", whole_blocks=int(whole_blocks))],
+                              "move", places + [info(n, k, list(t.shape)) for n, k, t in zip(names, kinds, tensors)],
+                              [info(n + ".out", k, list(t.shape)) for n, k, t in zip(names, kinds, tensors)])
+        gpu = self.device.type == "cuda"
+        self.sess = InferenceSession(ol.make_model(graph, opset=17, extra_opsets={"com.ortb200": 1}).serialize(),
+                                     providers=[("CUDAExecutionProvider", {"device_id": str(self.device.index or 0)}) if gpu else "CPUExecutionProvider"])
+        self.binding = self.sess.io_binding()
+        for n, t in zip(names, tensors):
+            self.binding.bind_torch_input(n, t)
+            self.binding.bind_torch_output(n + ".out", t)
+
+    def __call__(self, sources: Sequence[int], targets: Sequence[int]) -> None:
+        moves = [(s, t) for s, t in zip(sources, targets) if s != t]
+        if not moves:
+            return
+        both = torch.tensor(moves, dtype=torch.int64).t().contiguous().to(self.device)
+        self.binding.bind_torch_input("sources", both[0])
+        self.binding.bind_torch_input("targets", both[1])
+        self.sess.run_with_iobinding(self.binding)
+
+
 class CachePool:
     def __init__(self, spec: Sequence[CacheTensor], num_blocks: int, block_size: int, num_slots: int, device: torch.device):
         self.spec = list(spec)
@@ -47,6 +84,16 @@ class CachePool:
         self.free_slots = list(range(num_slots - 1, -1, -1))
         self.sequences: Dict[Hashable, SequenceEntry] = {}
         self.owners: Dict[int, int] = {}                         # blocks of more than one sequence: how many
+        self._movers: Dict[bool, CacheMover] = {}
+
+    def _move(self, sources: Sequence[int], targets: Sequence[int], whole_blocks: bool) -> None:
+        """Entries or blocks of the paged tensors to other places."""
+        paged = [self.tensors[c.input] for c in self.spec if c.kind == "paged"]
+        if not paged or not sources:
+            return
+        if whole_blocks not in self._movers:
+            self._movers[whole_blocks] = CacheMover(paged, whole_blocks)
+        self._movers[whole_blocks](sources, targets)
 
     def open(self, seq: Hashable) -> SequenceEntry:
         if seq in self.sequences:
@@ -78,13 +125,29 @@ class CachePool:
             self.owners[block] = self.owners.get(block, 1) + 1
         if rest:
             entry.blocks.append(self.free_blocks.pop())
+        if rest:
+            self._move([src.blocks[whole]], [entry.blocks[-1]], True)
         for c in self.spec:
-            t = self.tensors[c.input]
             if c.kind == "slot":
+                t = self.tensors[c.input]
                 t[entry.slot].copy_(t[src.slot])
-            elif rest:
-                t[entry.blocks[-1]].copy_(t[src.blocks[whole]])
         return entry
+
+    def keep(self, chosen: Dict[Hashable, Tuple[int, Sequence[int]]]) -> None:
+        """Of the tokens behind the first ``held`` of a sequence, only those at the places ``path`` (ascending, counted from
+        ``held``), which close up: ``chosen`` names (held, path) for each sequence."""
+        sources, targets = [], []
+        for seq, (held, path) in chosen.items():
+            entry = self.sequences[seq]
+            if not 0 <= held <= held + len(path) <= entry.length or any(not 0 <= p < entry.length - held for p in path) or any(a >= b for a, b in zip(path, path[1:])):
+                raise ValueError(f"sequence {seq!r} holds no such tokens")
+        for seq, (held, path) in chosen.items():
+            entry = self.sequences[seq]
+            place = lambda t: entry.blocks[t // self.block_size] * self.block_size + t % self.block_size  # noqa: E731, B023
+            sources += [place(held + p) for p in path]
+            targets += [place(held + i) for i in range(len(path))]
+            entry.length = held + len(path)
+        self._move(sources, targets, False)
 
     def common_tokens(self, seqs: Sequence[Hashable]) -> int:
         """How many leading tokens of all ``seqs`` lie in the same blocks."""
@@ -129,10 +192,11 @@ class CachePool:
         if any(len(a.blocks) != len(b.blocks) for a, b in zip(src, dst)):
             raise ValueError("sequences hold different numbers of blocks")
         lengths = [e.length for e in src]
+        self._move(src_blocks, dst_blocks, True)
         for c in self.spec:
-            t = self.tensors[c.input]
-            a = torch.tensor(src_blocks if c.kind == "paged" else [e.slot for e in src], device=t.device)
-            b = torch.tensor(dst_blocks if c.kind == "paged" else [e.slot for e in dst], device=t.device)
-            t.index_copy_(0, b, t.index_select(0, a))
+            if c.kind == "slot":
+                t = self.tensors[c.input]
+                a, b = (torch.tensor([e.slot for e in entries], device=t.device) for entries in (src, dst))
+                t.index_copy_(0, b, t.index_select(0, a))
         for e, n in zip(dst, lengths):
             e.length = n

@@ -10,8 +10,9 @@ session captures it on the first step and replays it afterwards.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
-from typing import Dict, Hashable, List, Optional, Sequence, Tuple, Union
+from typing import Callable, Dict, Hashable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -19,6 +20,9 @@ from .. import onnx_lite as ol
 from ..capi import InferenceSession, RunOptions
 from .decoder_cache import CacheFull, CachePool
 from .llama import LlamaConfig, empty_kv_cache
+
+
+MOST_DRAFTED = 256   # tokens of a sequence's tree (com.ortb200.TreePagedAttention)
 
 
 class DecoderRunner:
@@ -159,6 +163,9 @@ class PagedDecoderRunner:
     ``decode_step`` drive a fixed batch of ``batch`` rows on top of the same pool.  A step that brings one token per
     sequence has fixed shapes and addresses and is captured as one CUDA graph per batch size.
 
+    ``draft_step`` (models built with ``draft_trees``) runs a tree of drafted tokens for each sequence, ``accept`` keeps one of
+    its paths.
+
     ``fork`` opens a sequence behind the tokens of another one, with the blocks that these fill in common.  A model built with
     ``shared_prefix`` attends to what all sequences of a batch have in common once for all of them, and extends its block
     tables on the device."""
@@ -179,6 +186,8 @@ class PagedDecoderRunner:
         self.has_slots = "state_slots" in in_names
         self.has_key_starts = "key_starts" in in_names
         self.has_layout = "free_blocks" in in_names
+        self.has_trees = "parents" in in_names
+        self._drafted: Dict[Hashable, Tuple[int, List[int]]] = {}   # sequences with drafted tokens: tokens held before, parents
         self.logits_dtype = {"tensor(float)": torch.float32, "tensor(float16)": torch.float16,
                              "tensor(bfloat16)": torch.bfloat16}[out_info["logits"].type]
         self._steps: Dict[int, "_DecodeBuffers"] = {}
@@ -226,8 +235,10 @@ class PagedDecoderRunner:
             got += e.blocks[-(-e.length // self.block_size):-(-(e.length + n) // self.block_size)]
         return got
 
-    def _bind(self, binding, ids, cum, past, table, slots, key_starts, rows, logits, nxt, free=None, shared=None, used=None) -> None:
+    def _bind(self, binding, ids, cum, past, table, slots, key_starts, rows, logits, nxt, free=None, shared=None, used=None, parents=None) -> None:
         binding.bind_torch_input("input_ids", ids)
+        if self.has_trees:
+            binding.bind_torch_input("parents", parents)
         if self.has_layout:      # `cum` holds the new tokens of every sequence; the extended table goes where the table is
             binding.bind_torch_input("new_tokens", cum)
             binding.bind_torch_input("free_blocks", free)
@@ -255,9 +266,61 @@ class PagedDecoderRunner:
         """One batch: ``entries`` = (sequence, its next tokens, places among them whose logits are wanted).  A sequence
         seen for the first time is opened.  Returns the logits [wanted, vocab] in the order of the entries."""
         entries = [e for e in entries if len(e[1]) > 0]
+        self._make_room(entries)
+        if not entries:
+            return torch.empty(0, self.cfg.vocab_size, dtype=self.logits_dtype, device=self.device)
+        seqs = [e[0] for e in entries]
+        if all(len(e[1]) == 1 for e in entries):
+            buf = self._decode_buffers(len(entries))
+            buf.ids.copy_(torch.tensor([int(e[1][0]) for e in entries], dtype=torch.int64))
+            self._run_decode(buf, seqs)
+            wanted = [b for b, e in enumerate(entries) for _ in e[2]]
+            return buf.logits[torch.tensor(wanted, dtype=torch.int64, device=self.device)]
+        return self._run_wanted(entries, None)
+
+    def draft_step(self, entries: Sequence[Tuple[Hashable, Sequence[int], Sequence[int], Sequence[int]]]) -> torch.Tensor:
+        """One batch of trees: ``entries`` = (sequence, its tokens, the place of each token's parent among them or -1, places whose
+        logits are wanted).  A parent stands in front of its children; a token sees what the sequence holds, its ancestors and
+        itself.  Returns the logits [wanted, vocab] in the order of the entries.  ``accept`` has to follow for every sequence."""
+        if not self.has_trees:
+            raise ValueError("the model has no form for drafted tokens (draft_trees)")
+        entries = [e for e in entries if len(e[1]) > 0]
+        if len({e[0] for e in entries}) != len(entries):
+            raise ValueError("a sequence comes twice in a batch")
+        for seq, tokens, parents, _ in entries:
+            if len(parents) != len(tokens) or any(not -1 <= p < i for i, p in enumerate(parents)):
+                raise ValueError(f"sequence {seq!r}: every token has one parent, in front of it")
+            if len(tokens) > MOST_DRAFTED and any(p != i - 1 for i, p in enumerate(parents)):
+                raise ValueError(f"sequence {seq!r}: a tree of more than {MOST_DRAFTED} tokens")
+        plain = [(seq, tokens, want) for seq, tokens, _, want in entries]
+        self._make_room(plain)
+        if not entries:
+            return torch.empty(0, self.cfg.vocab_size, dtype=self.logits_dtype, device=self.device)
+        before = {seq: self.pool.sequences[seq].length for seq, *_ in entries}
+        logits = self._run_wanted(plain, [int(p) for _, _, parents, _ in entries for p in parents])
+        for seq, _, parents, _ in entries:
+            self._drafted[seq] = (before[seq], [int(p) for p in parents])
+        return logits
+
+    def accept(self, paths: Dict[Hashable, Sequence[int]]) -> None:
+        """What sequences keep of their drafted tokens: for each a path of its tree, the places of its tokens from a root on.  The
+        others are forgotten."""
+        for seq, path in paths.items():
+            if seq not in self._drafted:
+                raise ValueError(f"sequence {seq!r} has no drafted tokens")
+            parents = self._drafted[seq][1]
+            if any(not 0 <= p < len(parents) or parents[p] != q for p, q in zip(path, [-1, *path])):
+                raise ValueError(f"sequence {seq!r}: {list(path)} is no path of its tree")
+        self.pool.keep({seq: (self._drafted[seq][0], list(path)) for seq, path in paths.items()})
+        for seq in paths:
+            del self._drafted[seq]
+
+    def _make_room(self, entries) -> None:
         opened = []
         try:
             for seq, tokens, want in entries:
+                if seq in self._drafted:
+                    raise ValueError(f"the drafted tokens of sequence {seq!r} wait for accept()")
                 if any(not 0 <= w < len(tokens) for w in want):
                     raise ValueError(f"sequence {seq!r}: a wanted place lies outside its {len(tokens)} tokens")
                 if seq not in self.pool.sequences:
@@ -270,32 +333,28 @@ class PagedDecoderRunner:
             for seq in opened:
                 self.pool.close(seq)
             raise
-        if not entries:
-            return torch.empty(0, self.cfg.vocab_size, dtype=self.logits_dtype, device=self.device)
-        seqs = [e[0] for e in entries]
-        if all(len(e[1]) == 1 for e in entries):
-            buf = self._decode_buffers(len(entries))
-            buf.ids.copy_(torch.tensor([int(e[1][0]) for e in entries], dtype=torch.int64))
-            self._run_decode(buf, seqs)
-            wanted = [b for b, e in enumerate(entries) for _ in e[2]]
-            return buf.logits[torch.tensor(wanted, dtype=torch.int64, device=self.device)]
+
+    def _run_wanted(self, entries, parents) -> torch.Tensor:
         ids = torch.cat([torch.as_tensor(e[1], dtype=torch.int64).reshape(-1).cpu() for e in entries])
         starts, rows = [0], []
         for _, tokens, want in entries:
             rows += [starts[-1] + int(w) for w in want]
             starts.append(starts[-1] + len(tokens))
-        logits, _ = self._run_packed(ids, starts, seqs, rows or [0])
+        logits, _ = self._run_packed(ids, starts, [e[0] for e in entries], rows or [0], parents)
         return logits if rows else logits[:0]
 
     def fork(self, seq: Hashable, source: Hashable, tokens: Optional[int] = None) -> None:
         """Opens ``seq`` behind the first ``tokens`` (default: all) tokens that ``source`` holds."""
+        if source in self._drafted:
+            raise ValueError(f"the drafted tokens of sequence {source!r} wait for accept()")
         self.pool.fork(seq, source, tokens)
 
     def release(self, seq: Hashable) -> None:
         """The sequence is finished: its blocks and slot go back to the pool."""
         self.pool.close(seq)
+        self._drafted.pop(seq, None)
 
-    def _run_packed(self, ids: torch.Tensor, starts, seqs, rows) -> Tuple[torch.Tensor, torch.Tensor]:
+    def _run_packed(self, ids: torch.Tensor, starts, seqs, rows, parents=None) -> Tuple[torch.Tensor, torch.Tensor]:
         dev = self.device
         lengths = [self.pool.sequences[s].length for s in seqs]
         past = torch.tensor(lengths, dtype=torch.int32)
@@ -306,6 +365,8 @@ class PagedDecoderRunner:
         binding = self.sess.io_binding()
         i32 = lambda v: torch.tensor(v, dtype=torch.int32).to(dev)  # noqa: E731
         cum, layout = starts, {}
+        if self.has_trees:
+            layout = dict(parents=i32(parents if parents is not None else [i - 1 for a, b in zip(starts, starts[1:]) for i in range(b - a)]))
         if self.has_layout:
             cum = [starts[b + 1] - starts[b] for b in range(len(seqs))]
             layout = dict(free=i32(self._granted(seqs, cum)), shared=i32([self.pool.common_tokens(seqs)]), used=i32([0]))
@@ -323,7 +384,7 @@ class PagedDecoderRunner:
             buf = _DecodeBuffers(rows, self.blocks_per_seq, self.cfg.vocab_size, self.logits_dtype, self.device)
             buf.binding = self.sess.io_binding()
             self._bind(buf.binding, buf.ids, buf.new if self.has_layout else buf.cum, buf.past, buf.table, buf.slots, buf.key_starts, buf.rows, buf.logits, buf.next,
-                       buf.free, buf.shared, buf.used)
+                       buf.free, buf.shared, buf.used, buf.parents)
             buf.options.add_run_config_entry("gpu_graph_id", str(self._graph_id + len(self._steps)))
             self._steps[rows] = buf
         return self._steps[rows]
@@ -432,6 +493,7 @@ class _DecodeBuffers:
         self.free = torch.zeros(rows, dtype=torch.int32, device=device)     # a token enters one new block at most
         self.shared = torch.zeros(1, dtype=torch.int32, device=device)
         self.used = torch.zeros(1, dtype=torch.int32, device=device)
+        self.parents = torch.full((rows,), -1, dtype=torch.int32, device=device)
         self.layout = None
         self.tokens = None       # lengths that the next step of the same batch finds
         self.binding = None
@@ -448,8 +510,14 @@ class GenerationConfig:
                  pad_token_id: int = 0, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
                  repetition_penalty: float = 1.0, no_repeat_ngram_size: int = 0, num_beams: int = 1,
                  length_penalty: float = 1.0, early_stopping: bool = False, num_return_sequences: int = 1,
-                 vocab_mask: Optional[torch.Tensor] = None, seed: Optional[int] = None, logprobs: Optional[int] = None):
-        """``logprobs``: report log probabilities, entropies and that many best alternatives (``generate_requests``)."""
+                 vocab_mask: Optional[torch.Tensor] = None, seed: Optional[int] = None, logprobs: Optional[int] = None,
+                 presence_penalty: float = 0.0, frequency_penalty: float = 0.0, logit_bias: Optional[Dict[int, float]] = None,
+                 grammar: Optional[Callable[[List[int]], Optional[Sequence[int]]]] = None, draft_tokens: int = 0, draft_ngram: int = 3):
+        """For ``generate_requests``: ``logprobs``: report log probabilities, entropies and that many best alternatives.
+        ``presence_penalty`` and ``frequency_penalty`` are subtracted from the logits of generated tokens, once and as often as they
+        occur; ``logit_bias`` is added to tokens' logits; ``grammar`` names the tokens that may follow the generated ones (None: all).
+        ``draft_tokens`` (runners with ``draft_trees``): up to so many tokens a step are drafted from what followed the last
+        ``draft_ngram`` tokens, or fewer, earlier in the request's own text; the step keeps those that it would have chosen."""
         self.__dict__.update(locals())
         del self.__dict__["self"]
 
@@ -529,6 +597,139 @@ def generate(runner: Union[DecoderRunner, PagedDecoderRunner], input_ids: torch.
             runner.decode_step(nxt.view(-1, 1))
             logits = _last_logits(runner, prefill=False)
     return seqs
+
+
+class LogitsProcessor:
+    """The logits processors of ``generate_requests`` for all rows of a step at once: ``com.ortb200.ProcessLogits`` as a session of its
+    own on the provider of the logits' device, with the inputs that the configuration needs."""
+
+    def __init__(self, vocab_size: int, dtype: torch.dtype, device: torch.device, cfg: GenerationConfig):
+        T, info = ol.TensorProto, ol.make_tensor_value_info
+        kind = {torch.float32: T.FLOAT, torch.float16: T.FLOAT16, torch.bfloat16: T.BFLOAT16}[dtype]
+        self.vocab_size, self.device, self.cfg = vocab_size, device, cfg
+        self.text = cfg.repetition_penalty != 1.0 or cfg.presence_penalty != 0.0 or cfg.frequency_penalty != 0.0
+        self.biased = (cfg.eos_token_id is not None and cfg.min_new_tokens > 0) or cfg.no_repeat_ngram_size > 0 or bool(cfg.logit_bias)
+        self.masked = cfg.vocab_mask is not None or cfg.grammar is not None
+        self.warm = cfg.temperature != 1.0 and cfg.temperature > 0
+        self.idle = not (self.text or self.biased or self.masked or self.warm)
+        ins = [info("logits", kind, ["rows", vocab_size])]
+        names = ["logits"] + [""] * 14
+
+        def add(place: int, name: str, onnx_type: int, shape) -> None:
+            names[place] = name
+            ins.append(info(name, onnx_type, shape))
+        if self.text:
+            for i, (name, shape) in enumerate((("history", ["total"]), ("history_starts", ["ends"]), ("generated_starts", ["lists"]))):
+                add(1 + i, name, T.INT64, shape)
+            add(4, "row_list", T.INT32, ["rows"])
+            add(5, "drafted", T.INT64, ["rows", "depth"])
+            for i, name in enumerate(("repetition", "presence", "frequency")):
+                add(6 + i, name, T.FLOAT, ["rows"])
+        if self.biased:
+            add(9, "bias_tokens", T.INT64, ["biases"])
+            add(10, "bias_values", T.FLOAT, ["biases"])
+            add(11, "bias_starts", T.INT64, ["bias_ends"])
+        if self.masked:
+            add(12, "allowed", T.INT32, ["masks", (vocab_size + 31) // 32])
+            add(13, "row_mask", T.INT32, ["rows"])
+        if self.warm:
+            add(14, "temperature", T.FLOAT, ["rows"])
+        while not names[-1]:
+            names.pop()
+        graph = ol.make_graph([ol.make_node("ProcessLogits", names, ["scores"], domain="com.ortb200")], "logits", ins, [info("scores", T.FLOAT, ["rows", vocab_size])])
+        gpu = device.type == "cuda"
+        self.sess = None if self.idle else InferenceSession(
+            ol.make_model(graph, opset=17, extra_opsets={"com.ortb200": 1}).serialize(),
+            providers=[("CUDAExecutionProvider", {"device_id": str(device.index or 0)}) if gpu else "CPUExecutionProvider"])
+
+    def _biases(self, text: Sequence[int], generated: int) -> Dict[int, float]:
+        """Of one row whose text ends with ``generated`` generated tokens."""
+        cfg, bias = self.cfg, dict(self.cfg.logit_bias or {})
+        if cfg.eos_token_id is not None and generated < cfg.min_new_tokens:
+            bias[cfg.eos_token_id] = -math.inf
+        n = cfg.no_repeat_ngram_size
+        if n > 0:
+            tail = list(text[len(text) - (n - 1):])
+            for i in range(len(text) - n + 1):
+                if list(text[i:i + n - 1]) == tail:
+                    bias[text[i + n - 1]] = -math.inf
+        return bias
+
+    def _mask(self, allowed: Optional[Sequence[int]]) -> torch.Tensor:
+        keep = torch.ones(self.vocab_size, dtype=torch.bool) if allowed is None else torch.zeros(self.vocab_size, dtype=torch.bool)
+        if allowed is not None:
+            keep[torch.as_tensor(list(allowed), dtype=torch.int64)] = True
+        if self.cfg.vocab_mask is not None:
+            keep &= self.cfg.vocab_mask.reshape(-1).cpu() != 0
+        words = torch.nn.functional.pad(keep, (0, -self.vocab_size % 32)).reshape(-1, 32).long()
+        packed = (words << torch.arange(32)).sum(-1)
+        return torch.where(packed >= 1 << 31, packed - (1 << 32), packed).int()
+
+    def __call__(self, logits: torch.Tensor, requests: Sequence[Tuple[Sequence[int], int, Sequence[Sequence[int]]]]) -> torch.Tensor:
+        """logits [rows, vocab] -> scores [rows, vocab] in 32 bits.  ``requests``: (text, how many tokens of it are generated, for each of
+        the request's rows the drafted tokens behind the text)."""
+        if self.idle:
+            return logits.float()
+        cfg, dev, rows = self.cfg, self.device, logits.shape[0]
+        ints = lambda v, t=torch.int64: torch.tensor(v, dtype=t).to(dev)  # noqa: E731
+        same = lambda v: torch.full((rows,), v, dtype=torch.float32, device=dev)  # noqa: E731
+        feeds = {"logits": logits}
+        if self.text:
+            starts, generated, lists = [0], [], []
+            for i, (text, new, paths) in enumerate(requests):
+                starts.append(starts[-1] + len(text))
+                generated.append(starts[-1] - new)
+                lists += [i] * len(paths)
+            deepest = max(len(p) for _, _, paths in requests for p in paths)
+            drafted = [list(p) + [-1] * (deepest - len(p)) for _, _, paths in requests for p in paths]
+            feeds.update(history=ints([t for text, _, _ in requests for t in text]), history_starts=ints(starts), generated_starts=ints(generated), row_list=ints(lists, torch.int32),
+                         drafted=ints(drafted).reshape(rows, deepest), repetition=same(cfg.repetition_penalty), presence=same(cfg.presence_penalty),
+                         frequency=same(cfg.frequency_penalty))
+        if self.biased:
+            bias = [self._biases([*text, *p], new + len(p)) for text, new, paths in requests for p in paths]
+            ends = [0]
+            for b in bias:
+                ends.append(ends[-1] + len(b))
+            feeds.update(bias_tokens=ints([t for b in bias for t in b]), bias_values=torch.tensor([v for b in bias for v in b.values()], dtype=torch.float32).to(dev), bias_starts=ints(ends))
+        if self.masked:
+            if cfg.grammar is None:
+                feeds.update(allowed=self._mask(None).reshape(1, -1).to(dev), row_mask=torch.zeros(rows, dtype=torch.int32, device=dev))
+            else:
+                masks = [self._mask(cfg.grammar([*text[len(text) - new:], *p])) for text, new, paths in requests for p in paths]
+                feeds.update(allowed=torch.stack(masks).to(dev), row_mask=torch.arange(rows, dtype=torch.int32, device=dev))
+        if self.warm:
+            feeds.update(temperature=same(cfg.temperature))
+        scores = torch.empty(rows, self.vocab_size, dtype=torch.float32, device=dev)
+        binding = self.sess.io_binding()
+        for name, t in feeds.items():
+            binding.bind_torch_input(name, t)
+        binding.bind_torch_output("scores", scores)
+        self.sess.run_with_iobinding(binding)
+        return scores
+
+
+def draft_tree(text: Sequence[int], most: int, ngram: int = 3) -> Tuple[List[int], List[int]]:
+    """A tree of the last token of ``text`` and up to ``most`` drafted ones: what followed earlier occurrences of the last ``ngram`` tokens, then
+    of fewer, the latest occurrences first and each up to half as many tokens as there may be.  Returns the tokens and their parents."""
+    tokens, parents, children = [int(text[-1])], [-1], {}
+    depth, end = max(1, (most + 1) // 2), len(text)
+    for n in range(min(ngram, end - 1), 0, -1):
+        tail = list(text[end - n:])
+        for at in range(end - 1, n - 1, -1):
+            if len(tokens) > most:
+                return tokens, parents
+            if list(text[at - n:at]) != tail:
+                continue
+            node = 0
+            for t in text[at:min(at + depth, end)]:
+                if (node, t) not in children:
+                    if len(tokens) > most:
+                        break
+                    children[node, t] = len(tokens)
+                    tokens.append(int(t))
+                    parents.append(node)
+                node = children[node, t]
+    return tokens, parents
 
 
 class TokenScorer:
@@ -620,7 +821,12 @@ def generate_requests(runner: PagedDecoderRunner, prompts: Sequence[Sequence[int
     the running batch in a step of its own.  Returns the generated tokens of every request (end token included).
 
     ``shared_prompt`` stands in front of every prompt: it runs once, the requests share the cache blocks that it fills, and it
-    takes one of the runner's sequences.  With ``cfg.logprobs`` the requests come back as ``Generated``."""
+    takes one of the runner's sequences.  With ``cfg.logprobs`` the requests come back as ``Generated``.  With ``cfg.draft_tokens``
+    a step may give a request several tokens, the same as without."""
+    if cfg.draft_tokens < 0 or cfg.draft_ngram < 1:
+        raise ValueError("draft_tokens is not negative, and draft_ngram positive")
+    if cfg.draft_tokens and not runner.has_trees:
+        raise ValueError("drafted tokens need a decoder with draft_trees")
     if len(shared_prompt):
         if any(len(p) == 0 for p in prompts):
             raise ValueError("a request behind a shared prompt has a token of its own at least")
@@ -651,15 +857,14 @@ def _generate_requests(runner: PagedDecoderRunner, prompts, cfg: GenerationConfi
     held_by_all = len(shared) // runner.block_size     # blocks that a request does not need for itself
     scorer = TokenScorer(runner.cfg.vocab_size, cfg.logprobs, runner.logits_dtype, runner.device) if cfg.logprobs is not None else None
     details = [Generated() for _ in texts]
+    processor = LogitsProcessor(runner.cfg.vocab_size, runner.logits_dtype, runner.device, cfg)
     waiting, running = list(range(len(texts))), []
 
-    def pick(i: int, logits: torch.Tensor) -> None:
-        seq = torch.tensor([texts[i] + new[i]], dtype=torch.int64, device=runner.device)
-        scores = process_logits(logits.reshape(1, -1), seq, len(new[i]), cfg)
+    def pick(i: int, logits: torch.Tensor, scores: torch.Tensor, best: int) -> int:
+        """The request's next token out of a row of logits, noted; a request that is finished leaves."""
+        tok = best
         if sampling:
-            tok = int(torch.multinomial(torch.softmax(top_k_top_p_filter(scores, cfg.top_k, cfg.top_p), -1), 1, generator=gen))
-        else:
-            tok = int(scores.argmax(-1))
+            tok = int(torch.multinomial(torch.softmax(top_k_top_p_filter(scores.reshape(1, -1), cfg.top_k, cfg.top_p), -1), 1, generator=gen))
         new[i].append(tok)
         if scorer is not None:
             lp, h, top_lp, top = (t.tolist() for t in scorer(logits.reshape(1, -1), torch.tensor([tok], dtype=torch.int64)))
@@ -673,6 +878,7 @@ def _generate_requests(runner: PagedDecoderRunner, prompts, cfg: GenerationConfi
             done[i] = new.pop(i)
             running.remove(i)
             runner.release(("request", i))
+        return tok
 
     while waiting or running:
         joining = waiting[:min(runner.batch - len(running), len(runner.pool.free_slots))]
@@ -693,14 +899,47 @@ def _generate_requests(runner: PagedDecoderRunner, prompts, cfg: GenerationConfi
             running += joining
             for i in joining:
                 new[i] = []
+            trees = {i: ([-1], [-1]) for i in joining}   # a row for the last token of each
+            drafted = False
         elif running:
             joining = list(running)
-            logits = runner.step([(("request", i), [new[i][-1]], [0]) for i in joining])
+            # room has been kept for the tokens that a request will generate: no more of them are drafted
+            trees = {i: draft_tree(texts[i] + new[i], min(cfg.draft_tokens, cfg.max_new_tokens - len(new[i]) - 1), cfg.draft_ngram) if cfg.draft_tokens else ([new[i][-1]], [-1])
+                     for i in joining}
+            drafted = any(len(tokens) > 1 for tokens, _ in trees.values())
+            if drafted:
+                logits = runner.draft_step([(("request", i), *trees[i], range(len(trees[i][0]))) for i in joining])
+            else:
+                logits = runner.step([(("request", i), [new[i][-1]], [0]) for i in joining])
         else:
             raise CacheFull(f"request {waiting[0]} does not fit into the cache")
-        for row, i in enumerate(joining):
-            pick(i, logits[row])
+        paths = {i: _paths(*trees[i]) for i in joining}
+        scores = processor(logits, [(texts[i] + new[i], len(new[i]), [[trees[i][0][j] for j in path[1:]] for path in paths[i]]) for i in joining])
+        best = [0] * len(scores) if sampling else scores.argmax(-1).tolist()
+        row, kept = 0, {}
+        for i in joining:   # from the root on, as far as the tree has what is chosen
+            tokens, parents = trees[i]
+            node = 0
+            while True:
+                tok = pick(i, logits[row + node], scores[row + node], best[row + node])
+                child = [j for j in range(node + 1, len(tokens)) if parents[j] == node and tokens[j] == tok]
+                if i not in running or not child:
+                    break
+                node = child[0]
+            if drafted and i in running:
+                kept[("request", i)] = paths[i][node]
+            row += len(tokens)
+        if drafted:
+            runner.accept(kept)
     return done if scorer is None else details
+
+
+def _paths(tokens: Sequence[int], parents: Sequence[int]) -> List[List[int]]:
+    """Of every token of a tree, the places from its root to it."""
+    paths: List[List[int]] = []
+    for i, p in enumerate(parents):
+        paths.append((paths[p] if p >= 0 else []) + [i])
+    return paths
 
 
 def _last_logits(runner: DecoderRunner, prefill: bool) -> torch.Tensor:

@@ -95,7 +95,8 @@ def build_llama(cfg: LlamaConfig, tp_rank: int = 0, tp_size: int = 1, external_w
                 device: str = "cpu", with_argmax: bool = True, last_token_logits: bool = True,
                 weight_std: float = 0.02, shard_lm_head: bool = True, quant_bits: int = 0,
                 quant_block: int = 32, paged: bool = False, moe_experts: int = 0, moe_top_k: int = 2, ep_rank: int = 0,
-                ep_size: int = 1, state: Optional[Mapping[str, torch.Tensor]] = None, shared_prefix: bool = False, block_size: int = 256) -> Tuple[bytes, Dict[str, torch.Tensor]]:
+                ep_size: int = 1, state: Optional[Mapping[str, torch.Tensor]] = None, shared_prefix: bool = False, block_size: int = 256,
+                draft_trees: bool = False) -> Tuple[bytes, Dict[str, torch.Tensor]]:
     """Returns (ModelProto bytes, weights).  ``state`` holds a checkpoint's tensors under their usual names
     (``model.layers.0.self_attn.q_proj.weight`` [out, in], ...); without it the weights are random.  With ``external_weights`` the dict holds every weight (on
     ``device``) to pass to ``SessionOptions.add_external_initializers``; otherwise it is empty and the
@@ -120,6 +121,10 @@ def build_llama(cfg: LlamaConfig, tp_rank: int = 0, tp_size: int = 1, external_w
     layers, and ``com.ortb200.SharedPrefixPagedAttention`` attends to the first ``shared_prefix`` tokens, which are the
     same in every sequence of the batch, once for all of them.
 
+    ``draft_trees=True`` (with ``paged``) builds the form for steps with drafted tokens: the new tokens of a sequence form a
+    tree, which the input ``parents`` [tokens] describes (the place of a token's parent among its sequence's new tokens, -1
+    for the last token in the cache), and ``com.ortb200.TreePagedAttention`` lets a token see the cache and its ancestors.
+
     ``moe_experts > 0`` replaces the dense SwiGLU block of every layer by a top-``moe_top_k`` softmax-routed mixture of
     that many SwiGLU experts (the Mixtral shape): ``com.microsoft.MoE`` on one device, or ``com.microsoft.ShardedMoE``
     holding experts ``[ep_rank * E / ep_size, (ep_rank + 1) * E / ep_size)`` when ``ep_size > 1`` (expert parallelism:
@@ -130,7 +135,8 @@ def build_llama(cfg: LlamaConfig, tp_rank: int = 0, tp_size: int = 1, external_w
     assert moe_experts % max(ep_size, 1) == 0
     if paged:
         last_token_logits = False
-    assert paged or not shared_prefix, "a shared prefix lies in paged caches"
+    assert paged or not (shared_prefix or draft_trees), "a shared prefix and drafted tokens lie in paged caches"
+    assert not (shared_prefix and draft_trees), "one form of attention at a time"
     assert quant_bits in (0, 4)
     assert cfg.num_heads % tp_size == 0 and cfg.num_kv_heads % tp_size == 0 and cfg.ffn_size % tp_size == 0
     dt, odt = _TORCH_DT[cfg.dtype], _ONNX_DT[cfg.dtype]
@@ -234,6 +240,8 @@ def build_llama(cfg: LlamaConfig, tp_rank: int = 0, tp_size: int = 1, external_w
             ol.make_tensor_value_info("block_table", T.INT32, ["batch", "max_blocks"]),
             ol.make_tensor_value_info("logits_indices", T.INT64, ["rows"]),
         ]
+        if draft_trees:
+            inputs.append(ol.make_tensor_value_info("parents", T.INT32, ["tokens"]))
         if shared_prefix:
             inputs += [ol.make_tensor_value_info("free_blocks", T.INT32, ["free"]), ol.make_tensor_value_info("shared_prefix", T.INT32, [1])]
             nodes.append(ol.make_node("PagedBatchLayout", ["past_seqlens", "new_tokens", "block_table", "free_blocks", "input_ids"],
@@ -281,11 +289,11 @@ def build_llama(cfg: LlamaConfig, tp_rank: int = 0, tp_size: int = 1, external_w
                 outputs.append(ol.make_tensor_value_info(f"{kv}_cache_out.{i}", odt, ["num_blocks", "block_size", Nk, H]))
             attn_ins = [f"{p}.qkv", "", "", f"key_cache.{i}", f"value_cache.{i}", "cumulative_sequence_length", "past_seqlens"]
             attn_ins += (["block_table_out", "shared_prefix", "cos_cache", "sin_cache", "positions", "slot_mapping"] if shared_prefix else
-                         ["block_table", "cos_cache", "sin_cache"])
+                         ["block_table"] + (["parents"] if draft_trees else []) + ["cos_cache", "sin_cache"])
             nodes.append(ol.make_node(
-                "SharedPrefixPagedAttention" if shared_prefix else "PagedAttention", attn_ins,
+                "SharedPrefixPagedAttention" if shared_prefix else "TreePagedAttention" if draft_trees else "PagedAttention", attn_ins,
                 [f"{p}.attn_out", f"key_cache_out.{i}", f"value_cache_out.{i}"], name=f"{p}.attn",
-                domain="com.ortb200" if shared_prefix else "com.microsoft", num_heads=N, kv_num_heads=Nk, do_rotary=1, rotary_interleaved=0))
+                domain="com.ortb200" if shared_prefix or draft_trees else "com.microsoft", num_heads=N, kv_num_heads=Nk, do_rotary=1, rotary_interleaved=0))
         else:
             inputs.append(ol.make_tensor_value_info(f"past_key_values.{i}.key", odt, ["batch", Nk, "past_seq", H]))
             inputs.append(ol.make_tensor_value_info(f"past_key_values.{i}.value", odt, ["batch", Nk, "past_seq", H]))
@@ -370,7 +378,7 @@ def build_llama(cfg: LlamaConfig, tp_rank: int = 0, tp_size: int = 1, external_w
         outputs += [ol.make_tensor_value_info("block_table_out", T.INT32, ["batch", "max_blocks"]), ol.make_tensor_value_info("blocks_used", T.INT32, [1])]
     graph = ol.make_graph(nodes, "llama", inputs, outputs, inits)
     meta = {"tp_rank": str(tp_rank), "tp_size": str(tp_size), "architecture": "mixtral" if moe_experts else "llama"}
-    model = ol.make_model(graph, opset=17, metadata=meta, **({"extra_opsets": {"com.ortb200": 1}} if shared_prefix else {}))
+    model = ol.make_model(graph, opset=17, metadata=meta, **({"extra_opsets": {"com.ortb200": 1}} if shared_prefix or draft_trees else {}))
     return model.serialize(), weights
 
 

@@ -23,6 +23,8 @@ class DecoderFamily:
     build: Callable[[Any, Optional[Mapping[str, torch.Tensor]], str], Tuple[bytes, Dict[str, torch.Tensor]]]
     # the form for sequences that begin with the same tokens, for caches of blocks of a given size
     build_shared: Optional[Callable[[Any, Optional[Mapping[str, torch.Tensor]], str, int], Tuple[bytes, Dict[str, torch.Tensor]]]] = None
+    # the form for steps with drafted tokens
+    build_drafts: Optional[Callable[[Any, Optional[Mapping[str, torch.Tensor]], str], Tuple[bytes, Dict[str, torch.Tensor]]]] = None
 
 
 FAMILIES: Dict[str, DecoderFamily] = {}
@@ -38,7 +40,8 @@ register_family("Rovurax", DecoderFamily(rovurax.RovuraxConfig.from_json, lambda
     cfg, w if w is not None else rovurax.random_weights(cfg, device=dev), device=dev)))
 register_family("LlamaForCausalLM", DecoderFamily(
     llama.LlamaConfig.from_json, lambda cfg, w, dev: llama.build_llama(cfg, external_weights=True, device=dev, paged=True, state=w),
-    lambda cfg, w, dev, block: llama.build_llama(cfg, external_weights=True, device=dev, paged=True, state=w, shared_prefix=True, block_size=block)))
+    lambda cfg, w, dev, block: llama.build_llama(cfg, external_weights=True, device=dev, paged=True, state=w, shared_prefix=True, block_size=block),
+    lambda cfg, w, dev: llama.build_llama(cfg, external_weights=True, device=dev, paged=True, state=w, draft_trees=True)))
 
 DTYPES = {"bfloat16": "bf16", "float16": "fp16", "float32": "fp32"}
 
@@ -52,19 +55,25 @@ def family_of(config: Mapping[str, Any]) -> DecoderFamily:
 
 def create_decoder(config: Mapping[str, Any], tensors: Optional[Mapping[str, torch.Tensor]], dtype: str = "bfloat16", *, batch: int = 1,
                    max_len: int = 2048, max_tokens: Optional[int] = None, block_size: int = 256, provider: str = "CUDAExecutionProvider",
-                   cuda_graph: bool = True, session_entries: Optional[Mapping[str, str]] = None, shared_prefix: bool = False) -> PagedDecoderRunner:
+                   cuda_graph: bool = True, session_entries: Optional[Mapping[str, str]] = None, shared_prefix: bool = False,
+                   draft_trees: bool = False) -> PagedDecoderRunner:
     """A decoder with room for ``batch`` sequences of at most ``max_len`` tokens; ``max_tokens`` bounds the tokens that all
     of them hold together (default: no further bound).  float32 runs every product in true 32-bit.  ``shared_prefix``: the
     form that attends to the tokens that all sequences of a batch begin with once for all of them, with room for one
-    sequence more, which holds them."""
+    sequence more, which holds them.  ``draft_trees``: the form for steps with drafted tokens."""
     family = family_of(config)
+    if draft_trees and family.build_drafts is None:
+        raise ValueError(f"architecture {config.get('architecture') or config.get('architectures')!r} has no form for drafted tokens")
+    if shared_prefix and draft_trees:
+        raise ValueError("a decoder has the form for a shared prefix or the one for drafted tokens")
     per_seq = (max_len + block_size - 1) // block_size
     cfg = family.config(config, DTYPES[dtype], per_seq * block_size)
     gpu = provider == "CUDAExecutionProvider"
     if shared_prefix and family.build_shared is None:
         raise ValueError(f"architecture {config.get('architecture') or config.get('architectures')!r} has no form for a shared prefix")
     device = "cuda" if gpu else "cpu"
-    model, weights = family.build_shared(cfg, tensors, device, block_size) if shared_prefix else family.build(cfg, tensors, device)
+    model, weights = (family.build_shared(cfg, tensors, device, block_size) if shared_prefix else family.build_drafts(cfg, tensors, device) if draft_trees else
+                      family.build(cfg, tensors, device))
     so = SessionOptions()
     so.add_external_initializers(list(weights.keys()), list(weights.values()))
     for k, v in {"ortb200.pdl": "1", **(session_entries or {})}.items():

@@ -23,6 +23,9 @@ def main(argv=None) -> int:
     ap.add_argument("--top-k", type=int, default=0)
     ap.add_argument("--top-p", type=float, default=1.0)
     ap.add_argument("--repetition-penalty", type=float, default=1.0)
+    ap.add_argument("--presence-penalty", type=float, default=0.0)
+    ap.add_argument("--frequency-penalty", type=float, default=0.0)
+    ap.add_argument("--draft-tokens", type=int, default=0, help="tokens that a step may draft from the request's own text")
     ap.add_argument("--seed", type=int, default=None, help="sampling with this seed (greedy without it, top-k and top-p)")
     ap.add_argument("--shared-prompt-ids", default="", help="comma-separated token ids in front of every prompt; they run once")
     ap.add_argument("--logprobs", type=int, default=None, help="also report log probabilities, entropies and that many alternatives")
@@ -34,10 +37,12 @@ def main(argv=None) -> int:
     shared = [int(t) for t in a.shared_prompt_ids.split(",") if t]
     longest = len(shared) + max(len(p) for p in prompts) + a.max_new_tokens
     runner = load_decoder(a.model, a.dtype, batch=min(a.batch, len(prompts)), max_len=longest,
-                          provider="CUDAExecutionProvider" if a.provider == "cuda" else "CPUExecutionProvider", shared_prefix=bool(shared))
+                          provider="CUDAExecutionProvider" if a.provider == "cuda" else "CPUExecutionProvider", shared_prefix=bool(shared),
+                          draft_trees=a.draft_tokens > 0)
     outs = generate_requests(runner, prompts, GenerationConfig(
         max_new_tokens=a.max_new_tokens, eos_token_id=a.eos_token_id, temperature=a.temperature, top_k=a.top_k, top_p=a.top_p,
-        repetition_penalty=a.repetition_penalty, seed=a.seed, logprobs=a.logprobs), shared)
+        repetition_penalty=a.repetition_penalty, seed=a.seed, logprobs=a.logprobs,
+        presence_penalty=a.presence_penalty, frequency_penalty=a.frequency_penalty, draft_tokens=a.draft_tokens), shared)
     for prompt, out in zip(prompts, outs):
         if a.logprobs is None:
             print(json.dumps({"prompt": prompt, "generated": out}), flush=True)
