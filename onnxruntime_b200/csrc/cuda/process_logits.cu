@@ -1,9 +1,10 @@
 // Penalties for repeated tokens, biases, masks and temperatures on logits (com.ortb200.ProcessLogits).
 //
 // Every logit is read once and every score written once.  A CTA has a chunk of a row's vocabulary, with a counter per token in shared
-// memory, and three passes: it reads the row's whole text and counts the tokens of its chunk; it streams the chunk through
-// mask and temperature, which asks nothing of the counters; then it works the counted tokens out again, few of the chunk, and
-// last the biased ones.  No CTA waits for another, and counting commutes: no result depends on an order of arrival.
+// memory.  It asks its logits into L2, reads the row's whole text and biases and counts and flags the tokens of its chunk, and streams the
+// chunk through temperature and mask.  The few tokens that are touched are listed, and worked out again behind the stream; where
+// they are more than the list holds, the stream looks at every counter.  No CTA waits for another, and counting commutes: no result
+// depends on an order of arrival.
 #include <cuda_runtime.h>
 #include <math.h>
 #include "draft_ops.h"
@@ -12,10 +13,47 @@
 namespace ortb200 {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kMaxChunk = 16384;      // counters of a CTA: 64 KB, three CTAs to an SM
+constexpr int kMaxChunk = 16384;      // counters of a CTA: 64 KB
+constexpr int kList = 1024;           // touched tokens of a chunk that are listed
+constexpr int kBiases = 256;          // biases of a chunk that are
 constexpr int kMaxVocab = 0x7fff0000; // an index plus the tokens of a pass fits 31 bits
 constexpr unsigned kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3fffffffu;
+
+// Quotients by one divisor of a whole row: with its rounded reciprocal r, q = x r is off by a unit or so, the remainder x - q d is exact in
+// a fused multiply-add, and q + r (x - q d) is the quotient rounded once (P. Markstein, IBM Journal of Research and Development 34, 1990;
+// numbers below 2^-100, whose remainders 32 bits do not hold, are within 3 times that).
+// A division for every logit takes some twenty instructions, 48 in all for each logit of logits that are masked and
+// scaled.
+struct Divisor {
+  float d, r;   // r: NaN where the reciprocal's exponent leaves no room for the remainder
+  __device__ __forceinline__ explicit Divisor(float by) : d(by), r(fabsf(by) > 0x1p-100f && fabsf(by) < 0x1p100f ? 1.f / by : NAN) {}
+  __device__ __forceinline__ float special(float x, float q) const { return r == r ? q : x / d; }   // infinities, and what overflows
+  __device__ __forceinline__ float operator()(float x) const {
+    const float q = x * r, y = fmaf(fmaf(-q, d, x), r, q);
+    return y == y ? y : special(x, q);
+  }
+  template <int N>
+  __device__ __forceinline__ void all(float* f) const {
+    const f32x2 r2 = pack2(r, r), minus = pack2(-d, -d), one = pack2(1.f, 1.f);
+    f32x2 x[N / 2], q[N / 2], y[N / 2], sum = pack2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      x[i] = pack2(f[2 * i], f[2 * i + 1]);
+      q[i] = mul2(x[i], r2);
+      y[i] = fma2(fma2(q[i], minus, x[i]), r2, q[i]);
+      sum = fma2(y[i], one, sum);
+    }
+    float s0, s1;
+    unpack2(sum, s0, s1);
+    if (s0 + s1 == s0 + s1) {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) unpack2(y[i], f[2 * i], f[2 * i + 1]);
+    } else {   // one of them is no number, or the sum of two infinities
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = (*this)(f[i]);
+    }
+  }
+};
 
 // What a row asks for besides its text.
 struct RowRules {
@@ -49,18 +87,83 @@ __device__ __forceinline__ RowRules rules_of(const ortb200_process_logits_args& 
   if (bad && report && a.status) atomicExch(a.status, kStatusBadArgument);
   return q;
 }
-__device__ __forceinline__ float penalised(const RowRules& q, float x, unsigned word) {
+__device__ __forceinline__ float penalised(const RowRules& q, const Divisor& repeated, float x, unsigned word) {
   if (word & ~kBiased) {   // somewhere in the text
-    x = x < 0.f ? x * q.repetition : x / q.repetition;
+    x = x < 0.f ? x * q.repetition : repeated(x);
     const unsigned c = word & kCount;
     if (c) x -= q.frequency * static_cast<float>(c) + q.presence;
   }
   return x;
 }
-__device__ __forceinline__ float finished(const RowRules& q, float x, bool allowed) {
-  if (q.temperature != 1.f) x = x / q.temperature;
-  return allowed ? x : -INFINITY;
+
+// The text of a row: history [begin, end), of which what lies from `counted` on counts, and its row of drafted tokens.
+struct Text {
+  long long begin, end, counted;
+  int drafted;
+  bool bad;
+  // (Asked for beside the row's rules: every load that waits for another adds most of a microsecond to a CTA that has some eight.)
+  __device__ __forceinline__ Text(const ortb200_process_logits_args& a, long long r) : begin(0), end(0), counted(0), drafted(a.drafted ? a.drafted_width : 0), bad(false) {
+    if (!a.history) return;
+    const long long l = a.row_list ? a.row_list[r] : r;
+    bad = l >= a.lists;
+    if (l < 0 || bad) return;
+    begin = a.history_starts[l];
+    end = a.history_starts[l + 1];
+    counted = a.generated_starts ? a.generated_starts[l] : 0;
+    bad = begin < 0 || end < begin || end > a.history_len;
+    if (bad) begin = end = 0;
+  }
+  __device__ __forceinline__ bool any() const { return end > begin || drafted > 0; }
+};
+// add(token, whether it counts) for every token of the text, by all threads: two tokens to a load, AHEAD loads of a thread on their way
+template <int THREADS, int AHEAD, typename F>
+__device__ __forceinline__ void for_text(const ortb200_process_logits_args& a, const Text& t, long long r, F add) {
+  const long long odd = min(t.begin + static_cast<long long>((reinterpret_cast<uintptr_t>(a.history + t.begin) >> 3) & 1), t.end), pairs = (t.end - odd) / 2;
+  if (threadIdx.x == 0 && odd > t.begin) add(a.history[t.begin], t.begin >= t.counted);
+  if (threadIdx.x == 32 && odd + 2 * pairs < t.end) add(a.history[t.end - 1], t.end - 1 >= t.counted);
+  const longlong2* two = reinterpret_cast<const longlong2*>(a.history + odd);
+  const int n = static_cast<int>(pairs), from = static_cast<int>(min(max(t.counted - odd, -1ll), 2 * pairs));   // (a history has fewer than 2^30 tokens)
+  for (int i = threadIdx.x; i < n; i += AHEAD * THREADS) {
+    longlong2 v[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (i + k * THREADS < n) v[k] = __ldg(two + i + k * THREADS);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (i + k * THREADS < n) {
+        const int at = 2 * (i + k * THREADS);
+        add(v[k].x, at >= from);
+        add(v[k].y, at + 1 >= from);
+      }
+  }
+  for (int d = threadIdx.x; d < t.drafted; d += THREADS) add(a.drafted[r * a.drafted_width + d], true);
 }
+
+// A score from its logit: penalties by the token's counter, its bias, the temperature, the mask.
+template <typename T>
+struct Scorer {
+  const T* x;
+  float* y;
+  const RowRules& q;
+  const Divisor &warmth, &repeated;
+  __device__ __forceinline__ bool allowed(int v) const { return !q.mask || (__ldg(q.mask + (v >> 5)) >> (v & 31) & 1); }
+  __device__ __forceinline__ float finished(int v, float f) const {
+    if (q.temperature != 1.f) f = warmth(f);
+    return allowed(v) ? f : -INFINITY;
+  }
+  __device__ __forceinline__ void whole(int v, unsigned word, float bias) const { y[v] = finished(v, penalised(q, repeated, to_float<T>(x[v]), word) + bias); }
+};
+
+// How a row is divided: its vectors start at the first token whose place in the tensor E divides; what is in front of them is the first
+// CTA's, and the last tokens, fewer than a vector, belong to whoever has what is in front of those.
+struct Chunks {
+  int vocab, chunk, lead, tail, tail_part;
+  __device__ __forceinline__ Chunks(int vocabulary, long long r, int E, int size) : vocab(vocabulary), chunk(size) {
+    lead = E == 1 ? 0 : min(static_cast<int>((E - r * vocab % E) % E), vocab);
+    tail = lead + (vocab - lead) / E * E;
+    tail_part = tail > lead ? (tail - lead - 1) / chunk : 0;
+  }
+};
 
 template <typename T>
 __device__ __forceinline__ void unpack(const uint4& v, float* f) {
@@ -69,199 +172,197 @@ __device__ __forceinline__ void unpack(const uint4& v, float* f) {
   for (int i = 0; i < 16 / static_cast<int>(sizeof(T)); ++i) f[i] = to_float<T>(t[i]);
 }
 
-// E: logits of a vector (1: any alignment).  TEXT: rows may have texts.
-template <typename T, int E, bool TEXT>
-__global__ void __launch_bounds__(kThreads, 3) process_logits_kernel(const ortb200_process_logits_args a, const int chunk, const int parts) {
-  extern __shared__ __align__(16) unsigned counts[];   // [chunk + 2 E]: a row's first tokens may lie in front of the first vector, its last ones behind the last
+// Where a CTA is: tokens [first, end) of row r, the vectors among them, and the token of counter 0 (a row's first tokens may lie in front of
+// the first vector, its last ones behind the last).
+struct Place {
+  int body0, vectors, first, end, base;
+  __device__ __forceinline__ Place(const Chunks& c, int part, int E) {
+    body0 = c.lead + part * c.chunk;
+    const int body1 = min(body0 + c.chunk, c.tail);
+    vectors = max(body1 - body0, 0) / E;
+    first = part == 0 ? 0 : body0;
+    end = part == c.tail_part ? c.vocab : part < c.tail_part ? body1 : first;
+    base = body0 - E;
+  }
+};
+
+// E: logits of a vector (1: any alignment).  TOUCHED: rows may have texts or biases; else the stream alone.
+template <typename T, int E, bool TOUCHED, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 2) process_logits_kernel(const ortb200_process_logits_args a, const int chunk, const int parts) {
+  extern __shared__ __align__(16) unsigned counts[];            // [chunk + 2 E + 4]
+  __shared__ int listed, biases, twice;
+  __shared__ uint16_t list[TOUCHED ? kList : 1], biased[TOUCHED ? kBiases : 1];   // of counters
+  __shared__ float bias_of[TOUCHED ? kBiases : 1];
   const int part = static_cast<int>(blockIdx.x % parts);
   const long long r = blockIdx.x / parts;
   pdl_wait_prior_grids();
   const T* x = static_cast<const T*>(a.logits) + r * a.vocab;
   float* y = a.scores + r * a.vocab;
-  // the row's vectors start at the first token whose place in the tensor E divides; what is in front of them is the first CTA's
-  const int lead = E == 1 ? 0 : min(static_cast<int>((E - r * a.vocab % E) % E), a.vocab);
-  const int tail = lead + (a.vocab - lead) / E * E;                   // the last tokens, fewer than a vector: the CTA's that has what is in front of them
-  const int tail_part = tail > lead ? (tail - lead - 1) / chunk : 0;
-  const int body0 = lead + part * chunk, body1 = min(body0 + chunk, tail), vectors = max(body1 - body0, 0) / E;   // the chunk
-  const int first = part == 0 ? 0 : body0, end = part == tail_part ? a.vocab : part < tail_part ? body1 : first;  // with what is left over
-  const int base = body0 - E;                                         // the token of counter 0
+  const Chunks c(a.vocab, r, E, chunk);
+  const Place at(c, part, E);
+  for (int i = threadIdx.x; i * 128 < at.vectors * E * static_cast<int>(sizeof(T)); i += THREADS)   // on their way while the row's rules and text come
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(x + at.body0) + i * 128));
+  const Text t(a, r);
   const RowRules q = rules_of(a, r, part == 0 && threadIdx.x == 0);
+  const Divisor warmth(q.temperature), repeated(q.repetition);
+  const Scorer<T> s = {x, y, q, warmth, repeated};
 
-  bool text = false;
-  if constexpr (TEXT) {
-    long long h0 = 0, h1 = 0, counted = 0;
-    const bool asks = q.repetition != 1.f || q.presence != 0.f || q.frequency != 0.f;
-    if (asks && a.history) {
-      const long long l = a.row_list ? a.row_list[r] : r;
-      bool bad = l >= a.lists;
-      if (l >= 0 && !bad) {
-        h0 = a.history_starts[l];
-        h1 = a.history_starts[l + 1];
-        bad = h0 < 0 || h1 < h0 || h1 > a.history_len;
-        if (bad) h0 = h1 = 0;
-        counted = a.generated_starts ? a.generated_starts[l] : h0;
-      }
-      if (bad && part == 0 && threadIdx.x == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
-    }
-    const int drafted = asks && a.drafted ? a.drafted_width : 0;
-    text = h1 > h0 || drafted > 0;
-    if (text) {
-      for (int i = threadIdx.x; i < (chunk + 2 * E + 3) / 4; i += kThreads) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
+  bool touched = false, dense = false;   // dense: the stream looks at the counters, and there is no list
+  if constexpr (TOUCHED) {
+    const bool asks = q.repetition != 1.f || q.presence != 0.f || q.frequency != 0.f, text = asks && t.any();   // (a row without penalties has no use for its text)
+    if (asks && t.bad && part == 0 && threadIdx.x == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
+    touched = text || q.bias1 > q.bias0;
+    if (touched) {
+      if (threadIdx.x == 0) listed = biases = twice = 0;
+      for (int i = threadIdx.x; i < (chunk + 2 * E + 4) / 4; i += THREADS) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
       __syncthreads();
-      const unsigned size = static_cast<unsigned>(end - first);
-      auto add = [&](long long v, bool count) {
-        const unsigned long long at = static_cast<unsigned long long>(v - first);
-        if (at >= size) return;
-        unsigned* to = counts + (first - base) + static_cast<unsigned>(at);
-        if (count) atomicAdd(to, 1u);
-        else atomicOr(to, kSeen);
+      const unsigned size = static_cast<unsigned>(at.end - at.first);
+      auto counter_of = [&](long long v) -> int {   // -1: another CTA's token, or none
+        const unsigned u = static_cast<unsigned>(v) - static_cast<unsigned>(at.first);
+        return u >= size || static_cast<unsigned long long>(v) >> 32 ? -1 : at.first - at.base + static_cast<int>(u);
       };
-      // two tokens to a load, four loads of a thread on their way
-      constexpr int kAhead = 4;
-      const long long odd = min(h0 + static_cast<long long>((reinterpret_cast<uintptr_t>(a.history + h0) >> 3) & 1), h1), pairs = (h1 - odd) / 2;
-      if (threadIdx.x == 0 && odd > h0) add(a.history[h0], h0 >= counted);
-      if (threadIdx.x == 32 && odd + 2 * pairs < h1) add(a.history[h1 - 1], h1 - 1 >= counted);
-      const longlong2* two = reinterpret_cast<const longlong2*>(a.history + odd);
-      long long i = threadIdx.x;
-      for (; i + (kAhead - 1) * kThreads < pairs; i += kAhead * kThreads) {
-        longlong2 v[kAhead];
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) v[k] = __ldg(two + i + k * kThreads);
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-          const long long at = odd + 2 * (i + k * kThreads);
-          add(v[k].x, at >= counted);
-          add(v[k].y, at + 1 >= counted);
+      auto to_list = [&](int i) {
+        const int n = atomicAdd(&listed, 1);
+        if (n < kList) list[n] = static_cast<uint16_t>(i);
+      };
+      dense = text && t.end - t.begin > static_cast<long long>(parts) * kList;   // too many to be listed, most likely
+      for (long long b = q.bias0 + threadIdx.x; b < q.bias1; b += THREADS) {
+        const int i = counter_of(a.bias_tokens[b]);
+        if (i < 0) continue;
+        const unsigned was = atomicOr(&counts[i], kBiased);
+        if (was & kBiased) twice = 1;   // (whoever writes, writes the same)
+        if (was == 0) to_list(i);
+        const int n = atomicAdd(&biases, 1);
+        if (n < kBiases) {
+          biased[n] = static_cast<uint16_t>(i);
+          bias_of[n] = a.bias_values[b];
         }
       }
-      for (; i < pairs; i += kThreads) {
-        const longlong2 v = __ldg(two + i);
-        add(v.x, odd + 2 * i >= counted);
-        add(v.y, odd + 2 * i + 1 >= counted);
+      if (text) {
+        for_text<THREADS, THREADS == 256 ? 4 : 8>(a, t, r, [&](long long v, bool count) {
+          const int i = counter_of(v);
+          if (i < 0) return;
+          if (dense) {
+            if (count) atomicAdd(&counts[i], 1u);
+            else atomicOr(&counts[i], kSeen);
+          } else if ((count ? atomicAdd(&counts[i], 1u) : atomicOr(&counts[i], kSeen)) == 0) {
+            to_list(i);
+          }
+        });
       }
-      for (int d = threadIdx.x; d < drafted; d += kThreads) add(a.drafted[r * a.drafted_width + d], true);
+      __syncthreads();
+      dense = dense || listed > kList;
     }
   }
 
   // ------------------------------------------------------------------------------------------------------ the chunk's vectors
-  auto allowed = [&](int v) { return !q.mask || (__ldg(q.mask + (v >> 5)) >> (v & 31) & 1); };
   constexpr int kAhead = E == 1 ? 8 : 4;
-  for (int i0 = 0; i0 < vectors; i0 += kAhead * kThreads) {
+  for (int i0 = 0; i0 < at.vectors; i0 += kAhead * THREADS) {
     T one[E == 1 ? kAhead : 1];
     uint4 many[E == 1 ? 1 : kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int at = i0 + i * kThreads + threadIdx.x;
-      if (at < vectors) {
-        if constexpr (E == 1) one[i] = x[body0 + at];
-        else many[i] = __ldg(reinterpret_cast<const uint4*>(x + body0) + at);
+      const int n = i0 + i * THREADS + threadIdx.x;
+      if (n < at.vectors) {
+        if constexpr (E == 1) one[i] = x[at.body0 + n];
+        else many[i] = __ldg(reinterpret_cast<const uint4*>(x + at.body0) + n);
       }
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int at = i0 + i * kThreads + threadIdx.x, v = body0 + at * E;
-      if (at >= vectors) continue;
+      const int n = i0 + i * THREADS + threadIdx.x, v = at.body0 + n * E;
+      if (n >= at.vectors) continue;
       if constexpr (E == 1) {
-        y[v] = finished(q, to_float<T>(one[i]), allowed(v));
+        y[v] = s.finished(v, penalised(q, repeated, to_float<T>(one[i]), TOUCHED && dense ? counts[v - at.base] : 0u));
       } else {
         float f[E];
         unpack<T>(many[i], f);
-        if (q.temperature != 1.f)   // in front of the mask: infinities take the long way through a division (18 instead of 5 us for 150 rows of 32000)
+        if (TOUCHED && dense) {
+          unsigned w[E];
 #pragma unroll
-          for (int e = 0; e < E; ++e) f[e] = f[e] / q.temperature;
+          for (int e = 0; e < E; e += 4) *reinterpret_cast<uint4*>(w + e) = *reinterpret_cast<const uint4*>(counts + v - at.base + e);
+#pragma unroll
+          for (int e = 0; e < E; ++e) f[e] = penalised(q, repeated, f[e], w[e]);
+        }
+        if (q.temperature != 1.f) warmth.all<E>(f);
         if (q.mask) {   // E bits from bit v on; they may lie in two words
           const int w0 = v >> 5, w1 = (v + E - 1) >> 5;
           const unsigned lo = __ldg(q.mask + w0), hi = w1 != w0 ? __ldg(q.mask + w1) : 0u, bits = __funnelshift_r(lo, hi, v & 31);
 #pragma unroll
-          for (int e = 0; e < E; ++e) f[e] = bits >> e & 1 ? f[e] : -INFINITY;
+          for (int e = 0; e < E; ++e) f[e] = bits & 1u << e ? f[e] : -INFINITY;
         }
 #pragma unroll
         for (int e = 0; e < E; e += 4) __stcs(reinterpret_cast<float4*>(y + v + e), make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]));
       }
     }
   }
-  auto whole = [&](int v, unsigned word, float bias) { y[v] = finished(q, penalised(q, to_float<T>(x[v]), word) + bias, allowed(v)); };
   if (E > 1) {
-    if (part == 0 && static_cast<int>(threadIdx.x) < lead) whole(threadIdx.x, 0u, 0.f);
-    if (part == tail_part && static_cast<int>(threadIdx.x) < a.vocab - tail) whole(tail + threadIdx.x, 0u, 0.f);
-  }
-  if (text) {   // ----------------------------------------------------------------------------------------------------- the text's tokens
-    __syncthreads();
-    const int last = end - base;
-    for (int i = 4 * threadIdx.x; i < last; i += 4 * kThreads) {
-      const uint4 w = *reinterpret_cast<const uint4*>(counts + i);
-      if (w.x) whole(base + i, w.x, 0.f);
-      if (w.y) whole(base + i + 1, w.y, 0.f);
-      if (w.z) whole(base + i + 2, w.z, 0.f);
-      if (w.w) whole(base + i + 3, w.w, 0.f);
-    }
+    const int t = static_cast<int>(threadIdx.x), v = t < E ? t : c.tail + t - E;
+    if (t < E ? part == 0 && v < c.lead : part == c.tail_part && v < a.vocab) s.whole(v, touched ? counts[v - at.base] : 0u, 0.f);
   }
 
-  // --------------------------------------------------------------------------------------------------------------- biases
-  // A token's flag tells whether it has several: who finds it set has come second.  Without a text only the counters of biased tokens
-  // are in use.
-  if (q.bias1 > q.bias0) {
-    __shared__ int twice;
-    auto mine = [&](long long b) -> int {   // the counter of a bias's token, -1 where it is another CTA's or none
+  // -------------------------------------------------------------------------------------------------------- what is touched
+  if constexpr (TOUCHED) {
+    if (!touched) return;
+    __syncthreads();   // the stream's scores have been written
+    const bool apart = dense || twice || biases > kBiases;   // biases are worked out by themselves
+    if (!dense)
+      for (int i = threadIdx.x; i < listed; i += THREADS) {
+        const int n = list[i];
+        const unsigned word = counts[n];
+        float bias = 0.f;
+        if (word & kBiased) {
+          if (apart) continue;
+          for (int k = 0; k < biases; ++k)
+            if (biased[k] == n) bias = bias_of[k];
+        }
+        s.whole(at.base + n, word, bias);
+      }
+    if (!apart) return;
+    // rare, or a long text: of several biases of a token the first looks for the others and sums them up in their order
+    for (long long b = q.bias0 + threadIdx.x; b < q.bias1; b += THREADS) {
       const long long v = a.bias_tokens[b];
-      return v >= first && v < end ? static_cast<int>(v) - base : -1;
-    };
-    if (threadIdx.x == 0) twice = 0;
-    if (!text)
-      for (long long b = q.bias0 + threadIdx.x; b < q.bias1; b += kThreads) {
-        const int at = mine(b);
-        if (at >= 0) counts[at] = 0;
+      if (v < at.first || v >= at.end) continue;
+      bool leads = true;
+      float sum = a.bias_values[b];
+      if (twice) {
+        for (long long o = q.bias0; o < b && leads; ++o) leads = a.bias_tokens[o] != v;
+        for (long long o = b + 1; o < q.bias1 && leads; ++o)
+          if (a.bias_tokens[o] == v) sum += a.bias_values[o];
       }
-    __syncthreads();   // also: the passes above have written what is written again here
-    for (long long b = q.bias0 + threadIdx.x; b < q.bias1; b += kThreads) {
-      const int at = mine(b);
-      if (at < 0) continue;
-      const unsigned word = atomicOr(&counts[at], kBiased);
-      if (word & kBiased) twice = 1;   // (whoever writes, writes the same)
-      else whole(base + at, word, a.bias_values[b]);
+      if (leads) s.whole(static_cast<int>(v), counts[static_cast<int>(v) - at.base], sum);
     }
-    __syncthreads();
-    if (twice)   // rare: every bias looks for others of its token, and the first of several sums them up in their order
-      for (long long b = q.bias0 + threadIdx.x; b < q.bias1; b += kThreads) {
-        const int at = mine(b);
-        if (at < 0) continue;
-        const long long t = base + at;
-        bool leads = true, several = false;
-        for (long long o = q.bias0; o < b && leads; ++o) leads = a.bias_tokens[o] != t;
-        if (!leads) continue;
-        float sum = a.bias_values[b];
-        for (long long o = b + 1; o < q.bias1; ++o)
-          if (a.bias_tokens[o] == t) {
-            sum += a.bias_values[o];
-            several = true;
-          }
-        if (several) whole(base + at, counts[at], sum);
-      }
   }
 }
 
-template <typename T, int E, bool TEXT>
-int launch(const ortb200_process_logits_args* a, cudaStream_t stream) {
-  // Short chunks where rows are few, so that every SM has some; but a text is read once for each chunk, so not beyond where the usual text
-  // is as many bytes as the chunk.
-  const int64_t text = TEXT && a->history && a->lists > 0 ? 8 * (a->history_len / a->lists) : 0;
-  int chunk = kMaxChunk;
-  while (chunk > 2048 && a->rows * ((a->vocab + chunk - 1) / chunk) < 3 * 148 && text <= chunk / 2 * static_cast<int64_t>(sizeof(T) + 4)) chunk /= 2;
-  const long long parts = (a->vocab + chunk - 1) / chunk;
+template <typename T, int E, bool TOUCHED, int THREADS>
+int launch(const ortb200_process_logits_args* a, int64_t text_bytes, cudaStream_t stream) {
+  // Usually four vectors of logits to a thread.  Shorter chunks where rows are few, so that every SM has some, but, as a text is read once
+  // for each chunk, none that are fewer bytes than the usual text.
+  int chunk = THREADS == 512 ? kMaxChunk : 8192;
+  while (chunk > 2048 && a->rows * ((a->vocab + chunk - 1) / chunk) < 3 * 148 && text_bytes <= chunk / 2 * static_cast<int64_t>(sizeof(T) + 4)) chunk /= 2;
+  const long long parts = (a->vocab + static_cast<long long>(chunk) - 1) / chunk;
   if (a->rows * parts > 0x7fffffffll) return -2;
-  const int smem = TEXT || a->bias_tokens ? (chunk + 2 * E + 4) * 4 : 0;
-  auto kern = process_logits_kernel<T, E, TEXT>;
+  const int smem = TOUCHED ? (chunk + 2 * E + 4) * 4 : 0;
+  auto kern = process_logits_kernel<T, E, TOUCHED, THREADS>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMaxChunk + 64) * 4) != cudaSuccess) return -10;   // per device
-  return launch_kernel(kern, dim3(static_cast<unsigned>(a->rows * parts)), kThreads, smem, stream, a->use_pdl != 0, *a, chunk, static_cast<int>(parts));
+  return launch_kernel(kern, dim3(static_cast<unsigned>(a->rows * parts)), THREADS, smem, stream, a->use_pdl != 0, *a, chunk, static_cast<int>(parts));
+}
+
+template <typename T, int E>
+int launch_rows(const ortb200_process_logits_args* a, cudaStream_t stream) {
+  if (!a->history && !a->drafted && !a->bias_tokens) return launch<T, E, false, 256>(a, 0, stream);
+  // Every chunk reads the row's text.  Texts of up to 64 KB: chunks of 8192 and CTAs of 256 threads, six to an SM (384 rows of 128256 with 2250
+  // tokens 106 us; chunks of 16384 and CTAs of 512 threads 122).  Longer ones the other way: half as many bytes of text, and more of them on their
+  // way at a time (40 rows of 50257 with 45000 tokens 32 us instead of 45).
+  const int64_t text_bytes = a->history && a->lists > 0 ? 8 * (a->history_len / a->lists) : 0;
+  return text_bytes > 64 * 1024 ? launch<T, E, true, 512>(a, text_bytes, stream) : launch<T, E, true, 256>(a, text_bytes, stream);
 }
 
 template <typename T>
 int launch_type(const ortb200_process_logits_args* a, cudaStream_t stream) {
-  constexpr int E = 16 / sizeof(T);
   const bool aligned = ((reinterpret_cast<uintptr_t>(a->logits) | reinterpret_cast<uintptr_t>(a->scores)) & 15) == 0;
-  const bool text = a->history || a->drafted;
-  if (aligned) return text ? launch<T, E, true>(a, stream) : launch<T, E, false>(a, stream);
-  return text ? launch<T, 1, true>(a, stream) : launch<T, 1, false>(a, stream);
+  return aligned ? launch_rows<T, 16 / sizeof(T)>(a, stream) : launch_rows<T, 1>(a, stream);
 }
 
 }  // namespace

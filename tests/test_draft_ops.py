@@ -545,6 +545,31 @@ def test_logits_neutral_values(provider):
 
 
 @pytest.mark.parametrize("provider", PROVIDERS)
+def test_logits_quotients(provider):
+    """Temperatures and penalties of any size: quotients are rounded once, also where they overflow, underflow or divide infinities."""
+    g = torch.Generator().manual_seed(6)
+    by = torch.cat([torch.rand(40, generator=g) * 3 + 0.01, 10.0 ** torch.linspace(-44, 38, 40), torch.tensor([2 - 2.0 ** -23, 1 + 2.0 ** -23, 3.0, torch.finfo(torch.float32).max, 2.0 ** -149])])
+    x = torch.cat([torch.randn(3000, generator=g) * 10.0 ** (torch.rand(3000, generator=g) * 76 - 38), torch.tensor([0.0, -0.0, math.inf, -math.inf, math.nan, 2.0 ** -149, 3.4e38, -3.4e38])])
+    case = LogitsCase(torch.float32, len(by), len(x), without=NAMES[1:])
+    case.t.update(logits=x.expand(len(by), -1).contiguous(), temperature=by)
+    for repeated in (False, True):
+        if repeated:   # the same as penalties: only what is not below 0 is divided
+            case.t.pop("temperature")
+            case.t.update(history=torch.arange(len(x)), history_starts=i64(0, len(x)), row_list=torch.zeros(len(by), dtype=torch.int32), repetition=by)
+        got, exact = case.call(provider)()["scores"].double(), x.double() / by.double().unsqueeze(1)
+        if repeated:
+            exact = torch.where(x < 0, x.double() * by.double().unsqueeze(1), exact)
+        want = exact.float().double()
+        same = (got == want) | (got.isnan() & want.isnan())
+        # Half a unit in the last place of 32 bits (u = 2^-24 of the value), or of the smallest numbers.  A quotient q that is off by 1.5 u is mended with its
+        # remainder x - q d, which is exact unless it falls below what 32 bits hold, 2^-149: that takes |x| < 2^-100 (the remainder is at most 1.5 u |x|, and its
+        # last bit 2^-48 |x|).  There it is rounded to a multiple of 2^-149: to 0 while it is below 2^-150, which leaves 1.5 u, and otherwise
+        # |x| > 2^-150 / (1.5 u), so that an error of 2^-150 is 1.5 u of x.  With the last rounding that is within 3 u for such numbers.
+        units = torch.where(x.abs() < 2.0 ** -100, 3.0, 1.0).double()
+        assert (same | ((got - exact).abs() <= torch.clamp(units * exact.abs() * 2.0 ** -24, min=2.0 ** -149))).all()
+
+
+@pytest.mark.parametrize("provider", PROVIDERS)
 def test_logits_biases_of_one_token_count_in_their_order(provider):
     case = LogitsCase(torch.float32, 2, 64, without=NAMES[1:9] + ["allowed", "row_mask", "temperature"])
     case.t.update(bias_tokens=i64(*[3, 9, 3, 3, 9], *[5] * 300), bias_values=torch.cat([torch.tensor([1e8, 2.0, 1.0, -1e8, 0.5]), torch.full((300,), 0.25)]), bias_starts=i64(0, 5, 305))
@@ -596,6 +621,22 @@ def test_logits_on_odd_addresses(dt, vocab):
 def test_logits_sizes_of_models(dt, rows, vocab):
     """Up to what a cluster's counters hold, and one more."""
     LogitsCase(dt, rows, vocab, length=3000, biases=30, seed=1).run(GPU)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,rows,vocab,how", [(torch.bfloat16, 132, 128256, dict(lists=9, drafted=5)), (torch.float32, 335, 50257, dict(length=200, biases=300)),
+                                               (torch.float16, 525, 32003, dict(length=5500, lists=20)), (torch.bfloat16, 17000, 1000, dict(length=60)),
+                                               (torch.float32, 335, 50257, dict(without=NAMES[1:9])), (torch.float16, 525, 32003, dict(length=300, place=1))])
+def test_logits_of_large_batches(dt, rows, vocab, how):
+    """What rows touch is gathered in front of the stream; some of the texts of 5500 tokens touch more than is gathered."""
+    how = dict(how)
+    place = how.pop("place", None)
+    case = LogitsCase(dt, rows, vocab, seed=9, **{"biases": 12, **how})
+    got = case.call(GPU, place=place)()
+    rest = case.rows
+    assert rest * vocab >= 1 << 24
+    case.rows = min(rest, 100)                              # (the oracle takes its time)
+    case.check(got)
 
 
 @pytest.mark.gpu
