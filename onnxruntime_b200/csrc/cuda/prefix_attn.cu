@@ -216,12 +216,15 @@ __global__ void __launch_bounds__(128) prefix_rows_kernel(const ortb200_prefix_a
 // The reference maximum of a row is raised only when a tile exceeds it by 2^8 (weights stay below 256), so that O is rescaled a few
 // times per row.
 constexpr float kRaise = 8.f;
-constexpr int kQT = 128;          // query rows of a unit
+constexpr int kQT = 128;          // query rows of a unit, one for each lane of tensor memory
+constexpr int kWide = 256;        // of a unit of a batch whose sequences bring more rows than that: two tiles of rows, and one CTA to an SM
 constexpr int kKT = 64;           // keys of a tile
 constexpr int kFew = 8;           // units of so few rows go another way through the same tiles
-constexpr int kThreads = 192;
 constexpr int kGrid = 296;        // two CTAs on each of 148 SMs
-constexpr int kTmemCols = 256;    // two score buffers of 64 columns, O in up to 128
+constexpr int kTmemCols = 256;    // of a tile of rows: two score buffers of 64 columns, O in up to 128
+// Units of QT rows: CTAs of the grid, and their threads - a warp for loads, one for the products of each tile of rows, four for its softmax.
+template <int QT> constexpr int grid_of = QT == kQT ? kGrid : kGrid / 2;
+template <int QT> constexpr int threads_of = QT == kQT ? 192 : 384;
 constexpr int kPlanInSmem = 768;  // row tiles whose running sums a CTA keeps in shared memory
 
 // What follows from the lengths.
@@ -247,7 +250,7 @@ __host__ __device__ inline long long most_row_tiles(long long T, int B, int N, i
 __host__ __device__ inline long long plan_bytes(long long T, int B, int N, int Nk) {
   return up256(sizeof(Plan) + 8 * (most_row_tiles(T, B, N, Nk) + 1) + 4ll * (B + 1));
 }
-__host__ __device__ inline long long segment_rows(long long T, int N) { return 2 * T * N + static_cast<long long>(kGrid) * kQT; }
+__host__ __device__ inline long long segment_rows(long long T, int N) { return 2 * T * N + static_cast<long long>(kGrid) * kQT; }   // (grid_of<QT> x QT is the same for both)
 __host__ __device__ inline long long tree_bytes(long long T) { return up256(T * kTreeWords * 4); }
 template <bool TREE>
 __host__ __device__ inline Work work_of(const ortb200_prefix_attn_args& a) {
@@ -276,35 +279,45 @@ __host__ __device__ inline Work work_of(const ortb200_prefix_attn_args& a) {
 __device__ __forceinline__ int extra(int rows) { return rows > 32 ? 4 : 1; }
 __device__ __forceinline__ int places(int tiles, int rows) { return tiles > 0 ? tiles + extra(rows) : 0; }
 // The share of CTA i of `total` places starts at share(i); place x belongs to CTA owner(x).
-__device__ __forceinline__ long long share(long long total, int i) { return total * i / kGrid; }
+template <int QT>
+__device__ __forceinline__ long long share(long long total, int i) { return total * i / grid_of<QT>; }
+template <int QT>
 __device__ __forceinline__ int owner(long long total, long long x) {
-  if (total < 0x7fffffffll / kGrid) return static_cast<int>((static_cast<unsigned>(x + 1) * kGrid - 1) / static_cast<unsigned>(total));   // a 64-bit quotient costs five times as much
-  return static_cast<int>(((x + 1) * kGrid - 1) / total);
+  if (total < 0x7fffffffll / kGrid) return static_cast<int>((static_cast<unsigned>(x + 1) * grid_of<QT> - 1) / static_cast<unsigned>(total));   // a 64-bit quotient costs five times as much
+  return static_cast<int>(((x + 1) * grid_of<QT> - 1) / total);
 }
 
-// Unit `rt` (rows [128 rt, 128 rt + 128) of the sequence's rows x G) of a sequence: its keys [prefix keys, end) in tiles of 64.
+// Unit `rt` (rows [QT rt, QT rt + QT) of the sequence's rows x G) of a sequence: its keys [prefix keys, end) in tiles of 64.
+template <int QT>
 __device__ __forceinline__ int own_end(const ortb200_prefix_attn_args& a, int G, const Span& s, int rt) {
-  const int last = min(rt * kQT + kQT, s.rows * G) - 1;
+  const int last = min(rt * QT + QT, s.rows * G) - 1;
   return static_cast<int>(min(static_cast<long long>(s.past) + last / G + 1, static_cast<long long>(a.max_blocks) * a.block_size));
 }
+template <int QT>
 __device__ __forceinline__ int own_tiles(const ortb200_prefix_attn_args& a, int G, const Span& s, int rt, int prefix_tiles) {
-  return max((own_end(a, G, s, rt) + kKT - 1) / kKT - prefix_tiles, 0);
+  return max((own_end<QT>(a, G, s, rt) + kKT - 1) / kKT - prefix_tiles, 0);
 }
-__device__ __forceinline__ int row_tiles(int G, int rows) { return (rows * G + kQT - 1) / kQT; }
-__device__ __forceinline__ int unit_rows(int G, int rows, int rt) { return min(kQT, rows * G - rt * kQT); }
+template <int QT>
+__device__ __forceinline__ int row_tiles(int G, int rows) { return (rows * G + QT - 1) / QT; }
+template <int QT>
+__device__ __forceinline__ int unit_rows(int G, int rows, int rt) { return min(QT, rows * G - rt * QT); }
+template <int QT>
 __device__ __forceinline__ int own_places(const ortb200_prefix_attn_args& a, int G, const Span& s, int rt, int prefix_tiles) {
-  return places(own_tiles(a, G, s, rt, prefix_tiles), unit_rows(G, s.rows, rt));
+  return places(own_tiles<QT>(a, G, s, rt, prefix_tiles), unit_rows<QT>(G, s.rows, rt));
 }
 // all units of the prefix are numbered like the first
+template <int QT>
 __device__ __forceinline__ long long prefix_places(const ortb200_prefix_attn_args& a, int G, int all_rows, int prefix_tiles) {
-  return static_cast<long long>(row_tiles(G, all_rows)) * a.Nk * places(prefix_tiles, unit_rows(G, all_rows, 0));
+  return static_cast<long long>(row_tiles<QT>(G, all_rows)) * a.Nk * places(prefix_tiles, unit_rows<QT>(G, all_rows, 0));
 }
-// first row that the segments of a unit may use, before 128 rows per CTA number: units follow one another without a gap
+// first row that the segments of a unit may use, before QT rows per CTA number: units follow one another without a gap
+template <int QT>
 __device__ __forceinline__ long long prefix_slot(const ortb200_prefix_attn_args& a, int rt, int kvh, int rows) {
-  return static_cast<long long>(rt) * kQT * a.Nk + static_cast<long long>(kvh) * rows;
+  return static_cast<long long>(rt) * QT * a.Nk + static_cast<long long>(kvh) * rows;
 }
+template <int QT>
 __device__ __forceinline__ long long own_slot(const ortb200_prefix_attn_args& a, int G, int row0, int rt, int kvh, int rows) {
-  return a.T * a.N + static_cast<long long>(a.Nk) * (static_cast<long long>(row0) * G + static_cast<long long>(rt) * kQT) + static_cast<long long>(kvh) * rows;
+  return a.T * a.N + static_cast<long long>(a.Nk) * (static_cast<long long>(row0) * G + static_cast<long long>(rt) * QT) + static_cast<long long>(kvh) * rows;
 }
 
 // the last of n ascending places that is not behind x
@@ -319,7 +332,7 @@ __device__ __forceinline__ int sequence_with(const I* places, int n, I x) {
 }
 // All THREADS of a CTA: how many tokens all sequences share, and where the own units of each row tile start (`first` and `tile0`,
 // written for all to read after the next barrier).
-template <int THREADS>
+template <int THREADS, int QT>
 __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, long long* first, int* tile0, int* status) {
   __shared__ int least_sm[THREADS / 32], row_sm[THREADS / 32];
   __shared__ long long sum_sm[THREADS / 32];
@@ -333,7 +346,7 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
     if (s.rows == 0) continue;
     least = min(least, s.past);
     row = min(row, b);
-    several |= s.rows * G > kQT;
+    several |= s.rows * G > QT;
   }
   least = __reduce_min_sync(0xffffffffu, least);
   row = __reduce_min_sync(0xffffffffu, row);
@@ -379,7 +392,7 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
       const unsigned with = __ballot_sync(0xffffffffu, some);
       if (b0 > 0) __syncthreads();
       if (lane == 31) tiles_sm[warp] = __popc(with);   // read behind the next barrier, as sum_sm is
-      const long long at = running(some ? static_cast<long long>(own_places(a, G, s, 0, p.prefix_tiles)) * a.Nk : 0, base, false);
+      const long long at = running(some ? static_cast<long long>(own_places<QT>(a, G, s, 0, p.prefix_tiles)) * a.Nk : 0, base, false);
       int tile = tiles + __popc(with & ((1u << lane) - 1));
 #pragma unroll
       for (int i = 0; i < THREADS / 32; ++i) {
@@ -393,14 +406,14 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
       tile0[a.B] = tiles;
       first[tiles] = base;
     }
-    p.total = base + prefix_places(a, G, all_rows, p.prefix_tiles);
+    p.total = base + prefix_places<QT>(a, G, all_rows, p.prefix_tiles);
     return p;
   }
   const long long most = most_row_tiles(a.T, a.B, a.N, a.Nk);   // more than these only lengths that overlap have: the rest is left out
   long long tiles = 0, base = 0;
   for (int b0 = 0; b0 < a.B; b0 += THREADS) {
     const int b = b0 + threadIdx.x;
-    const long long at = running(b < a.B ? row_tiles(G, span_of(a, b).rows) : 0, tiles, b0 > 0);
+    const long long at = running(b < a.B ? row_tiles<QT>(G, span_of(a, b).rows) : 0, tiles, b0 > 0);
     if (b < a.B) tile0[b] = static_cast<int>(min(at, most));
   }
   tiles = min(tiles, most);
@@ -411,26 +424,26 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
     long long n = 0;
     if (r < tiles) {
       const int b = sequence_with(tile0, a.B, r);
-      n = static_cast<long long>(own_places(a, G, span_of(a, b), r - tile0[b], p.prefix_tiles)) * a.Nk;
+      n = static_cast<long long>(own_places<QT>(a, G, span_of(a, b), r - tile0[b], p.prefix_tiles)) * a.Nk;
     }
     const long long at = running(n, base, r0 > 0);
     if (r < tiles) first[r] = at;
   }
   if (threadIdx.x == 0) first[tiles] = base;
-  p.total = base + prefix_places(a, G, all_rows, p.prefix_tiles);
+  p.total = base + prefix_places<QT>(a, G, all_rows, p.prefix_tiles);
   return p;
 }
 
 // Step 1: one CTA (or, for few tokens, several) per token and one more for the plan.  VEC: whole heads rotated in halves or not
 // at all, every address a multiple of 16 bytes: a thread moves 2 x 16 bytes; otherwise one element.
-template <typename T, bool VEC, bool TREE>
+template <typename T, bool VEC, bool TREE, int QT>
 __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefix_attn_args a, const int* parents) {
   const Work w = work_of<TREE>(a);
   pdl_wait_prior_grids();
   pdl_launch_dependents();   // behind the wait: when step 2 begins, everything in front of this step has ended
   if (blockIdx.x == a.T) {
     if (blockIdx.y != 0) return;
-    const Plan p = make_plan<128>(a, w.first, w.tile0, a.status);
+    const Plan p = make_plan<128, QT>(a, w.first, w.tile0, a.status);
     if (threadIdx.x == 0) *w.plan = p;
     return;
   }
@@ -514,22 +527,28 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
   }
 }
 
-template <int HD>
+template <int HD, int QT>
 struct TcSmem {
-  static constexpr int kStages = HD == 64 ? 3 : 2;
+  static constexpr int kRowTiles = QT / kQT;
+  static constexpr bool kOnce = QT == kWide;              // weights are rounded to the type once
+  static constexpr int kStages = QT == kQT ? (HD == 64 ? 3 : 2) : 4;
   static constexpr int kBoxes = HD / 64;                  // boxes of 64 elements per row
   static constexpr int kQBox = kQT * 128, kBox = kKT * 128;
   static constexpr int kStageBytes = 2 * kBoxes * kBox;   // K, then V
-  static constexpr int kOffKV = kBoxes * kQBox;
+  static constexpr int kQTile = kBoxes * kQBox;           // queries of a tile of rows
+  static constexpr int kOffKV = kRowTiles * kQTile;
   static constexpr int kOffBar = kOffKV + kStages * kStageBytes;
-  static constexpr int kOffFirst = kOffBar + 256;
-  static constexpr int kHalf = kQT / 2 * 128;             // the second of two places for queries of up to 64 rows
+  static constexpr int kOffFirst = kOffBar + 512;
+  static constexpr int kHalf = kQT / 2 * 128;             // the second of two places for queries of up to 64 rows (units of 128)
   static constexpr int kOffTile0 = kOffFirst + 8 * (kPlanInSmem + 1);
   static constexpr int kTotal = kOffTile0 + 4 * (kPlanInSmem + 1) + 1024;
 };
-enum { BAR_Q = 0, BAR_Q_FREE = BAR_Q + 2, BAR_K_FULL = BAR_Q_FREE + 2, BAR_K_EMPTY = BAR_K_FULL + 3, BAR_V_FULL = BAR_K_EMPTY + 3, BAR_V_EMPTY = BAR_V_FULL + 3, BAR_S = BAR_V_EMPTY + 3,
-       BAR_P = BAR_S + 2, BAR_O = BAR_P + 2, BAR_END, BAR_O_FREE, BAR_FEW, BAR_FEW_END = BAR_FEW + 4, BAR_COUNT = BAR_FEW_END + 2 };
-static_assert(BAR_COUNT * 8 + 4 <= 256, "barriers do not fit");
+constexpr int kMostStages = 4;
+enum { BAR_Q = 0, BAR_Q_FREE = BAR_Q + 2, BAR_K_FULL = BAR_Q_FREE + 2, BAR_K_EMPTY = BAR_K_FULL + kMostStages, BAR_V_FULL = BAR_K_EMPTY + kMostStages,
+       BAR_V_EMPTY = BAR_V_FULL + kMostStages, BAR_FEW = BAR_V_EMPTY + kMostStages, BAR_FEW_END = BAR_FEW + 4, BAR_TILE = BAR_FEW_END + 2,
+       // of each tile of rows:
+       BAR_S = 0, BAR_P = 2, BAR_O = 4, BAR_END = 5, BAR_O_FREE = 6, BAR_OF_TILE = 7, BAR_COUNT = BAR_TILE + 2 * BAR_OF_TILE };
+static_assert(BAR_COUNT * 8 + 4 <= 512, "barriers do not fit");
 
 // A CTA's share of one unit.
 struct Segment {
@@ -543,6 +562,7 @@ struct Segment {
   long long slot;
 };
 // The segments of a CTA one after the other: its first unit is searched for, the others follow from the one before.
+template <int QT>
 struct Walk {
   const ortb200_prefix_attn_args& a;
   const int* tile0;
@@ -555,9 +575,9 @@ struct Walk {
   __device__ Walk(const ortb200_prefix_attn_args& args, const long long* first, const int* tiles_of, const Plan& p, int cta)
       : a(args), tile0(tiles_of), G(args.N / args.Nk), prefix_tiles(p.prefix_tiles), prefix_row(p.prefix_row) {
     all_rows = last_row(a);
-    const long long prefix_total = prefix_places(a, G, all_rows, prefix_tiles);
-    long long x = share(p.total, cta);
-    left = share(p.total, cta + 1) - x;
+    const long long prefix_total = prefix_places<QT>(a, G, all_rows, prefix_tiles);
+    long long x = share<QT>(p.total, cta);
+    left = share<QT>(p.total, cta + 1) - x;
     seq = -1;
     rt = kvh = at = 0;
     if (left == 0) return;
@@ -583,29 +603,29 @@ struct Walk {
   }
   __device__ void prefix_unit() {
     tiles = prefix_tiles;
-    before = extra(unit_rows(G, all_rows, 0));
+    before = extra(unit_rows<QT>(G, all_rows, 0));
     unit.seq = -1;
-    unit.q_row = rt * kQT;
-    unit.rows = unit_rows(G, all_rows, rt);
+    unit.q_row = rt * QT;
+    unit.rows = unit_rows<QT>(G, all_rows, rt);
     unit.key0 = 0;
     unit.end = tiles * kKT;
     unit.past = unit.in_seq = 0;
     unit.table_row = prefix_row;
     unit.tree = false;
-    unit.slot = prefix_slot(a, rt, 0, unit.rows);
+    unit.slot = prefix_slot<QT>(a, rt, 0, unit.rows);
   }
   __device__ void own_unit() {
-    tiles = own_tiles(a, G, s, rt, prefix_tiles);
-    unit.rows = unit_rows(G, s.rows, rt);
+    tiles = own_tiles<QT>(a, G, s, rt, prefix_tiles);
+    unit.rows = unit_rows<QT>(G, s.rows, rt);
     before = tiles > 0 ? extra(unit.rows) : 0;
     unit.seq = unit.table_row = seq;
-    unit.in_seq = rt * kQT;
+    unit.in_seq = rt * QT;
     unit.q_row = s.row0 * G + unit.in_seq;
     unit.key0 = prefix_tiles * kKT;
-    unit.end = own_end(a, G, s, rt);
+    unit.end = own_end<QT>(a, G, s, rt);
     unit.past = s.past;
     unit.tree = s.rows <= kTreeNodes;
-    unit.slot = own_slot(a, G, s.row0, rt, 0, unit.rows);
+    unit.slot = own_slot<QT>(a, G, s.row0, rt, 0, unit.rows);
   }
   __device__ void step() {   // to the next unit that has tiles; there is one while places are left
     at = 0;
@@ -613,7 +633,7 @@ struct Walk {
     kvh = 0;
     ++rt;
     if (seq < 0) {
-      if (rt < row_tiles(G, all_rows)) {
+      if (rt < row_tiles<QT>(G, all_rows)) {
         prefix_unit();
         return;
       }
@@ -656,7 +676,8 @@ struct Walk {
   }
 };
 // Queries of up to 64 rows take one of two places in turn, so that the next segment's arrive while this one's are in use; more
-// take both.
+// take both.  (Wide units have one place: their segments are long.)
+template <int QT>
 struct QueryPlace {
   int place = 0;             // 0 or 1; 0 with `both`
   bool both = false;
@@ -666,6 +687,7 @@ struct QueryPlace {
   __device__ int fills() const { return place ? fills1 : fills0; }
   __device__ int uses() const { return place ? uses1 : uses0; }
   __device__ void take(int rows) {
+    if (QT != kQT) return;
     both = rows > kQT / 2;
     place = both ? 0 : turn;
     turn = both ? 0 : turn ^ 1;
@@ -805,10 +827,10 @@ __device__ __forceinline__ float sum_over_keys(float x) {
 // S, softmax and O with its hand-overs; so each of the four warps multiplies a quarter of a tile's keys itself, keys and dims as
 // the 16 rows of a product and the queries as its 8 columns: S^T = K Q^T, O^T += V^T P^T.  A warp has its own running maximum and
 // sums; they meet once per segment, in the place of the queries.
-template <int HD, bool BF16, int CAP, bool TREE>
+template <int HD, bool BF16, int CAP, bool TREE, int QT>
 __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, const Work& w, const Segment& g, uint8_t* smem, uint64_t* bars, float2 (*part)[kFew],
-                                         const QueryPlace& qp, float scale, int qw, int lane, int& stage, uint32_t& parity, int& few_tiles, int few_segments, bool& ok) {
-  using L = TcSmem<HD>;
+                                         const QueryPlace<QT>& qp, float scale, int qw, int lane, int& stage, uint32_t& parity, int& few_tiles, int few_segments, bool& ok) {
+  using L = TcSmem<HD, QT>;
   const int G = a.N / a.Nk, n0 = (lane & 3) * 2;
   float fs = scale * 1.4426950408889634f;
   const Cap<CAP> cap(scale, a.softcap);
@@ -954,7 +976,7 @@ __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, cons
         v[x + 3] += f * y.w;
       }
     }
-    const long long row = g.slot + static_cast<long long>(blockIdx.x) * kQT + n;
+    const long long row = g.slot + static_cast<long long>(blockIdx.x) * QT + n;
     if ((lane & 15) == 0) w.ml[row] = make_float2(m, l);
 #pragma unroll
     for (int x = 0; x < E; x += 4) *reinterpret_cast<float4*>(w.o + row * HD + d0 + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
@@ -964,12 +986,12 @@ __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, cons
   if (lane == 0) mbar_arrive(&bars[BAR_FEW_END + (few_segments & 1)]);
 }
 
-template <int HD, bool BF16, int CAP, bool TREE>
-__global__ void __launch_bounds__(kThreads, 2)
+template <int HD, bool BF16, int CAP, bool TREE, int QT>
+__global__ void __launch_bounds__(threads_of<QT>, QT == kQT ? 2 : 1)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                    const ortb200_prefix_attn_args a, const float scale) {
-  using L = TcSmem<HD>;
-  constexpr int STAGES = L::kStages;
+  using L = TcSmem<HD, QT>;
+  constexpr int STAGES = L::kStages, TILES = L::kRowTiles;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
@@ -983,11 +1005,15 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
-    for (int i = 0; i < BAR_COUNT; ++i) mbar_init(&bars[i], i == BAR_P || i == BAR_P + 1 || i >= BAR_O_FREE ? 4 : 1);
+    for (int i = 0; i < BAR_TILE + TILES * BAR_OF_TILE; ++i) {
+      const int of_tile = i < BAR_TILE ? -1 : (i - BAR_TILE) % BAR_OF_TILE;
+      const bool freed = (i >= BAR_Q_FREE && i < BAR_K_FULL) || (i >= BAR_K_EMPTY && i < BAR_V_FULL) || (i >= BAR_V_EMPTY && i < BAR_FEW);   // by each tile of rows
+      mbar_init(&bars[i], freed ? TILES : (i >= BAR_FEW && i < BAR_TILE) || of_tile == BAR_P || of_tile == BAR_P + 1 || of_tile == BAR_O_FREE ? 4 : 1);
+    }
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_alloc(tmem_slot, kTmemCols * TILES);
     tmem_relinquish();
   }
   // Step 1 has begun when this step begins, and what came before has ended: lengths, table and old cache entries may be read at
@@ -996,7 +1022,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   Plan plan;
   const bool kept = most_row_tiles(a.T, a.B, a.N, a.Nk) <= kPlanInSmem;
   if (kept) {
-    plan = make_plan<kThreads>(a, first_sm, tile0_sm, nullptr);
+    plan = make_plan<threads_of<QT>, QT>(a, first_sm, tile0_sm, nullptr);
   } else {
     pdl_wait_prior_grids();
     plan = *w.plan;
@@ -1004,10 +1030,13 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem_s = __reduce_or_sync(0xffffffffu, *tmem_slot);   // S / P: two buffers of 64 columns; the same for all, and known to be
+  const int tile = TILES == 1 ? 0 : warp >= 4 ? (warp - 4) >> 2 : max(warp - 1, 0);   // of rows, that a warp of the products or the softmax works on
+  const uint32_t tmem_base = __reduce_or_sync(0xffffffffu, *tmem_slot);                // the same for all, and known to be
+  const uint32_t tmem_s = tmem_base + tile * kTmemCols;                                // S / P: two buffers of 64 columns
   const uint32_t tmem_o = tmem_s + 2 * kKT;
+  uint64_t* tile_bars = bars + BAR_TILE + tile * BAR_OF_TILE;
 
-  Walk walk(a, kept ? first_sm : w.first, kept ? tile0_sm : w.tile0, plan, blockIdx.x);
+  Walk<QT> walk(a, kept ? first_sm : w.first, kept ? tile0_sm : w.tile0, plan, blockIdx.x);
   Segment g;
   bool ok = true;
 
@@ -1016,7 +1045,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const int piece = min(a.block_size, kKT), pieces = kKT / piece;   // rows that one block gives a tile
     int s = 0, k_tiles = 0, v_tiles = 0;
     uint32_t parity = 1;   // the first round over the stages waits for nothing
-    QueryPlace qp;
+    QueryPlace<QT> qp;
     bool waited = !kept, outside = false;
     auto wait_step1 = [&]() {
       if (waited) return;
@@ -1038,7 +1067,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         __syncwarp();
         if (lane < boxes)
           for (int bx = 0; bx < L::kBoxes; ++bx)
-            tma_load_3d(smem + bx * L::kQBox + qp.place * L::kHalf + lane * 2048, &tm_q, &bars[BAR_Q + qp.place], bx * 64, g.q_row + lane * 16, g.kvh);
+            tma_load_3d(smem + (TILES == 1 ? qp.place * L::kHalf + lane * 2048 : (lane >> 3) * L::kQTile + (lane & 7) * 2048) + bx * L::kQBox, &tm_q, &bars[BAR_Q + qp.place], bx * 64, g.q_row + lane * 16, g.kvh);
         qp.done();
         return true;
       };
@@ -1086,20 +1115,20 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     }
     if (outside && a.status) atomicExch(a.status, kStatusBadArgument);
     if (!ok && lane == 0 && a.status) atomicExch(a.status, kStatusTimeoutProducer);
-  } else if (warp == 1) {
+  } else if (warp <= TILES) {
     // ------------------------------------------------------------------------------------------------- products
     if (elect_one()) {
       constexpr uint32_t idesc_s = umma_idesc_f16(BF16, kQT, kKT), idesc_o = umma_idesc_f16_bmn(BF16, kQT, HD);
       const uint32_t kv_low = desc_low(smem_u32(smem + L::kOffKV), 16), v_low = desc_low(smem_u32(smem + L::kOffKV + L::kBoxes * L::kBox), L::kBox);
       int s = 0, seg = 0, it = 0;   // stage, segment and tile of this CTA
       uint32_t parity = 0;
-      QueryPlace qp;
-      auto issue_s = [&](int tile, int stage, bool last) {
-        const uint32_t q_low = desc_low(smem_u32(smem + qp.place * L::kHalf), 16), k_low = kv_low + stage * (L::kStageBytes >> 4), d = tmem_s + (tile & 1) * kKT;
+      QueryPlace<QT> qp;
+      auto issue_s = [&](int keys, int stage, bool last) {
+        const uint32_t q_low = desc_low(smem_u32(smem + (TILES == 1 ? qp.place * L::kHalf : tile * L::kQTile)), 16), k_low = kv_low + stage * (L::kStageBytes >> 4), d = tmem_s + (keys & 1) * kKT;
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
           mma_ss(d, q_low + (kk / 4) * (L::kQBox >> 4) + (kk % 4) * 2, k_low + (kk / 4) * (L::kBox >> 4) + (kk % 4) * 2, idesc_s, kk > 0 ? 1u : 0u);
-        umma_commit(&bars[BAR_S + (tile & 1)]);
+        umma_commit(&tile_bars[BAR_S + (keys & 1)]);
         umma_commit(&bars[BAR_K_EMPTY + stage]);
         if (last) {
           umma_commit(&bars[BAR_Q_FREE + qp.place]);
@@ -1108,6 +1137,23 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       };
       int few_tiles = 0, few_segments = 0;
       while (ok && walk.next(g)) {
+        if (TILES > 1 && tile > 0 && (g.rows <= kFew || g.rows <= tile * kQT)) {   // no rows here: what arrives is given back
+          for (int t = 0; t < g.tiles; ++t) {
+            if (!wait_bar(&bars[BAR_K_FULL + s], parity)) { ok = false; break; }
+            mbar_arrive(&bars[BAR_K_EMPTY + s]);
+            if (!wait_bar(&bars[BAR_V_FULL + s], parity)) { ok = false; break; }
+            mbar_arrive(&bars[BAR_V_EMPTY + s]);
+            if (++s == STAGES) {
+              s = 0;
+              parity ^= 1u;
+            }
+          }
+          // (the queries' own arrival keeps this tile from giving them back twice while the other one has them once)
+          if (ok && !wait_bar(&bars[BAR_Q + qp.place], qp.fills() & 1)) ok = false;
+          mbar_arrive(&bars[BAR_Q_FREE + qp.place]);
+          qp.done();
+          continue;
+        }
         if (g.rows <= kFew) {   // the other warps do these; what they have read goes back in the order of the tiles
           qp.take(g.rows);
           for (int t = 0; t < g.tiles; ++t, ++few_tiles) {
@@ -1126,7 +1172,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           continue;
         }
         // scores go over the weights of two tiles before; the products that read those are behind the last tile's, which are over
-        if (it > 0 && !wait_bar(&bars[BAR_O], (it - 1) & 1)) { ok = false; break; }
+        if (it > 0 && !wait_bar(&tile_bars[BAR_O], (it - 1) & 1)) { ok = false; break; }
         qp.take(g.rows);
         if (!wait_bar(&bars[BAR_Q + qp.place], qp.fills() & 1) || !wait_bar(&bars[BAR_K_FULL + s], parity)) { ok = false; break; }
         tcgen05_fence_after();
@@ -1135,22 +1181,23 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           const int s1 = s + 1 == STAGES ? 0 : s + 1;
           const uint32_t parity1 = s1 == 0 ? parity ^ 1u : parity;
           if (t + 1 < g.tiles) {
-            if (it > 0 && !wait_bar(&bars[BAR_O], (it - 1) & 1)) { ok = false; break; }
+            if (it > 0 && !wait_bar(&tile_bars[BAR_O], (it - 1) & 1)) { ok = false; break; }
             if (!wait_bar(&bars[BAR_K_FULL + s1], parity1)) { ok = false; break; }
             tcgen05_fence_after();
             issue_s(it + 1, s1, t + 2 == g.tiles);
           }
-          if (!wait_bar(&bars[BAR_V_FULL + s], parity) || !wait_bar(&bars[BAR_P + (it & 1)], (it >> 1) & 1)) { ok = false; break; }
-          if (t == 0 && seg > 0 && !wait_bar(&bars[BAR_O_FREE], (seg - 1) & 1)) { ok = false; break; }
+          if (!wait_bar(&bars[BAR_V_FULL + s], parity) || !wait_bar(&tile_bars[BAR_P + (it & 1)], (it >> 1) & 1)) { ok = false; break; }
+          if (t == 0 && seg > 0 && !wait_bar(&tile_bars[BAR_O_FREE], (seg - 1) & 1)) { ok = false; break; }
           tcgen05_fence_after();
           const uint32_t low = v_low + s * (L::kStageBytes >> 4), p = tmem_s + (it & 1) * kKT;
 #pragma unroll
           for (int kk = 0; kk < kKT / 16; ++kk) mma_ts(tmem_o, p + kk * 8, low + kk * (2048 >> 4), idesc_o, t > 0 || kk > 0 ? 1u : 0u);
 #pragma unroll
-          for (int kk = 0; kk < kKT / 16; ++kk) mma_ts(tmem_o, p + kKT / 2 + kk * 8, low + kk * (2048 >> 4), idesc_o, 1u);
-          umma_commit(&bars[BAR_O]);
+          for (int kk = 0; kk < kKT / 16; ++kk)
+            if (!L::kOnce) mma_ts(tmem_o, p + kKT / 2 + kk * 8, low + kk * (2048 >> 4), idesc_o, 1u);
+          umma_commit(&tile_bars[BAR_O]);
           umma_commit(&bars[BAR_V_EMPTY + s]);
-          if (t == g.tiles - 1) umma_commit(&bars[BAR_END]);
+          if (t == g.tiles - 1) umma_commit(&tile_bars[BAR_END]);
           s = s1;
           parity = parity1;
         }
@@ -1160,30 +1207,37 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       if (!ok && a.status) atomicExch(a.status, kStatusTimeoutMma);
     }
     __syncwarp();
-  } else {
+  } else if (TILES == 1 || warp >= 4) {
     // --------------------------------------------------------------------------------- softmax, one thread per row
-    const int qw = warp & 3, r = qw * 32 + lane, G = a.N / a.Nk;
+    const int qw = warp & 3, in_tile = qw * 32 + lane, r = tile * kQT + in_tile, G = a.N / a.Nk;
     const uint32_t lane_addr = static_cast<uint32_t>(qw * 32) << 16;
     const float scale_log2 = scale * 1.4426950408889634f;
     int seg = 0, it = 0, few_tiles = 0, few_segments = 0, stage = 0;
     uint32_t parity = 0;
-    QueryPlace qp;
+    QueryPlace<QT> qp;
     while (walk.next(g)) {   // to the end even when a wait gave up: the four warps meet at barriers
       qp.take(g.rows);
+      if (TILES > 1 && tile > 0 && (g.rows <= kFew || g.rows <= tile * kQT)) {
+        qp.done();
+        const int passed = stage + g.tiles;
+        stage = passed % STAGES;
+        parity ^= (passed / STAGES) & 1u;
+        continue;
+      }
       if (g.rows <= kFew) {
-        few_rows<HD, BF16, CAP, TREE>(a, w, g, smem, bars, part, qp, scale, qw, lane, stage, parity, few_tiles, few_segments, ok);
+        few_rows<HD, BF16, CAP, TREE, QT>(a, w, g, smem, bars, part, qp, scale, qw, lane, stage, parity, few_tiles, few_segments, ok);
         ++few_segments;
         qp.done();
         continue;
       }
       qp.done();
-      const bool idle = qw * 32 >= g.rows;   // a warp without rows keeps the barriers going
+      const bool idle = tile * kQT + qw * 32 >= g.rows;   // a warp without rows keeps the barriers going
       const int pos = g.seq < 0 ? 0x7fffffff : g.past + (g.in_seq + r) / G;
       const int first_pos = g.seq < 0 ? 0x7fffffff : g.past + g.in_seq / G;
       float m = -INFINITY, l = 0.f;
       for (int t = 0; t < g.tiles; ++t, ++it) {
         const int key0 = g.key0 + t * kKT;
-        if (ok && !wait_warp(&bars[BAR_S + (it & 1)], (it >> 1) & 1)) ok = false;
+        if (ok && !wait_warp(&tile_bars[BAR_S + (it & 1)], (it >> 1) & 1)) ok = false;
         tcgen05_fence_after();
         if (!idle) {
           const uint32_t s_addr = tmem_s + (it & 1) * kKT + lane_addr;
@@ -1219,7 +1273,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           if (__any_sync(0xffffffffu, raise)) {
             const float corr = raise ? (m == -INFINITY ? 0.f : ex2_approx(m - m_tile)) : 1.f;
             if (t > 0) {
-              if (ok && !wait_warp(&bars[BAR_O], (it - 1) & 1)) ok = false;
+              if (ok && !wait_warp(&tile_bars[BAR_O], (it - 1) & 1)) ok = false;
               tcgen05_fence_after();
 #pragma unroll 1
               for (int c = 0; c < HD; c += 32) {
@@ -1247,6 +1301,10 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
               const f32x2 p = pack2(ex2_approx(p0), ex2_approx(p1));
               sum = fma2(p, one, sum);
               unpack2(p, p0, p1);
+              if (L::kOnce) {
+                packed[j / 2] = pack16<BF16>(p0, p1);
+                continue;
+              }
               if (BF16) {   // the upper halves of the two, not rounded, and what is left
                 h0 = __uint_as_float(__float_as_uint(p0) & 0xffff0000u);
                 h1 = __uint_as_float(__float_as_uint(p1) & 0xffff0000u);
@@ -1262,7 +1320,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
               rest[j / 2] = pack16<BF16>(d0, d1);
             }
             tmem_st_x16_u32(s_addr + c / 2, packed);
-            tmem_st_x16_u32(s_addr + kKT / 2 + c / 2, rest);
+            if (!L::kOnce) tmem_st_x16_u32(s_addr + kKT / 2 + c / 2, rest);
           }
           float sum0, sum1;
           unpack2(sum, sum0, sum1);
@@ -1274,23 +1332,23 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           // what lies behind the last key may be anything, and 0 * NaN would reach the product: these rows of V become 0
           if (!wait_warp(&bars[BAR_V_FULL + stage], parity)) ok = false;
           uint8_t* v = smem + L::kOffKV + stage * L::kStageBytes + L::kBoxes * L::kBox + live * 128;
-          for (int i = r; i < (kKT - live) * 8; i += 128)
+          for (int i = in_tile; i < (kKT - live) * 8; i += 128)
 #pragma unroll
             for (int bx = 0; bx < L::kBoxes; ++bx) *reinterpret_cast<uint4*>(v + bx * L::kBox + i * 16) = make_uint4(0, 0, 0, 0);
           fence_proxy_async();
         }
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[BAR_P + (it & 1)]);
+        if (lane == 0) mbar_arrive(&tile_bars[BAR_P + (it & 1)]);
         if (++stage == STAGES) {
           stage = 0;
           parity ^= 1u;
         }
       }
-      if (ok && !wait_warp(&bars[BAR_END], seg & 1)) ok = false;
+      if (ok && !wait_warp(&tile_bars[BAR_END], seg & 1)) ok = false;
       tcgen05_fence_after();
       if (!idle) {
-        const long long row = g.slot + static_cast<long long>(blockIdx.x) * kQT + r;
+        const long long row = g.slot + static_cast<long long>(blockIdx.x) * QT + r;
         const bool mine = ok && r < g.rows;
         if (mine) w.ml[row] = make_float2(m, l);
 #pragma unroll 1
@@ -1305,7 +1363,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       }
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[BAR_O_FREE]);
+      if (lane == 0) mbar_arrive(&tile_bars[BAR_O_FREE]);
       ++seg;
     }
     if (!ok && lane == 0 && a.status) atomicExch(a.status, kStatusTimeoutEpilogue);
@@ -1315,7 +1373,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   __syncthreads();
   if (warp == 1) {
     tcgen05_fence_after();
-    tmem_dealloc(tmem_s, kTmemCols);
+    tmem_dealloc(tmem_base, kTmemCols * TILES);
   }
 }
 
@@ -1332,7 +1390,7 @@ __device__ __forceinline__ void load_cg(const float* p, float* v) {
 // Step 3: a warp joins `per` neighbouring rows of a key head (32 at most).  Each lane looks one row's sequence up; where the
 // segments of a unit are is worked out once for all of its rows.  SPLIT: few rows, whose segments may be hundreds; the four warps of
 // a CTA share one row's.
-template <typename T, int HD, bool SPLIT, bool TREE>
+template <typename T, int HD, bool SPLIT, bool TREE, int QT>
 __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_attn_args a, const int per) {
   constexpr int E = HD / 32;
   const int lane = threadIdx.x & 31, G = a.N / a.Nk, all_rows = last_row(a);
@@ -1351,9 +1409,9 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
   const int4 my_tok = __ldcg(&w.token[my_t]);
   const bool my_live = my_t < all_rows && my_t >= my_tok.y && my_t < my_tok.y + my_tok.z && plan.total > 0;   // lengths that start behind 0 leave rows to nobody
   // where the own units of the row's row tile start
-  const int my_ort = my_live ? (static_cast<int>(row0) + min(lane, count - 1) - my_tok.y * G) / kQT : 0, my_tile = my_live ? __ldcg(&w.tile0[my_tok.x]) + my_ort : 0;
+  const int my_ort = my_live ? (static_cast<int>(row0) + min(lane, count - 1) - my_tok.y * G) / QT : 0, my_tile = my_live ? __ldcg(&w.tile0[my_tok.x]) + my_ort : 0;
   const bool counted = my_live && my_tile < __ldcg(&w.tile0[my_tok.x + 1]);
-  const long long my_start = counted ? prefix_places(a, G, all_rows, plan.prefix_tiles) + __ldcg(&w.first[my_tile]) : 0;
+  const long long my_start = counted ? prefix_places<QT>(a, G, all_rows, plan.prefix_tiles) + __ldcg(&w.first[my_tile]) : 0;
   // the units of a row, 0 of the prefix and 1 of its own keys: first tile in the numbering, tiles, first slot
   int prt = -1, ort = -1, seq = -1, tiles0 = 0, tiles1 = 0, first0 = 0, first1 = 0, count0 = 0, count1 = 0;
   long long from0 = 0, from1 = 0, slot0 = 0, slot1 = 0, start = 0;
@@ -1364,8 +1422,8 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
     own = k >= count0;
     const int i = own ? first1 + k - count0 : first0 + k;
     const long long from = own ? from1 : from0;
-    has = k < count0 + count1 && max(from, share(plan.total, i)) < min(from + (own ? tiles1 : tiles0), share(plan.total, i + 1));
-    base = (own ? slot1 : slot0) + static_cast<long long>(i) * kQT;
+    has = k < count0 + count1 && max(from, share<QT>(plan.total, i)) < min(from + (own ? tiles1 : tiles0), share<QT>(plan.total, i + 1));
+    base = (own ? slot1 : slot0) + static_cast<long long>(i) * QT;
   };
   // rows of up to four segments, the usual ones: their places, the same in all lanes
   constexpr int kShort = 4;
@@ -1384,24 +1442,24 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
     if (!live) {
       count0 = count1 = n = 0;
       prt = -1;
-    } else if (pr / kQT != prt || tok.x != seq || orow / kQT != ort) {
+    } else if (pr / QT != prt || tok.x != seq || orow / QT != ort) {
       const Span s = {tok.y, tok.z, tok.w};
-      prt = pr / kQT;
+      prt = pr / QT;
       tiles0 = plan.prefix_tiles;
-      const int before0 = extra(unit_rows(G, all_rows, 0));
+      const int before0 = extra(unit_rows<QT>(G, all_rows, 0));
       from0 = (static_cast<long long>(prt) * a.Nk + kvh) * (tiles0 + before0) + before0;
-      slot0 = prefix_slot(a, prt, kvh, unit_rows(G, all_rows, prt));
+      slot0 = prefix_slot<QT>(a, prt, kvh, unit_rows<QT>(G, all_rows, prt));
       seq = tok.x;
-      ort = orow / kQT;
+      ort = orow / QT;
       start = __shfl_sync(0xffffffffu, my_start, r);
-      tiles1 = own_tiles(a, G, s, ort, tiles0);
-      const int rows1 = unit_rows(G, s.rows, ort);
+      tiles1 = own_tiles<QT>(a, G, s, ort, tiles0);
+      const int rows1 = unit_rows<QT>(G, s.rows, ort);
       from1 = start + static_cast<long long>(kvh) * places(tiles1, rows1) + extra(rows1);
-      slot1 = own_slot(a, G, s.row0, ort, kvh, rows1);
-      first0 = tiles0 > 0 ? owner(plan.total, from0) : 0;
-      first1 = tiles1 > 0 ? owner(plan.total, from1) : 0;
-      count0 = tiles0 > 0 ? owner(plan.total, from0 + tiles0 - 1) - first0 + 1 : 0;
-      count1 = tiles1 > 0 ? owner(plan.total, from1 + tiles1 - 1) - first1 + 1 : 0;
+      slot1 = own_slot<QT>(a, G, s.row0, ort, kvh, rows1);
+      first0 = tiles0 > 0 ? owner<QT>(plan.total, from0) : 0;
+      first1 = tiles1 > 0 ? owner<QT>(plan.total, from1) : 0;
+      count0 = tiles0 > 0 ? owner<QT>(plan.total, from0 + tiles0 - 1) - first0 + 1 : 0;
+      count1 = tiles1 > 0 ? owner<QT>(plan.total, from1 + tiles1 - 1) - first1 + 1 : 0;
       segment(lane);
       unsigned left = __ballot_sync(0xffffffffu, has);
       n = count0 + count1 > 32 ? kShort + 1 : __popc(left);
@@ -1423,7 +1481,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
       for (int i = 0; i < kShort; ++i) {
         ml[i] = make_float2(-INFINITY, 0.f);
         if (i < n) {
-          const unsigned row = (places4[i] >> 1) + static_cast<unsigned>(places4[i] & 1 ? orow : pr) % kQT;
+          const unsigned row = (places4[i] >> 1) + static_cast<unsigned>(places4[i] & 1 ? orow : pr) % QT;
           ml[i] = __ldcg(&w.ml[row]);
           load_cg<E>(w.o + static_cast<unsigned long long>(row) * HD + lane * E, v[i]);
         }
@@ -1440,7 +1498,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
     }
     for (int k0 = SPLIT ? warp * 32 : 0; n > kShort && k0 < count0 + count1; k0 += SPLIT ? 128 : 32) {
       segment(k0 + lane);
-      const long long row = base + (own ? orow : pr) % kQT;
+      const long long row = base + (own ? orow : pr) % QT;
       const float2 ml = has ? __ldcg(&w.ml[row]) : make_float2(-INFINITY, 0.f);
       unsigned left = __ballot_sync(0xffffffffu, has);
       const float mm = fmaxf(m, warp_max(ml.x));
@@ -1512,9 +1570,9 @@ bool vectorised(const ortb200_prefix_attn_args* a) {
   return (p & 15) == 0;
 }
 
-template <typename T, int HD, bool TREE>
+template <typename T, int HD, bool TREE, int QT>
 int launch_tc(const ortb200_prefix_attn_args* a, const int* parents, cudaStream_t stream) {
-  using L = TcSmem<HD>;
+  using L = TcSmem<HD, QT>;
   const CUtensorMapDataType dt = a->dtype == ORTB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const int64_t rows = a->T * (a->N / a->Nk), entry = static_cast<int64_t>(a->Nk) * HD * 2;
   CUtensorMap tq, tk, tv;
@@ -1524,27 +1582,36 @@ int launch_tc(const ortb200_prefix_attn_args* a, const int* parents, cudaStream_
   if (make_tensor_map_4d(&tk, a->k_cache, dt, 2, dims, strides, 64, box) != 0) return -6;
   if (make_tensor_map_4d(&tv, a->v_cache, dt, 2, dims, strides, 64, box) != 0) return -6;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  auto kern = a->softcap > 64.f ? prefix_attn_kernel<HD, kBf16, 2, TREE> : a->softcap > 0.f ? prefix_attn_kernel<HD, kBf16, 1, TREE> : prefix_attn_kernel<HD, kBf16, 0, TREE>;
+  auto kern = a->softcap > 64.f ? prefix_attn_kernel<HD, kBf16, 2, TREE, QT> : a->softcap > 0.f ? prefix_attn_kernel<HD, kBf16, 1, TREE, QT> : prefix_attn_kernel<HD, kBf16, 0, TREE, QT>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) != cudaSuccess) return -10;   // per device
   const int heads = a->N + 2 * a->Nk;
   const long long spread = 2 * kGrid / (a->T + 1), most = (heads + 15) / 16;   // few tokens: several CTAs per token, 16 heads at least to each
   const dim3 prep_grid(static_cast<unsigned>(a->T + 1), static_cast<unsigned>(spread < 1 ? 1 : spread > most ? most : spread));
-  int rc = vectorised<T>(a) ? launch_kernel(prefix_prep_tc_kernel<T, true, TREE>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a, parents)
-                            : launch_kernel(prefix_prep_tc_kernel<T, false, TREE>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a, parents);
+  int rc = vectorised<T>(a) ? launch_kernel(prefix_prep_tc_kernel<T, true, TREE, QT>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a, parents)
+                            : launch_kernel(prefix_prep_tc_kernel<T, false, TREE, QT>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a, parents);
   if (rc != 0) return rc;
   const float scale = a->scale != 0.f ? a->scale : 1.f / sqrtf(static_cast<float>(HD));
   // the two later steps may set up while the step before them ends: they wait for it before they read
-  rc = launch_kernel(kern, dim3(kGrid), kThreads, L::kTotal, stream, true, tq, tk, tv, *a, scale);
+  rc = launch_kernel(kern, dim3(grid_of<QT>), threads_of<QT>, L::kTotal, stream, true, tq, tk, tv, *a, scale);
   if (rc != 0) return rc;
   // Up to four rows per SM: a CTA each (one token of 32 heads over two key heads behind 18529 tokens: 23 us instead of 74 with one
   // warp a row).  Then one row per warp until there are rows for 16 warps on each SM, which is what fits at once: warps that come
   // later would look their segments up when the others have ended (24 prompts of up to 150 tokens: 37 us behind the product kernel
   // instead of 80).
-  if (a->T * a->N <= 2 * kGrid) return launch_kernel(prefix_join_kernel<T, HD, true, TREE>, dim3(static_cast<unsigned>(a->T * a->N)), 128, 0, stream, true, *a, 1);
+  if (a->T * a->N <= 2 * kGrid) return launch_kernel(prefix_join_kernel<T, HD, true, TREE, QT>, dim3(static_cast<unsigned>(a->T * a->N)), 128, 0, stream, true, *a, 1);
   const long long fit = 16 * kGrid / 2;
   const int per = static_cast<int>(std::min<long long>(32, (a->T * a->N + fit - 1) / fit));
   const long long warps = (rows + per - 1) / per * a->Nk;
-  return launch_kernel(prefix_join_kernel<T, HD, false, TREE>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0, stream, true, *a, per);
+  return launch_kernel(prefix_join_kernel<T, HD, false, TREE, QT>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0, stream, true, *a, per);
+}
+
+// Wide units where sequences bring more than 128 rows on average (G for each token): two tiles of rows share what is loaded.
+template <typename T, int HD, bool TREE>
+int launch_width(const ortb200_prefix_attn_args* a, const int* parents, cudaStream_t stream) {
+  if constexpr (TREE) {
+    if (a->T * (a->N / a->Nk) > static_cast<int64_t>(kQT) * a->B) return launch_tc<T, HD, TREE, kWide>(a, parents, stream);
+  }
+  return launch_tc<T, HD, TREE, kQT>(a, parents, stream);
 }
 
 template <typename T>
@@ -1577,8 +1644,8 @@ int launch_attn(const ortb200_prefix_attn_args* a, const int* parents, cudaStrea
     if ((a->H != 64 && a->H != 128) || !blocks || a->N / a->Nk > kQT) return -2;
     if ((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache) | reinterpret_cast<uintptr_t>(a->out)) & 15) return -3;
     if (reinterpret_cast<uintptr_t>(a->workspace) & 255) return -3;
-    if (a->dtype == ORTB200_BF16) return a->H == 128 ? launch_tc<__nv_bfloat16, 128, TREE>(a, parents, stream) : launch_tc<__nv_bfloat16, 64, TREE>(a, parents, stream);
-    if (a->dtype == ORTB200_F16) return a->H == 128 ? launch_tc<__half, 128, TREE>(a, parents, stream) : launch_tc<__half, 64, TREE>(a, parents, stream);
+    if (a->dtype == ORTB200_BF16) return a->H == 128 ? launch_width<__nv_bfloat16, 128, TREE>(a, parents, stream) : launch_width<__nv_bfloat16, 64, TREE>(a, parents, stream);
+    if (a->dtype == ORTB200_F16) return a->H == 128 ? launch_width<__half, 128, TREE>(a, parents, stream) : launch_width<__half, 64, TREE>(a, parents, stream);
     return -4;
   }
   switch (a->dtype) {

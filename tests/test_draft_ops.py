@@ -175,6 +175,24 @@ def test_tree_units_of_few_and_of_many_rows(dt, N, Nk, H, size):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cap", [0.0, 7.0, 90.0])
+@pytest.mark.parametrize("N,Nk,H,size", [(16, 2, 64, 16), (16, 2, 128, 64), (64, 4, 128, 32), (128, 1, 64, 64)])
+def test_tree_units_of_two_row_tiles(dt, cap, N, Nk, H, size):
+    """Batches whose sequences bring many rows: units of up to 256 rows, with fewer, with one tile's and with very few rows between them."""
+    nodes = [60, 1, 0, 33, 16, 17, 120, 2, 250, 31, 32, 5, 64, 1]
+    TreeCase(dt, N, Nk, H, size, [(29 * i) % 183 + (900 if i == 3 else 0) for i in range(len(nodes))], [tree(n, i) for i, n in enumerate(nodes)], seed=4, cap=cap).run(GPU)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nodes", [[256], [300, 256], [128, 129, 127], [64] * 50, [200] * 9 + [1] * 9])
+@pytest.mark.parametrize("N,Nk,H", [(8, 4, 128), (24, 3, 64)])
+def test_tree_batches_of_many_rows(N, Nk, H, nodes):
+    trees = [tree(n, i) if n <= 256 else list(range(-1, n - 1)) for i, n in enumerate(nodes)]
+    TreeCase(torch.bfloat16, N, Nk, H, 64, [(211 * i) % 700 for i in range(len(nodes))], trees, seed=5).run(GPU)
+
+
+@pytest.mark.gpu
 def test_tree_many_sequences_and_long_prompts():
     """More row tiles than a CTA keeps the running sums of, trees and a prompt among them."""
     trees = [tree((1, 9, 0, 2)[i % 4], i) for i in range(900)] + [list(range(-1, 699))]
