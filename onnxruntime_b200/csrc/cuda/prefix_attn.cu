@@ -434,6 +434,13 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
   return p;
 }
 
+// sequence_of by a CTA of 128: one round of loads instead of a chain of them
+__device__ __forceinline__ int sequence_among(const int* cu, int B, int t) {
+  int before = 0;
+  for (int b0 = 0; b0 < B; b0 += 128) before += __syncthreads_count(b0 + static_cast<int>(threadIdx.x) < B && cu[b0 + threadIdx.x] <= t);
+  return max(before - 1, 0);
+}
+
 // Step 1: one CTA (or, for few tokens, several) per token and one more for the plan.  VEC: whole heads rotated in halves or not
 // at all, every address a multiple of 16 bytes: a thread moves 2 x 16 bytes; otherwise one element.
 template <typename T, bool VEC, bool TREE, int QT>
@@ -448,8 +455,12 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
     return;
   }
   const int t = blockIdx.x, H = a.H, heads = a.N + 2 * a.Nk, G = a.N / a.Nk;
+  if (TREE && a.k == nullptr) {   // the token's row is on its way while its place is found
+    const char* row = static_cast<const char*>(a.qkv) + static_cast<long long>(t) * heads * H * sizeof(T);
+    for (int i = threadIdx.x * 128; i < heads * H * static_cast<int>(sizeof(T)); i += 128 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + i));
+  }
   if (t >= last_row(a)) return;
-  const int b = sequence_of(a.cu_seqlens, a.B, t);
+  const int b = TREE ? sequence_among(a.cu_seqlens, a.B, t) : sequence_of(a.cu_seqlens, a.B, t);
   if (blockIdx.y == 0 && threadIdx.x == 0) {
     const Span sp = span_of(a, b);
     w.token[t] = make_int4(b, sp.row0, sp.rows, sp.past);
