@@ -12,6 +12,7 @@
 //  * step loop -> StreamExecutionContext::RunSince (stream_execution_context.cc:180).
 #pragma once
 #include <map>
+#include <unordered_map>
 #include <memory>
 #include <string>
 #include <vector>
@@ -63,7 +64,7 @@ class GraphExecutor {
   std::map<std::string, bool> outer_on_gpu_;
   std::map<std::string, bool> on_gpu_;  // value name -> location
   std::vector<Step> steps_;
-  std::map<std::string, int> slot_of_;
+  std::unordered_map<std::string, int> slot_of_;
   std::vector<std::string> slot_names_;
   std::vector<Value> constant_slots_;
   std::vector<std::string> input_names_, output_names_, outer_names_;

@@ -525,10 +525,12 @@ std::vector<Value> InferenceSession::RunImpl(const RunOptions& ro, const std::ve
   c10::cuda::OptionalCUDAGuard guard;
   if (device_.is_cuda()) guard.set_device(device_);
 
-  std::vector<std::string> output_names = output_names_in.empty() ? output_names_ : output_names_in;
-  for (auto& n : output_names)
-    if (std::find(output_names_.begin(), output_names_.end(), n) == output_names_.end())
+  const std::vector<std::string>& output_names = output_names_in.empty() ? output_names_ : output_names_in;
+  for (size_t i = 0; i < output_names.size(); ++i) {   // usually all of them, in the model's order (a search for each of 64 took half of such a call)
+    const std::string& n = output_names[i];
+    if ((i >= output_names_.size() || output_names_[i] != n) && std::find(output_names_.begin(), output_names_.end(), n) == output_names_.end())
       ORTB_THROW(INVALID_ARGUMENT, "Invalid output name:", n);
+  }
 
   // order the feeds as the plan expects and validate them
   const Graph& g = *model_->graph_;
@@ -706,15 +708,13 @@ std::vector<Value> InferenceSession::Run(const RunOptions& ro, const std::vector
 }
 
 void InferenceSession::RunWithBinding(const RunOptions& ro, IOBinding& b) {
-  std::vector<std::string> names = b.out_names_;
-  std::vector<Value> res = RunImpl(ro, b.in_names_, b.in_values_, names, &b.out_values_);
-  b.results_.clear();
+  std::vector<Value> res = RunImpl(ro, b.in_names_, b.in_values_, b.out_names_, &b.out_values_);
   for (size_t i = 0; i < res.size(); ++i) {
-    Value v = res[i];
+    Value& v = res[i];
     if (!b.out_values_[i].t.defined() && v.t.defined() && v.t.device() != b.out_devices_[i])
       v.t = v.t.to(b.out_devices_[i]);
-    b.results_.push_back(v);
   }
+  b.results_ = std::move(res);
 }
 
 std::string InferenceSession::EndProfiling() { return profiler_.End(); }

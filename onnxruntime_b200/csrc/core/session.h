@@ -10,6 +10,7 @@
 #include <atomic>
 #include <chrono>
 #include <map>
+#include <unordered_map>
 #include <memory>
 #include <mutex>
 #include <set>
@@ -216,7 +217,7 @@ class InferenceSession {
   int64_t launch_count_ = 0;
   int64_t last_run_launches_ = 0;
   std::map<std::string, MemoryPlan> memory_plans_;
-  std::map<std::string, size_t> input_index_;
+  std::unordered_map<std::string, size_t> input_index_;
   std::vector<const ValueInfo*> input_info_;
   at::Tensor gemm_ws_, attn_ws_, status_word_;
   std::vector<at::Tensor> retired_ws_;  // outgrown workspaces that captured graphs still point to
