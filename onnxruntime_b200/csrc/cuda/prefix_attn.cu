@@ -541,7 +541,6 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
 template <int HD, int QT>
 struct TcSmem {
   static constexpr int kRowTiles = QT / kQT;
-  static constexpr bool kOnce = QT == kWide;              // weights are rounded to the type once
   static constexpr int kStages = QT == kQT ? (HD == 64 ? 3 : 2) : 4;
   static constexpr int kBoxes = HD / 64;                  // boxes of 64 elements per row
   static constexpr int kQBox = kQT * 128, kBox = kKT * 128;
@@ -1204,8 +1203,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 #pragma unroll
           for (int kk = 0; kk < kKT / 16; ++kk) mma_ts(tmem_o, p + kk * 8, low + kk * (2048 >> 4), idesc_o, t > 0 || kk > 0 ? 1u : 0u);
 #pragma unroll
-          for (int kk = 0; kk < kKT / 16; ++kk)
-            if (!L::kOnce) mma_ts(tmem_o, p + kKT / 2 + kk * 8, low + kk * (2048 >> 4), idesc_o, 1u);
+          for (int kk = 0; kk < kKT / 16; ++kk) mma_ts(tmem_o, p + kKT / 2 + kk * 8, low + kk * (2048 >> 4), idesc_o, 1u);
           umma_commit(&tile_bars[BAR_O]);
           umma_commit(&bars[BAR_V_EMPTY + s]);
           if (t == g.tiles - 1) umma_commit(&tile_bars[BAR_END]);
@@ -1277,8 +1275,15 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             for (int j = 0; j < kKT; ++j) sv[j] = j < hi ? sv[j] : -INFINITY;
           }
           float m_raw = -INFINITY;
+          if (!TREE) {
 #pragma unroll
-          for (int j = 0; j < kKT; j += 2) m_raw = fmax3(m_raw, sv[j], sv[j + 1]);
+            for (int j = 0; j < kKT; j += 2) m_raw = fmax3(m_raw, sv[j], sv[j + 1]);
+          } else {   // four chains
+            float four[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < kKT; j += 2) four[j / 2 % 4] = fmax3(four[j / 2 % 4], sv[j], sv[j + 1]);
+            m_raw = fmaxf(fmax3(four[0], four[1], four[2]), four[3]);
+          }
           const float m_tile = m_raw * fs;
           const bool raise = m_tile > m + kRaise;   // also the first finite maximum of a row
           if (__any_sync(0xffffffffu, raise)) {
@@ -1312,10 +1317,6 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
               const f32x2 p = pack2(ex2_approx(p0), ex2_approx(p1));
               sum = fma2(p, one, sum);
               unpack2(p, p0, p1);
-              if (L::kOnce) {
-                packed[j / 2] = pack16<BF16>(p0, p1);
-                continue;
-              }
               if (BF16) {   // the upper halves of the two, not rounded, and what is left
                 h0 = __uint_as_float(__float_as_uint(p0) & 0xffff0000u);
                 h1 = __uint_as_float(__float_as_uint(p1) & 0xffff0000u);
@@ -1331,7 +1332,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
               rest[j / 2] = pack16<BF16>(d0, d1);
             }
             tmem_st_x16_u32(s_addr + c / 2, packed);
-            if (!L::kOnce) tmem_st_x16_u32(s_addr + kKT / 2 + c / 2, rest);
+            tmem_st_x16_u32(s_addr + kKT / 2 + c / 2, rest);
           }
           float sum0, sum1;
           unpack2(sum, sum0, sum1);
@@ -1616,11 +1617,13 @@ int launch_tc(const ortb200_prefix_attn_args* a, const int* parents, cudaStream_
   return launch_kernel(prefix_join_kernel<T, HD, false, TREE, QT>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0, stream, true, *a, per);
 }
 
-// Wide units where sequences bring more than 128 rows on average (G for each token): two tiles of rows share what is loaded.
+// Wide units where sequences bring more than 192 rows on average (G for each token), heads of 128: two tiles of rows share what is
+// loaded.  6 trees of 48 tokens on average behind 25000, eight query heads to a key head: 408 -> 352 us, of 27 behind 3000 in a batch of 24 149 ->
+// 142, of 30 tokens and four heads 111 and 111; but heads of 64, whose tiles are half as many bytes, 82 -> 94 us.
 template <typename T, int HD, bool TREE>
 int launch_width(const ortb200_prefix_attn_args* a, const int* parents, cudaStream_t stream) {
-  if constexpr (TREE) {
-    if (a->T * (a->N / a->Nk) > static_cast<int64_t>(kQT) * a->B) return launch_tc<T, HD, TREE, kWide>(a, parents, stream);
+  if constexpr (TREE && HD == 128) {
+    if (a->T * (a->N / a->Nk) > 192ll * a->B) return launch_tc<T, HD, TREE, kWide>(a, parents, stream);
   }
   return launch_tc<T, HD, TREE, kQT>(a, parents, stream);
 }
