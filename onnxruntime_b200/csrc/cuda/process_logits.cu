@@ -188,7 +188,7 @@ struct Place {
 
 // E: logits of a vector (1: any alignment).  TOUCHED: rows may have texts or biases; else the stream alone.
 template <typename T, int E, bool TOUCHED, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 2) process_logits_kernel(const ortb200_process_logits_args a, const int chunk, const int parts) {
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 1) process_logits_kernel(const ortb200_process_logits_args a, const int chunk, const int parts) {
   extern __shared__ __align__(16) unsigned counts[];            // [chunk + 2 E + 4]
   __shared__ int listed, biases, twice;
   __shared__ uint16_t list[TOUCHED ? kList : 1], biased[TOUCHED ? kBiases : 1];   // of counters
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 2) process_logit
         }
       }
       if (text) {
-        for_text<THREADS, THREADS == 256 ? 4 : 8>(a, t, r, [&](long long v, bool count) {
+        for_text<THREADS, 4>(a, t, r, [&](long long v, bool count) {
           const int i = counter_of(v);
           if (i < 0) return;
           if (dense) {
@@ -339,7 +339,7 @@ template <typename T, int E, bool TOUCHED, int THREADS>
 int launch(const ortb200_process_logits_args* a, int64_t text_bytes, cudaStream_t stream) {
   // Usually four vectors of logits to a thread.  Shorter chunks where rows are few, so that every SM has some, but, as a text is read once
   // for each chunk, none that are fewer bytes than the usual text.
-  int chunk = THREADS == 512 ? kMaxChunk : 8192;
+  int chunk = THREADS == 256 ? 8192 : kMaxChunk;
   while (chunk > 2048 && a->rows * ((a->vocab + chunk - 1) / chunk) < 3 * 148 && text_bytes <= chunk / 2 * static_cast<int64_t>(sizeof(T) + 4)) chunk /= 2;
   const long long parts = (a->vocab + static_cast<long long>(chunk) - 1) / chunk;
   if (a->rows * parts > 0x7fffffffll) return -2;
@@ -353,10 +353,10 @@ template <typename T, int E>
 int launch_rows(const ortb200_process_logits_args* a, cudaStream_t stream) {
   if (!a->history && !a->drafted && !a->bias_tokens) return launch<T, E, false, 256>(a, 0, stream);
   // Every chunk reads the row's text.  Texts of up to 64 KB: chunks of 8192 and CTAs of 256 threads, six to an SM (384 rows of 128256 with 2250
-  // tokens 106 us; chunks of 16384 and CTAs of 512 threads 122).  Longer ones the other way: half as many bytes of text, and more of them on their
-  // way at a time (40 rows of 50257 with 45000 tokens 32 us instead of 45).
+  // tokens 108 us, with 10 tokens 70; chunks of 16384 and three CTAs of 512 threads 104 and 80, two of them 122 and 92).  Longer ones: chunks of 16384,
+  // half as many bytes of text, and 1024 threads that read them (40 rows of 50257 with 45000 tokens 27 us, 512 threads 32, the short texts' way 45).
   const int64_t text_bytes = a->history && a->lists > 0 ? 8 * (a->history_len / a->lists) : 0;
-  return text_bytes > 64 * 1024 ? launch<T, E, true, 512>(a, text_bytes, stream) : launch<T, E, true, 256>(a, text_bytes, stream);
+  return text_bytes > 64 * 1024 ? launch<T, E, true, 1024>(a, text_bytes, stream) : launch<T, E, true, 256>(a, text_bytes, stream);
 }
 
 template <typename T>
