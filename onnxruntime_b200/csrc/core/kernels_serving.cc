@@ -166,7 +166,18 @@ void PagedQueries(Ctx& ctx, const SharedPrefixSizes& z) {
     at::Tensor hidden = kpos.gt(qpos);
     if (tree.first.defined()) hidden.narrow(1, pl, S).copy_(tree.first.logical_not());
     s = s.masked_fill(hidden.unsqueeze(0), -std::numeric_limits<float>::infinity());
-    out.narrow(0, t0, S).copy_(at::matmul(at::softmax(s, -1), gather(vc)).permute({1, 0, 2}));
+    at::Tensor values = gather(vc), weights = at::softmax(s, -1), product;
+    if (z.tree && !at::isfinite(values.narrow(1, pl, S)).all().item<bool>()) {
+      // values that are not finite count for rows that see them, and 0 times them not for the others
+      at::Tensor finite = at::isfinite(values).all(2, true);   // [N, L, 1]
+      finite.narrow(1, 0, pl).fill_(true);
+      product = at::matmul(weights, at::where(finite, values, at::zeros_like(values)));
+      at::Tensor spoilt = at::matmul(hidden.logical_not().to(values.scalar_type()).unsqueeze(0), finite.logical_not().to(values.scalar_type()));   // [N, S, 1]
+      product = product.masked_fill(spoilt.gt(0), std::numeric_limits<float>::quiet_NaN());
+    } else {
+      product = at::matmul(weights, values);
+    }
+    out.narrow(0, t0, S).copy_(product.permute({1, 0, 2}));
   }
   ctx.SetOutput(0, out.reshape({z.T, z.N * z.H}));
   if (ctx.OutputCount() > 1) ctx.SetOutput(1, kc);

@@ -140,7 +140,6 @@ extern "C" int ortb200_cache_move(const ortb200_cache_move_args* a, ortb200_stre
     all |= reinterpret_cast<uintptr_t>(a->caches[i]) | static_cast<uint64_t>(a->unit_bytes[i]);
     widest = a->unit_bytes[i] > widest ? a->unit_bytes[i] : widest;
   }
-  if (widest == 0) return 0;
   if (all % 16 == 0) return launch_move<uint4>(a, widest, stream);
   if (all % 4 == 0) return launch_move<uint32_t>(a, widest, stream);
   if (all % 2 == 0) return launch_move<uint16_t>(a, widest, stream);

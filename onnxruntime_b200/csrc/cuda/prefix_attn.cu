@@ -75,6 +75,21 @@ __device__ __forceinline__ bool owned(const ortb200_prefix_attn_args& a, int b, 
 
 // Trees of drafted tokens: the rows of a sequence that a row sees, as bits, which step 1 works out.
 constexpr int kTreeWords = 8, kTreeNodes = 32 * kTreeWords;
+// Behind a row's bits lie as many words that are not 0 where one of its values is no finite number: 0 times such a value would reach rows
+// that do not see it, and a drafted token that goes wrong would take the others with it.  These values count as 0, and rows that do see
+// one become NaN.
+constexpr int kTreeStride = 2 * kTreeWords;
+__device__ __forceinline__ bool tree_spoilt(const uint32_t* ancestors, long long t) {
+  const uint4* w = reinterpret_cast<const uint4*>(ancestors + t * kTreeStride + kTreeWords);
+  const uint4 x = __ldcg(w), y = __ldcg(w + 1);
+  return (x.x | x.y | x.z | x.w | y.x | y.y | y.z | y.w) != 0;
+}
+// one of the two 16-bit numbers is an infinity or NaN
+template <typename T>
+__device__ __forceinline__ bool spoilt2(uint32_t w) {
+  const uint32_t e = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  return (w & e) == e || (w >> 16 & e) == e;
+}
 // All threads of row t's CTA, row i of the `rows` of its sequence: writes the row's bits, returns how deep it lies.  The walk from
 // parent to parent goes through shared memory; trees are a few levels deep.
 __device__ __forceinline__ int tree_row(const int* parents, int row0, int rows, int i, uint32_t* ancestors, int* status, bool write) {
@@ -127,7 +142,7 @@ __global__ void __launch_bounds__(128) prefix_prep_kernel(const ortb200_prefix_a
   }
   if (parents) {
     const Span s = span_of(a, b);
-    pos += tree_row(parents, s.row0, s.rows, t - s.row0, ancestors + static_cast<long long>(t) * kTreeWords, a.status, true) - (t - s.row0);
+    pos += tree_row(parents, s.row0, s.rows, t - s.row0, ancestors + static_cast<long long>(t) * kTreeStride, a.status, true) - (t - s.row0);
   }
   const bool keep = slot >= 0 && slot < static_cast<long long>(a.num_blocks) * a.block_size;
   if (!keep && threadIdx.x == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
@@ -181,7 +196,7 @@ __global__ void __launch_bounds__(128) prefix_rows_kernel(const ortb200_prefix_a
     for (int r = 0; r < R; ++r) qv[r] = r * 32 + lane < H ? to_float<T>(q[item * H + r * 32 + lane]) : 0.f;
     const bool tree = ancestors && s.rows <= kTreeNodes;
     for (int j = 0; j < keys; ++j) {
-      if (tree && j >= s.past && !tree_sees(ancestors + static_cast<long long>(t) * kTreeWords, j - s.past)) continue;
+      if (tree && j >= s.past && !tree_sees(ancestors + static_cast<long long>(t) * kTreeStride, j - s.past)) continue;
       const int block = a.block_table[static_cast<long long>(b) * a.max_blocks + j / a.block_size];
       if (block < 0 || block >= a.num_blocks) {
         if (lane == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
@@ -239,7 +254,7 @@ struct Work {            // the workspace's parts
   long long* first;      // [row tiles of all sequences + 1]: where the own units of each start, behind the prefix's
   int* tile0;            // [B + 1]: which of those row tiles are a sequence's
   int4* token;           // [T]: the token's sequence, that sequence's first row, rows and past
-  uint32_t* ancestors;   // [T, 8]: trees only
+  uint32_t* ancestors;   // [T, 16]: trees only
   uint16_t* q;           // [Nk, T G, H]
   float2* ml;            // per row of a segment: m (in units of log 2) and l
   float* o;              // per row of a segment: H values
@@ -251,7 +266,7 @@ __host__ __device__ inline long long plan_bytes(long long T, int B, int N, int N
   return up256(sizeof(Plan) + 8 * (most_row_tiles(T, B, N, Nk) + 1) + 4ll * (B + 1));
 }
 __host__ __device__ inline long long segment_rows(long long T, int N) { return 2 * T * N + static_cast<long long>(kGrid) * kQT; }   // (grid_of<QT> x QT is the same for both)
-__host__ __device__ inline long long tree_bytes(long long T) { return up256(T * kTreeWords * 4); }
+__host__ __device__ inline long long tree_bytes(long long T) { return up256(T * kTreeStride * 4); }
 template <bool TREE>
 __host__ __device__ inline Work work_of(const ortb200_prefix_attn_args& a) {
   char* p = static_cast<char*>(a.workspace);
@@ -477,7 +492,7 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
   }
   if (TREE) {
     const Span s = span_of(a, b);
-    pos += tree_row(parents, s.row0, s.rows, t - s.row0, w.ancestors + static_cast<long long>(t) * kTreeWords, a.status, blockIdx.y == 0) - (t - s.row0);
+    pos += tree_row(parents, s.row0, s.rows, t - s.row0, w.ancestors + static_cast<long long>(t) * kTreeStride, a.status, blockIdx.y == 0) - (t - s.row0);
   }
   const bool keep = slot >= 0 && slot < static_cast<long long>(a.num_blocks) * a.block_size;
   if (!keep && threadIdx.x == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
@@ -488,6 +503,7 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
   }
   const T* cosr = a.cos_cache ? static_cast<const T*>(a.cos_cache) + pos * half : nullptr;
   const T* sinr = a.cos_cache ? static_cast<const T*>(a.sin_cache) + pos * half : nullptr;
+  bool spoilt = false;
   const int per_block = (heads + gridDim.y - 1) / gridDim.y;
   const int lo = blockIdx.y * per_block, hi = min(heads, lo + per_block), items = VEC ? H / 16 : H;
   for (int idx = lo * items + threadIdx.x; idx < hi * items; idx += 128) {
@@ -508,6 +524,8 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
     if (VEC) {
       const int far = H / 2;
       const uint4 u4 = *reinterpret_cast<const uint4*>(src + d), v4 = *reinterpret_cast<const uint4*>(src + d + far);
+      if (TREE && kind == 2)
+        spoilt |= spoilt2<T>(u4.x) || spoilt2<T>(u4.y) || spoilt2<T>(u4.z) || spoilt2<T>(u4.w) || spoilt2<T>(v4.x) || spoilt2<T>(v4.y) || spoilt2<T>(v4.z) || spoilt2<T>(v4.w);
       if (!turn) {
         *reinterpret_cast<uint4*>(dst + d) = u4;
         *reinterpret_cast<uint4*>(dst + d + far) = v4;
@@ -526,6 +544,7 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
       *reinterpret_cast<uint4*>(dst + d + far) = *reinterpret_cast<const uint4*>(y1);
     } else {
       T y = src[d];
+      if (TREE && kind == 2) spoilt |= spoilt2<T>(*reinterpret_cast<const uint16_t*>(&y));
       if (turn && d < a.rot_dim) {
         const int i = a.interleaved ? d >> 1 : d % half;
         const bool upper = a.interleaved ? d & 1 : d >= half;
@@ -535,6 +554,12 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
       }
       dst[d] = y;
     }
+  }
+  if (TREE) {
+    spoilt = __syncthreads_or(spoilt);
+    uint32_t* word = w.ancestors + static_cast<long long>(t) * kTreeStride + kTreeWords;
+    if (threadIdx.x == 0) word[blockIdx.y] = spoilt;
+    if (blockIdx.y == 0 && threadIdx.x >= gridDim.y && threadIdx.x < kTreeWords) word[threadIdx.x] = 0;
   }
 }
 
@@ -882,13 +907,23 @@ __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, cons
       if (key + 8 >= seen0) c[2] = -INFINITY;
       if (key + 8 >= seen1) c[3] = -INFINITY;
       if (TREE && g.tree && first + 16 > g.past) {   // (rows behind the unit's last take its bits)
-        const uint32_t* bits0 = w.ancestors + static_cast<long long>((g.q_row + min(n0, g.rows - 1)) / G) * kTreeWords;
-        const uint32_t* bits1 = w.ancestors + static_cast<long long>((g.q_row + min(n0 + 1, g.rows - 1)) / G) * kTreeWords;
+        const uint32_t* bits0 = w.ancestors + static_cast<long long>((g.q_row + min(n0, g.rows - 1)) / G) * kTreeStride;
+        const uint32_t* bits1 = w.ancestors + static_cast<long long>((g.q_row + min(n0 + 1, g.rows - 1)) / G) * kTreeStride;
         const int j = key - g.past;
         if (j >= 0 && !tree_sees(bits0, j)) c[0] = -INFINITY;
         if (j >= 0 && !tree_sees(bits1, j)) c[1] = -INFINITY;
         if (j + 8 >= 0 && !tree_sees(bits0, j + 8)) c[2] = -INFINITY;
         if (j + 8 >= 0 && !tree_sees(bits1, j + 8)) c[3] = -INFINITY;
+      }
+      uint32_t spoilt = 0;   // keys of this warp whose values are not finite
+      if (TREE && first + 16 > g.past) {
+        const int at = first + (lane & 15);
+        spoilt = __ballot_sync(0xffffffffu, lane < 16 && at >= g.past && at < g.end && tree_spoilt(w.ancestors, (g.q_row - g.in_seq) / G + at - g.past));
+        if (spoilt) {
+          const bool near = spoilt >> (lane >> 2) & 1, far = spoilt >> ((lane >> 2) + 8) & 1;
+          if ((near && c[0] != -INFINITY) || (far && c[2] != -INFINITY)) l0 = NAN;
+          if ((near && c[1] != -INFINITY) || (far && c[3] != -INFINITY)) l1 = NAN;
+        }
       }
       float t0 = fmaxf(c[0], c[2]) * fs, t1 = fmaxf(c[1], c[3]) * fs;
       if (__any_sync(0xffffffffu, t0 > m0 + kRaise || t1 > m1 + kRaise)) {
@@ -927,6 +962,15 @@ __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, cons
         for (int i = lane; i < (16 - live) * 8; i += 32)
 #pragma unroll
           for (int bx = 0; bx < L::kBoxes; ++bx) *reinterpret_cast<uint4*>(v + bx * L::kBox + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+        __syncwarp();
+      }
+      if (TREE && spoilt) {
+        uint8_t* v = smem + L::kOffKV + stage * L::kStageBytes + L::kBoxes * L::kBox + qw * 16 * 128;
+        for (int i = lane; i < 16 * 8; i += 32)
+          if (spoilt >> (i >> 3) & 1)
+#pragma unroll
+            for (int bx = 0; bx < L::kBoxes; ++bx) *reinterpret_cast<uint4*>(v + bx * L::kBox + i * 16) = make_uint4(0, 0, 0, 0);
         fence_proxy_async();
         __syncwarp();
       }
@@ -1248,6 +1292,23 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         const int key0 = g.key0 + t * kKT;
         if (ok && !wait_warp(&tile_bars[BAR_S + (it & 1)], (it >> 1) & 1)) ok = false;
         tcgen05_fence_after();
+        if (TREE && key0 + kKT > g.past) {   // keys of the tile whose values are not finite
+          const int at = key0 + lane, row0 = (g.q_row - g.in_seq) / G - g.past;
+          const uint32_t spoilt0 = __ballot_sync(0xffffffffu, at >= g.past && at < g.end && tree_spoilt(w.ancestors, row0 + at));
+          const uint32_t spoilt1 = __ballot_sync(0xffffffffu, at + 32 >= g.past && at + 32 < g.end && tree_spoilt(w.ancestors, row0 + at + 32));
+          if (spoilt0 | spoilt1) {
+            if (ok && !wait_warp(&bars[BAR_V_FULL + stage], parity)) ok = false;
+            uint8_t* v = smem + L::kOffKV + stage * L::kStageBytes + L::kBoxes * L::kBox;
+            for (int i = in_tile; ok && i < kKT * 8; i += 128)
+              if ((i < 256 ? spoilt0 >> (i >> 3) : spoilt1 >> ((i >> 3) - 32)) & 1)
+#pragma unroll
+                for (int bx = 0; bx < L::kBoxes; ++bx) *reinterpret_cast<uint4*>(v + bx * L::kBox + i * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async();
+            const uint32_t* bits = w.ancestors + static_cast<long long>((g.q_row + min(r, g.rows - 1)) / G) * kTreeStride;
+            for (int j = 0; j < kKT; ++j)
+              if ((j < 32 ? spoilt0 >> j : spoilt1 >> (j - 32)) & 1 && (g.tree ? tree_sees(bits, key0 + j - g.past) : key0 + j <= pos)) l = NAN;
+          }
+        }
         if (!idle) {
           const uint32_t s_addr = tmem_s + (it & 1) * kKT + lane_addr;
           float sv[kKT];
@@ -1262,7 +1323,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             for (int j = 0; j < kKT; ++j) sv[j] = cap(sv[j]);
           }
           if (TREE && g.tree && key0 + kKT > g.past) {   // 64 of the row's bits, the cache's all set (rows behind the unit's last take its bits)
-            const uint32_t* bits = w.ancestors + static_cast<long long>((g.q_row + min(r, g.rows - 1)) / G) * kTreeWords;
+            const uint32_t* bits = w.ancestors + static_cast<long long>((g.q_row + min(r, g.rows - 1)) / G) * kTreeStride;
             const int lo = key0 - g.past, w0 = lo >> 5;
             auto word = [&](int i) { return i < 0 ? 0xffffffffu : i < kTreeWords ? __ldcg(bits + i) : 0u; };
             const uint32_t b0 = word(w0), b1 = word(w0 + 1), b2 = word(w0 + 2);
@@ -1597,7 +1658,7 @@ int launch_tc(const ortb200_prefix_attn_args* a, const int* parents, cudaStream_
   auto kern = a->softcap > 64.f ? prefix_attn_kernel<HD, kBf16, 2, TREE, QT> : a->softcap > 0.f ? prefix_attn_kernel<HD, kBf16, 1, TREE, QT> : prefix_attn_kernel<HD, kBf16, 0, TREE, QT>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) != cudaSuccess) return -10;   // per device
   const int heads = a->N + 2 * a->Nk;
-  const long long spread = 2 * kGrid / (a->T + 1), most = (heads + 15) / 16;   // few tokens: several CTAs per token, 16 heads at least to each
+  const long long spread = 2 * kGrid / (a->T + 1), most = std::min((heads + 15) / 16, TREE ? kTreeWords : heads);   // few tokens: several CTAs per token, 16 heads at least to each
   const dim3 prep_grid(static_cast<unsigned>(a->T + 1), static_cast<unsigned>(spread < 1 ? 1 : spread > most ? most : spread));
   int rc = vectorised<T>(a) ? launch_kernel(prefix_prep_tc_kernel<T, true, TREE, QT>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a, parents)
                             : launch_kernel(prefix_prep_tc_kernel<T, false, TREE, QT>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a, parents);

@@ -197,7 +197,8 @@ def test_draft_step_refusals():
 
 @pytest.mark.parametrize("provider", PROVIDERS)
 @pytest.mark.parametrize("kw", [dict(), dict(repetition_penalty=1.2, frequency_penalty=0.1), dict(no_repeat_ngram_size=2, temperature=0.8), dict(eos_token_id=7, min_new_tokens=5),
-                                dict(presence_penalty=0.3, logit_bias={4: 1.0}, grammar=lambda done: range(0, 40, 2) if len(done) % 2 else None)], ids=str)
+                                dict(presence_penalty=0.3, logit_bias={4: 1.0}, grammar=lambda done: range(0, 40, 2) if len(done) % 2 else None)],
+                         ids=["greedy", "repetition", "ngrams", "end", "grammar"])
 def test_drafted_requests_equal_requests_without(provider, kw):
     """Greedy tokens, with 32-bit layers, in which rows of a tree and single rows differ far less than the best tokens do; a small vocabulary, so
     that drafts are often right; more requests than run at a time."""

@@ -193,6 +193,60 @@ def test_tree_batches_of_many_rows(N, Nk, H, nodes):
 
 
 @pytest.mark.gpu
+def test_tree_wide_units_of_many_sequences():
+    """More units of two row tiles than a CTA keeps the running sums of."""
+    TreeCase(torch.bfloat16, 64, 1, 128, 16, [i % 67 for i in range(300)], [tree(4 + (i % 5 == 0), i) for i in range(300)], seed=8).run(GPU)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_tree_tokens_without_a_sequence(kind):
+    """Rows that belong to no sequence: nothing is cached, and their results are 0."""
+    case = TreeCase(kind[1], 4, 2, 64, 16, [], [], behind=5)
+    case.table = torch.zeros(0, 3, dtype=torch.int32)
+    got = case.call(kind[0])()
+    assert (got["out"] == 0).all() and torch.equal(got["kc_out"].nan_to_num(7.0), case.caches[0].nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("past,nodes", [(0, 3), (70, 9), (130, 40)])
+def test_tree_hidden_scores_of_any_size(kind, past, nodes):
+    """What a row does not see has no say, however large its scores are: keys of infinities, NaN and the type's largest numbers in siblings."""
+    trees = [[-1] + [0] * (nodes - 1)]
+    case = TreeCase(kind[1], 4, 2, 64, 16, [past], trees, rotary=0.0, seed=nodes)
+    want = case.call(kind[0])()["out"]
+    for i, v in ((1, math.inf), (2, math.nan)) if nodes < 9 else ((1, math.inf), (2, math.nan), (5, torch.finfo(kind[1]).max), (8, -math.inf)):
+        case.qkv[i, 4:6] = v
+    got = case.call(kind[0])()["out"]
+    rows = [0] + [i for i in range(3, nodes) if i not in (5, 8)]
+    assert torch.equal(got[rows], want[rows])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("N,H,past,nodes", [(4, 64, 0, 3), (4, 64, 57, 7), (4, 128, 130, 40), (16, 128, 100, 100), (2, 128, 70, 300), (2, 40, 20, 9)])
+def test_tree_hidden_values_of_any_size(kind, N, H, past, nodes):
+    """A drafted token whose values overflow spoils the rows that see it, and no others: to the bit, these are what they are without it."""
+    parents = [-1] + [(i - 1) // 2 if nodes <= 256 else i - 1 for i in range(1, nodes)]
+    other = tree(6, 3)
+    case = TreeCase(kind[1], N, 2, H, 16, [past, 33], [parents, other], seed=nodes)
+    bad = {1: math.inf, 2: math.nan} if nodes < 40 else {5: -math.inf, nodes // 2: math.nan, nodes - 1: math.inf}
+    # what is not finite counts as 0 for all others
+    for i in bad:
+        case.qkv[i, -2:, ::3] = 0.0
+    whole = [case.qkv[i, -2:].clone() for i in bad]
+    for i in bad:
+        case.qkv[i, -2:] = 0.0
+    want = case.call(kind[0])()["out"]
+    for (i, v), row in zip(bad.items(), whole):
+        case.qkv[i, -2:] = row
+        case.qkv[i, -2:, 1::3] = v
+    got = case.call(kind[0])()["out"]
+    sees = oracle.sees(parents) if nodes <= 256 else torch.ones(nodes, nodes, dtype=torch.bool).tril()
+    spoilt = sees[:, list(bad)].any(1)
+    assert torch.equal(got[:nodes][~spoilt], want[:nodes][~spoilt]) and torch.equal(got[nodes:], want[nodes:])
+    assert not got[:nodes][spoilt].isfinite().all(1).any()
+
+
+@pytest.mark.gpu
 def test_tree_many_sequences_and_long_prompts():
     """More row tiles than a CTA keeps the running sums of, trees and a prompt among them."""
     trees = [tree((1, 9, 0, 2)[i % 4], i) for i in range(900)] + [list(range(-1, 699))]
@@ -385,6 +439,15 @@ def test_move_places_that_are_none(provider, sources, targets):
     """Reported; what lies outside the cache is neither read nor written, and the other moves take place on the GPU."""
     with pytest.raises((InvalidArgument, EPFail)):
         move_call(provider, sources, targets, some_caches(3))()
+
+
+@pytest.mark.parametrize("provider", PROVIDERS)
+def test_move_in_a_cache_of_nothing(provider):
+    """Caches without a block have no place that a move could name."""
+    move_call(provider, [], [], some_caches(2, blocks=0))()
+    move_call(provider, [3], [-1], some_caches(2, blocks=0))()
+    with pytest.raises((InvalidArgument, EPFail)):
+        move_call(provider, [0], [0], some_caches(2, blocks=0))()
 
 
 @pytest.mark.parametrize("provider", PROVIDERS)
