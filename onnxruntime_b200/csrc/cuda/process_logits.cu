@@ -5,6 +5,12 @@
 // chunk through temperature and mask.  The few tokens that are touched are listed, and worked out again behind the stream; where
 // they are more than the list holds, the stream looks at every counter.  No CTA waits for another, and counting commutes: no result
 // depends on an order of arrival.
+//
+// What bounds it: without texts the stream (384 rows of 128256 bf16 logits 55 us, 295 MB; the bytes need 45).  With a text of 2250 tokens to a
+// row 108 us: reading and counting it in each of 16 chunks, 112 MB out of L2 and half of the instructions; issue slots are 67 % busy.  A text of
+// 45000 tokens and 50257 32-bit logits, 40 rows: 27 us, nearly all of it the text.  Slower, for the same 384 rows: a text read once by a cluster of
+// the row's CTAs, which add to each other's counters, 212 us; a kernel that gathers what a row touches in a hash table, behind the stream or
+// in front of it, 105 to 111 and a second launch; a warp's tokens of the chunk queued and counted 32 at a time 123.
 #include <cuda_runtime.h>
 #include <math.h>
 #include "draft_ops.h"
@@ -22,8 +28,7 @@ constexpr unsigned kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3fffff
 // Quotients by one divisor of a whole row: with its rounded reciprocal r, q = x r is off by a unit or so, the remainder x - q d is exact in
 // a fused multiply-add, and q + r (x - q d) is the quotient rounded once (P. Markstein, IBM Journal of Research and Development 34, 1990;
 // numbers below 2^-100, whose remainders 32 bits do not hold, are within 3 times that).
-// A division for every logit takes some twenty instructions, 48 in all for each logit of logits that are masked and
-// scaled.
+// A division takes some twenty instructions, and the long way for infinities: with one for every logit the kernel had 48 instructions to a logit.
 struct Divisor {
   float d, r;   // r: NaN where the reciprocal's exponent leaves no room for the remainder
   __device__ __forceinline__ explicit Divisor(float by) : d(by), r(fabsf(by) > 0x1p-100f && fabsf(by) < 0x1p100f ? 1.f / by : NAN) {}
