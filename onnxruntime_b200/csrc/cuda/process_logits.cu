@@ -120,28 +120,42 @@ struct Text {
   }
   __device__ __forceinline__ bool any() const { return end > begin || drafted > 0; }
 };
-// add(token, whether it counts) for every token of the text, by all threads: two tokens to a load, AHEAD loads of a thread on their way
+// add(token) for tokens [begin, end) of the history, by all threads: two tokens to a load, AHEAD loads of a thread on their way
 template <int THREADS, int AHEAD, typename F>
-__device__ __forceinline__ void for_text(const ortb200_process_logits_args& a, const Text& t, long long r, F add) {
-  const long long odd = min(t.begin + static_cast<long long>((reinterpret_cast<uintptr_t>(a.history + t.begin) >> 3) & 1), t.end), pairs = (t.end - odd) / 2;
-  if (threadIdx.x == 0 && odd > t.begin) add(a.history[t.begin], t.begin >= t.counted);
-  if (threadIdx.x == 32 && odd + 2 * pairs < t.end) add(a.history[t.end - 1], t.end - 1 >= t.counted);
-  const longlong2* two = reinterpret_cast<const longlong2*>(a.history + odd);
-  const int n = static_cast<int>(pairs), from = static_cast<int>(min(max(t.counted - odd, -1ll), 2 * pairs));   // (a history has fewer than 2^30 tokens)
-  for (int i = threadIdx.x; i < n; i += AHEAD * THREADS) {
+__device__ __forceinline__ void for_tokens(const int64_t* history, long long begin, long long end, F add) {
+  if (begin >= end) return;
+  const int64_t* p = history + begin;
+  const int len = static_cast<int>(end - begin), odd = static_cast<int>((reinterpret_cast<uintptr_t>(p) >> 3) & 1), pairs = (len - odd) / 2;   // (a history has fewer than 2^30 tokens)
+  if (threadIdx.x == 0 && odd) add(p[0]);
+  if (threadIdx.x == 32 && odd + 2 * pairs < len) add(p[len - 1]);
+  const longlong2* two = reinterpret_cast<const longlong2*>(p + odd);
+  for (int i = threadIdx.x; i < pairs; i += AHEAD * THREADS) {
     longlong2 v[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
-      if (i + k * THREADS < n) v[k] = __ldg(two + i + k * THREADS);
+      if (i + k * THREADS < pairs) v[k] = __ldg(two + i + k * THREADS);
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
-      if (i + k * THREADS < n) {
-        const int at = 2 * (i + k * THREADS);
-        add(v[k].x, at >= from);
-        add(v[k].y, at + 1 >= from);
+      if (i + k * THREADS < pairs) {
+        add(v[k].x);
+        add(v[k].y);
       }
   }
-  for (int d = threadIdx.x; d < t.drafted; d += THREADS) add(a.drafted[r * a.drafted_width + d], true);
+}
+// seen(token) for what does not count of a text, count(token) for what does
+template <int THREADS, int AHEAD, typename S, typename C>
+__device__ __forceinline__ void for_text(const ortb200_process_logits_args& a, const Text& t, long long r, S seen, C count) {
+  const long long counts_from = min(max(t.counted, t.begin), t.end);
+  for_tokens<THREADS, AHEAD>(a.history, t.begin, counts_from, seen);
+  for_tokens<THREADS, AHEAD>(a.history, counts_from, t.end, count);
+  for (int d = threadIdx.x; d < t.drafted; d += THREADS) count(a.drafted[r * a.drafted_width + d]);
+}
+// (as an instruction of its own: the compiler makes one addition for a warp out of atomicAdd to one place, which costs more than the two
+// lanes that usually come)
+__device__ __forceinline__ int next_place(int* counter) {
+  int n;
+  asm volatile("atom.shared.add.u32 %0, [%1], 1;" : "=r"(n) : "r"(smem_u32(counter)) : "memory");
+  return n;
 }
 
 // A score from its logit: penalties by the token's counter, its bias, the temperature, the mask.
@@ -227,7 +241,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 1) process_logit
         return u >= size || static_cast<unsigned long long>(v) >> 32 ? -1 : at.first - at.base + static_cast<int>(u);
       };
       auto to_list = [&](int i) {
-        const int n = atomicAdd(&listed, 1);
+        const int n = next_place(&listed);
         if (n < kList) list[n] = static_cast<uint16_t>(i);
       };
       dense = text && t.end - t.begin > static_cast<long long>(parts) * kList;   // too many to be listed, most likely
@@ -243,17 +257,28 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 1) process_logit
           bias_of[n] = a.bias_values[b];
         }
       }
-      if (text) {
-        for_text<THREADS, 4>(a, t, r, [&](long long v, bool count) {
-          const int i = counter_of(v);
-          if (i < 0) return;
-          if (dense) {
-            if (count) atomicAdd(&counts[i], 1u);
-            else atomicOr(&counts[i], kSeen);
-          } else if ((count ? atomicAdd(&counts[i], 1u) : atomicOr(&counts[i], kSeen)) == 0) {
-            to_list(i);
-          }
-        });
+      if (text && dense) {
+        for_text<THREADS, 4>(
+            a, t, r,
+            [&](long long v) {
+              const int i = counter_of(v);
+              if (i >= 0) atomicOr(&counts[i], kSeen);
+            },
+            [&](long long v) {
+              const int i = counter_of(v);
+              if (i >= 0) atomicAdd(&counts[i], 1u);
+            });
+      } else if (text) {
+        for_text<THREADS, 4>(
+            a, t, r,
+            [&](long long v) {
+              const int i = counter_of(v);
+              if (i >= 0 && atomicOr(&counts[i], kSeen) == 0) to_list(i);
+            },
+            [&](long long v) {
+              const int i = counter_of(v);
+              if (i >= 0 && atomicAdd(&counts[i], 1u) == 0) to_list(i);
+            });
       }
       __syncthreads();
       dense = dense || listed > kList;
