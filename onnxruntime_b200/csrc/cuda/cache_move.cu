@@ -18,7 +18,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kCaches = 128;        // caches of one launch: their addresses are kernel arguments
-constexpr int kMaxMoves = 3072;     // times the narrowest range, 64 bytes, fits shared memory
+constexpr int kMaxMoves = 3000;     // times the narrowest range, 64 bytes, fits shared memory
 
 struct Caches {
   uint8_t* at[kCaches];

@@ -377,7 +377,7 @@ def test_move_orders(provider, sources, targets, blocks):
 
 
 @pytest.mark.parametrize("provider", PROVIDERS)
-@pytest.mark.parametrize("moves", [1, 31, 32, 33, 300, 767, 768, 769, 3071, 3072, 3073, 4000])
+@pytest.mark.parametrize("moves", [1, 31, 32, 33, 300, 749, 750, 751, 2999, 3000, 3001, 4000])
 def test_move_numbers(provider, moves):
     """Permutations with cycles of all lengths, up to what one pass of the kernel holds and beyond."""
     caches = some_caches(2, blocks=260, inner=(1, 40))
@@ -623,6 +623,17 @@ def test_logits_neutral_values(provider):
     got = case.call(provider)()["scores"]
     x = case.t["logits"]
     assert torch.equal(got[[0, 1, 2, 3, 5]], x[[0, 1, 2, 3, 5]]) and torch.equal(got[4], x[4] / 0.5)
+
+
+@pytest.mark.parametrize("kind", LOGITS_KINDS)
+@pytest.mark.parametrize("text,biases", [(2000, 0), (0, 2000), (1023, 300), (1500, 1500)])
+def test_logits_touched_tokens_side_by_side(kind, text, biases):
+    """More touched tokens of one part of the vocabulary than are listed, whether by texts that are short for the whole of it or by biases."""
+    case = LogitsCase(kind[1], 3, 20000, without=["drafted", "row_list"], seed=text)
+    case.t.update(history=torch.arange(3 * text) % max(text, 1) + 5, history_starts=torch.arange(4) * text, generated_starts=torch.arange(3) * text + text // 2,
+                  bias_tokens=(torch.arange(3 * biases) * 2) % max(2 * biases, 1), bias_values=torch.linspace(-3, 3, 3 * biases), bias_starts=torch.arange(4) * biases,
+                  repetition=torch.full((3,), 1.25))
+    case.run(kind[0])
 
 
 @pytest.mark.parametrize("provider", PROVIDERS)
