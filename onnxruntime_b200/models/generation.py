@@ -14,6 +14,7 @@ import math
 from dataclasses import dataclass, field
 from typing import Callable, Dict, Hashable, List, Optional, Sequence, Tuple, Union
 
+import numpy as np
 import torch
 
 from .. import onnx_lite as ol
@@ -642,17 +643,16 @@ class LogitsProcessor:
             ol.make_model(graph, opset=17, extra_opsets={"com.ortb200": 1}).serialize(),
             providers=[("CUDAExecutionProvider", {"device_id": str(device.index or 0)}) if gpu else "CPUExecutionProvider"])
 
-    def _biases(self, text: Sequence[int], generated: int) -> Dict[int, float]:
-        """Of one row whose text ends with ``generated`` generated tokens."""
+    def _biases(self, text: Sequence[int], path: Sequence[int], generated: int) -> Dict[int, float]:
+        """Of one row: a request's text, of which ``generated`` tokens are generated, and the drafted tokens behind it."""
         cfg, bias = self.cfg, dict(self.cfg.logit_bias or {})
-        if cfg.eos_token_id is not None and generated < cfg.min_new_tokens:
+        if cfg.eos_token_id is not None and generated + len(path) < cfg.min_new_tokens:
             bias[cfg.eos_token_id] = -math.inf
         n = cfg.no_repeat_ngram_size
         if n > 0:
-            tail = list(text[len(text) - (n - 1):])
-            for i in range(len(text) - n + 1):
-                if list(text[i:i + n - 1]) == tail:
-                    bias[text[i + n - 1]] = -math.inf
+            whole = np.concatenate([np.asarray(text, dtype=np.int64), np.asarray(path, dtype=np.int64)])
+            if len(whole) >= n:
+                bias.update(dict.fromkeys(whole[_places_of(whole[:-1], whole[len(whole) - (n - 1):])].tolist(), -math.inf))
         return bias
 
     def _mask(self, allowed: Optional[Sequence[int]]) -> torch.Tensor:
@@ -682,11 +682,11 @@ class LogitsProcessor:
                 lists += [i] * len(paths)
             deepest = max(len(p) for _, _, paths in requests for p in paths)
             drafted = [list(p) + [-1] * (deepest - len(p)) for _, _, paths in requests for p in paths]
-            feeds.update(history=ints([t for text, _, _ in requests for t in text]), history_starts=ints(starts), generated_starts=ints(generated), row_list=ints(lists, torch.int32),
+            feeds.update(history=torch.from_numpy(np.concatenate([np.asarray(text, dtype=np.int64) for text, _, _ in requests])).to(dev), history_starts=ints(starts), generated_starts=ints(generated), row_list=ints(lists, torch.int32),
                          drafted=ints(drafted).reshape(rows, deepest), repetition=same(cfg.repetition_penalty), presence=same(cfg.presence_penalty),
                          frequency=same(cfg.frequency_penalty))
         if self.biased:
-            bias = [self._biases([*text, *p], new + len(p)) for text, new, paths in requests for p in paths]
+            bias = [self._biases(text, p, new) for text, new, paths in requests for p in paths]
             ends = [0]
             for b in bias:
                 ends.append(ends[-1] + len(b))
@@ -695,7 +695,7 @@ class LogitsProcessor:
             if cfg.grammar is None:
                 feeds.update(allowed=self._mask(None).reshape(1, -1).to(dev), row_mask=torch.zeros(rows, dtype=torch.int32, device=dev))
             else:
-                masks = [self._mask(cfg.grammar([*text[len(text) - new:], *p])) for text, new, paths in requests for p in paths]
+                masks = [self._mask(cfg.grammar([int(t) for t in (*text[len(text) - new:], *p)])) for text, new, paths in requests for p in paths]
                 feeds.update(allowed=torch.stack(masks).to(dev), row_mask=torch.arange(rows, dtype=torch.int32, device=dev))
         if self.warm:
             feeds.update(temperature=same(cfg.temperature))
@@ -710,26 +710,33 @@ class LogitsProcessor:
 
 def draft_tree(text: Sequence[int], most: int, ngram: int = 3) -> Tuple[List[int], List[int]]:
     """A tree of the last token of ``text`` and up to ``most`` drafted ones: what followed earlier occurrences of the last ``ngram`` tokens, then
-    of fewer, the latest occurrences first and each up to half as many tokens as there may be.  Returns the tokens and their parents."""
+    of fewer; the latest occurrences first, 64 at most, and of each up to half as many tokens as there may be.  Returns the tokens and their parents."""
+    text = np.asarray(text, dtype=np.int64)
     tokens, parents, children = [int(text[-1])], [-1], {}
     depth, end = max(1, (most + 1) // 2), len(text)
-    for n in range(min(ngram, end - 1), 0, -1):
-        tail = list(text[end - n:])
-        for at in range(end - 1, n - 1, -1):
+    for n in range(min(ngram, end - 1) if most > 0 else 0, 0, -1):
+        for at in _places_of(text[:-1], text[end - n:])[:-65:-1].tolist():
             if len(tokens) > most:
                 return tokens, parents
-            if list(text[at - n:at]) != tail:
-                continue
             node = 0
-            for t in text[at:min(at + depth, end)]:
+            for t in text[at:min(at + depth, end)].tolist():
                 if (node, t) not in children:
                     if len(tokens) > most:
                         break
                     children[node, t] = len(tokens)
-                    tokens.append(int(t))
+                    tokens.append(t)
                     parents.append(node)
                 node = children[node, t]
     return tokens, parents
+
+
+def _places_of(text: np.ndarray, tail: np.ndarray) -> np.ndarray:
+    """The places behind every occurrence of ``tail`` in ``text``, ascending (of an empty tail: all places of tokens and the one behind)."""
+    starts = len(text) - len(tail) + 1
+    found = np.ones(max(starts, 0), dtype=bool)
+    for k, t in enumerate(tail):
+        found &= text[k:starts + k] == t
+    return np.flatnonzero(found) + len(tail)
 
 
 class TokenScorer:
@@ -852,6 +859,7 @@ def _generate_requests(runner: PagedDecoderRunner, prompts, cfg: GenerationConfi
     if cfg.seed is not None:
         gen.manual_seed(cfg.seed)
     texts = [shared + [int(t) for t in p] for p in prompts]
+    flat = [np.array(t + [0] * max(cfg.max_new_tokens, 1), dtype=np.int64) for t in texts]   # the same, and what is generated
     done: List[Optional[List[int]]] = [None] * len(texts)
     new: Dict[int, List[int]] = {}
     held_by_all = len(shared) // runner.block_size     # blocks that a request does not need for itself
@@ -865,6 +873,7 @@ def _generate_requests(runner: PagedDecoderRunner, prompts, cfg: GenerationConfi
         tok = best
         if sampling:
             tok = int(torch.multinomial(torch.softmax(top_k_top_p_filter(scores.reshape(1, -1), cfg.top_k, cfg.top_p), -1), 1, generator=gen))
+        flat[i][len(texts[i]) + len(new[i])] = tok
         new[i].append(tok)
         if scorer is not None:
             lp, h, top_lp, top = (t.tolist() for t in scorer(logits.reshape(1, -1), torch.tensor([tok], dtype=torch.int64)))
@@ -904,7 +913,7 @@ def _generate_requests(runner: PagedDecoderRunner, prompts, cfg: GenerationConfi
         elif running:
             joining = list(running)
             # room has been kept for the tokens that a request will generate: no more of them are drafted
-            trees = {i: draft_tree(texts[i] + new[i], min(cfg.draft_tokens, cfg.max_new_tokens - len(new[i]) - 1), cfg.draft_ngram) if cfg.draft_tokens else ([new[i][-1]], [-1])
+            trees = {i: draft_tree(flat[i][:len(texts[i]) + len(new[i])], min(cfg.draft_tokens, cfg.max_new_tokens - len(new[i]) - 1), cfg.draft_ngram) if cfg.draft_tokens else ([new[i][-1]], [-1])
                      for i in joining}
             drafted = any(len(tokens) > 1 for tokens, _ in trees.values())
             if drafted:
@@ -914,7 +923,7 @@ def _generate_requests(runner: PagedDecoderRunner, prompts, cfg: GenerationConfi
         else:
             raise CacheFull(f"request {waiting[0]} does not fit into the cache")
         paths = {i: _paths(*trees[i]) for i in joining}
-        scores = processor(logits, [(texts[i] + new[i], len(new[i]), [[trees[i][0][j] for j in path[1:]] for path in paths[i]]) for i in joining])
+        scores = processor(logits, [(flat[i][:len(texts[i]) + len(new[i])], len(new[i]), [[trees[i][0][j] for j in path[1:]] for path in paths[i]]) for i in joining])
         best = [0] * len(scores) if sampling else scores.argmax(-1).tolist()
         row, kept = 0, {}
         for i in joining:   # from the root on, as far as the tree has what is chosen

@@ -84,6 +84,8 @@ def test_draft_trees():
     tokens, parents = draft_tree([1, 2, 3, 4, 9, 1, 2, 5, 6, 2, 8, 1, 2], 9, 2)
     assert tokens[:4] == [2, 5, 6, 2] and len(tokens) <= 10 and all(p < i for i, p in enumerate(parents)) and len(set(zip(tokens, parents))) == len(tokens)
     assert draft_tree([5, 5, 5, 5], 3) == ([5, 5, 5], [-1, 0, 1]) or len(draft_tree([5, 5, 5, 5], 3)[0]) <= 4
+    # many occurrences of a token that always goes on the same way
+    assert draft_tree([1, 2] * 5000 + [1], 3, 1) == ([1, 2, 1], [-1, 0, 1])
     for most in range(1, 20):
         tokens, parents = draft_tree([i * i % 7 for i in range(60)], most)
         assert 1 < len(tokens) <= most + 1 and parents[0] == -1 and all(0 <= p < i for i, p in enumerate(parents) if i)
