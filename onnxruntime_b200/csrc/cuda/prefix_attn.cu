@@ -17,6 +17,7 @@
 // so that one long prefix and many short tails fill the machine alike, without a word about it from the host, which does not
 // know the lengths.  A CTA's share of a unit is a segment; it leaves (m, l, o) of its rows in 32 bits, and step 3 joins the
 // segments of a row.  Which CTA wrote what follows from the same arithmetic: nothing is counted, nothing waited for.
+// (Trees: a unit that one CTA has needs no joining, and the CTA writes the results.)
 //
 // Within a CTA (192 threads, two per SM): warp 0 loads tiles by TMA through the block table, warp 1 issues the products
 // (S = Q K^T into tensor memory, O += P V with P in tensor memory over the scores), warps 2 to 5 hold one row per thread.  Units of
@@ -301,8 +302,12 @@ __host__ __device__ inline Work work_of(const ortb200_prefix_attn_args& a) {
 // costs a CTA as much time as some tiles, and a share of many short units has to be worth as much as one of a long unit.  For 24
 // prompts of up to 150 tokens behind 6000 (28 heads) 1, 2, 3 and 5 places took 303, 257, 234 and 238 us where rows are many; with
 // few rows 0, 1 and 2 make 108, 104 and 112 us (180 single tokens behind 20011), 54, 52 and 52 us (64 behind 8192).
-__device__ __forceinline__ int extra(int rows) { return rows > 32 ? 4 : 1; }
-__device__ __forceinline__ int places(int tiles, int rows) { return tiles > 0 ? tiles + extra(rows) : 0; }
+// Trees, whose units end with fewer stores where one CTA has all of one, take 2 between 9 and 32 rows: 1, 2 and 4 make 37, 34 and 31 us (57 trees of up
+// to 12 tokens behind 54, 32 heads over 8), 114, 110 and 112 (200 of up to 3 behind 500), but 123, 123 and 136 (64 of up to 16 behind 500, 32 key heads).
+template <bool TREE>
+__device__ __forceinline__ int extra(int rows) { return rows > 32 ? 4 : TREE && rows > kFew ? 2 : 1; }
+template <bool TREE>
+__device__ __forceinline__ int places(int tiles, int rows) { return tiles > 0 ? tiles + extra<TREE>(rows) : 0; }
 // The share of CTA i of `total` places starts at share(i); place x belongs to CTA owner(x).
 template <int QT>
 __device__ __forceinline__ long long share(long long total, int i) { return total * i / grid_of<QT>; }
@@ -326,14 +331,14 @@ template <int QT>
 __device__ __forceinline__ int row_tiles(int G, int rows) { return (rows * G + QT - 1) / QT; }
 template <int QT>
 __device__ __forceinline__ int unit_rows(int G, int rows, int rt) { return min(QT, rows * G - rt * QT); }
-template <int QT>
+template <bool TREE, int QT>
 __device__ __forceinline__ int own_places(const ortb200_prefix_attn_args& a, int G, const Span& s, int rt, int prefix_tiles) {
-  return places(own_tiles<QT>(a, G, s, rt, prefix_tiles), unit_rows<QT>(G, s.rows, rt));
+  return places<TREE>(own_tiles<QT>(a, G, s, rt, prefix_tiles), unit_rows<QT>(G, s.rows, rt));
 }
 // all units of the prefix are numbered like the first
-template <int QT>
+template <bool TREE, int QT>
 __device__ __forceinline__ long long prefix_places(const ortb200_prefix_attn_args& a, int G, int all_rows, int prefix_tiles) {
-  return static_cast<long long>(row_tiles<QT>(G, all_rows)) * a.Nk * places(prefix_tiles, unit_rows<QT>(G, all_rows, 0));
+  return static_cast<long long>(row_tiles<QT>(G, all_rows)) * a.Nk * places<TREE>(prefix_tiles, unit_rows<QT>(G, all_rows, 0));
 }
 // first row that the segments of a unit may use, before QT rows per CTA number: units follow one another without a gap
 template <int QT>
@@ -357,17 +362,18 @@ __device__ __forceinline__ int sequence_with(const I* places, int n, I x) {
 }
 // All THREADS of a CTA: how many tokens all sequences share, and where the own units of each row tile start (`first` and `tile0`,
 // written for all to read after the next barrier).
-template <int THREADS, int QT>
+template <int THREADS, bool TREE, int QT>
 __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, long long* first, int* tile0, int* status) {
   __shared__ int least_sm[THREADS / 32], row_sm[THREADS / 32];
   __shared__ long long sum_sm[THREADS / 32];
   __shared__ int tiles_sm[THREADS / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.N / a.Nk;
-  int least = 0x7fffffff, row = 0x7fffffff, several = 0;
+  int least = 0x7fffffff, row = 0x7fffffff, several = 0, backwards = 0;
   const int promised = a.shared_prefix ? *a.shared_prefix : 0, all_rows = last_row(a);
   for (int b = threadIdx.x; b < a.B; b += THREADS) {
     const Span s = span_of(a, b);
     if (status) check_lengths(a, b, s, status);
+    if (TREE) backwards |= a.cu_seqlens[b + 1] < a.cu_seqlens[b];
     if (s.rows == 0) continue;
     least = min(least, s.past);
     row = min(row, b);
@@ -380,6 +386,7 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
     row_sm[warp] = row;
   }
   several = __syncthreads_or(several);
+  if (TREE) backwards = __syncthreads_or(backwards);   // sequences that overlap would write one another's results: reported, and nothing is computed
 #pragma unroll
   for (int i = 0; i < THREADS / 32; ++i) {
     least = min(least, least_sm[i]);
@@ -417,7 +424,7 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
       const unsigned with = __ballot_sync(0xffffffffu, some);
       if (b0 > 0) __syncthreads();
       if (lane == 31) tiles_sm[warp] = __popc(with);   // read behind the next barrier, as sum_sm is
-      const long long at = running(some ? static_cast<long long>(own_places<QT>(a, G, s, 0, p.prefix_tiles)) * a.Nk : 0, base, false);
+      const long long at = running(some ? static_cast<long long>(own_places<TREE, QT>(a, G, s, 0, p.prefix_tiles)) * a.Nk : 0, base, false);
       int tile = tiles + __popc(with & ((1u << lane) - 1));
 #pragma unroll
       for (int i = 0; i < THREADS / 32; ++i) {
@@ -431,7 +438,7 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
       tile0[a.B] = tiles;
       first[tiles] = base;
     }
-    p.total = base + prefix_places<QT>(a, G, all_rows, p.prefix_tiles);
+    p.total = backwards ? 0 : base + prefix_places<TREE, QT>(a, G, all_rows, p.prefix_tiles);
     return p;
   }
   const long long most = most_row_tiles(a.T, a.B, a.N, a.Nk);   // more than these only lengths that overlap have: the rest is left out
@@ -449,20 +456,28 @@ __device__ __forceinline__ Plan make_plan(const ortb200_prefix_attn_args& a, lon
     long long n = 0;
     if (r < tiles) {
       const int b = sequence_with(tile0, a.B, r);
-      n = static_cast<long long>(own_places<QT>(a, G, span_of(a, b), r - tile0[b], p.prefix_tiles)) * a.Nk;
+      n = static_cast<long long>(own_places<TREE, QT>(a, G, span_of(a, b), r - tile0[b], p.prefix_tiles)) * a.Nk;
     }
     const long long at = running(n, base, r0 > 0);
     if (r < tiles) first[r] = at;
   }
   if (threadIdx.x == 0) first[tiles] = base;
-  p.total = base + prefix_places<QT>(a, G, all_rows, p.prefix_tiles);
+  p.total = backwards ? 0 : base + prefix_places<TREE, QT>(a, G, all_rows, p.prefix_tiles);
   return p;
 }
 
-// sequence_of by a CTA of 128: one round of loads instead of a chain of them
-__device__ __forceinline__ int sequence_among(const int* cu, int B, int t) {
+// sequence_of by a CTA of 128: one round of loads instead of a chain of them.  `backwards`: the lengths run backwards somewhere, which alone
+// makes sequences overlap.
+__device__ __forceinline__ int sequence_among(const int* cu, int B, int t, bool* backwards) {
   int before = 0;
-  for (int b0 = 0; b0 < B; b0 += 128) before += __syncthreads_count(b0 + static_cast<int>(threadIdx.x) < B && cu[b0 + threadIdx.x] <= t);
+  bool back = false;
+  for (int b0 = 0; b0 < B; b0 += 128) {
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    const int from = b < B ? cu[b] : 0, to = b < B ? cu[b + 1] : 0;
+    back |= to < from;
+    before += __syncthreads_count(b < B && from <= t);
+  }
+  *backwards = __syncthreads_or(back);
   return max(before - 1, 0);
 }
 
@@ -475,7 +490,7 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
   pdl_launch_dependents();   // behind the wait: when step 2 begins, everything in front of this step has ended
   if (blockIdx.x == a.T) {
     if (blockIdx.y != 0) return;
-    const Plan p = make_plan<128, QT>(a, w.first, w.tile0, a.status);
+    const Plan p = make_plan<128, TREE, QT>(a, w.first, w.tile0, a.status);
     if (threadIdx.x == 0) *w.plan = p;
     return;
   }
@@ -484,13 +499,26 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
     const char* row = static_cast<const char*>(a.qkv) + static_cast<long long>(t) * heads * H * sizeof(T);
     for (int i = threadIdx.x * 128; i < heads * H * static_cast<int>(sizeof(T)); i += 128 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + i));
   }
-  if (t >= last_row(a)) return;
-  const int b = TREE ? sequence_among(a.cu_seqlens, a.B, t) : sequence_of(a.cu_seqlens, a.B, t);
+  auto nobodys = [&]() {   // a row of no sequence: its result is 0 (without trees step 3 sees to it)
+    if (!TREE || blockIdx.y != 0) return;
+    T* out = static_cast<T*>(a.out) + static_cast<long long>(t) * a.N * H;
+    for (int i = threadIdx.x; i < a.N * H; i += 128) out[i] = from_float<T>(0.f);
+  };
+  if (t >= last_row(a)) {
+    nobodys();
+    return;
+  }
+  bool backwards = false;
+  const int b = TREE ? sequence_among(a.cu_seqlens, a.B, t, &backwards) : sequence_of(a.cu_seqlens, a.B, t);
+  if (backwards) nobodys();   // (of such lengths the plan is empty)
   if (blockIdx.y == 0 && threadIdx.x == 0) {
     const Span sp = span_of(a, b);
     w.token[t] = make_int4(b, sp.row0, sp.rows, sp.past);
   }
-  if (!owned(a, b, t)) return;   // (its queries stay what the workspace holds; no row's result reaches another's)
+  if (!owned(a, b, t)) {   // (its queries stay what the workspace holds; no row's result reaches another's)
+    nobodys();
+    return;
+  }
   long long slot, pos;
   if (a.positions) {
     pos = a.positions[t];
@@ -604,10 +632,10 @@ struct Segment {
   int past, in_seq;      // own units: tokens in front of the sequence's rows, first row of the unit among the sequence's rows x G
   int table_row;
   bool tree;             // own units: new keys are seen by the rows' bits
-  long long slot;
+  long long slot;        // -1: an own unit without a prefix, and the segment is all of it (trees)
 };
 // The segments of a CTA one after the other: its first unit is searched for, the others follow from the one before.
-template <int QT>
+template <bool TREE, int QT>
 struct Walk {
   const ortb200_prefix_attn_args& a;
   const int* tile0;
@@ -620,7 +648,7 @@ struct Walk {
   __device__ Walk(const ortb200_prefix_attn_args& args, const long long* first, const int* tiles_of, const Plan& p, int cta)
       : a(args), tile0(tiles_of), G(args.N / args.Nk), prefix_tiles(p.prefix_tiles), prefix_row(p.prefix_row) {
     all_rows = last_row(a);
-    const long long prefix_total = prefix_places<QT>(a, G, all_rows, prefix_tiles);
+    const long long prefix_total = prefix_places<TREE, QT>(a, G, all_rows, prefix_tiles);
     long long x = share<QT>(p.total, cta);
     left = share<QT>(p.total, cta + 1) - x;
     seq = -1;
@@ -648,7 +676,7 @@ struct Walk {
   }
   __device__ void prefix_unit() {
     tiles = prefix_tiles;
-    before = extra(unit_rows<QT>(G, all_rows, 0));
+    before = extra<TREE>(unit_rows<QT>(G, all_rows, 0));
     unit.seq = -1;
     unit.q_row = rt * QT;
     unit.rows = unit_rows<QT>(G, all_rows, rt);
@@ -662,7 +690,7 @@ struct Walk {
   __device__ void own_unit() {
     tiles = own_tiles<QT>(a, G, s, rt, prefix_tiles);
     unit.rows = unit_rows<QT>(G, s.rows, rt);
-    before = tiles > 0 ? extra(unit.rows) : 0;
+    before = tiles > 0 ? extra<TREE>(unit.rows) : 0;
     unit.seq = unit.table_row = seq;
     unit.in_seq = rt * QT;
     unit.q_row = s.row0 * G + unit.in_seq;
@@ -714,12 +742,18 @@ struct Walk {
       g.tiles = n;
       g.kvh = kvh;
       g.key0 += t0 * kKT;
-      g.slot += static_cast<long long>(kvh) * g.rows;
+      g.slot = TREE && n == tiles ? -1 : g.slot + static_cast<long long>(kvh) * g.rows;
       return true;
     }
     return false;
   }
 };
+// Trees: a segment that is all of its unit has its rows' results, which need no step 3.  Row r's place among them.
+template <int HD>
+__device__ __forceinline__ uint16_t* result_of(const ortb200_prefix_attn_args& a, const Segment& g, int r) {
+  const int G = a.N / a.Nk, t = (g.q_row + r) / G;
+  return static_cast<uint16_t*>(a.out) + (static_cast<long long>(t) * a.N + g.kvh * G + (g.q_row + r - t * G)) * HD;
+}
 // Queries of up to 64 rows take one of two places in turn, so that the next segment's arrive while this one's are in use; more
 // take both.  (Wide units have one place: their segments are long.)
 template <int QT>
@@ -1003,6 +1037,7 @@ __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, cons
   }
   l0 = sum_over_keys(l0);
   l1 = sum_over_keys(l1);
+  const bool whole = TREE && g.slot < 0;
   named_barrier(1, 128);   // all have read the queries, and the sums of the segment before
   if (lane < 4) {
     part[qw][n0] = make_float2(m0, l0);
@@ -1040,10 +1075,17 @@ __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, cons
         v[x + 3] += f * y.w;
       }
     }
-    const long long row = g.slot + static_cast<long long>(blockIdx.x) * QT + n;
-    if ((lane & 15) == 0) w.ml[row] = make_float2(m, l);
+    if (whole) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      uint16_t* const result = result_of<HD>(a, g, n);
 #pragma unroll
-    for (int x = 0; x < E; x += 4) *reinterpret_cast<float4*>(w.o + row * HD + d0 + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+      for (int x = 0; x < E; x += 4) *reinterpret_cast<uint2*>(result + d0 + x) = make_uint2(pack16<BF16>(v[x] * inv, v[x + 1] * inv), pack16<BF16>(v[x + 2] * inv, v[x + 3] * inv));
+    } else {
+      const long long row = g.slot + static_cast<long long>(blockIdx.x) * QT + n;
+      if ((lane & 15) == 0) w.ml[row] = make_float2(m, l);
+#pragma unroll
+      for (int x = 0; x < E; x += 4) *reinterpret_cast<float4*>(w.o + row * HD + d0 + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+    }
   }
   fence_proxy_async();   // the next queries arrive where the sums were
   __syncwarp();
@@ -1086,7 +1128,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   Plan plan;
   const bool kept = most_row_tiles(a.T, a.B, a.N, a.Nk) <= kPlanInSmem;
   if (kept) {
-    plan = make_plan<threads_of<QT>, QT>(a, first_sm, tile0_sm, nullptr);
+    plan = make_plan<threads_of<QT>, TREE, QT>(a, first_sm, tile0_sm, nullptr);
   } else {
     pdl_wait_prior_grids();
     plan = *w.plan;
@@ -1100,7 +1142,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   const uint32_t tmem_o = tmem_s + 2 * kKT;
   uint64_t* tile_bars = bars + BAR_TILE + tile * BAR_OF_TILE;
 
-  Walk<QT> walk(a, kept ? first_sm : w.first, kept ? tile0_sm : w.tile0, plan, blockIdx.x);
+  Walk<TREE, QT> walk(a, kept ? first_sm : w.first, kept ? tile0_sm : w.tile0, plan, blockIdx.x);
   Segment g;
   bool ok = true;
 
@@ -1433,15 +1475,31 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       if (!idle) {
         const long long row = g.slot + static_cast<long long>(blockIdx.x) * QT + r;
         const bool mine = ok && r < g.rows;
-        if (mine) w.ml[row] = make_float2(m, l);
+        if (TREE && g.slot < 0) {
+          uint16_t* const result = result_of<HD>(a, g, r);
+          const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 32) {
-          float v[32];
-          tmem_ld_x32(tmem_o + lane_addr + c, v);
-          tmem_ld_wait();
-          if (mine)
+          for (int c = 0; c < HD; c += 32) {
+            float v[32];
+            tmem_ld_x32(tmem_o + lane_addr + c, v);
+            tmem_ld_wait();
+            if (mine)
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) store8(w.o + row * HD + c + j, v + j);
+              for (int j = 0; j < 32; j += 8)
+                *reinterpret_cast<uint4*>(result + c + j) = make_uint4(pack16<BF16>(v[j] * inv, v[j + 1] * inv), pack16<BF16>(v[j + 2] * inv, v[j + 3] * inv),
+                                                                       pack16<BF16>(v[j + 4] * inv, v[j + 5] * inv), pack16<BF16>(v[j + 6] * inv, v[j + 7] * inv));
+          }
+        } else {
+          if (mine) w.ml[row] = make_float2(m, l);
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 32) {
+            float v[32];
+            tmem_ld_x32(tmem_o + lane_addr + c, v);
+            tmem_ld_wait();
+            if (mine)
+#pragma unroll
+              for (int j = 0; j < 32; j += 8) store8(w.o + row * HD + c + j, v + j);
+          }
         }
       }
       tcgen05_fence_before();
@@ -1494,7 +1552,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
   // where the own units of the row's row tile start
   const int my_ort = my_live ? (static_cast<int>(row0) + min(lane, count - 1) - my_tok.y * G) / QT : 0, my_tile = my_live ? __ldcg(&w.tile0[my_tok.x]) + my_ort : 0;
   const bool counted = my_live && my_tile < __ldcg(&w.tile0[my_tok.x + 1]);
-  const long long my_start = counted ? prefix_places<QT>(a, G, all_rows, plan.prefix_tiles) + __ldcg(&w.first[my_tile]) : 0;
+  const long long my_start = counted ? prefix_places<TREE, QT>(a, G, all_rows, plan.prefix_tiles) + __ldcg(&w.first[my_tile]) : 0;
   // the units of a row, 0 of the prefix and 1 of its own keys: first tile in the numbering, tiles, first slot
   int prt = -1, ort = -1, seq = -1, tiles0 = 0, tiles1 = 0, first0 = 0, first1 = 0, count0 = 0, count1 = 0;
   long long from0 = 0, from1 = 0, slot0 = 0, slot1 = 0, start = 0;
@@ -1529,7 +1587,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
       const Span s = {tok.y, tok.z, tok.w};
       prt = pr / QT;
       tiles0 = plan.prefix_tiles;
-      const int before0 = extra(unit_rows<QT>(G, all_rows, 0));
+      const int before0 = extra<TREE>(unit_rows<QT>(G, all_rows, 0));
       from0 = (static_cast<long long>(prt) * a.Nk + kvh) * (tiles0 + before0) + before0;
       slot0 = prefix_slot<QT>(a, prt, kvh, unit_rows<QT>(G, all_rows, prt));
       seq = tok.x;
@@ -1537,7 +1595,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
       start = __shfl_sync(0xffffffffu, my_start, r);
       tiles1 = own_tiles<QT>(a, G, s, ort, tiles0);
       const int rows1 = unit_rows<QT>(G, s.rows, ort);
-      from1 = start + static_cast<long long>(kvh) * places(tiles1, rows1) + extra(rows1);
+      from1 = start + static_cast<long long>(kvh) * places<TREE>(tiles1, rows1) + extra<TREE>(rows1);
       slot1 = own_slot<QT>(a, G, s.row0, ort, kvh, rows1);
       first0 = tiles0 > 0 ? owner<QT>(plan.total, from0) : 0;
       first1 = tiles1 > 0 ? owner<QT>(plan.total, from1) : 0;
@@ -1554,6 +1612,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
       }
     }
     if (r == 0) pdl_wait_prior_grids();
+    if (TREE && n == 1) return;   // step 2 has written it (a CTA of these has one row)
     float o[E], m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
@@ -1645,6 +1704,131 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
   }
 }
 
+// Step 3 for trees of more rows.  There is no prefix, and step 2 has written the rows of the units that one CTA has.  The others are those that the
+// start of a share lies within: so the grid goes over the shares and not over the rows.  The first start within a unit has its rows, a CTA up to 32 of
+// them and a warp four.  What it takes beside step 2 is waiting for loads, so that few rows behind one another matter, and not how many CTAs look in vain.  All segments
+// written and all rows joined, up to 32 by a warp one after the other, against this, whole calls back to back: 146 and 95 us (75 trees of up to 60 tokens
+// behind 779, 24 heads over 8 of 64), 107 and 78 (52 of up to 58 behind 382, 32 over 8 of 128), 131 and 112 (512 of up to 4 behind 500), but 28.7 and 30.7
+// (20 of up to 10 behind 500).
+constexpr int kJoinRows = 32, kJoinThreads = 256;
+// the last of n ascending places that is not behind x, by all of a CTA
+template <typename I>
+__device__ __forceinline__ int place_among(const I* places, int n, I x) {
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + kJoinThreads - 1) / kJoinThreads, at = static_cast<int>(threadIdx.x) * step;
+    const int count = __syncthreads_count(at < n && __ldcg(places + lo + at) <= x);
+    const int before = max(count - 1, 0) * step;
+    lo += before;
+    n = min(n - before, step);
+  }
+  return lo;
+}
+template <typename T, int HD, int QT>
+__global__ void __launch_bounds__(kJoinThreads, 4) tree_join_kernel(const ortb200_prefix_attn_args a) {
+  constexpr int E = HD / 32, kRows = kJoinRows / (kJoinThreads / 32), R = 2, S = 2;   // S segments of R rows on their way at a time
+  __shared__ long long base[grid_of<QT>];
+  __shared__ int found;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.N / a.Nk, row0 = blockIdx.y * kJoinRows;
+  const Work w = work_of<true>(a);
+  // (step 1 has ended when this step begins: only the segments are waited for)
+  const long long total = __ldcg(&w.plan->total);
+  const int units = __ldcg(&w.tile0[a.B]);
+  int rows = 0, b = 0, rt = 0, kvh = 0;
+  Span s = {0, 0, 0};
+  if (total > 0) {
+    const int i = blockIdx.x;
+    const long long x = share<QT>(total, i);
+    const int r = place_among(w.first, units, x);
+    b = place_among(w.tile0, a.B, r);
+    s = span_of(a, b);
+    rt = r - __ldcg(&w.tile0[b]);
+    rows = unit_rows<QT>(G, s.rows, rt);
+    const int tiles = own_tiles<QT>(a, G, s, rt, 0), each = places<true>(tiles, rows);
+    const long long first = __ldcg(&w.first[r]);
+    kvh = static_cast<int>((x - first) / each);
+    const long long from = first + static_cast<long long>(kvh) * each + extra<true>(rows), slot = own_slot<QT>(a, G, s.row0, rt, kvh, rows);
+    if (i == 0 || !(x > from && x < from + tiles && share<QT>(total, i - 1) <= from)) rows = 0;
+    if (row0 < rows && warp == 0) {
+      int n = 0;
+      for (int k0 = i - 1; k0 < grid_of<QT> && share<QT>(total, k0) < from + tiles; k0 += 32) {
+        const int k = k0 + lane;
+        const bool has = k < grid_of<QT> && max(from, share<QT>(total, k)) < min(from + tiles, share<QT>(total, k + 1));
+        const unsigned all = __ballot_sync(0xffffffffu, has);
+        if (has) base[n + __popc(all & ((1u << lane) - 1))] = slot + static_cast<long long>(k) * QT;
+        n += __popc(all);
+      }
+      if (lane == 0) found = n;
+    }
+  }
+  const int mine0 = row0 + warp * kRows, in_seq = rt * QT, live = min(rows - mine0, kRows);
+  pdl_wait_prior_grids();
+  if (row0 >= rows) return;
+  __syncthreads();
+  const int n = found;
+#pragma unroll 1
+  for (int q0 = 0; q0 < kRows; q0 += R) {
+    if (q0 >= live) break;
+    float o[R][E], m[R], l[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      m[q] = -INFINITY;
+      l[q] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[q][e] = 0.f;
+    }
+#pragma unroll 1
+    for (int k = 0; k < n; k += S) {
+      float2 ml[S][R];
+      float v[S][R][E];
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+          const bool some = k + i < n && q0 + q < live;
+          const long long at = base[min(k + i, n - 1)] + mine0 + q0 + q;
+          ml[i][q] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[i][q][e] = 0.f;
+          if (some) {
+            ml[i][q] = __ldcg(&w.ml[at]);
+            load_cg<E>(w.o + at * HD + lane * E, v[i][q]);
+          }
+        }
+#pragma unroll
+      for (int q = 0; q < R; ++q) {
+        float mm = m[q];
+#pragma unroll
+        for (int i = 0; i < S; ++i) mm = fmaxf(mm, ml[i][q].x);
+        const float keep = m[q] == -INFINITY ? 0.f : exp2f(m[q] - mm);
+        l[q] = m[q] == -INFINITY ? l[q] : l[q] * keep;   // (a sum without a maximum is 0 or NaN)
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[q][e] *= keep;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          const float f = ml[i][q].x == -INFINITY ? 0.f : exp2f(ml[i][q].x - mm);
+          l[q] += ml[i][q].x == -INFINITY ? ml[i][q].y : ml[i][q].y * f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[q][e] += f * v[i][q][e];
+        }
+        m[q] = mm;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      if (q0 + q < live) {
+        const int row = in_seq + mine0 + q0 + q, t = s.row0 + row / G;
+        const float inv = l[q] == 0.f ? 0.f : 1.f / l[q];
+        T* out = static_cast<T*>(a.out) + (static_cast<long long>(t) * a.N + kvh * G + row % G) * HD + lane * E;
+        __align__(8) T y[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = from_float<T>(o[q][e] * inv);
+        if (E == 4) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(y);
+        else *reinterpret_cast<uint32_t*>(out) = *reinterpret_cast<const uint32_t*>(y);
+      }
+  }
+}
+
 template <typename T>
 bool vectorised(const ortb200_prefix_attn_args* a) {
   if (a->cos_cache && (a->interleaved || a->rot_dim != a->H)) return false;
@@ -1682,10 +1866,14 @@ int launch_tc(const ortb200_prefix_attn_args* a, const int* parents, cudaStream_
   // later would look their segments up when the others have ended (24 prompts of up to 150 tokens: 37 us behind the product kernel
   // instead of 80).
   if (a->T * a->N <= 2 * kGrid) return launch_kernel(prefix_join_kernel<T, HD, true, TREE, QT>, dim3(static_cast<unsigned>(a->T * a->N)), 128, 0, stream, true, *a, 1);
-  const long long fit = 16 * kGrid / 2;
-  const int per = static_cast<int>(std::min<long long>(32, (a->T * a->N + fit - 1) / fit));
-  const long long warps = (rows + per - 1) / per * a->Nk;
-  return launch_kernel(prefix_join_kernel<T, HD, false, TREE, QT>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0, stream, true, *a, per);
+  if constexpr (TREE) {
+    return launch_kernel(tree_join_kernel<T, HD, QT>, dim3(grid_of<QT>, QT / kJoinRows), kJoinThreads, 0, stream, true, *a);
+  } else {
+    const long long fit = 16 * kGrid / 2;
+    const int per = static_cast<int>(std::min<long long>(32, (a->T * a->N + fit - 1) / fit));
+    const long long warps = (rows + per - 1) / per * a->Nk;
+    return launch_kernel(prefix_join_kernel<T, HD, false, TREE, QT>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0, stream, true, *a, per);
+  }
 }
 
 // Wide units where sequences bring more than 192 rows on average (G for each token), heads of 128: two tiles of rows share what is

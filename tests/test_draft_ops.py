@@ -193,6 +193,16 @@ def test_tree_batches_of_many_rows(N, Nk, H, nodes):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N,Nk,H", [(24, 8, 64), (32, 8, 128), (32, 32, 64), (16, 1, 128)])
+@pytest.mark.parametrize("long", [0, 6000])
+def test_tree_units_of_one_and_of_several_ctas(dt, N, Nk, H, long):
+    """Units of every size, most of which one CTA has; with a long sequence some are spread over many."""
+    pasts = [(97 * i) % 400 + (long if i == 9 else 0) for i in range(45)]
+    TreeCase(dt, N, Nk, H, 32, pasts, [tree((37 * i) % 61, i) for i in range(45)], seed=11, behind=3).run(GPU)
+
+
+@pytest.mark.gpu
 def test_tree_wide_units_of_many_sequences():
     """More units of two row tiles than a CTA keeps the running sums of."""
     TreeCase(torch.bfloat16, 64, 1, 128, 16, [i % 67 for i in range(300)], [tree(4 + (i % 5 == 0), i) for i in range(300)], seed=8).run(GPU)
@@ -281,6 +291,15 @@ def test_tree_lengths_and_tables_that_fit_nothing(kind, change):
     else:
         for n, t in change.items():
             call.ins[n].copy_(t)
+    with pytest.raises((InvalidArgument, EPFail)):
+        call()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("N,Nk", [(4, 2), (64, 2)])
+def test_tree_lengths_that_run_backwards(kind, N, Nk):
+    call = TreeCase(kind[1], N, Nk, 64, 16, [20, 40, 70], [[-1, 0], [-1, 0, 0], [-1, 0, 1, 1]]).call(kind[0])
+    call.ins["cum"].copy_(i32(0, 6, 2, 9))
     with pytest.raises((InvalidArgument, EPFail)):
         call()
 
