@@ -8,7 +8,7 @@
 //
 // What bounds it: without texts the stream (384 rows of 128256 bf16 logits 55 us, 295 MB; the bytes need 45).  With a text of 2250 tokens to a
 // row 108 us: reading and counting it in each of 16 chunks, 112 MB out of L2 and half of the instructions; issue slots are 67 % busy.  A text of
-// 45000 tokens and 50257 32-bit logits, 40 rows: 27 us, nearly all of it the text.  Slower, for the same 384 rows: a text read once by a cluster of
+// 45000 tokens and 50257 32-bit logits, 40 rows: 24 us, nearly all of it the text.  Slower, for the same 384 rows: a text read once by a cluster of
 // the row's CTAs, which add to each other's counters, 212 us; a kernel that gathers what a row touches in a hash table, behind the stream or
 // in front of it, 105 to 111 and a second launch; a warp's tokens of the chunk queued and counted 32 at a time 123.
 #include <cuda_runtime.h>
@@ -384,7 +384,7 @@ int launch_rows(const ortb200_process_logits_args* a, cudaStream_t stream) {
   if (!a->history && !a->drafted && !a->bias_tokens) return launch<T, E, false, 256>(a, 0, stream);
   // Every chunk reads the row's text.  Texts of up to 64 KB: chunks of 8192 and CTAs of 256 threads, six to an SM (384 rows of 128256 with 2250
   // tokens 108 us, with 10 tokens 70; chunks of 16384 and three CTAs of 512 threads 104 and 80, two of them 122 and 92).  Longer ones: chunks of 16384,
-  // half as many bytes of text, and 1024 threads that read them (40 rows of 50257 with 45000 tokens 27 us, 512 threads 32, the short texts' way 45).
+  // half as many bytes of text, and 1024 threads that read them (40 rows of 50257 with 45000 tokens 24 us; before a text's two parts had loops of their own 27, 512 threads 32, the short texts' way 45).
   const int64_t text_bytes = a->history && a->lists > 0 ? 8 * (a->history_len / a->lists) : 0;
   return text_bytes > 64 * 1024 ? launch<T, E, true, 1024>(a, text_bytes, stream) : launch<T, E, true, 256>(a, text_bytes, stream);
 }
