@@ -117,7 +117,7 @@ void ProcessLogitsImpl(Ctx& ctx) {
         }
       }
       for (const auto& [v, s] : sums) {
-        to[v] += s;
+        to[v] = s == -std::numeric_limits<float>::infinity() ? s : to[v] + s;   // a ban holds for logits that are infinite or NaN, too
         sum_of[v] = 0;
       }
     }

@@ -45,7 +45,7 @@ int64_t ortb200_cache_move_max_moves(void);
 //   c: how often the token occurs in the row's text, counted from generated_starts of its list on, and seen: whether it occurs at all
 //   seen:      x = x < 0 ? x repetition : x / repetition
 //   always:    x = x - (frequency c + presence [c > 0])
-//   biased:    x = x + the sum of the token's biases, in their order
+//   biased:    x = x + the sum of the token's biases, in their order; -inf where that sum is -inf, whatever x is
 //   masked:    x = -inf where the row's mask has the bit 0
 //   always:    x = x / temperature (a temperature that is not above 0 leaves x)
 // The text of a row is the tokens of its list, history[history_starts[l], history_starts[l + 1]), and the `drafted_width` tokens of its

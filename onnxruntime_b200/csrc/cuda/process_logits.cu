@@ -170,7 +170,10 @@ struct Scorer {
     if (q.temperature != 1.f) f = warmth(f);
     return allowed(v) ? f : -INFINITY;
   }
-  __device__ __forceinline__ void whole(int v, unsigned word, float bias) const { y[v] = finished(v, penalised(q, repeated, to_float<T>(x[v]), word) + bias); }
+  // (a bias of -inf is a ban: added to an infinite logit, or to one that is no number, it would leave a NaN, which a search for the largest takes)
+  __device__ __forceinline__ void whole(int v, unsigned word, float bias) const {
+    y[v] = bias == -INFINITY ? bias : finished(v, penalised(q, repeated, to_float<T>(x[v]), word) + bias);
+  }
 };
 
 // How a row is divided: its vectors start at the first token whose place in the tensor E divides; what is in front of them is the first

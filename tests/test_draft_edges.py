@@ -1,0 +1,48 @@
+"""Edges of the decode step with drafted tokens: what its operators, the pool and the generation loop make of infinities, shared blocks, drafts
+that a grammar forbids, and limits.  The definitions are draft_oracle.py's."""
+import math
+
+import pytest
+import torch
+
+from onnxruntime_b200.models.generation import GenerationConfig, LogitsProcessor
+from test_draft_generation import PROVIDERS
+from test_draft_ops import LOGITS_KINDS, LogitsCase
+
+
+# ----------------------------------------------------------------------------------------------------------------------- bans
+HARD = [math.inf, -math.inf, math.nan, 0.0]
+
+
+@pytest.mark.parametrize("kind", LOGITS_KINDS)
+@pytest.mark.parametrize("biases", [4, 400])
+@pytest.mark.parametrize("twice", [False, True])
+def test_banned_tokens_of_any_logit(kind, biases, twice):
+    """A token whose biases sum to -inf has -inf, whatever its logit is: infinities, NaN, the type's largest number; on rows with few biases and
+    with more than are listed, named once and twice, inside and outside of the text."""
+    vocab, tokens = 3001, torch.arange(biases) * 7 + 1
+    case = LogitsCase(kind[1], 2, vocab, without=["row_list", "drafted", "allowed", "row_mask"], seed=biases)
+    hard = torch.tensor([*HARD, torch.finfo(kind[1]).max])
+    case.t["logits"][:, tokens] = hard[torch.arange(biases) % 5].to(kind[1])
+    named = torch.cat([tokens, tokens[::2]]) if twice else tokens
+    per = len(named)
+    case.t.update(history=torch.arange(2 * 50) % 50, history_starts=torch.tensor([0, 50, 100]), generated_starts=torch.tensor([20, 60]), bias_tokens=named.repeat(2),
+                  bias_values=torch.full((2 * per,), -math.inf), bias_starts=torch.tensor([0, per, 2 * per]), repetition=torch.tensor([1.0, 1.5]), presence=torch.tensor([0.5, 0.0]),
+                  frequency=torch.tensor([0.25, 0.0]), temperature=torch.tensor([0.5, 1.0]))
+    got = case.call(kind[0])()["scores"]
+    assert (got[:, tokens] == -math.inf).all()
+    free = torch.ones(vocab, dtype=torch.bool)
+    free[tokens] = False
+    assert got[:, free].isfinite().all()
+
+
+@pytest.mark.parametrize("provider", PROVIDERS)
+@pytest.mark.parametrize("hard", [math.inf, math.nan])
+@pytest.mark.parametrize("kw", [dict(eos_token_id=5, min_new_tokens=4), dict(no_repeat_ngram_size=2), dict(no_repeat_ngram_size=1), dict(logit_bias={5: -math.inf})], ids=str)
+def test_a_banned_token_is_not_chosen(provider, hard, kw):
+    """An end token before its time, and one that would repeat an n-gram, are not the best of a row whatever the model says of them."""
+    device = torch.device("cuda" if provider == "CUDAExecutionProvider" else "cpu")
+    logits = torch.linspace(-1, 1, 40).repeat(2, 1)
+    logits[:, 5] = hard
+    scores = LogitsProcessor(40, torch.float32, device, GenerationConfig(**kw))(logits.to(device), [([1, 2, 5, 1, 2], 1, [[]]), ([2, 5, 3, 2], 0, [[]])]).cpu()
+    assert (scores[:, 5] == -math.inf).all() and scores.argmax(-1).tolist() == [39, 39]
