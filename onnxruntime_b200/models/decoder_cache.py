@@ -135,12 +135,19 @@ class CachePool:
 
     def keep(self, chosen: Dict[Hashable, Tuple[int, Sequence[int]]]) -> None:
         """Of the tokens behind the first ``held`` of a sequence, only those at the places ``path`` (ascending, counted from
-        ``held``), which close up: ``chosen`` names (held, path) for each sequence."""
+        ``held``), which close up: ``chosen`` names (held, path) for each sequence.  Blocks that several sequences share are not
+        written, now or by the tokens that follow, and state in slots has no memory of fewer tokens than all."""
         sources, targets = [], []
         for seq, (held, path) in chosen.items():
             entry = self.sequences[seq]
             if not 0 <= held <= held + len(path) <= entry.length or any(not 0 <= p < entry.length - held for p in path) or any(a >= b for a, b in zip(path, path[1:])):
                 raise ValueError(f"sequence {seq!r} holds no such tokens")
+            if held + len(path) == entry.length:
+                continue
+            if any(b in self.owners for b in entry.blocks[held // self.block_size:]):
+                raise ValueError(f"sequence {seq!r}: blocks that several sequences share are not written")
+            if any(c.kind == "slot" for c in self.spec):
+                raise ValueError(f"the state of sequence {seq!r} is that of all its {entry.length} tokens")
         for seq, (held, path) in chosen.items():
             entry = self.sequences[seq]
             place = lambda t: entry.blocks[t // self.block_size] * self.block_size + t % self.block_size  # noqa: E731, B023

@@ -5,8 +5,9 @@ import math
 import pytest
 import torch
 
+from onnxruntime_b200.models.decoder_cache import CachePool, CacheTensor
 from onnxruntime_b200.models.generation import GenerationConfig, LogitsProcessor
-from test_draft_generation import PROVIDERS
+from test_draft_generation import PROVIDERS, pool
 from test_draft_ops import LOGITS_KINDS, LogitsCase
 
 
@@ -46,3 +47,49 @@ def test_a_banned_token_is_not_chosen(provider, hard, kw):
     logits[:, 5] = hard
     scores = LogitsProcessor(40, torch.float32, device, GenerationConfig(**kw))(logits.to(device), [([1, 2, 5, 1, 2], 1, [[]]), ([2, 5, 3, 2], 0, [[]])]).cpu()
     assert (scores[:, 5] == -math.inf).all() and scores.argmax(-1).tolist() == [39, 39]
+
+
+# ------------------------------------------------------------------------------------------------------------------- the pool
+def hold(p, seq, tokens):
+    if seq not in p.sequences:
+        p.open(seq)
+    p.reserve(seq, tokens)
+    p.advance(seq, tokens)
+
+
+@pytest.mark.parametrize("held,path", [(2, [1, 3]), (0, []), (6, [0]), (8, []), (8, [1]), (7, [0, 1])])
+def test_pool_keeps_no_path_in_shared_blocks(held, path):
+    """What another sequence holds, or would see written by the tokens that follow a shorter path, stays: the call is refused before anything moves."""
+    p = pool()
+    hold(p, "a", 12)
+    p.fork("b", "a")
+    hold(p, "c", 3)
+    before = {n: t.clone() for n, t in p.tensors.items()}
+    with pytest.raises(ValueError):
+        p.keep({"c": (0, [1]), "a": (held, path)})
+    assert p.sequences["a"].length == 12 and p.sequences["c"].length == 3
+    assert all(torch.equal(t, before[n]) for n, t in p.tensors.items())
+
+
+def test_pool_keeps_paths_behind_shared_blocks():
+    p = pool()
+    hold(p, "a", 8)
+    p.fork("b", "a")
+    hold(p, "a", 3)
+    last = {n: t[p.sequences["a"].blocks[2], 2].clone() for n, t in p.tensors.items()}
+    p.keep({"a": (8, [2]), "b": (2, range(6))})       # (all of b's tokens: nothing moves)
+    assert p.sequences["a"].length == 9 and p.sequences["b"].length == 8
+    assert all(torch.equal(t[p.sequences["a"].blocks[2], 0], last[n]) for n, t in p.tensors.items())
+    p.close("b")
+    p.keep({"a": (1, [4])})                           # nobody else's any more
+    assert p.sequences["a"].length == 2
+
+
+def test_pool_keeps_no_path_of_state_in_slots():
+    spec = [CacheTensor("k", "k_out", "paged", (2,), torch.float32), CacheTensor("s", "s_out", "slot", (3,), torch.float32)]
+    p = CachePool(spec, 4, 4, 2, torch.device("cpu"))
+    hold(p, "a", 5)
+    with pytest.raises(ValueError):
+        p.keep({"a": (3, [1])})
+    p.keep({"a": (3, [0, 1])})
+    assert p.sequences["a"].length == 5
