@@ -516,7 +516,8 @@ class GenerationConfig:
                  grammar: Optional[Callable[[List[int]], Optional[Sequence[int]]]] = None, draft_tokens: int = 0, draft_ngram: int = 3):
         """For ``generate_requests``: ``logprobs``: report log probabilities, entropies and that many best alternatives.
         ``presence_penalty`` and ``frequency_penalty`` are subtracted from the logits of generated tokens, once and as often as they
-        occur; ``logit_bias`` is added to tokens' logits; ``grammar`` names the tokens that may follow the generated ones (None: all).
+        occur; ``logit_bias`` is added to tokens' logits; ``grammar`` names the tokens that may follow the generated ones (None: all), and is
+        asked only about tokens that it has named.
         ``draft_tokens`` (runners with ``draft_trees``): up to so many tokens a step are drafted from what followed the last
         ``draft_ngram`` tokens, or fewer, earlier in the request's own text; the step keeps those that it would have chosen."""
         self.__dict__.update(locals())
@@ -658,16 +659,17 @@ class LogitsProcessor:
     def _mask(self, allowed: Optional[Sequence[int]]) -> torch.Tensor:
         keep = torch.ones(self.vocab_size, dtype=torch.bool) if allowed is None else torch.zeros(self.vocab_size, dtype=torch.bool)
         if allowed is not None:
-            keep[torch.as_tensor(list(allowed), dtype=torch.int64)] = True
+            keep[torch.from_numpy(_token_array(allowed))] = True
         if self.cfg.vocab_mask is not None:
             keep &= self.cfg.vocab_mask.reshape(-1).cpu() != 0
         words = torch.nn.functional.pad(keep, (0, -self.vocab_size % 32)).reshape(-1, 32).long()
         packed = (words << torch.arange(32)).sum(-1)
         return torch.where(packed >= 1 << 31, packed - (1 << 32), packed).int()
 
-    def __call__(self, logits: torch.Tensor, requests: Sequence[Tuple[Sequence[int], int, Sequence[Sequence[int]]]]) -> torch.Tensor:
+    def __call__(self, logits: torch.Tensor, requests: Sequence[Tuple[Sequence[int], int, Sequence[Sequence[int]]]],
+                 named: Optional[Sequence[Optional[Sequence[int]]]] = None) -> torch.Tensor:
         """logits [rows, vocab] -> scores [rows, vocab] in 32 bits.  ``requests``: (text, how many tokens of it are generated, for each of
-        the request's rows the drafted tokens behind the text)."""
+        the request's rows the drafted tokens behind the text).  ``named``: what the grammar names for each row, where it has been asked."""
         if self.idle:
             return logits.float()
         cfg, dev, rows = self.cfg, self.device, logits.shape[0]
@@ -695,7 +697,9 @@ class LogitsProcessor:
             if cfg.grammar is None:
                 feeds.update(allowed=self._mask(None).reshape(1, -1).to(dev), row_mask=torch.zeros(rows, dtype=torch.int32, device=dev))
             else:
-                masks = [self._mask(cfg.grammar([int(t) for t in (*text[len(text) - new:], *p)])) for text, new, paths in requests for p in paths]
+                if named is None:
+                    named = [cfg.grammar([int(t) for t in (*text[len(text) - new:], *p)]) for text, new, paths in requests for p in paths]
+                masks = [self._mask(allowed) for allowed in named]
                 feeds.update(allowed=torch.stack(masks).to(dev), row_mask=torch.arange(rows, dtype=torch.int32, device=dev))
         if self.warm:
             feeds.update(temperature=same(cfg.temperature))
@@ -728,6 +732,35 @@ def draft_tree(text: Sequence[int], most: int, ngram: int = 3) -> Tuple[List[int
                     parents.append(node)
                 node = children[node, t]
     return tokens, parents
+
+
+def _permitted(cfg: GenerationConfig, generated: Sequence[int], tokens: Sequence[int], parents: Sequence[int]):
+    """Of a tree of drafted tokens behind ``generated`` those that can be chosen: tokens that the grammar names behind their parent, and no end
+    token, behind which nothing is.  The grammar is so asked for texts alone that it allows.  Returns the tokens, their parents, and for each what
+    the grammar names behind it (None: all)."""
+    kept: Dict[int, int] = {}
+    left, up, named, texts = [], [], [], []   # (texts: for a grammar)
+    for j, (token, parent) in enumerate(zip(tokens, parents)):
+        if parent >= 0:
+            if parent not in kept or token == cfg.eos_token_id:
+                continue
+            if named[kept[parent]] is not None and not (named[kept[parent]] == token).any():
+                continue
+        kept[j] = len(left)
+        left.append(token)
+        up.append(kept[parent] if parent >= 0 else -1)
+        if cfg.grammar is not None:
+            texts.append([*texts[up[-1]], token] if parent >= 0 else [int(t) for t in generated])
+        named.append(None if cfg.grammar is None else _token_array(cfg.grammar(list(texts[-1]))))
+    return left, up, named
+
+
+def _token_array(tokens: Optional[Sequence[int]]) -> Optional[np.ndarray]:
+    if tokens is None:
+        return None
+    if isinstance(tokens, torch.Tensor):
+        tokens = tokens.cpu().numpy()
+    return np.asarray(tokens if isinstance(tokens, np.ndarray) else list(tokens), dtype=np.int64).reshape(-1)
 
 
 def _places_of(text: np.ndarray, tail: np.ndarray) -> np.ndarray:
@@ -908,26 +941,28 @@ def _generate_requests(runner: PagedDecoderRunner, prompts, cfg: GenerationConfi
             running += joining
             for i in joining:
                 new[i] = []
-            trees = {i: ([-1], [-1]) for i in joining}   # a row for the last token of each
+            trees = {i: _permitted(cfg, [], [-1], [-1]) for i in joining}   # a row for the last token of each
             drafted = False
         elif running:
             joining = list(running)
             # room has been kept for the tokens that a request will generate: no more of them are drafted
             trees = {i: draft_tree(flat[i][:len(texts[i]) + len(new[i])], min(cfg.draft_tokens, cfg.max_new_tokens - len(new[i]) - 1), cfg.draft_ngram) if cfg.draft_tokens else ([new[i][-1]], [-1])
                      for i in joining}
-            drafted = any(len(tokens) > 1 for tokens, _ in trees.values())
+            trees = {i: _permitted(cfg, new[i], *tree) for i, tree in trees.items()}
+            drafted = any(len(tokens) > 1 for tokens, _, _ in trees.values())
             if drafted:
-                logits = runner.draft_step([(("request", i), *trees[i], range(len(trees[i][0]))) for i in joining])
+                logits = runner.draft_step([(("request", i), *trees[i][:2], range(len(trees[i][0]))) for i in joining])
             else:
                 logits = runner.step([(("request", i), [new[i][-1]], [0]) for i in joining])
         else:
             raise CacheFull(f"request {waiting[0]} does not fit into the cache")
-        paths = {i: _paths(*trees[i]) for i in joining}
-        scores = processor(logits, [(flat[i][:len(texts[i]) + len(new[i])], len(new[i]), [[trees[i][0][j] for j in path[1:]] for path in paths[i]]) for i in joining])
+        paths = {i: _paths(*trees[i][:2]) for i in joining}
+        scores = processor(logits, [(flat[i][:len(texts[i]) + len(new[i])], len(new[i]), [[trees[i][0][j] for j in path[1:]] for path in paths[i]]) for i in joining],
+                           [allowed for i in joining for allowed in trees[i][2]])
         best = [0] * len(scores) if sampling else scores.argmax(-1).tolist()
         row, kept = 0, {}
         for i in joining:   # from the root on, as far as the tree has what is chosen
-            tokens, parents = trees[i]
+            tokens, parents, _ = trees[i]
             node = 0
             while True:
                 tok = pick(i, logits[row + node], scores[row + node], best[row + node])

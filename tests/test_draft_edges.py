@@ -6,8 +6,8 @@ import pytest
 import torch
 
 from onnxruntime_b200.models.decoder_cache import CachePool, CacheTensor
-from onnxruntime_b200.models.generation import GenerationConfig, LogitsProcessor
-from test_draft_generation import PROVIDERS, pool
+from onnxruntime_b200.models.generation import GenerationConfig, LogitsProcessor, generate_requests
+from test_draft_generation import PROVIDERS, decoder, pool
 from test_draft_ops import LOGITS_KINDS, LogitsCase
 
 
@@ -93,3 +93,38 @@ def test_pool_keeps_no_path_of_state_in_slots():
         p.keep({"a": (3, [1])})
     p.keep({"a": (3, [0, 1])})
     assert p.sequences["a"].length == 5
+
+
+# --------------------------------------------------------------------------------------------------------------- grammars
+class Strict:
+    """Even and odd tokens by turns, as a state machine: a text that it has not allowed is an error."""
+
+    def __init__(self, end=None, kind=list):
+        self.end, self.kind, self.asked = end, kind, 0
+
+    def __call__(self, done):
+        self.asked += 1
+        assert self.end not in done, "nothing follows the end"
+        for i, t in enumerate(done):
+            assert t % 2 == i % 2, "never allowed: %s" % done
+        return self.kind(t for t in range(40) if t % 2 == len(done) % 2 or t == self.end)
+
+
+@pytest.mark.parametrize("provider", PROVIDERS)
+@pytest.mark.parametrize("end", [None, 7])
+@pytest.mark.parametrize("kind", [list, set, lambda g: torch.tensor(list(g)), lambda g: g], ids=["list", "set", "tensor", "iterator"])
+def test_a_grammar_is_asked_only_about_what_it_allows(provider, end, kind):
+    """Drafts out of prompts that break the grammar everywhere, and that repeat an end token."""
+    prompts = [[1, 3, 7, 1, 3, 8, 1, 3, 9, 1] * 2, [4, 4, 5, 5, 4, 4, 7, 5, 5], [0, 1, 2, 3] * 5]
+    r = decoder(provider, dtype="fp32", batch=2, vocab=40)
+    want = generate_requests(r, prompts, GenerationConfig(max_new_tokens=20, eos_token_id=end, grammar=Strict(end, kind)))
+    for drafts in (1, 6, 30):
+        steps, whole = [], r.draft_step
+        r.draft_step = lambda entries: steps.extend((e[1], e[2]) for e in entries) or whole(entries)
+        got = generate_requests(r, prompts, GenerationConfig(max_new_tokens=20, eos_token_id=end, grammar=Strict(end, kind), draft_tokens=drafts))
+        r.draft_step = whole
+        assert got == want
+        assert any(len(tokens) > 1 for tokens, _ in steps)
+        for tokens, parents in steps:     # what is drafted could be chosen
+            assert all(p < 0 or (tokens[p] % 2 != t % 2 and t != end) for t, p in zip(tokens, parents) if p > 0)
+            assert end not in tokens[1:]
