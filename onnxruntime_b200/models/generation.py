@@ -867,6 +867,7 @@ def generate_requests(runner: PagedDecoderRunner, prompts: Sequence[Sequence[int
         raise ValueError("draft_tokens is not negative, and draft_ngram positive")
     if cfg.draft_tokens and not runner.has_trees:
         raise ValueError("drafted tokens need a decoder with draft_trees")
+    key = None
     if len(shared_prompt):
         if any(len(p) == 0 for p in prompts):
             raise ValueError("a request behind a shared prompt has a token of its own at least")
@@ -874,14 +875,14 @@ def generate_requests(runner: PagedDecoderRunner, prompts: Sequence[Sequence[int
             raise CacheFull(f"the shared prompt exceeds {runner.max_len} tokens")
         key = ("shared prompt",)
         runner.step([(key, shared_prompt, [])])
-        try:
-            return _generate_requests(runner, prompts, cfg, [int(t) for t in shared_prompt], key)
-        finally:
-            for i in range(len(prompts)):   # of a call that was given up
-                if ("request", i) in runner.pool.sequences:
-                    runner.release(("request", i))
+    try:
+        return _generate_requests(runner, prompts, cfg, [int(t) for t in shared_prompt], key)
+    finally:
+        for i in range(len(prompts)):   # of a call that was given up, or a grammar that raised: a later call starts anew
+            if ("request", i) in runner.pool.sequences:
+                runner.release(("request", i))
+        if key is not None:
             runner.release(key)
-    return _generate_requests(runner, prompts, cfg, [], None)
 
 
 def _generate_requests(runner: PagedDecoderRunner, prompts, cfg: GenerationConfig, shared: List[int], key):

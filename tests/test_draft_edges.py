@@ -128,3 +128,19 @@ def test_a_grammar_is_asked_only_about_what_it_allows(provider, end, kind):
         for tokens, parents in steps:     # what is drafted could be chosen
             assert all(p < 0 or (tokens[p] % 2 != t % 2 and t != end) for t, p in zip(tokens, parents) if p > 0)
             assert end not in tokens[1:]
+
+
+@pytest.mark.parametrize("drafts", [0, 6])
+def test_requests_of_a_call_that_fails_are_given_back(drafts):
+    """A grammar that raises ends its call; the next one starts anew, with all blocks, and does not go on behind what the first one left."""
+    r = decoder("CPUExecutionProvider", dtype="fp32", batch=2, vocab=40)
+    prompts = [[1, 2, 3, 1, 2, 3, 1, 2], [5, 6, 5, 6, 5]]
+    want = generate_requests(r, prompts, GenerationConfig(max_new_tokens=8, draft_tokens=drafts))
+
+    def broken(done):
+        if len(done) >= 3:
+            raise KeyError(done[-1])
+    with pytest.raises(KeyError):
+        generate_requests(r, prompts, GenerationConfig(max_new_tokens=8, draft_tokens=drafts, grammar=broken))
+    assert not r.pool.sequences and len(r.pool.free_blocks) == r.pool.num_blocks and r._drafted == {}
+    assert generate_requests(r, prompts, GenerationConfig(max_new_tokens=8, draft_tokens=drafts)) == want
