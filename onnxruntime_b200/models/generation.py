@@ -518,8 +518,8 @@ class GenerationConfig:
         ``presence_penalty`` and ``frequency_penalty`` are subtracted from the logits of generated tokens, once and as often as they
         occur; ``logit_bias`` is added to tokens' logits; ``grammar`` names the tokens that may follow the generated ones (None: all), and is
         asked only about tokens that it has named.
-        ``draft_tokens`` (runners with ``draft_trees``): up to so many tokens a step are drafted from what followed the last
-        ``draft_ngram`` tokens, or fewer, earlier in the request's own text; the step keeps those that it would have chosen."""
+        ``draft_tokens`` (runners with ``draft_trees``): up to so many tokens a step, and 255 at most, are drafted from what followed
+        the last ``draft_ngram`` tokens, or fewer, earlier in the request's own text; the step keeps those that it would have chosen."""
         self.__dict__.update(locals())
         del self.__dict__["self"]
 
@@ -947,7 +947,7 @@ def _generate_requests(runner: PagedDecoderRunner, prompts, cfg: GenerationConfi
         elif running:
             joining = list(running)
             # room has been kept for the tokens that a request will generate: no more of them are drafted
-            trees = {i: draft_tree(flat[i][:len(texts[i]) + len(new[i])], min(cfg.draft_tokens, cfg.max_new_tokens - len(new[i]) - 1), cfg.draft_ngram) if cfg.draft_tokens else ([new[i][-1]], [-1])
+            trees = {i: draft_tree(flat[i][:len(texts[i]) + len(new[i])], min(cfg.draft_tokens, MOST_DRAFTED - 1, cfg.max_new_tokens - len(new[i]) - 1), cfg.draft_ngram) if cfg.draft_tokens else ([new[i][-1]], [-1])
                      for i in joining}
             trees = {i: _permitted(cfg, new[i], *tree) for i, tree in trees.items()}
             drafted = any(len(tokens) > 1 for tokens, _, _ in trees.values())

@@ -25,7 +25,7 @@ def main(argv=None) -> int:
     ap.add_argument("--repetition-penalty", type=float, default=1.0)
     ap.add_argument("--presence-penalty", type=float, default=0.0)
     ap.add_argument("--frequency-penalty", type=float, default=0.0)
-    ap.add_argument("--draft-tokens", type=int, default=0, help="tokens that a step may draft from the request's own text")
+    ap.add_argument("--draft-tokens", type=int, default=0, help="tokens that a step may draft from the request's own text (255 at most)")
     ap.add_argument("--seed", type=int, default=None, help="sampling with this seed (greedy without it, top-k and top-p)")
     ap.add_argument("--shared-prompt-ids", default="", help="comma-separated token ids in front of every prompt; they run once")
     ap.add_argument("--logprobs", type=int, default=None, help="also report log probabilities, entropies and that many alternatives")

@@ -144,3 +144,17 @@ def test_requests_of_a_call_that_fails_are_given_back(drafts):
         generate_requests(r, prompts, GenerationConfig(max_new_tokens=8, draft_tokens=drafts, grammar=broken))
     assert not r.pool.sequences and len(r.pool.free_blocks) == r.pool.num_blocks and r._drafted == {}
     assert generate_requests(r, prompts, GenerationConfig(max_new_tokens=8, draft_tokens=drafts)) == want
+
+
+# ----------------------------------------------------------------------------------------------------------------- limits of drafts
+@pytest.mark.parametrize("drafts", [255, 256, 300, 1 << 40])
+def test_drafts_beyond_the_largest_tree(drafts):
+    """A text that offers more drafts than a tree has: the step takes the largest tree, and the call goes on."""
+    g = torch.Generator().manual_seed(1)
+    prompt = torch.randint(0, 4, (500,), generator=g).tolist()
+    r = decoder("CPUExecutionProvider", dtype="fp32", batch=1, max_len=1024, vocab=40)
+    want = generate_requests(r, [prompt], GenerationConfig(max_new_tokens=400, vocab_mask=torch.arange(40) < 4, repetition_penalty=1.5))
+    sizes, whole = [], r.draft_step
+    r.draft_step = lambda entries: sizes.extend(len(e[1]) for e in entries) or whole(entries)
+    got = generate_requests(r, [prompt], GenerationConfig(max_new_tokens=400, vocab_mask=torch.arange(40) < 4, repetition_penalty=1.5, draft_tokens=drafts))
+    assert got == want and max(sizes) == 256
