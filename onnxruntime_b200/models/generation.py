@@ -862,7 +862,9 @@ def generate_requests(runner: PagedDecoderRunner, prompts: Sequence[Sequence[int
 
     ``shared_prompt`` stands in front of every prompt: it runs once, the requests share the cache blocks that it fills, and it
     takes one of the runner's sequences.  With ``cfg.logprobs`` the requests come back as ``Generated``.  With ``cfg.draft_tokens``
-    a step may give a request several tokens, the same as without."""
+    a step may give a request several tokens.  Without sampling they are the same as without drafts, as far as rows of a tree and single rows
+    round alike.  Sampled tokens have the same distribution; as all requests draw from one generator, a seed gives the same ones as without
+    drafts only to a request that runs alone."""
     if cfg.draft_tokens < 0 or cfg.draft_ngram < 1:
         raise ValueError("draft_tokens is not negative, and draft_ngram positive")
     if cfg.draft_tokens and not runner.has_trees:

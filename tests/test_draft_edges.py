@@ -158,3 +158,25 @@ def test_drafts_beyond_the_largest_tree(drafts):
     r.draft_step = lambda entries: sizes.extend(len(e[1]) for e in entries) or whole(entries)
     got = generate_requests(r, [prompt], GenerationConfig(max_new_tokens=400, vocab_mask=torch.arange(40) < 4, repetition_penalty=1.5, draft_tokens=drafts))
     assert got == want and max(sizes) == 256
+
+
+# --------------------------------------------------------------------------------------------------------------------- sampling
+@pytest.mark.parametrize("provider", PROVIDERS)
+def test_sampled_drafts_of_a_request_that_runs_alone(provider):
+    """One request's draws come in the order of its tokens, whether a step gives one or several: a seed gives the same tokens with and without drafts."""
+    prompt = [1, 2, 3, 4, 1, 2, 3, 4, 1, 2]
+    kw = dict(max_new_tokens=24, top_k=2, temperature=0.2, vocab_mask=torch.arange(40) < 5)
+    r = decoder(provider, dtype="fp32", batch=1, vocab=40)
+    for seed in range(3):
+        want = generate_requests(r, [prompt], GenerationConfig(seed=seed, **kw))
+        assert generate_requests(r, [prompt], GenerationConfig(seed=seed, draft_tokens=6, **kw)) == want
+
+
+@pytest.mark.parametrize("provider", PROVIDERS)
+def test_sampled_drafts_of_requests_that_run_together(provider):
+    """They share the draws, in another order than without drafts; a seed gives the same tokens again, and none that may not be chosen."""
+    prompts = [[1, 2, 3, 4, 1, 2, 3, 4, 1, 2], [3, 2, 3, 2, 3], [4, 4, 4]]
+    cfg = GenerationConfig(max_new_tokens=24, top_k=2, temperature=0.5, vocab_mask=torch.arange(40) < 5, seed=1, draft_tokens=6)
+    r = decoder(provider, dtype="fp32", batch=2, vocab=40)
+    first = generate_requests(r, prompts, cfg)
+    assert generate_requests(r, prompts, cfg) == first and all(len(t) == 24 and max(t) < 5 for t in first)
