@@ -516,8 +516,8 @@ class GenerationConfig:
                  grammar: Optional[Callable[[List[int]], Optional[Sequence[int]]]] = None, draft_tokens: int = 0, draft_ngram: int = 3):
         """For ``generate_requests``: ``logprobs``: report log probabilities, entropies and that many best alternatives.
         ``presence_penalty`` and ``frequency_penalty`` are subtracted from the logits of generated tokens, once and as often as they
-        occur; ``logit_bias`` is added to tokens' logits; ``grammar`` names the tokens that may follow the generated ones (None: all), and is
-        asked only about tokens that it has named.
+        occur; ``logit_bias`` is added to tokens' logits; ``grammar`` names the tokens that may follow the generated ones (None: all; what lies
+        outside the vocabulary is no token), and is asked only about tokens that it has named.
         ``draft_tokens`` (runners with ``draft_trees``): up to so many tokens a step, and 255 at most, are drafted from what followed
         the last ``draft_ngram`` tokens, or fewer, earlier in the request's own text; the step keeps those that it would have chosen."""
         self.__dict__.update(locals())
@@ -659,7 +659,8 @@ class LogitsProcessor:
     def _mask(self, allowed: Optional[Sequence[int]]) -> torch.Tensor:
         keep = torch.ones(self.vocab_size, dtype=torch.bool) if allowed is None else torch.zeros(self.vocab_size, dtype=torch.bool)
         if allowed is not None:
-            keep[torch.from_numpy(_token_array(allowed))] = True
+            named = _token_array(allowed)
+            keep[torch.from_numpy(named[(named >= 0) & (named < self.vocab_size)])] = True
         if self.cfg.vocab_mask is not None:
             keep &= self.cfg.vocab_mask.reshape(-1).cpu() != 0
         words = torch.nn.functional.pad(keep, (0, -self.vocab_size % 32)).reshape(-1, 32).long()

@@ -130,6 +130,16 @@ def test_a_grammar_is_asked_only_about_what_it_allows(provider, end, kind):
             assert end not in tokens[1:]
 
 
+@pytest.mark.parametrize("provider", PROVIDERS)
+def test_a_grammar_that_names_what_is_no_token(provider):
+    """-1 is not the last token of the vocabulary, and what lies behind it is none."""
+    device = torch.device("cuda" if provider == "CUDAExecutionProvider" else "cpu")
+    named = [[3, -1], [40, 5, 1 << 40], [], [-41, 39], None]
+    processor = LogitsProcessor(40, torch.float32, device, GenerationConfig(grammar=lambda done: named[done[0]]))
+    scores = processor(torch.zeros(5, 40, device=device), [([i], 1, [[]]) for i in range(5)]).cpu()
+    assert [(row == 0).nonzero().flatten().tolist() for row in scores] == [[3], [5], [], [39], list(range(40))]
+
+
 @pytest.mark.parametrize("drafts", [0, 6])
 def test_requests_of_a_call_that_fails_are_given_back(drafts):
     """A grammar that raises ends its call; the next one starts anew, with all blocks, and does not go on behind what the first one left."""
