@@ -603,7 +603,8 @@ def generate(runner: Union[DecoderRunner, PagedDecoderRunner], input_ids: torch.
 
 class LogitsProcessor:
     """The logits processors of ``generate_requests`` for all rows of a step at once: ``com.ortb200.ProcessLogits`` as a session of its
-    own on the provider of the logits' device, with the inputs that the configuration needs."""
+    own on the provider of the logits' device, with the inputs that the configuration needs.  ``vocab_mask`` is laid out when the
+    processor is made."""
 
     def __init__(self, vocab_size: int, dtype: torch.dtype, device: torch.device, cfg: GenerationConfig):
         T, info = ol.TensorProto, ol.make_tensor_value_info
@@ -613,6 +614,8 @@ class LogitsProcessor:
         self.biased = (cfg.eos_token_id is not None and cfg.min_new_tokens > 0) or cfg.no_repeat_ngram_size > 0 or bool(cfg.logit_bias)
         self.masked = cfg.vocab_mask is not None or cfg.grammar is not None
         self.warm = cfg.temperature != 1.0 and cfg.temperature > 0
+        self._vocab_words = None if cfg.vocab_mask is None else self._words((cfg.vocab_mask.reshape(-1).cpu() != 0).expand(vocab_size).numpy())
+        self._vocab_mask = None if cfg.vocab_mask is None else torch.from_numpy(self._vocab_words.reshape(1, -1).copy()).to(device)
         self.idle = not (self.text or self.biased or self.masked or self.warm)
         ins = [info("logits", kind, ["rows", vocab_size])]
         names = ["logits"] + [""] * 14
@@ -656,16 +659,25 @@ class LogitsProcessor:
                 bias.update(dict.fromkeys(whole[_places_of(whole[:-1], whole[len(whole) - (n - 1):])].tolist(), -math.inf))
         return bias
 
-    def _mask(self, allowed: Optional[Sequence[int]]) -> torch.Tensor:
-        keep = torch.ones(self.vocab_size, dtype=torch.bool) if allowed is None else torch.zeros(self.vocab_size, dtype=torch.bool)
-        if allowed is not None:
-            named = _token_array(allowed)
-            keep[torch.from_numpy(named[(named >= 0) & (named < self.vocab_size)])] = True
-        if self.cfg.vocab_mask is not None:
-            keep &= self.cfg.vocab_mask.reshape(-1).cpu() != 0
-        words = torch.nn.functional.pad(keep, (0, -self.vocab_size % 32)).reshape(-1, 32).long()
-        packed = (words << torch.arange(32)).sum(-1)
-        return torch.where(packed >= 1 << 31, packed - (1 << 32), packed).int()
+    def _words(self, keep: np.ndarray) -> np.ndarray:
+        """A truth value for each token as bits of 32-bit words."""
+        packed = np.zeros((self.vocab_size + 31) // 32 * 4, dtype=np.uint8)
+        packed[:(self.vocab_size + 7) // 8] = np.packbits(keep, bitorder="little")
+        return packed.view("<i4")
+
+    def _masks(self, named: Sequence[Optional[Sequence[int]]]) -> Tuple[np.ndarray, List[int]]:
+        """The different masks of rows for which a grammar names these tokens, and the mask of each row (-1: none)."""
+        places: Dict[bytes, int] = {}
+        rows = []
+        for tokens in named:
+            words = self._vocab_words
+            if tokens is not None:
+                tokens = _token_array(tokens)
+                keep = np.zeros(self.vocab_size, dtype=bool)
+                keep[tokens[(tokens >= 0) & (tokens < self.vocab_size)]] = True
+                words = self._words(keep) if words is None else self._words(keep) & words
+            rows.append(-1 if words is None else places.setdefault(words.tobytes(), len(places)))
+        return np.frombuffer(bytearray(b"".join(places)), dtype="<i4").reshape(len(places), (self.vocab_size + 31) // 32), rows
 
     def __call__(self, logits: torch.Tensor, requests: Sequence[Tuple[Sequence[int], int, Sequence[Sequence[int]]]],
                  named: Optional[Sequence[Optional[Sequence[int]]]] = None) -> torch.Tensor:
@@ -696,12 +708,12 @@ class LogitsProcessor:
             feeds.update(bias_tokens=ints([t for b in bias for t in b]), bias_values=torch.tensor([v for b in bias for v in b.values()], dtype=torch.float32).to(dev), bias_starts=ints(ends))
         if self.masked:
             if cfg.grammar is None:
-                feeds.update(allowed=self._mask(None).reshape(1, -1).to(dev), row_mask=torch.zeros(rows, dtype=torch.int32, device=dev))
+                feeds.update(allowed=self._vocab_mask, row_mask=torch.zeros(rows, dtype=torch.int32, device=dev))
             else:
                 if named is None:
                     named = [cfg.grammar([int(t) for t in (*text[len(text) - new:], *p)]) for text, new, paths in requests for p in paths]
-                masks = [self._mask(allowed) for allowed in named]
-                feeds.update(allowed=torch.stack(masks).to(dev), row_mask=torch.arange(rows, dtype=torch.int32, device=dev))
+                masks, of_row = self._masks(named)
+                feeds.update(allowed=torch.from_numpy(masks).to(dev), row_mask=ints(of_row, torch.int32))
         if self.warm:
             feeds.update(temperature=same(cfg.temperature))
         scores = torch.empty(rows, self.vocab_size, dtype=torch.float32, device=dev)

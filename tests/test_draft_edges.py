@@ -140,6 +140,29 @@ def test_a_grammar_that_names_what_is_no_token(provider):
     assert [(row == 0).nonzero().flatten().tolist() for row in scores] == [[3], [5], [], [39], list(range(40))]
 
 
+@pytest.mark.parametrize("provider", PROVIDERS)
+@pytest.mark.parametrize("vocab", [1, 7, 8, 31, 32, 33, 77, 1000])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("kind", [torch.bool, torch.float32, torch.bfloat16, torch.int64])
+def test_masks_of_grammars_and_vocabularies(provider, vocab, masked, kind):
+    """Rows with equal masks, with masks of their own and with none, under a constant mask of any type; that one is laid out once."""
+    device, g = torch.device("cuda" if provider == "CUDAExecutionProvider" else "cpu"), torch.Generator().manual_seed(vocab)
+    keep = torch.rand(vocab, generator=g) < 0.7 if masked else torch.ones(vocab, dtype=torch.bool)
+    named = [torch.randint(0, vocab, (n,), generator=g).tolist() for n in (0, 1, 9, 300)] + [None]
+    rows = [4, 2, 2, 0, 3, 4, 1, 2]
+    processor = LogitsProcessor(vocab, torch.float32, device, GenerationConfig(grammar=lambda done: named[done[0]], vocab_mask=keep.to(kind) if masked else None))
+    scores = processor(torch.zeros(len(rows), vocab, device=device), [([r], 1, [[]]) for r in rows]).cpu()
+    for r, row in zip(rows, scores):
+        want = keep.clone()
+        if named[r] is not None:
+            want &= torch.isin(torch.arange(vocab), torch.tensor(named[r], dtype=torch.int64))
+        assert torch.equal(row == 0, want) and (row[~want] == -math.inf).all()
+    if masked:
+        alone = LogitsProcessor(vocab, torch.float32, device, GenerationConfig(vocab_mask=keep.to(kind)))
+        alone._words = None
+        assert torch.equal(alone(torch.zeros(2, vocab, device=device), [([1], 1, [[]]), ([2], 0, [[]])]).cpu() == 0, keep.expand(2, -1))
+
+
 @pytest.mark.parametrize("drafts", [0, 6])
 def test_requests_of_a_call_that_fails_are_given_back(drafts):
     """A grammar that raises ends its call; the next one starts anew, with all blocks, and does not go on behind what the first one left."""
