@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <limits>
 #include <set>
 
@@ -71,16 +72,20 @@ void ProcessLogitsImpl(Ctx& ctx) {
   const auto repetition = Host<float>(ctx, 6, at::kFloat), presence = Host<float>(ctx, 7, at::kFloat), frequency = Host<float>(ctx, 8, at::kFloat);
   const auto bias_values = Host<float>(ctx, 10, at::kFloat), temperature = Host<float>(ctx, 14, at::kFloat);
   const char* op = "ProcessLogits";
-  std::vector<int64_t> count(z.vocab), sum_of(z.vocab);
+  constexpr float kNever = -std::numeric_limits<float>::infinity();
+  // of the tokens that a row touches, which are few beside its vocabulary; all 0 between rows
+  std::vector<int64_t> count(z.vocab), sum_of(z.vocab), touched, banned;
   std::vector<char> seen(z.vocab);
   for (int64_t r = 0; r < z.rows; ++r) {
     const float* from = x.data_ptr<float>() + r * z.vocab;
     float* to = out.data_ptr<float>() + r * z.vocab;
     const float rep = repetition.empty() ? 1.f : repetition[r], pres = presence.empty() ? 0.f : presence[r], freq = frequency.empty() ? 0.f : frequency[r];
-    std::fill(count.begin(), count.end(), 0);
-    std::fill(seen.begin(), seen.end(), 0);
+    std::copy(from, from + z.vocab, to);
+    touched.clear();
+    banned.clear();
     const auto add = [&](int64_t v, bool counts) {
       if (v < 0 || v >= z.vocab) return;
+      if (!seen[v]) touched.push_back(v);
       seen[v] = 1;
       count[v] += counts;
     };
@@ -95,13 +100,11 @@ void ProcessLogitsImpl(Ctx& ctx) {
       }
       for (int64_t d = 0; d < z.drafted; ++d) add(drafted[r * z.drafted + d], true);
     }
-    for (int64_t v = 0; v < z.vocab; ++v) {
-      float f = from[v];
-      if (seen[v]) {
-        f = f < 0.f ? f * rep : f / rep;
-        if (count[v]) f -= freq * static_cast<float>(count[v]) + pres;
-      }
-      to[v] = f;
+    for (const int64_t v : touched) {
+      to[v] = to[v] < 0.f ? to[v] * rep : to[v] / rep;
+      if (count[v]) to[v] -= freq * static_cast<float>(count[v]) + pres;
+      seen[v] = 0;
+      count[v] = 0;
     }
     if (!bias_tokens.empty() || ctx.HasInput(9)) {
       ORTB_ENFORCE_ARG(bias_starts[r] >= 0 && bias_starts[r] <= bias_starts[r + 1] && bias_starts[r + 1] <= z.biases, op, ": the biases of row ", r, " leave their list");
@@ -117,18 +120,32 @@ void ProcessLogitsImpl(Ctx& ctx) {
         }
       }
       for (const auto& [v, s] : sums) {
-        to[v] = s == -std::numeric_limits<float>::infinity() ? s : to[v] + s;   // a ban holds for logits that are infinite or NaN, too
+        if (s == kNever) banned.push_back(v);   // holds for logits that are infinite or NaN, too
+        else to[v] += s;
         sum_of[v] = 0;
       }
     }
+    if (!temperature.empty() && temperature[r] > 0.f && temperature[r] != 1.f) {
+      const float t = temperature[r];
+      for (int64_t v = 0; v < z.vocab; ++v) to[v] /= t;
+    }
+    for (const int64_t v : banned) to[v] = kNever;
     if (!row_mask.empty()) {
       ORTB_ENFORCE_ARG(row_mask[r] < z.masks, op, ": row ", r, " names mask ", row_mask[r], " of ", z.masks);
-      if (row_mask[r] >= 0)
-        for (int64_t v = 0; v < z.vocab; ++v)
-          if (!(static_cast<unsigned>(allowed[row_mask[r] * z.mask_words + v / 32]) >> (v % 32) & 1)) to[v] = -std::numeric_limits<float>::infinity();
+      for (int64_t w = 0; w < z.mask_words && row_mask[r] >= 0; ++w) {
+        const unsigned bits = static_cast<unsigned>(allowed[row_mask[r] * z.mask_words + w]);
+        float* const of = to + 32 * w;
+        const int n = static_cast<int>(std::min<int64_t>(32, z.vocab - 32 * w));
+        for (int b = 0; b < n && bits != ~0u; ++b) {   // (without a branch, which masks give no way to foresee)
+          uint32_t f, never;
+          std::memcpy(&f, of + b, 4);
+          std::memcpy(&never, &kNever, 4);
+          const uint32_t keep = 0u - (bits >> b & 1);
+          f = (f & keep) | (never & ~keep);
+          std::memcpy(of + b, &f, 4);
+        }
+      }
     }
-    if (!temperature.empty() && temperature[r] > 0.f && temperature[r] != 1.f)
-      for (int64_t v = 0; v < z.vocab; ++v) to[v] /= temperature[r];
   }
   ctx.SetOutput(0, out.to(ctx.Input(0).device()));
 }

@@ -37,6 +37,19 @@ def test_banned_tokens_of_any_logit(kind, biases, twice):
     assert got[:, free].isfinite().all()
 
 
+@pytest.mark.parametrize("kind", LOGITS_KINDS)
+def test_masked_and_banned_tokens_under_an_infinite_temperature(kind):
+    """x / inf is 0 for every finite logit; what is masked or banned stays -inf, on every provider."""
+    case = LogitsCase(kind[1], 2, 300, without=["history", "history_starts", "generated_starts", "row_list", "drafted", "repetition", "presence", "frequency"], seed=3)
+    case.t.update(temperature=torch.full((2,), math.inf), bias_tokens=torch.tensor([1, 2, 1, 2]), bias_values=torch.tensor([-math.inf, 1.0] * 2), bias_starts=torch.tensor([0, 2, 4]),
+                  allowed=torch.full((1, 10), 0x5555555f, dtype=torch.int32), row_mask=torch.tensor([0, -1], dtype=torch.int32))
+    got = case.call(kind[0])()["scores"]
+    want = torch.zeros(2, 300)
+    want[:, 1] = -math.inf
+    want[0, [v for v in range(300) if not 0x5555555f >> (v % 32) & 1]] = -math.inf
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("provider", PROVIDERS)
 @pytest.mark.parametrize("hard", [math.inf, math.nan])
 @pytest.mark.parametrize("kw", [dict(eos_token_id=5, min_new_tokens=4), dict(no_repeat_ngram_size=2), dict(no_repeat_ngram_size=1), dict(logit_bias={5: -math.inf})], ids=str)
