@@ -352,18 +352,47 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 1) process_logit
         s.whole(at.base + n, word, bias);
       }
     if (!apart) return;
-    // rare, or a long text: of several biases of a token the first looks for the others and sums them up in their order
+    auto here = [&](long long v) { return v >= at.first && v < at.end; };
+    if (!twice) {   // many biases, or a long text
+      for (long long b = q.bias0 + threadIdx.x; b < q.bias1; b += THREADS) {
+        const long long v = a.bias_tokens[b];
+        if (here(v)) s.whole(static_cast<int>(v), counts[static_cast<int>(v) - at.base], a.bias_values[b]);
+      }
+      return;
+    }
+    // Rare: a token has several biases.  One warp goes through all of them in their order, 32 at a time, and keeps the sums where the scores go; a
+    // counter's flag tells whether its token has no sum yet.  Then whoever sets the flag again makes the score of the sum.  (A search for each bias
+    // among all others would take the square of their number.)
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const int lane = static_cast<int>(threadIdx.x);
+      for (long long b0 = q.bias0; b0 < q.bias1; b0 += 32) {
+        const long long v = b0 + lane < q.bias1 ? a.bias_tokens[b0 + lane] : -1;
+        const bool mine = here(v);
+        if (!__any_sync(0xffffffffu, mine)) continue;
+        const float value = mine ? a.bias_values[b0 + lane] : 0.f;
+        const unsigned same = __match_any_sync(0xffffffffu, mine ? static_cast<int>(v) : -1 - lane);   // of a token the first lane sums up
+        const bool leads = mine && __ffs(same) - 1 == lane;
+        float sum = value;
+        if (leads) {
+          unsigned& word = counts[static_cast<int>(v) - at.base];
+          if (!(word & kBiased)) sum = y[v] + value;
+          word &= ~kBiased;
+        }
+        for (unsigned rest = leads ? same & (same - 1) : 0; __any_sync(0xffffffffu, rest != 0); rest &= rest - 1) {
+          const float next = __shfl_sync(0xffffffffu, value, rest ? __ffs(rest) - 1 : lane);
+          if (rest) sum += next;
+        }
+        if (leads) y[v] = sum;
+        __syncwarp();
+      }
+    }
+    __syncthreads();
     for (long long b = q.bias0 + threadIdx.x; b < q.bias1; b += THREADS) {
       const long long v = a.bias_tokens[b];
-      if (v < at.first || v >= at.end) continue;
-      bool leads = true;
-      float sum = a.bias_values[b];
-      if (twice) {
-        for (long long o = q.bias0; o < b && leads; ++o) leads = a.bias_tokens[o] != v;
-        for (long long o = b + 1; o < q.bias1 && leads; ++o)
-          if (a.bias_tokens[o] == v) sum += a.bias_values[o];
-      }
-      if (leads) s.whole(static_cast<int>(v), counts[static_cast<int>(v) - at.base], sum);
+      if (!here(v)) continue;
+      const unsigned word = atomicOr(&counts[static_cast<int>(v) - at.base], kBiased);
+      if (!(word & kBiased)) s.whole(static_cast<int>(v), word, y[v]);
     }
   }
 }

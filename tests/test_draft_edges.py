@@ -62,6 +62,42 @@ def test_a_banned_token_is_not_chosen(provider, hard, kw):
     assert (scores[:, 5] == -math.inf).all() and scores.argmax(-1).tolist() == [39, 39]
 
 
+# -------------------------------------------------------------------------------------------------------------------- biases
+def sums_in_order(vocab, tokens, values):
+    """Of each token its biases, added in 32 bits one after the other, and whether it has one."""
+    sums, some = torch.zeros(vocab), torch.zeros(vocab, dtype=torch.bool)
+    for t, v in zip(tokens.tolist(), values):
+        if 0 <= t < vocab:
+            sums[t] = sums[t] + v if some[t] else v
+            some[t] = True
+    return sums, some
+
+
+@pytest.mark.parametrize("kind", LOGITS_KINDS)
+@pytest.mark.parametrize("vocab,biases,pool_of", [(50257, 30000, 20000), (1000, 3001, 40), (9001, 33, 2), (300, 64, 1), (20000, 1025, 1024)])
+def test_biases_of_the_same_tokens(kind, vocab, biases, pool_of):
+    """Thousands of biases, tokens named again side by side and far apart: each sum in its order, to the bit; magnitudes so far apart that another
+    order shows."""
+    g = torch.Generator().manual_seed(biases)
+    case = LogitsCase(kind[1], 3, vocab, without=["row_list", "drafted", "allowed", "row_mask", "temperature", "history", "history_starts", "generated_starts", "repetition", "presence",
+                                                  "frequency"], seed=1)
+    tokens = torch.randint(-1, pool_of, (2 * biases,), generator=g) * (vocab // pool_of)
+    tokens[:64] = tokens[0]
+    tokens[5::97] = vocab
+    values = torch.randn(2 * biases, generator=g) * 10.0 ** torch.randint(-3, 6, (2 * biases,), generator=g)
+    case.t.update(bias_tokens=tokens, bias_values=values, bias_starts=torch.tensor([0, biases, biases, 2 * biases]))
+    got, x = case.call(kind[0])()["scores"], case.t["logits"].float()
+    for row, part in ((0, slice(0, biases)), (1, slice(0, 0)), (2, slice(biases, 2 * biases))):
+        sums, some = sums_in_order(vocab, tokens[part], values[part])
+        assert torch.equal(got[row], torch.where(some, x[row] + sums, x[row]))
+
+
+@pytest.mark.parametrize("kind", LOGITS_KINDS)
+def test_biases_of_the_same_tokens_beside_texts(kind):
+    case = LogitsCase(kind[1], 3, 5003, length=3000, biases=900, drafted=3, seed=8)
+    case.run(kind[0])
+
+
 # ------------------------------------------------------------------------------------------------------------------- the pool
 def hold(p, seq, tokens):
     if seq not in p.sequences:
