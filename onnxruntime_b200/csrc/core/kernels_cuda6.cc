@@ -155,8 +155,8 @@ class ProcessLogitsKernel final : public WithGeneric {
     if (z.biases > 0) {
       a.bias_tokens = static_cast<int64_t*>(given(9, at::kLong));
       a.bias_values = static_cast<float*>(given(10, at::kFloat));
-      a.bias_starts = static_cast<int64_t*>(given(11, at::kLong));
     }
+    a.bias_starts = static_cast<int64_t*>(given(11, at::kLong));   // without biases, too: starts that are none are reported
     a.allowed = static_cast<int*>(given(12, at::kInt));
     a.row_mask = static_cast<int*>(given(13, at::kInt));
     a.temperature = static_cast<float*>(given(14, at::kFloat));

@@ -64,7 +64,7 @@ typedef struct {
   const float* frequency;           // [rows]; null: 0
   const int64_t* bias_tokens;       // [bias_len]
   const float* bias_values;         // [bias_len]
-  const int64_t* bias_starts;       // [rows + 1]
+  const int64_t* bias_starts;       // [rows + 1]; may be given without biases
   const int* allowed;               // [masks, mask_words]: bit v % 32 of word v / 32 is token v's
   const int* row_mask;              // [rows]; a negative one: no mask
   const float* temperature;         // [rows]; null: 1

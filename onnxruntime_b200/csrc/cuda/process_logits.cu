@@ -81,7 +81,7 @@ __device__ __forceinline__ RowRules rules_of(const ortb200_process_logits_args& 
     else if (m >= 0) q.mask = reinterpret_cast<const unsigned*>(a.allowed) + static_cast<long long>(m) * a.mask_words;
   }
   q.bias0 = q.bias1 = 0;
-  if (a.bias_tokens) {
+  if (a.bias_starts) {
     q.bias0 = a.bias_starts[r];
     q.bias1 = a.bias_starts[r + 1];
     if (q.bias0 < 0 || q.bias1 < q.bias0 || q.bias1 > a.bias_len) {

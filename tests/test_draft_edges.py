@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from onnxruntime_b200.capi import EPFail, InvalidArgument
 from onnxruntime_b200.models.decoder_cache import CachePool, CacheTensor
 from onnxruntime_b200.models.generation import GenerationConfig, LogitsProcessor, generate_requests
 from test_draft_generation import PROVIDERS, decoder, pool
@@ -96,6 +97,20 @@ def test_biases_of_the_same_tokens(kind, vocab, biases, pool_of):
 def test_biases_of_the_same_tokens_beside_texts(kind):
     case = LogitsCase(kind[1], 3, 5003, length=3000, biases=900, drafted=3, seed=8)
     case.run(kind[0])
+
+
+@pytest.mark.parametrize("kind", LOGITS_KINDS)
+@pytest.mark.parametrize("starts", [[0, 1, 0, 0], [0, 0, 0, 5], [-1, 0, 0, 0]])
+@pytest.mark.parametrize("texts", [False, True])
+def test_starts_of_no_biases(kind, starts, texts):
+    """Starts that leave a list of biases are an error for an empty list, too; those of an empty list are none."""
+    left_out = ["row_list", "drafted", "allowed", "row_mask"] + ([] if texts else ["history", "history_starts", "generated_starts"])
+    case = LogitsCase(kind[1], 3, 40, biases=0, without=left_out)
+    assert len(case.t["bias_tokens"]) == 0
+    case.run(kind[0])
+    case.t["bias_starts"] = torch.tensor(starts)
+    with pytest.raises((InvalidArgument, EPFail)):
+        case.call(kind[0])()
 
 
 # ------------------------------------------------------------------------------------------------------------------- the pool
