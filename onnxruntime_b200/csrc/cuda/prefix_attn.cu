@@ -86,14 +86,12 @@ __device__ __forceinline__ bool owned(const ortb200_prefix_attn_args& a, int b, 
 
 // Trees of drafted tokens: the rows of a sequence that a row sees, as bits, which step 1 works out.
 constexpr int kTreeWords = 8, kTreeNodes = 32 * kTreeWords;
-// Behind a row's bits lie as many words that are not 0 where one of its values is no finite number: 0 times such a value would reach rows
-// that do not see it, and a drafted token that goes wrong would take the others with it.  These values count as 0, and rows that do see
-// one become NaN.
-constexpr int kTreeStride = 2 * kTreeWords;
-__device__ __forceinline__ bool tree_spoilt(const uint32_t* ancestors, long long t) {
-  const uint4* w = reinterpret_cast<const uint4*>(ancestors + t * kTreeStride + kTreeWords);
-  const uint4 x = __ldcg(w), y = __ldcg(w + 1);
-  return (x.x | x.y | x.z | x.w | y.x | y.y | y.z | y.w) != 0;
+// Behind a row's bits lies a byte for each key head, not 0 where one of the row's values of that head is no finite number: 0 times such a value would
+// reach rows that do not see it, and a drafted token that goes wrong would take the others with it.  These values count as 0, and for rows that do see
+// one the results of the query heads that read the key head become NaN.
+__host__ __device__ inline int tree_stride(int Nk) { return kTreeWords + (Nk + 3) / 4; }   // words of a row
+__device__ __forceinline__ bool tree_spoilt(const uint32_t* ancestors, int Nk, long long t, int kvh) {
+  return __ldcg(reinterpret_cast<const unsigned char*>(ancestors + t * tree_stride(Nk) + kTreeWords) + kvh) != 0;
 }
 // one of the two 16-bit numbers is an infinity or NaN
 template <typename T>
@@ -153,7 +151,7 @@ __global__ void __launch_bounds__(128) prefix_prep_kernel(const ortb200_prefix_a
   }
   if (parents) {
     const Span s = span_of(a, b);
-    pos += tree_row(parents, s.row0, s.rows, t - s.row0, ancestors + static_cast<long long>(t) * kTreeStride, a.status, true) - (t - s.row0);
+    pos += tree_row(parents, s.row0, s.rows, t - s.row0, ancestors + static_cast<long long>(t) * tree_stride(a.Nk), a.status, true) - (t - s.row0);
   }
   const bool keep = slot >= 0 && slot < static_cast<long long>(a.num_blocks) * a.block_size;
   if (!keep && threadIdx.x == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
@@ -207,7 +205,7 @@ __global__ void __launch_bounds__(128) prefix_rows_kernel(const ortb200_prefix_a
     for (int r = 0; r < R; ++r) qv[r] = r * 32 + lane < H ? to_float<T>(q[item * H + r * 32 + lane]) : 0.f;
     const bool tree = ancestors && s.rows <= kTreeNodes;
     for (int j = 0; j < keys; ++j) {
-      if (tree && j >= s.past && !tree_sees(ancestors + static_cast<long long>(t) * kTreeStride, j - s.past)) continue;
+      if (tree && j >= s.past && !tree_sees(ancestors + static_cast<long long>(t) * tree_stride(a.Nk), j - s.past)) continue;
       const int block = a.block_table[static_cast<long long>(b) * a.max_blocks + j / a.block_size];
       if (block < 0 || block >= a.num_blocks) {
         if (lane == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
@@ -220,6 +218,16 @@ __global__ void __launch_bounds__(128) prefix_rows_kernel(const ortb200_prefix_a
         if (r * 32 + lane < H) dot += qv[r] * to_float<T>(static_cast<const T*>(a.k_cache)[at + r * 32 + lane]);
       float sc = warp_sum(dot) * scale;
       if (a.softcap > 0.f) sc = a.softcap * tanhf(sc / a.softcap);
+      if (ancestors && j >= s.past) {   // of a tree's tokens, values that are not finite: as in the tensor-core form
+        bool finite = true;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (r * 32 + lane < H) finite &= isfinite(to_float<T>(static_cast<const T*>(a.v_cache)[at + r * 32 + lane]));
+        if (!__all_sync(0xffffffffu, finite)) {
+          l = NAN;
+          continue;
+        }
+      }
       if (sc == -INFINITY) continue;
       const float mm = fmaxf(m, sc), c = m == -INFINITY ? 0.f : expf(m - mm), p = expf(sc - mm);
       l = l * c + p;
@@ -265,7 +273,7 @@ struct Work {            // the workspace's parts
   long long* first;      // [row tiles of all sequences + 1]: where the own units of each start, behind the prefix's
   int* tile0;            // [B + 1]: which of those row tiles are a sequence's
   int4* token;           // [T]: the token's sequence, that sequence's first row, rows and past
-  uint32_t* ancestors;   // [T, 16]: trees only
+  uint32_t* ancestors;   // [T, tree_stride(Nk)]: trees only
   uint16_t* q;           // [Nk, T G, H]
   float2* ml;            // per row of a segment: m (in units of log 2) and l
   float* o;              // per row of a segment: H values
@@ -277,7 +285,7 @@ __host__ __device__ inline long long plan_bytes(long long T, int B, int N, int N
   return up256(sizeof(Plan) + 8 * (most_row_tiles(T, B, N, Nk) + 1) + 4ll * (B + 1));
 }
 __host__ __device__ inline long long segment_rows(long long T, int N) { return 2 * T * N + static_cast<long long>(kGrid) * kQT; }   // (grid_of<QT> x QT is the same for both)
-__host__ __device__ inline long long tree_bytes(long long T) { return up256(T * kTreeStride * 4); }
+__host__ __device__ inline long long tree_bytes(long long T, int Nk) { return up256(T * tree_stride(Nk) * 4); }
 template <bool TREE>
 __host__ __device__ inline Work work_of(const ortb200_prefix_attn_args& a) {
   char* p = static_cast<char*>(a.workspace);
@@ -289,7 +297,7 @@ __host__ __device__ inline Work work_of(const ortb200_prefix_attn_args& a) {
   w.token = reinterpret_cast<int4*>(p);
   p += up256(a.T * 16);
   w.ancestors = reinterpret_cast<uint32_t*>(p);
-  if (TREE) p += tree_bytes(a.T);
+  if (TREE) p += tree_bytes(a.T, a.Nk);
   w.q = reinterpret_cast<uint16_t*>(p);
   p += up256(a.T * a.N * a.H * 2);
   w.ml = reinterpret_cast<float2*>(p);
@@ -499,6 +507,10 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
     const char* row = static_cast<const char*>(a.qkv) + static_cast<long long>(t) * heads * H * sizeof(T);
     for (int i = threadIdx.x * 128; i < heads * H * static_cast<int>(sizeof(T)); i += 128 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + i));
   }
+  const int per_block = (heads + gridDim.y - 1) / gridDim.y, lo = blockIdx.y * per_block, hi = min(heads, lo + per_block);
+  unsigned char* const spoilt = TREE ? reinterpret_cast<unsigned char*>(w.ancestors + static_cast<long long>(t) * tree_stride(a.Nk) + kTreeWords) - a.N - a.Nk : nullptr;   // by head
+  if (TREE)   // (the search for the sequence has a barrier before any is set)
+    for (int head = max(lo, a.N + a.Nk) + threadIdx.x; head < hi; head += 128) spoilt[head] = 0;
   auto nobodys = [&]() {   // a row of no sequence: its result is 0 (without trees step 3 sees to it)
     if (!TREE || blockIdx.y != 0) return;
     T* out = static_cast<T*>(a.out) + static_cast<long long>(t) * a.N * H;
@@ -530,7 +542,7 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
   }
   if (TREE) {
     const Span s = span_of(a, b);
-    pos += tree_row(parents, s.row0, s.rows, t - s.row0, w.ancestors + static_cast<long long>(t) * kTreeStride, a.status, blockIdx.y == 0) - (t - s.row0);
+    pos += tree_row(parents, s.row0, s.rows, t - s.row0, w.ancestors + static_cast<long long>(t) * tree_stride(a.Nk), a.status, blockIdx.y == 0) - (t - s.row0);
   }
   const bool keep = slot >= 0 && slot < static_cast<long long>(a.num_blocks) * a.block_size;
   if (!keep && threadIdx.x == 0 && a.status) atomicExch(a.status, kStatusBadArgument);
@@ -541,9 +553,7 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
   }
   const T* cosr = a.cos_cache ? static_cast<const T*>(a.cos_cache) + pos * half : nullptr;
   const T* sinr = a.cos_cache ? static_cast<const T*>(a.sin_cache) + pos * half : nullptr;
-  bool spoilt = false;
-  const int per_block = (heads + gridDim.y - 1) / gridDim.y;
-  const int lo = blockIdx.y * per_block, hi = min(heads, lo + per_block), items = VEC ? H / 16 : H;
+  const int items = VEC ? H / 16 : H;
   for (int idx = lo * items + threadIdx.x; idx < hi * items; idx += 128) {
     const int head = idx / items, d = VEC ? idx % items * 8 : idx % items;
     const int kind = head < a.N ? 0 : head < a.N + a.Nk ? 1 : 2, kh = head - (kind == 1 ? a.N : a.N + a.Nk);
@@ -562,8 +572,8 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
     if (VEC) {
       const int far = H / 2;
       const uint4 u4 = *reinterpret_cast<const uint4*>(src + d), v4 = *reinterpret_cast<const uint4*>(src + d + far);
-      if (TREE && kind == 2)
-        spoilt |= spoilt2<T>(u4.x) || spoilt2<T>(u4.y) || spoilt2<T>(u4.z) || spoilt2<T>(u4.w) || spoilt2<T>(v4.x) || spoilt2<T>(v4.y) || spoilt2<T>(v4.z) || spoilt2<T>(v4.w);
+      if (TREE && kind == 2 && (spoilt2<T>(u4.x) || spoilt2<T>(u4.y) || spoilt2<T>(u4.z) || spoilt2<T>(u4.w) || spoilt2<T>(v4.x) || spoilt2<T>(v4.y) || spoilt2<T>(v4.z) || spoilt2<T>(v4.w)))
+        spoilt[head] = 1;
       if (!turn) {
         *reinterpret_cast<uint4*>(dst + d) = u4;
         *reinterpret_cast<uint4*>(dst + d + far) = v4;
@@ -582,7 +592,7 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
       *reinterpret_cast<uint4*>(dst + d + far) = *reinterpret_cast<const uint4*>(y1);
     } else {
       T y = src[d];
-      if (TREE && kind == 2) spoilt |= spoilt2<T>(*reinterpret_cast<const uint16_t*>(&y));
+      if (TREE && kind == 2 && spoilt2<T>(*reinterpret_cast<const uint16_t*>(&y))) spoilt[head] = 1;
       if (turn && d < a.rot_dim) {
         const int i = a.interleaved ? d >> 1 : d % half;
         const bool upper = a.interleaved ? d & 1 : d >= half;
@@ -592,12 +602,6 @@ __global__ void __launch_bounds__(128) prefix_prep_tc_kernel(const ortb200_prefi
       }
       dst[d] = y;
     }
-  }
-  if (TREE) {
-    spoilt = __syncthreads_or(spoilt);
-    uint32_t* word = w.ancestors + static_cast<long long>(t) * kTreeStride + kTreeWords;
-    if (threadIdx.x == 0) word[blockIdx.y] = spoilt;
-    if (blockIdx.y == 0 && threadIdx.x >= gridDim.y && threadIdx.x < kTreeWords) word[threadIdx.x] = 0;
   }
 }
 
@@ -951,8 +955,8 @@ __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, cons
       if (key + 8 >= seen0) c[2] = -INFINITY;
       if (key + 8 >= seen1) c[3] = -INFINITY;
       if (TREE && g.tree && first + 16 > g.past) {   // (rows behind the unit's last take its bits)
-        const uint32_t* bits0 = w.ancestors + static_cast<long long>((g.q_row + min(n0, g.rows - 1)) / G) * kTreeStride;
-        const uint32_t* bits1 = w.ancestors + static_cast<long long>((g.q_row + min(n0 + 1, g.rows - 1)) / G) * kTreeStride;
+        const uint32_t* bits0 = w.ancestors + static_cast<long long>((g.q_row + min(n0, g.rows - 1)) / G) * tree_stride(a.Nk);
+        const uint32_t* bits1 = w.ancestors + static_cast<long long>((g.q_row + min(n0 + 1, g.rows - 1)) / G) * tree_stride(a.Nk);
         const int j = key - g.past;
         if (j >= 0 && !tree_sees(bits0, j)) c[0] = -INFINITY;
         if (j >= 0 && !tree_sees(bits1, j)) c[1] = -INFINITY;
@@ -962,11 +966,14 @@ __device__ __forceinline__ void few_rows(const ortb200_prefix_attn_args& a, cons
       uint32_t spoilt = 0;   // keys of this warp whose values are not finite
       if (TREE && first + 16 > g.past) {
         const int at = first + (lane & 15);
-        spoilt = __ballot_sync(0xffffffffu, lane < 16 && at >= g.past && at < g.end && tree_spoilt(w.ancestors, (g.q_row - g.in_seq) / G + at - g.past));
+        spoilt = __ballot_sync(0xffffffffu, lane < 16 && at >= g.past && at < g.end && tree_spoilt(w.ancestors, a.Nk, (g.q_row - g.in_seq) / G + at - g.past, g.kvh));
         if (spoilt) {
           const bool near = spoilt >> (lane >> 2) & 1, far = spoilt >> ((lane >> 2) + 8) & 1;
-          if ((near && c[0] != -INFINITY) || (far && c[2] != -INFINITY)) l0 = NAN;
-          if ((near && c[1] != -INFINITY) || (far && c[3] != -INFINITY)) l1 = NAN;
+          auto sees = [&](int n, int k, int seen) {   // (a score may be -inf without being hidden)
+            return k < seen && (!g.tree || k < g.past || tree_sees(w.ancestors + static_cast<long long>((g.q_row + min(n, g.rows - 1)) / G) * tree_stride(a.Nk), k - g.past));
+          };
+          if ((near && sees(n0, key, seen0)) || (far && sees(n0, key + 8, seen0))) l0 = NAN;
+          if ((near && sees(n0 + 1, key, seen1)) || (far && sees(n0 + 1, key + 8, seen1))) l1 = NAN;
         }
       }
       float t0 = fmaxf(c[0], c[2]) * fs, t1 = fmaxf(c[1], c[3]) * fs;
@@ -1346,8 +1353,8 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         tcgen05_fence_after();
         if (TREE && key0 + kKT > g.past) {   // keys of the tile whose values are not finite
           const int at = key0 + lane, row0 = (g.q_row - g.in_seq) / G - g.past;
-          const uint32_t spoilt0 = __ballot_sync(0xffffffffu, at >= g.past && at < g.end && tree_spoilt(w.ancestors, row0 + at));
-          const uint32_t spoilt1 = __ballot_sync(0xffffffffu, at + 32 >= g.past && at + 32 < g.end && tree_spoilt(w.ancestors, row0 + at + 32));
+          const uint32_t spoilt0 = __ballot_sync(0xffffffffu, at >= g.past && at < g.end && tree_spoilt(w.ancestors, a.Nk, row0 + at, g.kvh));
+          const uint32_t spoilt1 = __ballot_sync(0xffffffffu, at + 32 >= g.past && at + 32 < g.end && tree_spoilt(w.ancestors, a.Nk, row0 + at + 32, g.kvh));
           if (spoilt0 | spoilt1) {
             if (ok && !wait_warp(&bars[BAR_V_FULL + stage], parity)) ok = false;
             uint8_t* v = smem + L::kOffKV + stage * L::kStageBytes + L::kBoxes * L::kBox;
@@ -1356,7 +1363,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 #pragma unroll
                 for (int bx = 0; bx < L::kBoxes; ++bx) *reinterpret_cast<uint4*>(v + bx * L::kBox + i * 16) = make_uint4(0, 0, 0, 0);
             fence_proxy_async();
-            const uint32_t* bits = w.ancestors + static_cast<long long>((g.q_row + min(r, g.rows - 1)) / G) * kTreeStride;
+            const uint32_t* bits = w.ancestors + static_cast<long long>((g.q_row + min(r, g.rows - 1)) / G) * tree_stride(a.Nk);
             for (int j = 0; j < kKT; ++j)
               if ((j < 32 ? spoilt0 >> j : spoilt1 >> (j - 32)) & 1 && (g.tree ? tree_sees(bits, key0 + j - g.past) : key0 + j <= pos)) l = NAN;
           }
@@ -1375,7 +1382,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             for (int j = 0; j < kKT; ++j) sv[j] = cap(sv[j]);
           }
           if (TREE && g.tree && key0 + kKT > g.past) {   // 64 of the row's bits, the cache's all set (rows behind the unit's last take its bits)
-            const uint32_t* bits = w.ancestors + static_cast<long long>((g.q_row + min(r, g.rows - 1)) / G) * kTreeStride;
+            const uint32_t* bits = w.ancestors + static_cast<long long>((g.q_row + min(r, g.rows - 1)) / G) * tree_stride(a.Nk);
             const int lo = key0 - g.past, w0 = lo >> 5;
             auto word = [&](int i) { return i < 0 ? 0xffffffffu : i < kTreeWords ? __ldcg(bits + i) : 0u; };
             const uint32_t b0 = word(w0), b1 = word(w0 + 1), b2 = word(w0 + 2);
@@ -1852,7 +1859,7 @@ int launch_tc(const ortb200_prefix_attn_args* a, const int* parents, cudaStream_
   auto kern = a->softcap > 64.f ? prefix_attn_kernel<HD, kBf16, 2, TREE, QT> : a->softcap > 0.f ? prefix_attn_kernel<HD, kBf16, 1, TREE, QT> : prefix_attn_kernel<HD, kBf16, 0, TREE, QT>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) != cudaSuccess) return -10;   // per device
   const int heads = a->N + 2 * a->Nk;
-  const long long spread = 2 * kGrid / (a->T + 1), most = std::min((heads + 15) / 16, TREE ? kTreeWords : heads);   // few tokens: several CTAs per token, 16 heads at least to each
+  const long long spread = 2 * kGrid / (a->T + 1), most = (heads + 15) / 16;   // few tokens: several CTAs per token, 16 heads at least to each
   const dim3 prep_grid(static_cast<unsigned>(a->T + 1), static_cast<unsigned>(spread < 1 ? 1 : spread > most ? most : spread));
   int rc = vectorised<T>(a) ? launch_kernel(prefix_prep_tc_kernel<T, true, TREE, QT>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a, parents)
                             : launch_kernel(prefix_prep_tc_kernel<T, false, TREE, QT>, prep_grid, 128, 0, stream, a->use_pdl != 0, *a, parents);
@@ -1952,7 +1959,7 @@ extern "C" int ortb200_tree_attn_max_nodes(void) { return kTreeNodes; }
 
 extern "C" int64_t ortb200_tree_attn_workspace_bytes(int64_t T, int B, int N, int Nk, int H, int tensor_cores) {
   const int64_t bytes = ortb200_prefix_attn_workspace_bytes(T, B, N, Nk, H, tensor_cores);
-  return bytes < 0 ? bytes : bytes + tree_bytes(T);
+  return bytes < 0 ? bytes : bytes + tree_bytes(T, Nk);
 }
 
 extern "C" int ortb200_tree_attn(const ortb200_tree_attn_args* args, ortb200_stream_t stream_) {

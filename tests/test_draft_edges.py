@@ -5,11 +5,13 @@ import math
 import pytest
 import torch
 
+import draft_oracle as oracle
+
 from onnxruntime_b200.capi import EPFail, InvalidArgument
 from onnxruntime_b200.models.decoder_cache import CachePool, CacheTensor
 from onnxruntime_b200.models.generation import GenerationConfig, LogitsProcessor, generate_requests
 from test_draft_generation import PROVIDERS, decoder, pool
-from test_draft_ops import LOGITS_KINDS, LogitsCase
+from test_draft_ops import KINDS, LOGITS_KINDS, LogitsCase, TreeCase, tree
 
 
 # ----------------------------------------------------------------------------------------------------------------------- bans
@@ -61,6 +63,39 @@ def test_a_banned_token_is_not_chosen(provider, hard, kw):
     logits[:, 5] = hard
     scores = LogitsProcessor(40, torch.float32, device, GenerationConfig(**kw))(logits.to(device), [([1, 2, 5, 1, 2], 1, [[]]), ([2, 5, 3, 2], 0, [[]])]).cpu()
     assert (scores[:, 5] == -math.inf).all() and scores.argmax(-1).tolist() == [39, 39]
+
+
+# ------------------------------------------------------------------------------------------------------ values that are not finite
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("N,Nk,H,past,nodes", [(4, 2, 64, 0, 3), (8, 2, 64, 57, 7), (6, 3, 128, 130, 40), (32, 2, 128, 100, 100), (2, 2, 128, 70, 300), (40, 40, 64, 9, 3), (64, 64, 64, 70, 2),
+                                              (35, 5, 64, 200, 60), (6, 3, 40, 20, 9), (2, 2, 256, 65, 270)])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_a_value_that_is_not_finite_reaches_its_key_head(kind, N, Nk, H, past, nodes, bad):
+    """One element of one key head of one drafted token: the query heads that read it, in the rows that see the token, become NaN; all other results are,
+    to the bit, what they are without it, on every provider and in every form of the kernels."""
+    parents = [-1] + [(i - 1) // 2 if nodes <= 256 else i - 1 for i in range(1, nodes)]
+    case = TreeCase(kind[1], N, Nk, H, 16, [past, 33], [parents, tree(6, 3)], seed=nodes)
+    token, head, group = nodes // 2, Nk // 2, N // Nk
+    case.qkv[token, N + Nk + head] = 0.0
+    want = case.call(kind[0])()["out"].reshape(-1, N, H)
+    case.qkv[token, N + Nk + head, H // 3] = bad
+    got = case.call(kind[0])()["out"].reshape(-1, N, H)
+    spoilt = torch.zeros(nodes + 6, N, dtype=torch.bool)
+    sees = oracle.sees(parents)[:, token] if nodes <= 256 else torch.arange(nodes) >= token
+    spoilt[:nodes, head * group:(head + 1) * group] = sees.unsqueeze(1)
+    assert got[spoilt].isnan().all() and torch.equal(got[~spoilt], want[~spoilt])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("N,H,nodes", [(4, 64, 3), (32, 64, 40), (32, 128, 100), (4, 40, 3)])
+def test_a_value_that_is_not_finite_behind_a_score_of_minus_infinity(kind, N, H, nodes):
+    """A token that a row sees is seen, also with a weight of 0 because its score is -inf."""
+    case = TreeCase(kind[1], N, 2, H, 16, [20], [[-1, 0] + [1] * (nodes - 2)], rotary=0.0, seed=nodes)
+    case.qkv[:, :N] = case.qkv[:, :N].abs() + 0.125
+    case.qkv[1, N:N + 2] = -math.inf
+    case.qkv[1, N + 2, 3] = math.inf
+    got = case.call(kind[0])()["out"].reshape(nodes, N, H)
+    assert got[1:, :N // 2].isnan().all() and got[0].isfinite().all() and got[:, N // 2:].isfinite().all()
 
 
 # -------------------------------------------------------------------------------------------------------------------- biases
