@@ -571,6 +571,9 @@ def generate(runner: Union[DecoderRunner, PagedDecoderRunner], input_ids: torch.
     """Greedy (``num_beams == 1``, ``top_k == 0``, ``top_p == 1``, temperature 1), sampling or beam search.
     Returns [batch * num_return_sequences, prompt + generated] token ids, padded with ``pad_token_id`` after EOS.
     For beam search the runner must have been created with ``batch = prompts * num_beams``."""
+    for name in ("presence_penalty", "frequency_penalty", "logit_bias", "grammar", "draft_tokens"):
+        if getattr(cfg, name):
+            raise ValueError(f"{name} is an option of generate_requests()")
     if cfg.num_beams > 1:
         return _beam_search(runner, input_ids, cfg)
     dev = runner.device

@@ -9,7 +9,7 @@ import draft_oracle as oracle
 
 from onnxruntime_b200.capi import EPFail, InvalidArgument
 from onnxruntime_b200.models.decoder_cache import CachePool, CacheTensor
-from onnxruntime_b200.models.generation import GenerationConfig, LogitsProcessor, generate_requests
+from onnxruntime_b200.models.generation import GenerationConfig, LogitsProcessor, generate, generate_requests
 from test_draft_generation import PROVIDERS, decoder, pool
 from test_draft_ops import KINDS, LOGITS_KINDS, LogitsCase, TreeCase, tree
 
@@ -312,3 +312,14 @@ def test_sampled_drafts_of_requests_that_run_together(provider):
     r = decoder(provider, dtype="fp32", batch=2, vocab=40)
     first = generate_requests(r, prompts, cfg)
     assert generate_requests(r, prompts, cfg) == first and all(len(t) == 24 and max(t) < 5 for t in first)
+
+
+# ---------------------------------------------------------------------------------------------------------------------- options
+@pytest.mark.parametrize("option", [dict(presence_penalty=0.5), dict(frequency_penalty=-0.1), dict(logit_bias={3: 1.0}), dict(grammar=lambda done: None), dict(draft_tokens=2)], ids=lambda o: list(o)[0])
+@pytest.mark.parametrize("beams", [1, 2])
+def test_a_fixed_batch_refuses_options_that_it_does_not_have(option, beams):
+    """What only generate_requests() applies is an error in generate(), and not without effect."""
+    r = decoder("CPUExecutionProvider", trees=False, dtype="fp32", batch=beams, vocab=40)
+    with pytest.raises(ValueError, match=list(option)[0]):
+        generate(r, torch.tensor([[1, 2, 3]]), GenerationConfig(max_new_tokens=2, num_beams=beams, **option))
+    assert generate(r, torch.tensor([[1, 2, 3]]), GenerationConfig(max_new_tokens=2, num_beams=beams, logit_bias={}, draft_ngram=2)).shape == (1, 5)
