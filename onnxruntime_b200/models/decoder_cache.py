@@ -42,13 +42,14 @@ class CacheMover:
     """``com.ortb200.PagedCacheMove`` over given cache tensors, as a session of its own: one launch moves entries of tokens, or whole
     blocks, in all of them.  All sources are read before any target is written."""
 
-    _TYPES = {torch.float32: ol.TensorProto.FLOAT, torch.float16: ol.TensorProto.FLOAT16, torch.bfloat16: ol.TensorProto.BFLOAT16, torch.float64: ol.TensorProto.DOUBLE,
-              torch.int8: ol.TensorProto.INT8, torch.uint8: ol.TensorProto.UINT8, torch.int32: ol.TensorProto.INT32, torch.int64: ol.TensorProto.INT64}
+    # bytes are moved, whatever type they are of: by the size of an element
+    _TYPES = {1: (torch.uint8, ol.TensorProto.UINT8), 2: (torch.int16, ol.TensorProto.INT16), 4: (torch.int32, ol.TensorProto.INT32), 8: (torch.int64, ol.TensorProto.INT64)}
 
     def __init__(self, tensors: Sequence[torch.Tensor], whole_blocks: bool):
         self.device = tensors[0].device
         info = ol.make_tensor_value_info
-        kinds = [self._TYPES[t.dtype] for t in tensors]
+        types = [self._TYPES[min(t.element_size(), 8)] for t in tensors]
+        tensors, kinds = [t.view(dtype) for t, (dtype, _) in zip(tensors, types)], [kind for _, kind in types]
         places = [info(n, ol.TensorProto.INT64, ["moves"]) for n in ("sources", "targets")]
         names = ["cache.%d" % i for i in range(len(tensors))]
         graph = ol.make_graph([ol.make_node("PagedCacheMove", ["sources", "targets"] + names, [n + ".out" for n in names], domain="com.ortb200", whole_blocks=int(whole_blocks))],

@@ -194,6 +194,28 @@ def test_pool_keeps_no_path_of_state_in_slots():
     assert p.sequences["a"].length == 5
 
 
+@pytest.mark.parametrize("provider", PROVIDERS)
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float8_e5m2, torch.bool, torch.int16, torch.bfloat16, torch.complex64, torch.complex128], ids=str)
+@pytest.mark.parametrize("shape", [(3,), (2, 8)])
+def test_pools_of_any_type(provider, dtype, shape):
+    """Forks, kept paths and beams move bytes: caches of 8-bit floats, truth values and complex numbers, beside one of another type."""
+    device = torch.device("cuda:0" if provider == "CUDAExecutionProvider" else "cpu")
+    p = CachePool([CacheTensor("k", "k_out", "paged", shape, dtype), CacheTensor("v", "v_out", "paged", (2,), torch.float32)], 8, 4, 3, device)
+    for t in p.tensors.values():
+        raw = t.view(torch.uint8)
+        raw.copy_(torch.randint(0, 2 if dtype == torch.bool else 256, raw.shape, generator=torch.Generator().manual_seed(1)))
+    entries = lambda n, s: p.tensors[n].view(torch.uint8)[p.sequences[s].blocks].flatten(0, 1)[:p.sequences[s].length].clone()  # noqa: E731
+    hold(p, "a", 7)
+    hold(p, "c", 6)
+    before = {n: entries(n, "a") for n in "kv"}
+    p.fork("b", "a", 6)
+    assert all(torch.equal(entries(n, "b"), before[n][:6]) for n in "kv")
+    p.close("b")
+    p.copy_sequence_state(["a"], ["c"])
+    p.keep({"a": (1, [2, 5])})
+    assert all(torch.equal(entries(n, "a"), before[n][[0, 3, 6]]) and torch.equal(entries(n, "c"), before[n]) for n in "kv")
+
+
 # --------------------------------------------------------------------------------------------------------------- grammars
 class Strict:
     """Even and odd tokens by turns, as a state machine: a text that it has not allowed is an error."""
