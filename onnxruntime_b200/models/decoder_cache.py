@@ -46,7 +46,7 @@ class CacheMover:
     _TYPES = {1: (torch.uint8, ol.TensorProto.UINT8), 2: (torch.int16, ol.TensorProto.INT16), 4: (torch.int32, ol.TensorProto.INT32), 8: (torch.int64, ol.TensorProto.INT64)}
 
     def __init__(self, tensors: Sequence[torch.Tensor], whole_blocks: bool):
-        self.device = tensors[0].device
+        self.tensors, self.device = list(tensors), tensors[0].device
         info = ol.make_tensor_value_info
         types = [self._TYPES[min(t.element_size(), 8)] for t in tensors]
         tensors, kinds = [t.view(dtype) for t, (dtype, _) in zip(tensors, types)], [kind for _, kind in types]
@@ -92,7 +92,8 @@ class CachePool:
         paged = [self.tensors[c.input] for c in self.spec if c.kind == "paged"]
         if not paged or not sources:
             return
-        if whole_blocks not in self._movers:
+        mover = self._movers.get(whole_blocks)
+        if mover is None or any(a is not b for a, b in zip(mover.tensors, paged)):   # (another tensor may have taken one's place)
             self._movers[whole_blocks] = CacheMover(paged, whole_blocks)
         self._movers[whole_blocks](sources, targets)
 

@@ -216,6 +216,18 @@ def test_pools_of_any_type(provider, dtype, shape):
     assert all(torch.equal(entries(n, "a"), before[n][[0, 3, 6]]) and torch.equal(entries(n, "c"), before[n]) for n in "kv")
 
 
+def test_pool_moves_in_the_tensors_that_it_has_now():
+    """A pool's tensor may be another one than in the call before."""
+    p = pool()
+    hold(p, "a", 6)
+    p.fork("b", "a")
+    p.close("b")
+    old, p.tensors["k"] = p.tensors["k"], p.tensors["k"] + 1000
+    untouched = old.clone()
+    e = p.fork("b", "a")
+    assert torch.equal(old, untouched) and torch.equal(p.tensors["k"][e.blocks[1]], p.tensors["k"][p.sequences["a"].blocks[1]])
+
+
 # --------------------------------------------------------------------------------------------------------------- grammars
 class Strict:
     """Even and odd tokens by turns, as a state machine: a text that it has not allowed is an error."""
