@@ -222,7 +222,7 @@ def test_pool_moves_in_the_tensors_that_it_has_now():
     hold(p, "a", 6)
     p.fork("b", "a")
     p.close("b")
-    old, p.tensors["k"] = p.tensors["k"], p.tensors["k"] + 1000
+    old, p.tensors["k"] = p.tensors["k"], torch.randn(p.tensors["k"].shape)
     untouched = old.clone()
     e = p.fork("b", "a")
     assert torch.equal(old, untouched) and torch.equal(p.tensors["k"][e.blocks[1]], p.tensors["k"][p.sequences["a"].blocks[1]])
