@@ -148,6 +148,23 @@ def test_starts_of_no_biases(kind, starts, texts):
         case.call(kind[0])()
 
 
+# ---------------------------------------------------------------------------------------------------------------------- texts
+@pytest.mark.parametrize("kind", LOGITS_KINDS)
+@pytest.mark.parametrize("vocab,lengths,place", [(50257, [20000, 8193, 9001], None), (50257, [20000, 8193, 9001], 1), (300007, [9000, 12001, 8200], None), (4099, [30000, 1, 12000], None),
+                                                 (16384, [8193, 8193, 8193], 1)])
+def test_texts_of_more_than_64_kilobytes(kind, vocab, lengths, place):
+    """Texts of more than 8192 tokens to a list on average, which a form of its own reads: fewer tokens than are listed and more, parts that count and
+    parts that do not, at odd places; with drafted tokens, biases and masks, and rows that share a list."""
+    g = torch.Generator().manual_seed(vocab)
+    case = LogitsCase(kind[1], 5, vocab, lists=3, drafted=4, biases=300, seed=vocab)
+    starts = torch.tensor([0, *lengths]).cumsum(0)
+    tokens = torch.randint(-1, vocab + 1, (sum(lengths),), generator=g)
+    tokens[::3] = torch.randint(0, 50, (len(tokens[::3]),), generator=g)
+    case.t.update(history=tokens, history_starts=starts, generated_starts=starts[:-1] + torch.tensor([lengths[0] // 3, 0, lengths[2]]),
+                  row_list=torch.tensor([1, 0, 2, -1, 0], dtype=torch.int32), repetition=torch.tensor([1.2, 1.0, 1.5, 1.3, 1.1]))
+    case.run(kind[0], place=place)
+
+
 # ------------------------------------------------------------------------------------------------------------------- the pool
 def hold(p, seq, tokens):
     if seq not in p.sequences:
