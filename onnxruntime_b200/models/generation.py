@@ -686,7 +686,7 @@ class LogitsProcessor:
                  named: Optional[Sequence[Optional[Sequence[int]]]] = None) -> torch.Tensor:
         """logits [rows, vocab] -> scores [rows, vocab] in 32 bits.  ``requests``: (text, how many tokens of it are generated, for each of
         the request's rows the drafted tokens behind the text).  ``named``: what the grammar names for each row, where it has been asked."""
-        if self.idle:
+        if self.idle or not len(logits):
             return logits.float()
         cfg, dev, rows = self.cfg, self.device, logits.shape[0]
         ints = lambda v, t=torch.int64: torch.tensor(v, dtype=t).to(dev)  # noqa: E731

@@ -9,7 +9,7 @@ import draft_oracle as oracle
 
 from onnxruntime_b200.capi import EPFail, InvalidArgument
 from onnxruntime_b200.models.decoder_cache import CachePool, CacheTensor
-from onnxruntime_b200.models.generation import GenerationConfig, LogitsProcessor, generate, generate_requests
+from onnxruntime_b200.models.generation import GenerationConfig, LogitsProcessor, draft_tree, generate, generate_requests
 from test_draft_generation import PROVIDERS, decoder, pool
 from test_draft_ops import KINDS, LOGITS_KINDS, LogitsCase, TreeCase, tree
 
@@ -329,7 +329,24 @@ def test_requests_of_a_call_that_fails_are_given_back(drafts):
     assert generate_requests(r, prompts, GenerationConfig(max_new_tokens=8, draft_tokens=drafts)) == want
 
 
+@pytest.mark.parametrize("kw", [dict(repetition_penalty=1.2), dict(logit_bias={1: 1.0}), dict(grammar=lambda done: [1]), dict(temperature=0.5), dict()], ids=lambda k: " ".join(k) or "idle")
+def test_no_rows(kw):
+    """A batch without a request."""
+    processor = LogitsProcessor(40, torch.bfloat16, torch.device("cpu"), GenerationConfig(**kw))
+    got = processor(torch.zeros(0, 40, dtype=torch.bfloat16), [])
+    assert got.shape == (0, 40) and got.dtype == torch.float32
+    assert processor(torch.zeros(1, 40, dtype=torch.bfloat16), [([1], 0, [[]])]).shape == (1, 40)
+
+
 # ----------------------------------------------------------------------------------------------------------------- limits of drafts
+def test_drafts_of_a_text_that_overlaps_itself():
+    """The longest tail first, of its occurrences the latest first, each with half as many tokens as there may be: worked out by hand."""
+    assert draft_tree([5, 5, 5, 5], 3) == ([5, 5, 5], [-1, 0, 1])
+    assert draft_tree([5, 5, 5, 5], 1) == ([5, 5], [-1, 0])
+    assert draft_tree([5, 5, 5, 5, 5], 6, 2) == ([5, 5, 5, 5], [-1, 0, 1, 2])
+    assert draft_tree([1, 2, 1, 2, 1], 4, 2) == ([1, 2, 1], [-1, 0, 1])
+
+
 @pytest.mark.parametrize("drafts", [255, 256, 300, 1 << 40])
 def test_drafts_beyond_the_largest_tree(drafts):
     """A text that offers more drafts than a tree has: the step takes the largest tree, and the call goes on."""
