@@ -13,7 +13,18 @@ inline int DtypeCode(at::ScalarType t) {
 }
 inline int Pdl(OpKernelContext& ctx) { return ctx.session()->config().Get("ortb200.pdl", "0") == "1" ? 1 : 0; }
 
-// The bound buffer of output i where it fits and is none of the inputs (but `in_place`), else a new tensor, which the executor
+// Two tensors have memory in common.  (By addresses: buffers that are bound by their pointers have storages of their own.)
+inline bool Overlap(const at::Tensor& a, const at::Tensor& b) {
+  const auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  return a.defined() && b.defined() && a.numel() > 0 && b.numel() > 0 && a.device() == b.device() && a.data_ptr() < static_cast<const void*>(end(b)) &&
+         b.data_ptr() < static_cast<const void*>(end(a));
+}
+
+// The bound buffer of output i where it fits and shares no memory with an input (but `in_place`, all of it), else a new tensor, which the executor
 // copies to whatever is bound.
 inline at::Tensor Output(OpKernelContext& ctx, int i, at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like, int in_place = -1) {
   if (i < ctx.OutputCount()) {
@@ -21,9 +32,9 @@ inline at::Tensor Output(OpKernelContext& ctx, int i, at::IntArrayRef sizes, at:
     if (b.defined() && b.device() == like.device() && b.scalar_type() == type && b.sizes() == sizes && b.is_contiguous()) {
       bool apart = true;
       for (int j = 0; j < ctx.InputCount(); ++j)
-        if (ctx.HasInput(j) && ctx.Input(j).is_alias_of(b) && !(j == in_place && ctx.Input(j).data_ptr() == b.data_ptr())) apart = false;
+        if (ctx.HasInput(j) && Overlap(ctx.Input(j), b) && !(j == in_place && ctx.Input(j).data_ptr() == b.data_ptr())) apart = false;
       for (int j = 0; j < i; ++j)
-        if (ctx.Preallocated(j).defined() && ctx.Preallocated(j).is_alias_of(b)) apart = false;
+        if (Overlap(ctx.Preallocated(j), b)) apart = false;
       if (apart) return b;
     }
   }

@@ -391,3 +391,32 @@ def test_a_fixed_batch_refuses_options_that_it_does_not_have(option, beams):
     with pytest.raises(ValueError, match=list(option)[0]):
         generate(r, torch.tensor([[1, 2, 3]]), GenerationConfig(max_new_tokens=2, num_beams=beams, **option))
     assert generate(r, torch.tensor([[1, 2, 3]]), GenerationConfig(max_new_tokens=2, num_beams=beams, logit_bias={}, draft_ngram=2)).shape == (1, 5)
+
+
+# ------------------------------------------------------------------------------------------------------------ buffers by address
+def by_address(call, provider, shared):
+    """Runs with output `shared[0]` bound, by its address, to the memory of input `shared[1]`; returns the outputs as they are there."""
+    out, into = shared
+    gpu = provider == "CUDAExecutionProvider"
+    t = call.ins[into].clone()
+    call.binding.bind_input(into, "cuda" if gpu else "cpu", 0, t.dtype, list(t.shape), t.data_ptr())
+    call.binding.bind_output(out, "cuda" if gpu else "cpu", 0, t.dtype, list(call.outs[out].shape), t.data_ptr())
+    call.sess.run_with_iobinding(call.binding)
+    if gpu:
+        torch.cuda.synchronize()
+        call.sess.check_device_status()
+    return {**{n: v.cpu() for n, v in call.outs.items()}, out: t.cpu().reshape(call.outs[out].shape)}
+
+
+@pytest.mark.parametrize("provider", PROVIDERS)
+@pytest.mark.parametrize("vocab", [200, 50257])
+def test_scores_in_the_memory_of_the_logits(provider, vocab):
+    """32-bit scores bound, by their address, where the logits are: touched tokens are worked out of the logits, not of scores."""
+    case = LogitsCase(torch.float32, 6, vocab, length=300, seed=2)
+    case.check(by_address(case.call(provider), provider, ("scores", "logits")))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_results_in_the_memory_of_the_queries(kind):
+    case = TreeCase(kind[1], 4, 2, 64, 16, [90, 80, 120], [tree(1, 0), tree(3, 1), tree(20, 2)], separate=True, seed=3)
+    case.check(by_address(case.call(kind[0]), kind[0], ("out", "q")))
