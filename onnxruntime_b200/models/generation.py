@@ -316,12 +316,16 @@ class PagedDecoderRunner:
         for seq in paths:
             del self._drafted[seq]
 
+    def _want_accepted(self, seqs) -> None:
+        for seq in seqs if self._drafted else ():
+            if seq in self._drafted:
+                raise ValueError(f"the drafted tokens of sequence {seq!r} wait for accept()")
+
     def _make_room(self, entries) -> None:
         opened = []
         try:
             for seq, tokens, want in entries:
-                if seq in self._drafted:
-                    raise ValueError(f"the drafted tokens of sequence {seq!r} wait for accept()")
+                self._want_accepted([seq])
                 if any(not 0 <= w < len(tokens) for w in want):
                     raise ValueError(f"sequence {seq!r}: a wanted place lies outside its {len(tokens)} tokens")
                 if seq not in self.pool.sequences:
@@ -346,8 +350,7 @@ class PagedDecoderRunner:
 
     def fork(self, seq: Hashable, source: Hashable, tokens: Optional[int] = None) -> None:
         """Opens ``seq`` behind the first ``tokens`` (default: all) tokens that ``source`` holds."""
-        if source in self._drafted:
-            raise ValueError(f"the drafted tokens of sequence {source!r} wait for accept()")
+        self._want_accepted([source])
         self.pool.fork(seq, source, tokens)
 
     def release(self, seq: Hashable) -> None:
@@ -427,7 +430,7 @@ class PagedDecoderRunner:
     def _reopen_rows(self) -> None:
         for r in self._rows:
             if r in self.pool.sequences:
-                self.pool.close(r)
+                self.release(r)
         for r in self._rows:
             self.pool.open(r)
         # full capacity at once, one block per row in turn: the block table of a row is fixed from here on, and no row owns
@@ -457,9 +460,11 @@ class PagedDecoderRunner:
             self._reopen_rows()
         for r in self._rows:
             self.pool.sequences[r].length = length
+            self._drafted.pop(r, None)
 
     def decode_step(self, tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One token per sequence; ``tokens`` [B] or None to feed back the previous step's output."""
+        self._want_accepted(self._rows)
         buf = self._decode_buffers(self.batch)
         buf.ids.copy_(tokens.reshape(-1) if tokens is not None else buf.next, non_blocking=True)
         self._run_decode(buf, self._rows)
@@ -468,6 +473,7 @@ class PagedDecoderRunner:
 
     def reorder_cache(self, rows: torch.Tensor) -> None:
         """Row i takes the content of row rows[i] (beam search: beams follow their parents)."""
+        self._want_accepted(self._rows)
         self.pool.copy_sequence_state([self._rows[int(r)] for r in rows.tolist()], self._rows)
 
     def generate(self, input_ids, max_new_tokens: int) -> torch.Tensor:

@@ -393,6 +393,29 @@ def test_a_fixed_batch_refuses_options_that_it_does_not_have(option, beams):
     assert generate(r, torch.tensor([[1, 2, 3]]), GenerationConfig(max_new_tokens=2, num_beams=beams, logit_bias={}, draft_ngram=2)).shape == (1, 5)
 
 
+def test_drafts_of_the_fixed_batch_wait_for_accept():
+    """The rows of prefill() and decode_step() are sequences like others: a step behind drafts that wait is refused, and new prompts forget them."""
+    r = decoder("CPUExecutionProvider", dtype="fp32", batch=2, max_len=32, vocab=40)
+    row = ("row", 0)
+    first = r.prefill([[1, 2, 3], [4, 5]]).clone()
+    want = r.decode_step(first).clone()
+    r.prefill([[1, 2, 3], [4, 5]])
+    r.draft_step([(row, [7, 8], [-1, 0], [1])])
+    for call in (lambda: r.decode_step(first), lambda: r.reorder_cache(torch.tensor([1, 0])), lambda: r.step([(row, [1], [0])]), lambda: r.fork("x", row)):
+        with pytest.raises(ValueError, match="accept"):
+            call()
+    r.accept({row: []})
+    assert torch.equal(r.decode_step(first), want)
+    r.draft_step([(row, [7, 8], [-1, 0], [1])])
+    r.prefill([[1, 2, 3], [4, 5]])
+    assert torch.equal(r.decode_step(first), want)
+    with pytest.raises(ValueError):
+        r.accept({row: [0]})
+    r.draft_step([(row, [7], [-1], [0])])
+    r.assume_context(9)
+    r.decode_step(first)
+
+
 # ------------------------------------------------------------------------------------------------------------ buffers by address
 def by_address(call, provider, shared):
     """Runs with output `shared[0]` bound, by its address, to the memory of input `shared[1]`; returns the outputs as they are there."""
