@@ -322,6 +322,8 @@ SharedPrefixSizes CheckTreeAttention(Ctx& ctx) {
   SharedPrefixSizes z = PagedQuerySizes(ctx, ": no window is known for trees; use PagedAttention");
   WantInts(ctx, 8, at::kInt, 1, "parents");
   ORTB_ENFORCE_ARG(ctx.Input(8).size(0) == z.T, "TreePagedAttention: parents have one entry per token");
+  const at::Tensor &kc = ctx.Input(3), &vc = ctx.Input(4);   // (views that lie side by side in one tensor are not contiguous)
+  ORTB_ENFORCE_ARG(!kc.is_contiguous() || !vc.is_contiguous() || !Overlap(kc, vc), "TreePagedAttention: key and value caches share memory");
   z.tree = true;
   return z;
 }

@@ -6,6 +6,17 @@
 
 namespace ortb {
 
+// Two tensors have memory in common.  (By addresses: buffers that are bound by their pointers have storages of their own.)
+inline bool Overlap(const at::Tensor& a, const at::Tensor& b) {
+  const auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  return a.defined() && b.defined() && a.numel() > 0 && b.numel() > 0 && a.device() == b.device() && a.data_ptr() < static_cast<const void*>(end(b)) &&
+         b.data_ptr() < static_cast<const void*>(end(a));
+}
+
 // com.ortb200 SharedPrefixPagedAttention and, with parents in the place of shared_prefix and nothing behind sin_cache, TreePagedAttention
 // inputs: query, key?, value?, key_cache, value_cache, cumulative_sequence_length, past_seqlens, block_table, shared_prefix,
 //         cos_cache?, sin_cache?, positions?, slot_mapping?

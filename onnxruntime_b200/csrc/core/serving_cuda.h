@@ -4,6 +4,7 @@
 
 #include "kernel.h"
 #include "ortb200_kernels.h"
+#include "serving_checks.h"
 #include "session.h"
 
 namespace ortb {
@@ -12,17 +13,6 @@ inline int DtypeCode(at::ScalarType t) {
   return t == at::kHalf ? ORTB200_F16 : t == at::kBFloat16 ? ORTB200_BF16 : t == at::kFloat ? ORTB200_F32 : -1;
 }
 inline int Pdl(OpKernelContext& ctx) { return ctx.session()->config().Get("ortb200.pdl", "0") == "1" ? 1 : 0; }
-
-// Two tensors have memory in common.  (By addresses: buffers that are bound by their pointers have storages of their own.)
-inline bool Overlap(const at::Tensor& a, const at::Tensor& b) {
-  const auto end = [](const at::Tensor& t) {
-    int64_t last = 0;
-    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
-  };
-  return a.defined() && b.defined() && a.numel() > 0 && b.numel() > 0 && a.device() == b.device() && a.data_ptr() < static_cast<const void*>(end(b)) &&
-         b.data_ptr() < static_cast<const void*>(end(a));
-}
 
 // The bound buffer of output i where it fits and shares no memory with an input (but `in_place`, all of it), else a new tensor, which the executor
 // copies to whatever is bound.

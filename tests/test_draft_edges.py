@@ -416,6 +416,26 @@ def test_drafts_of_the_fixed_batch_wait_for_accept():
     r.decode_step(first)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_key_and_value_caches_in_the_same_memory(kind):
+    """New values would be written over new keys."""
+    case = TreeCase(kind[1], 4, 2, 64, 16, [20, 40], [[-1, 0], [-1, 0, 0]])
+    call = case.call(kind[0])
+    both = torch.cat([call.ins["kc"], call.ins["vc"]])
+    n = len(call.ins["kc"])
+    for first, second in ((0, 0), (0, 1), (n - 1, 0)):
+        for name, at in (("kc", first), ("vc", second)):
+            call.binding.bind_torch_input(name, both[at:at + n])
+            call.binding.bind_torch_output(name + "_out", both[at:at + n])
+        with pytest.raises(InvalidArgument):
+            call()
+    for name, at in (("kc", 0), ("vc", n)):
+        call.binding.bind_torch_input(name, both[at:at + n])
+        call.binding.bind_torch_output(name + "_out", both[at:at + n])
+    got = call()
+    case.check({**got, "kc_out": both[:n].cpu(), "vc_out": both[n:].cpu()})
+
+
 # ------------------------------------------------------------------------------------------------------------ buffers by address
 def by_address(call, provider, shared):
     """Runs with output `shared[0]` bound, by its address, to the memory of input `shared[1]`; returns the outputs as they are there."""
