@@ -25,7 +25,7 @@ int64_t ortb200_tree_attn_workspace_bytes(int64_t T, int B, int N, int Nk, int H
 
 // cache[targets[m]] = cache[sources[m]] for every cache and every move, as if all sources were read before any target is written.
 // A cache is `units` units of unit_bytes[c] bytes.  A negative target is no move; a place outside the cache, or a target that is
-// named twice, is reported through the status word (the former is left out, of the latter one of the moves takes place).
+// named twice, is reported through the status word (the former is left out; what lies at the latter then comes from any of its moves, piece by piece).
 // The caches do not overlap.
 typedef struct {
   void* const* caches;          // [num_caches], host array

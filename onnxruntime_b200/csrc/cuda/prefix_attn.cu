@@ -35,10 +35,12 @@
 // scores and one for the products with V 147 and 72 instead of 140 and 67; few rows through tensor memory like all others 139 and 68
 // instead of 115 and 64.
 //
-// Trees, back to back: 24 of 8 to 16 tokens behind 2000 to 4000 (32 heads over 8 of 128) 76 us, of which the bytes need 46; a CTA's tiles come
-// at the rate of the memory, and what is left is the first 7 us, in which the step in front gives the queries, and the last segments'
-// ends.  6 of 38 to 59 tokens behind 20000 to 30000 (64 heads over 8) 368 us, of which the products need 138: a tile of 256 rows and 64 keys takes
-// a CTA 2450 clocks, the tensor pipe and the shared memory that feeds it 1500 of them, the exponentials 1024.  Slower or no better there:
+// Trees, back to back: 24 of 8 to 16 tokens behind 2000 to 4000 (32 heads over 8 of 128) 76 to 88 us, of which the bytes need 46; a CTA's tiles come
+// at the rate of the memory, and what is left is the first 7 us, in which the step in front gives the queries and a CTA has its first tiles on their way
+// and asks for no more, and the last segments' ends.  6 of 38 to 59 tokens behind 20000 to 30000 (64 heads over 8) 368 to 452 us, of which the products
+// need 138, and 207 with weights as two terms: a tile of 256 rows and 64 keys takes
+// a CTA 2450 clocks, the tensor pipe and the shared memory that feeds it 1500 of them, the exponentials 1024.  (The lower figures are the kernel alone
+// and short runs, the higher ones long runs with other inputs each time, under the power cap.)  Slower or no better there, in short runs:
 // units of 128 rows 398 us (keys and values are read from DRAM twice as often); weights rounded once 327 us, but an error of 0.0029
 // instead of 0.0024 against 64 bits; the two tiles' softmax half a tile apart 368 us (they fall into step again).  A loader
 // that asks for a tile's values behind the next tile's keys took 75 instead of 76 us and 410 instead of 419, but 73 instead of 59 for single tokens.
@@ -244,6 +246,8 @@ __global__ void __launch_bounds__(128) prefix_rows_kernel(const ortb200_prefix_a
 }
 
 // ------------------------------------------------------------------------------------------------------- tensor-core form
+// Rotated queries are rounded to the type, as rotated keys are in the cache and as an operator of its own that rotates them would leave them
+// (PagedAttention, rotary embedding).  A second 16-bit term would take half as much again of the product with K.
 // Weights reach the product with V as the sum of two 16-bit values.  Rounded once they would be off by as much as the rounded
 // queries are, and the result by 1.7 times the rounding of a 32-bit one instead of 1.4; it costs half a product more, 7 % of the
 // time where sequences bring single tokens and 12 % where the tensor pipe is full.
@@ -1716,7 +1720,9 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ortb200_prefix_a
 // them and a warp four.  What it takes beside step 2 is waiting for loads, so that few rows behind one another matter, and not how many CTAs look in vain.  All segments
 // written and all rows joined, up to 32 by a warp one after the other, against this, whole calls back to back: 146 and 95 us (75 trees of up to 60 tokens
 // behind 779, 24 heads over 8 of 64), 107 and 78 (52 of up to 58 behind 382, 32 over 8 of 128), 131 and 112 (512 of up to 4 behind 500), but 28.7 and 30.7
-// (20 of up to 10 behind 500).
+// (20 of up to 10 behind 500).  The join by itself, serialised, is slower where most units are spread over several CTAs: 14.2 instead of 12.5 us (24 of 8
+// to 16 behind 2000 to 4000) and 22.3 instead of 17.4 (6 of 38 to 59 behind 20000 to 30000), some 2 and 1 % of those calls; how many units are spread
+// is known on the device alone, so that all trees beyond few rows take this one.
 constexpr int kJoinRows = 32, kJoinThreads = 256;
 // the last of n ascending places that is not behind x, by all of a CTA
 template <typename I>

@@ -8,7 +8,8 @@
 //
 // What bounds it: without texts the stream (384 rows of 128256 bf16 logits 55 us, 295 MB; the bytes need 45).  With a text of 2250 tokens to a
 // row 108 us: reading and counting it in each of 16 chunks, 112 MB out of L2 and half of the instructions; issue slots are 67 % busy.  A text of
-// 45000 tokens and 50257 32-bit logits, 40 rows: 24 us, nearly all of it the text.  Slower, for the same 384 rows: a text read once by a cluster of
+// 45000 tokens and 50257 32-bit logits, 40 rows: 24 us, nearly all of it the text: four parts of a row read it, the last of which has 1105 tokens, and with
+// one CTA of 1024 threads to an SM 160 CTAs are two rounds.  Slower, for the same 384 rows: a text read once by a cluster of
 // the row's CTAs, which add to each other's counters, 212 us; a kernel that gathers what a row touches in a hash table, behind the stream or
 // in front of it, 105 to 111 and a second launch; a warp's tokens of the chunk queued and counted 32 at a time 123.
 #include <cuda_runtime.h>
