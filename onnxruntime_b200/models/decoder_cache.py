@@ -48,7 +48,8 @@ class CacheMover:
     def __init__(self, tensors: Sequence[torch.Tensor], whole_blocks: bool):
         self.tensors, self.device = list(tensors), tensors[0].device
         info = ol.make_tensor_value_info
-        types = [self._TYPES[min(t.element_size(), 8)] for t in tensors]
+        tensors = [torch.view_as_real(t) if t.is_complex() else t for t in tensors]
+        types = [self._TYPES[t.element_size()] for t in tensors]
         tensors, kinds = [t.view(dtype) for t, (dtype, _) in zip(tensors, types)], [kind for _, kind in types]
         places = [info(n, ol.TensorProto.INT64, ["moves"]) for n in ("sources", "targets")]
         names = ["cache.%d" % i for i in range(len(tensors))]

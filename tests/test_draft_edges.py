@@ -213,7 +213,7 @@ def test_pool_keeps_no_path_of_state_in_slots():
 
 @pytest.mark.parametrize("provider", PROVIDERS)
 @pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float8_e5m2, torch.bool, torch.int16, torch.bfloat16, torch.complex64, torch.complex128], ids=str)
-@pytest.mark.parametrize("shape", [(3,), (2, 8)])
+@pytest.mark.parametrize("shape", [(3,), (2, 8), ()])
 def test_pools_of_any_type(provider, dtype, shape):
     """Forks, kept paths and beams move bytes: caches of 8-bit floats, truth values and complex numbers, beside one of another type."""
     device = torch.device("cuda:0" if provider == "CUDAExecutionProvider" else "cpu")
@@ -221,7 +221,7 @@ def test_pools_of_any_type(provider, dtype, shape):
     for t in p.tensors.values():
         raw = t.view(torch.uint8)
         raw.copy_(torch.randint(0, 2 if dtype == torch.bool else 256, raw.shape, generator=torch.Generator().manual_seed(1)))
-    entries = lambda n, s: p.tensors[n].view(torch.uint8)[p.sequences[s].blocks].flatten(0, 1)[:p.sequences[s].length].clone()  # noqa: E731
+    entries = lambda n, s: p.tensors[n].view(torch.uint8).reshape(8, 4, -1)[p.sequences[s].blocks].flatten(0, 1)[:p.sequences[s].length].clone()  # noqa: E731
     hold(p, "a", 7)
     hold(p, "c", 6)
     before = {n: entries(n, "a") for n in "kv"}
